@@ -20,6 +20,7 @@
 #include "attention.h"
 #include "gemm.h"
 #include "gemv.h"
+#include "kv4.h"
 #include "layout.h"
 #include "link.h"
 #include "trace.h"
@@ -964,7 +965,9 @@ int dial_b200_device_status(int* status_out, int clear, char* err, size_t n) {
     }
     int v_noalloc = 0;
     DIAL_CUDA(noalloc_status(dev, clear != 0, &v_noalloc));
-    if (status_out) *status_out = v != 0 ? v : v_noalloc;
+    int v_kv4 = 0;
+    DIAL_CUDA(kv4_status(dev, clear != 0, &v_kv4));
+    if (status_out) *status_out = v != 0 ? v : v_noalloc != 0 ? v_noalloc : v_kv4;
   });
 }
 

@@ -1,0 +1,198 @@
+// Attention over the 4-bit KV cache.
+//
+//   o = sum_j p_j v_j,  p_j = exp(s_j - m) / l,  s_j = scale * q . k_j
+//
+// over the slots j a query sees.  One CTA of 8 warps per (query, query head,
+// sequence): warp w takes slots w, w + 8, ..., four dims a lane, with a running
+// maximum and sum; the warps' parts are merged in shared memory.  With running
+// weights a second kernel forms p_j again from each query's log-sum-exp, one
+// warp per (slot, kv head, sequence), so that no two warps add to one slot.
+#include <cmath>
+
+#include "kv4_dev.cuh"
+
+namespace dialb200 {
+namespace {
+
+struct AttnArgs {
+  Kv4Cache c;
+  const void* q;
+  const int32_t* sids;
+  const int32_t* lens;
+  const int32_t* q_starts;
+  void* out;
+  float* lse;  // [rows][q_heads], with weights
+  long long q_ld, out_ld;
+  int seqs, rows, max_q, max_len;
+  float scale;
+};
+
+struct Seq {
+  int sid, len, row0, n;
+};
+
+// The sequence's rows and slots; false (with the status recorded) for one
+// whose session, rows or length are out of range.
+__device__ __forceinline__ bool seq_of(const AttnArgs& a, int i, Seq& s) {
+  s.sid = a.sids[i];
+  s.len = a.lens[i];
+  s.row0 = a.q_starts ? a.q_starts[i] : i;
+  const int end = a.q_starts ? a.q_starts[i + 1] : i + 1;
+  if (static_cast<unsigned>(s.sid) >= static_cast<unsigned>(a.c.sessions) || s.len < 0 ||
+      s.len > a.max_len || s.row0 < 0 || end < s.row0 || end > a.rows || end - s.row0 > a.max_q) {
+    set_status(a.c.status, kStatusBadArgs);
+    return false;
+  }
+  s.n = end - s.row0;
+  return true;
+}
+
+template <typename Act>
+__global__ void __launch_bounds__(256) kv4_attn_kernel(const AttnArgs a) {
+  __shared__ float part[8][kHeadDim + 2];
+  const int j = blockIdx.x, h = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  Seq s;
+  if (!seq_of(a, blockIdx.z, s) || j >= s.n) return;
+  const int seen = max(0, s.len - s.n + 1 + j), kvh = h / (a.c.q_heads / a.c.kv_heads);
+  const int row = s.row0 + j;
+  float q[4], o[4] = {0.f, 0.f, 0.f, 0.f}, m = -INFINITY, l = 0.f;
+  load4(static_cast<const Act*>(a.q) + row * a.q_ld + h * kHeadDim + lane * 4, q);
+  for (int t = warp; t < seen; t += 8) {
+    const int block = max(0, kv4_block(a.c, a.c.block_table, s.sid, t / kPageTokens));
+    const uint8_t* slab = a.c.pages + kv4_slab_index(a.c, block, kvh) * kKv4Slab;
+    float k[4], v[4];
+    kv4_decode(slab, 0, kKv4KScales, t % kPageTokens, lane, a.c.k_scale, k);
+    kv4_decode(slab, kKv4VCodes, kKv4VScales, t % kPageTokens, lane, a.c.v_scale, v);
+    const float sc =
+        warp_sum(fmaf(q[0], k[0], q[1] * k[1]) + fmaf(q[2], k[2], q[3] * k[3])) * a.scale;
+    const float mn = fmaxf(m, sc);
+    const float keep = m == -INFINITY ? 0.f : expf(m - mn), p = expf(sc - mn);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = fmaf(o[e], keep, p * v[e]);
+    l = fmaf(l, keep, p);
+    m = mn;
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) part[warp][lane * 4 + e] = o[e];
+  if (lane == 0) {
+    part[warp][kHeadDim] = m;
+    part[warp][kHeadDim + 1] = l;
+  }
+  __syncthreads();
+  if (threadIdx.x < kHeadDim) {
+    float M = -INFINITY, L = 0.f, O = 0.f;
+    for (int w = 0; w < 8; ++w) M = fmaxf(M, part[w][kHeadDim]);
+    for (int w = 0; w < 8; ++w) {
+      const float f = part[w][kHeadDim] == -INFINITY ? 0.f : expf(part[w][kHeadDim] - M);
+      L = fmaf(f, part[w][kHeadDim + 1], L);
+      O = fmaf(f, part[w][threadIdx.x], O);
+    }
+    static_cast<Act*>(a.out)[row * a.out_ld + h * kHeadDim + threadIdx.x] =
+        ActTraits<Act>::from_f(seen > 0 ? O / L : 0.f);
+    if (a.lse && threadIdx.x == 0)
+      a.lse[static_cast<size_t>(row) * a.c.q_heads + h] = M + logf(L);
+  }
+}
+
+template <typename Act>
+__global__ void __launch_bounds__(256) kv4_weights_kernel(const AttnArgs a) {
+  const int t = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const int kvh = blockIdx.y, rep = a.c.q_heads / a.c.kv_heads;
+  Seq s;
+  if (!seq_of(a, blockIdx.z, s) || t >= s.len) return;
+  const int block = kv4_block(a.c, a.c.block_table, s.sid, t / kPageTokens);
+  const size_t si = kv4_slab_index(a.c, max(block, 0), kvh);
+  float k[4], sum = 0.f;
+  kv4_decode(a.c.pages + si * kKv4Slab, 0, kKv4KScales, t % kPageTokens, lane, a.c.k_scale, k);
+  for (int j = max(0, t - (s.len - s.n)); j < s.n; ++j)
+    for (int r = 0; r < rep; ++r) {
+      const int h = kvh * rep + r;
+      const size_t row = s.row0 + j;
+      float q[4];
+      load4(static_cast<const Act*>(a.q) + row * a.q_ld + h * kHeadDim + lane * 4, q);
+      const float sc =
+          warp_sum(fmaf(q[0], k[0], q[1] * k[1]) + fmaf(q[2], k[2], q[3] * k[3])) * a.scale;
+      sum += expf(sc - a.lse[row * a.c.q_heads + h]);
+    }
+  if (lane == 0 && block >= 0) a.c.weights[si * kPageTokens + t % kPageTokens] += sum;
+}
+
+template <typename Act>
+cudaError_t launch(const AttnArgs& a, cudaStream_t s) {
+  kv4_attn_kernel<Act><<<dim3(a.max_q, a.c.q_heads, a.seqs), 256, 0, s>>>(a);
+  cudaError_t e = cudaGetLastError();
+  if (e == cudaSuccess && a.c.weights) {
+    kv4_weights_kernel<Act><<<dim3((a.max_len + 7) / 8, a.c.kv_heads, a.seqs), 256, 0, s>>>(a);
+    e = cudaGetLastError();
+  }
+  return e;
+}
+
+}  // namespace
+}  // namespace dialb200
+
+using namespace dialb200;
+
+extern "C" int64_t dial_b200_kv4_attention_scratch_bytes(const dial_b200_kv4_shape* sh,
+                                                         int64_t seqs, int64_t rows, int64_t max_q,
+                                                         int64_t max_len, int32_t with_weights) {
+  if (!sh || sh->q_heads < 1 || sh->kv_heads < 1 || seqs < 0 || rows < 0 || max_q < 0 ||
+      max_len < 0)
+    return -1;
+  return with_weights ? rows * sh->q_heads * 4 : 0;
+}
+
+extern "C" int dial_b200_kv4_attention(const dial_b200_kv4_shape* sh, const void* q, int64_t q_ld,
+                                       const void* pages, float* weights,
+                                       const int32_t* block_table, int64_t sessions,
+                                       const int32_t* sids, const int32_t* lens,
+                                       const int32_t* q_starts, int64_t seqs, int64_t rows,
+                                       int64_t max_q, int64_t max_len, void* out, int64_t out_ld,
+                                       void* scratch, void* stream, char* err, size_t n) {
+  AttnArgs a{};
+  int rc = kv4_cache_of(sh, pages, weights, nullptr, block_table, sessions, &a.c, err, n);
+  if (rc != DIAL_OK) return rc;
+  if (!q || !sids || !lens || !out)
+    return kv4_fail(err, n, DIAL_ERR_INVALID, "null pointer argument");
+  if (seqs < 0 || seqs > 65535)
+    return kv4_fail(err, n, DIAL_ERR_INVALID, "seqs %lld outside [0, 65535]", (long long)seqs);
+  if (rows < 0 || rows > (1 << 26) || max_q < 0 || max_q > (1 << 24))
+    return kv4_fail(err, n, DIAL_ERR_INVALID, "rows %lld / max_q %lld out of range",
+                    (long long)rows, (long long)max_q);
+  if (!q_starts && rows != seqs)
+    return kv4_fail(err, n, DIAL_ERR_INVALID, "without q_starts rows %lld must equal seqs %lld",
+                    (long long)rows, (long long)seqs);
+  if (max_len < 0 || max_len > 16LL * sh->max_blocks)
+    return kv4_fail(err, n, DIAL_ERR_INVALID, "max_len %lld exceeds the block table's %lld slots",
+                    (long long)max_len, 16LL * sh->max_blocks);
+  if (!(sh->softmax_scale >= 0.f && sh->softmax_scale < 1e30f))
+    return kv4_fail(err, n, DIAL_ERR_INVALID, "softmax_scale %g out of range", sh->softmax_scale);
+  const int64_t width = 1LL * sh->q_heads * kHeadDim;
+  if (q_ld < width || out_ld < width || q_ld % 8 != 0 || out_ld % 8 != 0 ||
+      (reinterpret_cast<uintptr_t>(q) & 15) != 0 || (reinterpret_cast<uintptr_t>(out) & 15) != 0)
+    return kv4_fail(err, n, DIAL_ERR_INVALID,
+                    "q and out rows must hold q_heads heads and start on 16-byte boundaries");
+  if (seqs == 0 || rows == 0 || max_q == 0) return DIAL_OK;
+  if (dial_b200_kv4_attention_scratch_bytes(sh, seqs, rows, max_q, max_len, weights != nullptr) > 0 &&
+      (!scratch || (reinterpret_cast<uintptr_t>(scratch) & 15) != 0))
+    return kv4_fail(err, n, DIAL_ERR_INVALID, "scratch must be given, 16-byte aligned");
+  a.q = q;
+  a.sids = sids;
+  a.lens = lens;
+  a.q_starts = q_starts;
+  a.out = out;
+  a.lse = weights ? static_cast<float*>(scratch) : nullptr;
+  a.q_ld = q_ld;
+  a.out_ld = out_ld;
+  a.seqs = static_cast<int>(seqs);
+  a.rows = static_cast<int>(rows);
+  a.max_q = static_cast<int>(q_starts ? max_q : 1);
+  a.max_len = static_cast<int>(max_len);
+  a.scale = sh->softmax_scale > 0.f ? sh->softmax_scale : 1.f / sqrtf(static_cast<float>(kHeadDim));
+  if ((rc = kv4_ready(&a.c, err, n)) != DIAL_OK) return rc;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const cudaError_t e = sh->act == DIAL_ACT_BF16 ? launch<__nv_bfloat16>(a, s) : launch<__half>(a, s);
+  if (e != cudaSuccess)
+    return kv4_fail(err, n, DIAL_ERR_CUDA, "kv4 attention launch failed: %s", cudaGetErrorString(e));
+  return DIAL_OK;
+}

@@ -1,0 +1,97 @@
+// Device helpers of the 4-bit KV cache operators: the e2m1 / e4m3 codec and
+// the checked way from a session's slot to its slab.
+#pragma once
+
+#include "attn_dev.cuh"
+#include "common.cuh"
+#include "kv4.h"
+
+namespace dialb200 {
+
+// Page of slot `slot`, or -1 (with the status recorded) for a block id outside
+// the pool.  sid and slot / 16 are within the table.
+__device__ __forceinline__ int kv4_block(const Kv4Cache& c, const int32_t* table, int sid,
+                                         int page) {
+  const int b = table[static_cast<size_t>(sid) * c.max_blocks + page];
+  if (static_cast<unsigned>(b) >= static_cast<unsigned>(c.num_blocks)) {
+    set_status(c.status, kStatusBadArgs);
+    return -1;
+  }
+  return b;
+}
+
+__device__ __forceinline__ size_t kv4_slab_index(const Kv4Cache& c, int block, int head) {
+  return static_cast<size_t>(block) * c.kv_heads + head;
+}
+
+// e4m3 code nearest to a non-negative v, saturating at 448.
+__device__ __forceinline__ uint32_t e4m3_of(float v) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(0.f), "f"(v));
+  return r & 0xFFu;
+}
+
+__device__ __forceinline__ float e4m3_value(uint32_t code) {
+  const uint32_t h = e4m3x2_to_f16x2(static_cast<uint16_t>(code));
+  return __low2float(*reinterpret_cast<const __half2*>(&h));
+}
+
+// Two e2m1 codes, lo in the low nibble, nearest even, saturating at 6.
+__device__ __forceinline__ uint32_t e2m1x2_of(float lo, float hi) {
+  uint32_t r;
+  asm("{\n\t.reg .b8 b;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b, %1, %2;\n\t"
+      "cvt.u32.u8 %0, b;\n\t}"
+      : "=r"(r)
+      : "f"(hi), "f"(lo));
+  return r;
+}
+
+// Two e2m1 codes (one byte) to f16x2, exact.
+__device__ __forceinline__ uint32_t e2m1x2_to_f16x2(uint32_t byte) {
+  uint32_t r;
+  asm("{\n\t.reg .b8 b;\n\t"
+      "cvt.u8.u32 b, %1;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %0, b;\n\t}"
+      : "=r"(r)
+      : "r"(byte));
+  return r;
+}
+
+// Four values (dims 4 * lane ..) of a 128-dim row quantised by its warp: the
+// two code bytes, and the scale code of the lane's 16-dim group (4 lanes).
+__device__ __forceinline__ void kv4_encode(const float (&x)[4], float mult, uint32_t& codes,
+                                           uint32_t& scale) {
+  float v[4], amax = 0.f;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    v[e] = isnan(x[e]) ? 0.f : x[e];
+    amax = fmaxf(amax, fabsf(v[e]));
+  }
+  amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+  amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+  scale = e4m3_of(__fdiv_rn(__fdiv_rn(amax, 6.f), mult));
+  const float s = e4m3_value(scale) * mult;
+  codes = 0;
+  if (s > 0.f) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = __fdiv_rn(v[e], s);
+    codes = e2m1x2_of(v[0], v[1]) | e2m1x2_of(v[2], v[3]) << 8;
+  }
+}
+
+// The four values of the lane's dims (4 * lane ..) of token t of a slab's k
+// or v part; mult is the multiplier beside the e4m3 scales.
+__device__ __forceinline__ void kv4_decode(const uint8_t* slab, int codes_at, int scales_at, int t,
+                                           int lane, float mult, float (&v)[4]) {
+  const uint32_t c = *reinterpret_cast<const uint16_t*>(slab + codes_at + t * 64 + lane * 2);
+  const float s = e4m3_value(slab[scales_at + t * 8 + (lane >> 2)]) * mult;
+  const uint32_t a = e2m1x2_to_f16x2(c & 0xFFu), b = e2m1x2_to_f16x2(c >> 8);
+  const __half2 ha = *reinterpret_cast<const __half2*>(&a), hb = *reinterpret_cast<const __half2*>(&b);
+  v[0] = __low2float(ha) * s;
+  v[1] = __high2float(ha) * s;
+  v[2] = __low2float(hb) * s;
+  v[3] = __high2float(hb) * s;
+}
+
+}  // namespace dialb200

@@ -46,6 +46,22 @@ class AttnShape(C.Structure):
     ]
 
 
+class Kv4Shape(C.Structure):
+    _fields_ = [
+        ("q_heads", C.c_int32),
+        ("kv_heads", C.c_int32),
+        ("head_dim", C.c_int32),
+        ("max_blocks", C.c_int32),
+        ("num_blocks", C.c_int32),
+        ("max_pos", C.c_int32),
+        ("eps", C.c_float),
+        ("k_scale", C.c_float),
+        ("v_scale", C.c_float),
+        ("softmax_scale", C.c_float),
+        ("act", C.c_int32),
+    ]
+
+
 class GdnShape(C.Structure):
     _fields_ = [
         ("k_heads", C.c_int32),
@@ -112,6 +128,18 @@ _SIGS = {
     "dial_b200_stage_link_finish": (C.c_int, [_vp, _i64, _vp, _vp, *_err]),
     "dial_b200_gdn_forward": (C.c_int, [C.POINTER(GdnShape), _vp, _vp, _vp, _vp, _vp, _vp, _vp,
                                         _vp, _vp, _vp, _i64, _i64, _vp, _vp, _vp, *_err]),
+    "dial_b200_kv4_append": (C.c_int, [C.POINTER(Kv4Shape), _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp,
+                                       _vp, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _i64, _vp, *_err]),
+    "dial_b200_kv4_read": (C.c_int, [C.POINTER(Kv4Shape), _vp, _vp, _i64, _vp, _vp, _vp, _i64, _i64,
+                                     _vp, _vp, _vp, *_err]),
+    "dial_b200_kv4_attention_scratch_bytes": (_i64, [C.POINTER(Kv4Shape), _i64, _i64, _i64, _i64,
+                                                     _i32]),
+    "dial_b200_kv4_attention": (C.c_int, [C.POINTER(Kv4Shape), _vp, _i64, _vp, _vp, _vp, _i64, _vp,
+                                          _vp, _vp, _i64, _i64, _i64, _i64, _vp, _i64, _vp, _vp,
+                                          *_err]),
+    "dial_b200_kv4_evict_scratch_bytes": (_i64, [C.POINTER(Kv4Shape), _i64, _i64, _i64]),
+    "dial_b200_kv4_evict": (C.c_int, [C.POINTER(Kv4Shape), _vp, _vp, _vp, _vp, _vp, _i64, _vp, _vp,
+                                      _vp, _i64, _i64, _i64, _i64, _vp, _vp, *_err]),
     "dial_b200_engine_create": (C.c_int, [C.POINTER(ModelConfig), C.c_int, C.POINTER(_vp), *_err]),
     "dial_b200_engine_destroy": (None, [_vp]),
     "dial_b200_engine_load_synthetic": (C.c_int, [_vp, _u64, _vp, *_err]),

@@ -59,7 +59,8 @@ uint32_t dial_b200_abi_version(void);
  * out-of-range index a kernel saw since the last clear: the word shared by
  * the engines and the scratch-taking ops, else the word of
  * dial_b200_attention_decode_noalloc (clearing also resets that entry
- * point's split counters).  Synchronizes; allocates nothing. */
+ * point's split counters), else the word of the dial_b200_kv4 ops.
+ * Synchronizes; allocates nothing. */
 int dial_b200_device_status(int* status_out, int clear, char* err, size_t err_size);
 
 /* ------------------------------------------------------------------------ */
@@ -175,6 +176,126 @@ int dial_b200_attention_decode_noalloc(const dial_b200_attn_shape* sh, const voi
                                        const int32_t* sids, const int32_t* positions, void* out,
                                        int64_t out_ld, int64_t rows, int32_t splits, void* stream,
                                        char* err, size_t err_size);
+
+/* ------------------------------------------------------------------------ */
+/* 4-bit KV cache: append, read back, attention, eviction                    */
+/* ------------------------------------------------------------------------ */
+
+/* A KV cache in the NVFP4 form of the linears: e2m1 codes, two a byte, with an
+ * e4m3 scale for every 16 dims, 144 bytes a token and kv head (k and v)
+ * against 512 in the activation dtype.  No counterpart in the reference, whose
+ * cache holds the activation dtype (llama3/cache.rs:9-237).
+ *
+ * pages: uint8 [num_blocks][kv_heads][DIAL_B200_KV4_SLAB_BYTES]; a slab holds
+ * 16 tokens of one kv head: k codes [16][64] | v codes [16][64] | k scales
+ * [16][8] | v scales [16][8]; byte j of a code row holds dims 2j (low nibble)
+ * and 2j + 1.  A code c of a group with scale s stands for e2m1(c) * e4m3(s) *
+ * k_scale (v_scale).  Beside the pages, both optional: weights, f32
+ * [num_blocks][kv_heads][16], each slot's attention weight summed over the
+ * steps so far, and positions, int32 of the same shape, the position of the
+ * token in the slot (kv heads differ in both after an eviction).
+ * block_table: int32 [sessions][max_blocks]; slot i of a session is token i %
+ * 16 of page block_table[sid][i / 16].
+ *
+ * Device-side checks: a session id outside [0, sessions), a slot outside the
+ * table, a position outside the tables or a length outside [0, max_len]
+ * records the bad-argument device status, and that row or sequence is left
+ * out, its outputs as they were; a block id outside [0, num_blocks) records it
+ * too, and reads use page 0, writes are dropped. */
+#define DIAL_B200_KV4_SLAB_BYTES 2304
+
+typedef struct {
+  int32_t q_heads;
+  int32_t kv_heads;   /* q_heads is a multiple, at most 16 times as many */
+  int32_t head_dim;   /* must be 128 */
+  int32_t max_blocks; /* block-table row length (16-token pages per session) */
+  int32_t num_blocks; /* pages in the pool */
+  int32_t max_pos;    /* rows of the cos/sin tables (append with RoPE only) */
+  float eps;          /* q/k RMSNorm epsilon (append with norms only) */
+  float k_scale;      /* multipliers beside the e4m3 scales, positive: */
+  float v_scale;      /* amax / 6 / multiplier should fall in [2^-6, 448] */
+  float softmax_scale; /* 0: 1 / sqrt(head_dim) */
+  int32_t act;        /* DIAL_ACT_BF16 or DIAL_ACT_F16 */
+} dial_b200_kv4_shape;
+
+/* Rows of new tokens into their slots, the counterpart of the append half of
+ * dial_b200_attention_decode (text.rs:1466-1536, cache.rs:169-237):
+ *   qkv [rows, qkv_ld]: q | k | v, of which row m goes to slot slots[m] of
+ *   session sids[m]; slots[m] < 0 marks a padding row, which is skipped;
+ *   q_norm_w / k_norm_w [128]: per-head RMSNorm of q and k, both or neither
+ *   NULL; cos / sin [max_pos][64]: RoPE at positions[m], both or neither NULL
+ *   (each step rounded to the activation dtype, as in the decode op);
+ *   q_out [rows, q_out_ld] receives q after norm and RoPE (NULL: not wanted).
+ * k (after norm and RoPE) and v are quantised: s = e4m3(min(amax / 6 / scale,
+ * 448)) for each 16 dims, codes e2m1(x / (s * scale)), both to nearest even; NaN
+ * becomes 0, infinities the largest value.  weights (if not NULL) of the slot
+ * become 0, positions (if not NULL) positions[m].  Rows must name distinct
+ * slots.  `positions` may be NULL without RoPE and without a positions pool. */
+int dial_b200_kv4_append(const dial_b200_kv4_shape* sh, const void* qkv, int64_t qkv_ld,
+                         const void* q_norm_w, const void* k_norm_w, const void* cos,
+                         const void* sin, void* pages, float* weights, int32_t* positions_pool,
+                         const int32_t* block_table, int64_t sessions, const int32_t* sids,
+                         const int32_t* slots, const int32_t* positions, void* q_out,
+                         int64_t q_out_ld, int64_t rows, void* stream, char* err,
+                         size_t err_size);
+
+/* Slots back as the values they stand for: slot first[i] + j (first NULL: j)
+ * of session sids[i], j < count, into k_out / v_out [seqs][count][kv_heads]
+ * [128] in the activation dtype; slots at or past lens[i] (or below 0) become
+ * zeros.  For handing a session to a cache of the activation dtype. */
+int dial_b200_kv4_read(const dial_b200_kv4_shape* sh, const void* pages,
+                       const int32_t* block_table, int64_t sessions, const int32_t* sids,
+                       const int32_t* first, const int32_t* lens, int64_t seqs, int64_t count,
+                       void* k_out, void* v_out, void* stream, char* err, size_t err_size);
+
+/* Scratch of dial_b200_kv4_attention for calls of at most these sizes. */
+int64_t dial_b200_kv4_attention_scratch_bytes(const dial_b200_kv4_shape* sh, int64_t seqs,
+                                              int64_t rows, int64_t max_q, int64_t max_len,
+                                              int32_t with_weights);
+
+/* Attention over the cached slots, causal at the end of each sequence: the
+ * queries of sequence i are rows q_starts[i] .. q_starts[i + 1] - 1 of q [rows,
+ * q_ld] (q_starts NULL: row i), n of them, and query j sees slots 0 ..
+ * lens[i] - n + j of session sids[i]; a query that sees none gives zeros.
+ *   out [rows, out_ld] = softmax(softmax_scale * q . k) . v, f32 inside;
+ *   weights (if not NULL): weights[slot] += the slot's probabilities summed
+ *   over the sequence's queries and the query heads of the kv head.  Sequences
+ *   must then name distinct sessions.
+ * max_q and max_len bound n and lens[i] (host); rows no sequence names are left as
+ * they were.  `scratch` needs no preparation; two calls that may run at the
+ * same time need two. */
+int dial_b200_kv4_attention(const dial_b200_kv4_shape* sh, const void* q, int64_t q_ld,
+                            const void* pages, float* weights, const int32_t* block_table,
+                            int64_t sessions, const int32_t* sids, const int32_t* lens,
+                            const int32_t* q_starts, int64_t seqs, int64_t rows, int64_t max_q,
+                            int64_t max_len, void* out, int64_t out_ld, void* scratch,
+                            void* stream, char* err, size_t err_size);
+
+/* Scratch of dial_b200_kv4_evict for calls of at most these sizes. */
+int64_t dial_b200_kv4_evict_scratch_bytes(const dial_b200_kv4_shape* sh, int64_t seqs,
+                                          int64_t max_len, int64_t keep);
+
+/* Each sequence cut to its `keep` most attended entries, for every kv head on
+ * its own: among slots 0 .. lens[i] - 1 the entries whose position is above
+ * (newest position - recent) come first, then all by weight (NaN last), the lowest
+ * slot first among equals.  The kept entries below slot `keep` stay where they
+ * are; those at or above it move, in order, into the slots that the others
+ * leave, so that slots 0 .. lens_out[i] - 1 hold the kept ones, lens_out[i] =
+ * min(lens[i], keep).  Codes, scales, weights and positions move together.
+ * Attention does not depend on the order of slots: keys hold their RoPE.
+ *   dst_table [sessions][max_blocks]: where slots 0 .. keep - 1 go to, either
+ *   block_table itself (or NULL), which moves as little as possible, or other
+ *   pages, which leaves the source as it was (pages shared with another
+ *   session).  A page may be both source and destination only at the same
+ *   place of the same session.  Slots from lens_out[i] on are left as they were.
+ *   positions may be NULL with recent == 0; recent <= keep.  lens_out may be lens.
+ * Sequences must name distinct sessions. */
+int dial_b200_kv4_evict(const dial_b200_kv4_shape* sh, void* pages, float* weights,
+                        int32_t* positions, const int32_t* block_table,
+                        const int32_t* dst_table, int64_t sessions, const int32_t* sids,
+                        const int32_t* lens, int32_t* lens_out, int64_t seqs, int64_t max_len,
+                        int64_t keep, int64_t recent, void* scratch, void* stream, char* err,
+                        size_t err_size);
 
 /* ------------------------------------------------------------------------ */
 /* Gated-DeltaNet token mixer (Qwen3.8 hybrid linear-attention layers)      */

@@ -1,0 +1,346 @@
+"""The 4-bit KV cache operators against a plain 64-bit reference (kv4_case.py):
+codes, scales, read-back values and evictions equal it; attention is within the
+bound that the reference derives from the roundings."""
+
+import numpy as np
+import pytest
+import torch
+
+from kv4_case import DIM, PAGE, Cache, act_round, decode, encode, i32, norm_rope, same_slabs
+
+pytestmark = pytest.mark.gpu
+BF16, F16 = torch.bfloat16, torch.float16
+
+
+@pytest.fixture(autouse=True)
+def clear_status(cuda):
+    import dial_b200
+
+    dial_b200.device_status(clear=True)
+
+
+def host(t):
+    return t.double().cpu().numpy() if t.is_floating_point() else t.cpu().numpy()
+
+
+def check_attention(c, cuda, seqs, max_q=None, max_len=None, weights=True, q_scale=1.5, spare_rows=0,
+                    stride=0, dev=None, scratch=None):
+    """Run kv4_attention for seqs = [(sid, len, queries)] and compare out and
+    the running weights with the reference; returns the device cache."""
+    from dial_b200 import kv4
+
+    counts = [n for _, _, n in seqs]
+    rows = sum(counts) + spare_rows
+    q = act_round(c.rng.standard_normal((rows, c.QH * DIM)) * q_scale, c.dt)
+    cache, table = dev if dev else c.device(cuda)
+    qd = torch.zeros(rows, c.QH * DIM + stride, dtype=c.dt, device=cuda)
+    qd[:, :c.QH * DIM] = torch.from_numpy(q).to(cuda)
+    out = torch.full((rows, c.QH * DIM + stride), 7.0, dtype=c.dt, device=cuda)
+    starts = None if counts == [1] * len(counts) and not spare_rows else i32(
+        cuda, *([0] + np.cumsum(counts).tolist()))
+    before = host(cache.weights)
+    kv4.kv4_attention(c.sh, cache, qd[:, :c.QH * DIM], table, i32(cuda, *[s for s, _, _ in seqs]),
+                      i32(cuda, *[n for _, n, _ in seqs]),
+                      max(n for _, n, _ in seqs) if max_len is None else max_len, q_starts=starts,
+                      max_q=max(counts) if max_q is None else max_q, accumulate=weights,
+                      out=out[:, :c.QH * DIM], scratch=scratch)
+    torch.cuda.synchronize()
+    got, want, bound = host(out), np.full((rows, c.QH * DIM), 7.0), np.zeros((rows, c.QH * DIM))
+    w_want, w_bound = before.copy(), np.zeros_like(before)
+    at = 0
+    for sid, n, m in seqs:
+        o, b, s, sb = c.attend(q[at:at + m], sid, n)
+        want[at:at + m], bound[at:at + m] = o, b
+        blk, off = c.at(sid, n)
+        w_want[blk, :, off] += s
+        w_bound[blk, :, off] += sb
+        at += m
+    if stride:
+        assert (got[:, c.QH * DIM:] == 7.0).all()
+    d = np.abs(got[:, :c.QH * DIM] - want)
+    assert (d <= bound).all(), f"out off by {np.max(d / np.maximum(bound, 1e-30))} bounds"
+    w = host(cache.weights)
+    if weights:
+        d = np.abs(w - w_want)
+        w_bound = w_bound + 2.0 ** -23 * (np.abs(w_want) + np.abs(before)) * (w_bound > 0)
+        assert (d <= w_bound).all(), f"weights off by {np.max(d / np.maximum(w_bound, 1e-30))} bounds"
+    else:
+        np.testing.assert_array_equal(w, before)
+    c.weights = w.astype(np.float32)
+    return cache, table
+
+
+# ----------------------------------------------------------- append and read
+@pytest.mark.parametrize("dt", [BF16, F16])
+@pytest.mark.parametrize("norm", [True, False])
+@pytest.mark.parametrize("heads", [(32, 8), (5, 1), (3, 3)])
+def test_append_equals_the_reference(cuda, dt, norm, heads):
+    from dial_b200 import kv4
+
+    c = Cache(3, 4, 80, *heads, dt=dt, fill=False, max_pos=500)
+    cache, table = c.device(cuda)
+    rows = 41
+    sids = np.array([0] * 20 + [2] * 20 + [3], np.int32)
+    slots = np.array(list(range(13, 33)) + list(range(20)) + [79], np.int32)
+    slots[7] = -1  # a padding row
+    pos = (slots + 300).astype(np.int32)
+    x = act_round(c.rng.standard_normal((rows, (c.QH + 2 * c.H) * DIM)), dt)
+    x[3] = 0
+    x[4] *= 2.0 ** -13  # scales below e4m3's smallest
+    x[5, ::7] *= 64
+    x = act_round(x, dt)
+    w = [act_round(1 + 0.2 * c.rng.standard_normal(DIM), dt) for _ in range(2)]
+    ang = pos[:, None] * 1e6 ** (-np.arange(64) / 64)
+    t = lambda a: torch.from_numpy(np.ascontiguousarray(a)).to(cuda).to(dt)  # noqa: E731
+    tab = np.arange(500)[:, None] * 1e6 ** (-np.arange(64) / 64)
+    kw = dict(q_norm_w=t(w[0]), k_norm_w=t(w[1]), cos=t(np.cos(tab)), sin=t(np.sin(tab))) if norm else {}
+    q = kv4.kv4_append(c.sh, cache, t(x), table, *(torch.from_numpy(a).to(cuda)
+                                                   for a in (sids, slots, pos)), **kw)
+    hd = x.reshape(rows, -1, DIM)
+    cs = (act_round(np.cos(ang), dt), act_round(np.sin(ang), dt)) if norm else (None, None)
+    eps = float(np.float32(1e-6))
+    qr = norm_rope(hd[:, :c.QH], w[0] if norm else None, *cs, eps, dt)
+    kr = norm_rope(hd[:, c.QH:c.QH + c.H], w[1] if norm else None, *cs, eps, dt)
+    for m in range(rows):
+        if slots[m] >= 0:
+            c.put(sids[m], slots[m], kr[m], hd[m, c.QH + c.H:], pos[m])
+            np.testing.assert_array_equal(host(q[m]), qr[m].reshape(-1))
+    same_slabs(host(cache.pages), c.pages)
+    np.testing.assert_array_equal(host(cache.weights), c.weights)
+    np.testing.assert_array_equal(host(cache.positions), c.positions)
+    # read back: the values themselves, and zeros past the length
+    k, v = kv4.kv4_read(c.sh, cache, table, i32(cuda, 2, 0), i32(cuda, 20, 30), 27,
+                        first=i32(cuda, 0, 5))
+    for i, (sid, n, at) in enumerate(((2, 20, 0), (0, 30, 5))):
+        kk, vv = c.values(sid, n)
+        for got, want in ((k, kk), (v, vv)):
+            want = act_round(want[at:at + 27], dt)
+            np.testing.assert_array_equal(host(got[i])[:n - at], want)
+            assert (host(got[i])[n - at:] == 0).all()
+
+
+def test_append_of_nan_and_infinity(cuda):
+    from dial_b200 import kv4
+
+    c = Cache(5, 1, 16, 4, 2, fill=False)
+    cache, table = c.device(cuda)
+    x = act_round(c.rng.standard_normal((3, 8 * DIM)), BF16)
+    x[0, 4 * DIM:5 * DIM:9] = np.nan
+    x[0, 6 * DIM + 3] = np.inf
+    x[1, 7 * DIM + 20] = -np.inf
+    x[2, 4 * DIM:] = np.nan
+    z = i32(cuda, 0, 0, 0)
+    kv4.kv4_append(c.sh, cache, torch.from_numpy(x).to(cuda).to(BF16), table, z, i32(cuda, 0, 1, 2),
+                   positions=z, want_q=False)
+    for m in range(3):
+        h = x[m].reshape(-1, DIM)
+        c.put(0, m, h[4:6], h[6:], 0)
+    same_slabs(host(cache.pages), c.pages)
+    k, v = kv4.kv4_read(c.sh, cache, table, i32(cuda, 0), i32(cuda, 3), 3)
+    assert np.isfinite(host(k)).all() and np.isfinite(host(v)).all()
+    assert host(v)[0, 0, 0, 3] == 6 * 448 * c.v_scale and host(v)[0, 1, 1, 20] == -6 * 448 * c.v_scale
+    assert (host(k)[0, 2] == 0).all() and (host(v)[0, 2] == 0).all()
+
+
+def test_read_of_every_code_and_scale(cuda):
+    from dial_b200 import kv4
+
+    c = Cache(6, 1, 256 * 16, 2, 1, k_scale=1.0, v_scale=0.25, dt=F16)
+    codes = np.tile(np.arange(16, dtype=np.uint8), 8)
+    sc = np.array([s for s in range(127)], np.uint8)
+    from kv4_case import pack
+    for b in range(c.max_blocks):
+        s = np.full((1, PAGE, 8), sc[b % 127], np.uint8)
+        cc = np.broadcast_to(codes, (1, PAGE, DIM)).copy()
+        c.pages[c.table[0, b]] = pack(cc, s, cc, s)
+    cache, table = c.device(cuda)
+    n = 256 * 16
+    k, v = kv4.kv4_read(c.sh, cache, table, i32(cuda, 0), i32(cuda, n), n)
+    kk, vv = c.values(0, n)
+    np.testing.assert_array_equal(host(k)[0], act_round(kk, F16))
+    np.testing.assert_array_equal(host(v)[0], act_round(vv, F16))
+
+
+# ------------------------------------------------------------------ attention
+HEADS = [(32, 8), (4, 4), (4, 2), (6, 2), (10, 2), (16, 2), (16, 1)]
+
+
+@pytest.mark.parametrize("heads", HEADS)
+@pytest.mark.parametrize("dt", [BF16, F16])
+def test_attention_single_tokens(cuda, heads, dt):
+    c = Cache(11, 9, 700, *heads, dt=dt)
+    lens = [1, 2, 15, 16, 17, 255, 256, 700, 0]
+    check_attention(c, cuda, [(8 - i, n, 1) for i, n in enumerate(lens)])
+    check_attention(c, cuda, [(3, 33, 1)], weights=False)
+
+
+@pytest.mark.parametrize("heads", [(32, 8), (3, 3), (10, 2), (16, 1)])
+@pytest.mark.parametrize("weights", [False, True])
+def test_attention_few_queries(cuda, heads, weights):
+    c = Cache(12, 8, 300, *heads, dt=F16 if heads[0] == 32 else BF16)
+    check_attention(c, cuda, [(0, 300, 5), (1, 5, 5), (2, 3, 5), (4, 1, 1), (3, 17, 2), (6, 0, 3),
+                              (5, 64, 0), (7, 129, 8)], weights=weights, spare_rows=3)
+
+
+@pytest.mark.parametrize("queries,lens", [(16, (16, 40)), (33, (33, 90)), (64, (64, 257)),
+                                          (129, (129, 400)), (200, (150, 200))])
+@pytest.mark.parametrize("heads", [(8, 2), (5, 1), (2, 2)])
+def test_attention_prompts(cuda, queries, lens, heads):
+    c = Cache(13, 4, 416, *heads)
+    check_attention(c, cuda, [(2, lens[1], queries), (0, lens[0], queries), (3, 7, 3)],
+                    spare_rows=1, stride=64)
+
+
+def test_attention_long_split(cuda):
+    """One session long enough for every split, at an odd length; the largest
+    score in the first and in the last slot."""
+    for seed in (14, 15):
+        c = Cache(seed, 2, 20011, 8, 2, dt=F16)
+        check_attention(c, cuda, [(1, 20011, 1)])
+        check_attention(c, cuda, [(0, 9001, 1), (1, 3, 1)], max_len=20011)
+
+
+def test_attention_of_dominant_and_equal_scores(cuda):
+    """Queries large enough that one slot takes all the weight, and zero
+    queries, where every slot has the same."""
+    c = Cache(16, 2, 1000, 8, 2)
+    check_attention(c, cuda, [(0, 1000, 1), (1, 517, 1)], q_scale=40.0)
+    check_attention(c, cuda, [(0, 1000, 1), (1, 517, 1)], q_scale=0.0)
+    check_attention(c, cuda, [(0, 1000, 70), (1, 517, 40)], q_scale=30.0)
+
+
+def test_attention_scale_of_the_shape(cuda):
+    from dial_b200 import kv4
+
+    c = Cache(17, 1, 64, 4, 2)
+    sh = kv4.make_shape(4, 2, c.max_blocks, c.pages.shape[0], k_scale=c.k_scale, v_scale=c.v_scale,
+                        softmax_scale=0.03)
+    cache, table = c.device(cuda)
+    q = act_round(c.rng.standard_normal((1, 4 * DIM)), BF16)
+    got = kv4.kv4_attention(sh, cache, torch.from_numpy(q).to(cuda).to(BF16), table, i32(cuda, 0),
+                            i32(cuda, 61), 64)
+    o, b, _, _ = c.attend(q, 0, 61, float(np.float32(0.03)))
+    assert (np.abs(host(got) - o) <= b).all()
+
+
+# ------------------------------------------------------------------- eviction
+@pytest.mark.parametrize("n,keep,recent", [(1, 1, 0), (17, 16, 3), (100, 1, 1), (100, 99, 99),
+                                           (1023, 512, 64), (1025, 1000, 0), (5000, 1777, 300),
+                                           (40, 60, 10), (33, 0, 0), (0, 5, 5)])
+@pytest.mark.parametrize("out_of_place", [False, True])
+def test_evict_equals_the_reference(cuda, n, keep, recent, out_of_place):
+    from dial_b200 import kv4
+
+    cap = max(n, keep, 16)
+    c = Cache(21, 5, cap, 4, 2)
+    for s in range(5):  # positions that rise along the slots, other in each head
+        b, o = c.at(s, cap)
+        for h in range(2):
+            c.positions[b, h, o] = np.cumsum(c.rng.integers(1, 3, cap))
+    seqs = [(3, n), (1, max(0, n - 5)), (4, n // 2)]
+    dst = c.table.copy()
+    if out_of_place:
+        dst[:] = -1
+        kb = -(-keep // PAGE) if keep else 0
+        extra = 3 * kb
+        c.pages = np.concatenate([c.pages, c.pages[:1].repeat(extra, 0)])
+        c.weights = np.concatenate([c.weights, c.weights[:1].repeat(extra, 0)])
+        c.positions = np.concatenate([c.positions, c.positions[:1].repeat(extra, 0)])
+        first = c.sh.num_blocks
+        for i, (s, _) in enumerate(seqs):
+            dst[s, :kb] = np.arange(first + i * kb, first + (i + 1) * kb)[:c.max_blocks]
+        c.sh.num_blocks = first + extra
+    cache, table = c.device(cuda)
+    lens = i32(cuda, *[m for _, m in seqs])
+    new = kv4.kv4_evict(c.sh, cache, table, i32(cuda, *[s for s, _ in seqs]), lens, cap, keep, recent,
+                        dst_table=torch.from_numpy(dst).to(cuda) if out_of_place else None,
+                        lens_out=lens if not out_of_place else None)
+    want = [c.evict(s, m, keep, recent, dst) for s, m in seqs]
+    assert host(new).tolist() == want
+    np.testing.assert_array_equal(host(cache.pages), c.pages)
+    np.testing.assert_array_equal(host(cache.weights), c.weights)
+    np.testing.assert_array_equal(host(cache.positions), c.positions)
+
+
+@pytest.mark.parametrize("kind", ["equal", "ties", "special", "protected"])
+def test_evict_of_ties_and_special_weights(cuda, kind):
+    from dial_b200 import kv4
+
+    c = Cache(22, 1, 3000, 2, 2)
+    b, o = c.at(0, 3000)
+    c.positions[b, :, o] = np.arange(3000)[:, None]
+    if kind == "equal":
+        c.weights[:] = 0.25
+    elif kind == "ties":
+        c.weights = np.round(c.weights).astype(np.float32)
+    elif kind == "special":
+        pick = c.rng.integers(0, 7, c.weights.shape)
+        c.weights = np.array([np.nan, np.inf, -np.inf, 0.0, -0.0, -1.5, 1e-42],
+                             np.float32)[pick]
+    else:  # more entries protected than kept: positions all alike
+        c.positions[:] = 5
+    cache, table = c.device(cuda)
+    new = kv4.kv4_evict(c.sh, cache, table, i32(cuda, 0), i32(cuda, 3000), 3000, 1300, 200)
+    assert host(new).tolist() == [c.evict(0, 3000, 1300, 200)]
+    np.testing.assert_array_equal(host(cache.pages), c.pages)
+    np.testing.assert_array_equal(host(cache.weights), c.weights)
+    np.testing.assert_array_equal(host(cache.positions), c.positions)
+
+
+# ---------------------------------------------------------- a session's life
+def test_a_run_of_steps_with_eviction(cuda):
+    """Prompt, decode steps with running weights, eviction at the capacity, and
+    decoding on in the freed slots, three sessions at once, each step against
+    the reference."""
+    from dial_b200 import kv4
+
+    c = Cache(31, 3, 96, 8, 2, max_pos=400)
+    cache, table = c.device(cuda)
+    tab = np.arange(400)[:, None] * 1e6 ** (-np.arange(64) / 64)
+    cos, sin = (act_round(f(tab), BF16) for f in (np.cos, np.sin))
+    w = act_round(1 + 0.1 * c.rng.standard_normal(DIM), BF16)
+    t = lambda a: torch.from_numpy(np.ascontiguousarray(a)).to(cuda).to(BF16)  # noqa: E731
+    kw = dict(q_norm_w=t(w), k_norm_w=t(w), cos=t(cos), sin=t(sin))
+    lens, seen = np.array([0, 0, 0]), np.array([0, 0, 0])
+    steps = [np.array([90, 40, 7])] + [np.array([1, 1, 1])] * 9
+    for step, counts in enumerate(steps):
+        sids, slots, pos = [], [], []
+        for s in range(3):
+            sids += [s] * counts[s]
+            slots += range(lens[s], lens[s] + counts[s])
+            pos += range(seen[s], seen[s] + counts[s])
+        lens, seen = lens + counts, seen + counts
+        rows = len(sids)
+        x = act_round(c.rng.standard_normal((rows, 12 * DIM)), BF16)
+        q = kv4.kv4_append(c.sh, cache, t(x), table, i32(cuda, *sids), i32(cuda, *slots),
+                           i32(cuda, *pos), **kw)
+        hd = x.reshape(rows, -1, DIM)
+        eps = float(np.float32(1e-6))
+        qr = norm_rope(hd[:, :8], w, cos[pos], sin[pos], eps, BF16)
+        kr = norm_rope(hd[:, 8:10], w, cos[pos], sin[pos], eps, BF16)
+        np.testing.assert_array_equal(host(q), qr.reshape(rows, -1))
+        for m in range(rows):
+            c.put(sids[m], slots[m], kr[m], hd[m, 10:], pos[m])
+        same_slabs(host(cache.pages), c.pages)
+        starts = i32(cuda, 0, *np.cumsum(counts).tolist())
+        out = kv4.kv4_attention(c.sh, cache, q, table, i32(cuda, 0, 1, 2), i32(cuda, *lens.tolist()),
+                                96, q_starts=starts, max_q=int(counts.max()), accumulate=True)
+        at, before = 0, c.weights.astype(np.float64)
+        for s in range(3):
+            o, b, ws, wb = c.attend(qr.reshape(rows, -1)[at:at + counts[s]], s, lens[s])
+            assert (np.abs(host(out[at:at + counts[s]]) - o) <= b).all()
+            blk, off = c.at(s, lens[s])
+            got = host(cache.weights)[blk, :, off]
+            assert (np.abs(got - before[blk, :, off] - ws) <= wb + 2.0 ** -22 * (got + 1e-30)).all()
+            at += counts[s]
+        c.weights = host(cache.weights).astype(np.float32)
+        if step in (3, 6):
+            full = [s for s in range(3) if lens[s] > 60]
+            new = kv4.kv4_evict(c.sh, cache, table, i32(cuda, *full),
+                                i32(cuda, *lens[full].tolist()), 96, 60, 20)
+            for i, s in enumerate(full):
+                assert int(new[i]) == c.evict(s, int(lens[s]), 60, 20)
+                lens[s] = 60
+            same_slabs(host(cache.pages), c.pages)
+            np.testing.assert_array_equal(host(cache.weights), c.weights)
+            np.testing.assert_array_equal(host(cache.positions), c.positions)
