@@ -14,45 +14,14 @@
 namespace dialb200 {
 namespace {
 
-struct AttnArgs {
-  Kv4Cache c;
-  const void* q;
-  const int32_t* sids;
-  const int32_t* lens;
-  const int32_t* q_starts;
-  void* out;
-  float* lse;  // [rows][q_heads], with weights
-  long long q_ld, out_ld;
-  int seqs, rows, max_q, max_len;
-  float scale;
-};
-
-struct Seq {
-  int sid, len, row0, n;
-};
-
-// The sequence's rows and slots; false (with the status recorded) for one
-// whose session, rows or length are out of range.
-__device__ __forceinline__ bool seq_of(const AttnArgs& a, int i, Seq& s) {
-  s.sid = a.sids[i];
-  s.len = a.lens[i];
-  s.row0 = a.q_starts ? a.q_starts[i] : i;
-  const int end = a.q_starts ? a.q_starts[i + 1] : i + 1;
-  if (static_cast<unsigned>(s.sid) >= static_cast<unsigned>(a.c.sessions) || s.len < 0 ||
-      s.len > a.max_len || s.row0 < 0 || end < s.row0 || end > a.rows || end - s.row0 > a.max_q) {
-    set_status(a.c.status, kStatusBadArgs);
-    return false;
-  }
-  s.n = end - s.row0;
-  return true;
-}
+constexpr int kFewCols = 64;
 
 template <typename Act>
-__global__ void __launch_bounds__(256) kv4_attn_kernel(const AttnArgs a) {
+__global__ void __launch_bounds__(256) kv4_attn_kernel(const Kv4AttnArgs a) {
   __shared__ float part[8][kHeadDim + 2];
   const int j = blockIdx.x, h = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  Seq s;
-  if (!seq_of(a, blockIdx.z, s) || j >= s.n) return;
+  Kv4Seq s;
+  if (!kv4_seq(a, blockIdx.z, s) || j >= s.n) return;
   const int seen = max(0, s.len - s.n + 1 + j), kvh = h / (a.c.q_heads / a.c.kv_heads);
   const int row = s.row0 + j;
   float q[4], o[4] = {0.f, 0.f, 0.f, 0.f}, m = -INFINITY, l = 0.f;
@@ -89,17 +58,17 @@ __global__ void __launch_bounds__(256) kv4_attn_kernel(const AttnArgs a) {
     }
     static_cast<Act*>(a.out)[row * a.out_ld + h * kHeadDim + threadIdx.x] =
         ActTraits<Act>::from_f(seen > 0 ? O / L : 0.f);
-    if (a.lse && threadIdx.x == 0)
-      a.lse[static_cast<size_t>(row) * a.c.q_heads + h] = M + logf(L);
+    if (a.c.weights && threadIdx.x == 0)
+      static_cast<float*>(a.scratch)[static_cast<size_t>(row) * a.c.q_heads + h] = M + logf(L);
   }
 }
 
 template <typename Act>
-__global__ void __launch_bounds__(256) kv4_weights_kernel(const AttnArgs a) {
+__global__ void __launch_bounds__(256) kv4_weights_kernel(const Kv4AttnArgs a) {
   const int t = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   const int kvh = blockIdx.y, rep = a.c.q_heads / a.c.kv_heads;
-  Seq s;
-  if (!seq_of(a, blockIdx.z, s) || t >= s.len) return;
+  Kv4Seq s;
+  if (!kv4_seq(a, blockIdx.z, s) || t >= s.len) return;
   const int block = kv4_block(a.c, a.c.block_table, s.sid, t / kPageTokens);
   const size_t si = kv4_slab_index(a.c, max(block, 0), kvh);
   float k[4], sum = 0.f;
@@ -112,13 +81,13 @@ __global__ void __launch_bounds__(256) kv4_weights_kernel(const AttnArgs a) {
       load4(static_cast<const Act*>(a.q) + row * a.q_ld + h * kHeadDim + lane * 4, q);
       const float sc =
           warp_sum(fmaf(q[0], k[0], q[1] * k[1]) + fmaf(q[2], k[2], q[3] * k[3])) * a.scale;
-      sum += expf(sc - a.lse[row * a.c.q_heads + h]);
+      sum += expf(sc - static_cast<const float*>(a.scratch)[row * a.c.q_heads + h]);
     }
   if (lane == 0 && block >= 0) a.c.weights[si * kPageTokens + t % kPageTokens] += sum;
 }
 
 template <typename Act>
-cudaError_t launch(const AttnArgs& a, cudaStream_t s) {
+cudaError_t launch(const Kv4AttnArgs& a, cudaStream_t s) {
   kv4_attn_kernel<Act><<<dim3(a.max_q, a.c.q_heads, a.seqs), 256, 0, s>>>(a);
   cudaError_t e = cudaGetLastError();
   if (e == cudaSuccess && a.c.weights) {
@@ -136,9 +105,12 @@ using namespace dialb200;
 extern "C" int64_t dial_b200_kv4_attention_scratch_bytes(const dial_b200_kv4_shape* sh,
                                                          int64_t seqs, int64_t rows, int64_t max_q,
                                                          int64_t max_len, int32_t with_weights) {
-  if (!sh || sh->q_heads < 1 || sh->kv_heads < 1 || seqs < 0 || rows < 0 || max_q < 0 ||
+  if (!sh || sh->q_heads < 1 || sh->kv_heads < 1 || sh->q_heads % sh->kv_heads != 0 || seqs < 0 || rows < 0 || max_q < 0 ||
       max_len < 0)
     return -1;
+  if (max_q * (sh->q_heads / sh->kv_heads) <= kFewCols)
+    return static_cast<int64_t>(kv4_decode_scratch(sh->q_heads, sh->kv_heads, seqs, max_q, max_len,
+                                                   with_weights != 0));
   return with_weights ? rows * sh->q_heads * 4 : 0;
 }
 
@@ -149,7 +121,7 @@ extern "C" int dial_b200_kv4_attention(const dial_b200_kv4_shape* sh, const void
                                        const int32_t* q_starts, int64_t seqs, int64_t rows,
                                        int64_t max_q, int64_t max_len, void* out, int64_t out_ld,
                                        void* scratch, void* stream, char* err, size_t n) {
-  AttnArgs a{};
+  Kv4AttnArgs a{};
   int rc = kv4_cache_of(sh, pages, weights, nullptr, block_table, sessions, &a.c, err, n);
   if (rc != DIAL_OK) return rc;
   if (!q || !sids || !lens || !out)
@@ -181,7 +153,7 @@ extern "C" int dial_b200_kv4_attention(const dial_b200_kv4_shape* sh, const void
   a.lens = lens;
   a.q_starts = q_starts;
   a.out = out;
-  a.lse = weights ? static_cast<float*>(scratch) : nullptr;
+  a.scratch = scratch;
   a.q_ld = q_ld;
   a.out_ld = out_ld;
   a.seqs = static_cast<int>(seqs);
@@ -191,7 +163,9 @@ extern "C" int dial_b200_kv4_attention(const dial_b200_kv4_shape* sh, const void
   a.scale = sh->softmax_scale > 0.f ? sh->softmax_scale : 1.f / sqrtf(static_cast<float>(kHeadDim));
   if ((rc = kv4_ready(&a.c, err, n)) != DIAL_OK) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const cudaError_t e = sh->act == DIAL_ACT_BF16 ? launch<__nv_bfloat16>(a, s) : launch<__half>(a, s);
+  const cudaError_t e = a.max_q * (sh->q_heads / sh->kv_heads) <= kFewCols
+                            ? kv4_decode_launch(a, sh->act, s)
+                        : sh->act == DIAL_ACT_BF16 ? launch<__nv_bfloat16>(a, s) : launch<__half>(a, s);
   if (e != cudaSuccess)
     return kv4_fail(err, n, DIAL_ERR_CUDA, "kv4 attention launch failed: %s", cudaGetErrorString(e));
   return DIAL_OK;

@@ -211,7 +211,10 @@ int kv4_cache_of(const dial_b200_kv4_shape* sh, const void* pages, float* weight
     return kv4_fail(err, n, DIAL_ERR_INVALID,
                     "q_heads %d must be 1 to 16 times kv_heads %d (at most 1024)", sh->q_heads,
                     sh->kv_heads);
-  if (sh->max_blocks < 1 || sh->max_blocks > (1 << 26) || sh->num_blocks < 1)
+  // slabs and pages of a sequence are counted in 32 bits
+  if (sh->max_blocks < 1 || sh->num_blocks < 1 || sh->max_blocks > (1 << 26) ||
+      1LL * sh->max_blocks * sh->kv_heads > INT32_MAX ||
+      1LL * sh->num_blocks * sh->kv_heads > INT32_MAX)
     return kv4_fail(err, n, DIAL_ERR_INVALID, "max_blocks %d / num_blocks %d out of range",
                     sh->max_blocks, sh->num_blocks);
   if (!(sh->k_scale > 0.f && sh->k_scale < 1e30f && sh->v_scale > 0.f && sh->v_scale < 1e30f))

@@ -1,0 +1,660 @@
+// Attention of few queries over the 4-bit KV cache (single tokens, drafts).
+//
+//   o = sum_j p_j v_j / sum_j p_j,  p_j = 2^(x_j - m),  x_j = log2(e) scale q.k_j
+//
+// HBM-bound: 144 bytes a slot and kv head against 512 FLOP a column.  What
+// decides is the instructions a page takes, so its codes go from shared memory
+// straight into MMA operand registers, in the order the page has them:
+//   S^T = K Q^T  m16n8k16, A = 16 tokens x 16 dims.  Lane (g, c) holds row g's
+//                dims 32c .. 32c + 31 (16 bytes); MMA step t takes 4 of them, and
+//                the query operand is loaded in the same order of dims.
+//   O^T = V^T P^T  A = 16 dims x 16 tokens.  Lane (g, c) holds scale group g of 4
+//                tokens; nibbles of two tokens are interleaved before the
+//                conversion, which then gives the operand's token pairs.
+// e2m1 times e4m3 is exact in f16 (6 significant bits, 2^-10 .. 2688), so K and V
+// enter the MMA as the values the cache stands for; queries enter as f16 after
+// an exact power-of-two scale, P as f16 (2^-11 relative), and scores, sums and
+// accumulators are f32.  Columns are (query, head of the group) pairs, so the
+// 8 columns of an MMA cost the same for 1 and for 8.
+// The softmax reference m moves only when a score exceeds it by 2^8, found by
+// one vote a page instead of a shuffle tree.
+//
+// Work split: the pages of all (sequence, kv head) segments laid end to end and
+// cut into equal ranges, one a CTA, so ragged lengths balance; the pages of a
+// range go round its 4 warps, each with its own ring of bulk copies that runs on
+// across segment borders.  A segment inside one range is finished there; the
+// others leave (m, l, O) parts that kv4_join_kernel adds in order.  With running
+// weights the scores are kept in scratch (16 columns' f32 are a ninth of the
+// page's bytes at 4 heads a group) and the join turns them into probabilities
+// once m and l are known, one thread a slot, no atomics.
+#include <cmath>
+
+#include "kv4_attn.h"
+#include "kv4_dev.cuh"
+
+namespace dialb200 {
+namespace {
+
+// Warps a CTA: 16 warps an SM fit at up to 128 registers (one column tile) as two
+// CTAs of 8, 12 at 164 (two tiles) as three of 4.
+template <int NT>
+constexpr int kWarpsOf = NT == 1 ? 8 : 4;
+template <int NT>
+constexpr int kCtasPerSm = NT == 1 ? 2 : 3;
+constexpr int kRing = 4;           // pages in flight a warp
+constexpr int kSeqChunk = 1024;    // sequences a launch
+constexpr float kRaise = 8.f;      // log2 headroom of a probability above 1
+constexpr int kColStride = kHeadDim + 4;
+
+struct DecodeArgs {
+  Kv4AttnArgs a;
+  int cols_max;     // max_q * heads of a group
+  int groups;       // column groups of NT * 8
+  int ctas;         // ranges
+  int score_ld;     // floats a slot in `scores`
+  float* part_o;    // [ctas + segments][groups][NT * 8][128]
+  float* part_ml;   // [ctas + segments][groups][NT * 8][2]
+  float* scores;    // [pages of all segments][16][score_ld] or null
+};
+
+// cum[i]: pages of the sequences before i; the block's threads share the scan.
+template <int THREADS>
+__device__ __forceinline__ void page_prefix(const Kv4AttnArgs& a, int* cum, int* sums) {
+  constexpr int PER = kSeqChunk / THREADS;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  int v[PER], total = 0;
+#pragma unroll
+  for (int e = 0; e < PER; ++e) {
+    const int i = tid * PER + e;
+    Kv4Seq s;
+    v[e] = 0;
+    if (i < a.seqs && kv4_seq(a, i, s) && s.n > 0) v[e] = (s.len + kPageTokens - 1) / kPageTokens;
+    total += v[e];
+  }
+  int run = total;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int u = __shfl_up_sync(0xffffffffu, run, o);
+    if (lane >= o) run += u;
+  }
+  if (lane == 31) sums[warp] = run;
+  __syncthreads();
+  int before = run - total;
+  for (int w = 0; w < warp; ++w) before += sums[w];
+#pragma unroll
+  for (int e = 0; e < PER; ++e) {
+    const int i = tid * PER + e;
+    if (i <= a.seqs) cum[i] = before;
+    before += v[e];
+  }
+  if (tid == THREADS - 1 && a.seqs == kSeqChunk) cum[kSeqChunk] = before;
+  __syncthreads();
+}
+
+// The sequence whose pages hold page `fp` of the prefix.
+__device__ __forceinline__ int seq_at(const int* cum, int seqs, int fp) {
+  int lo = 0, hi = seqs;  // cum[lo] <= fp < cum[hi]
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (cum[mid] <= fp) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+// Ranges that `total` pages are cut into: no range is empty, and each warp of
+// a CTA has a page where the pages do not go round all CTAs.
+__device__ __forceinline__ int ranges_of(int total, int ctas, int warps) {
+  return min(ctas, (total + warps - 1) / warps);
+}
+// Range of pages (over all segments) of CTA b, and the CTA whose range holds f.
+__device__ __forceinline__ int range_start(int total, int b, int ctas) {
+  return static_cast<int>(static_cast<long long>(total) * b / ctas);
+}
+__device__ __forceinline__ int range_of(int total, int f, int ctas) {
+  int b = static_cast<int>(static_cast<long long>(f) * ctas / total);
+  while (b + 1 < ctas && range_start(total, b + 1, ctas) <= f) ++b;
+  return b;
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+__device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
+  const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+
+// Token of the page in row r of the K operand (and of the probabilities): the
+// row order in which a lane's 4 V tokens lie in both halves of a bank line.
+__device__ __forceinline__ int row_token(int r) { return r ^ ((r >> 1) & 1); }
+
+template <int NT>
+struct DecodeSmem {
+  static constexpr int kWarps = kWarpsOf<NT>;
+  uint8_t ring[kWarps][kRing][kKv4Slab];
+  float o[kWarps][8][kColStride];
+  float ml[kWarps][8][2];
+  uint64_t full[kWarps][kRing];
+  int cum[kSeqChunk + 1];
+  int sums[kWarps];
+};
+
+template <typename Act, int NT>
+__global__ void __launch_bounds__(kWarpsOf<NT> * 32, kCtasPerSm<NT>)
+    kv4_decode_kernel(const DecodeArgs d) {
+  constexpr int kWarps = kWarpsOf<NT>;
+  extern __shared__ __align__(128) uint8_t smem_raw[];
+  DecodeSmem<NT>& sm = *reinterpret_cast<DecodeSmem<NT>*>(smem_raw);
+  const Kv4AttnArgs& a = d.a;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
+  const int H = a.c.kv_heads, rep = a.c.q_heads / H;
+  const int b = blockIdx.x, col0 = blockIdx.y * NT * 8;
+  pdl_wait();
+  pdl_launch_dependents();
+  if (lane == 0) {
+    for (int i = 0; i < kRing; ++i) mbar_init(&sm.full[warp][i], 1);
+    fence_mbar_init();
+  }
+  page_prefix<kWarps * 32>(a, sm.cum, sm.sums);
+  const int total = sm.cum[a.seqs] * H;
+  // sequences without a slot: zeros
+  for (int i = b; i < a.seqs; i += d.ctas) {
+    Kv4Seq s;
+    if (sm.cum[i + 1] != sm.cum[i] || !kv4_seq(a, i, s) || blockIdx.y != 0) continue;
+    for (int r = 0; r < s.n; ++r)
+      for (int e = tid * 8; e < a.c.q_heads * kHeadDim; e += kWarps * 32 * 8)
+        *reinterpret_cast<uint4*>(static_cast<Act*>(a.out) + (s.row0 + r) * a.out_ld + e) =
+            make_uint4(0, 0, 0, 0);
+  }
+  const int ctas = ranges_of(total, d.ctas, kWarps);
+  if (b >= ctas) return;
+  const int f0 = range_start(total, b, ctas), f1 = range_start(total, b + 1, ctas);
+
+  // this warp's pages: f0 + warp + kWarps * i, i < mine; 32 slab numbers a window,
+  // the next window's loads a window ahead
+  const int mine = f1 - f0 > warp ? (f1 - f0 - warp + kWarps - 1) / kWarps : 0;
+  auto slab_of = [&](int i) -> int {
+    if (i >= mine) return 0;
+    const int f = f0 + warp + kWarps * i;
+    const int s = seq_at(sm.cum, a.seqs, f / H);
+    const int np = sm.cum[s + 1] - sm.cum[s], r = f - sm.cum[s] * H;
+    return max(0, kv4_block(a.c, a.c.block_table, a.sids[s], r % np)) * H + r / np;
+  };
+  int win = slab_of(lane), win_next = slab_of(32 + lane), issued = 0;
+  auto issue = [&]() {  // warp-uniform
+    if (issued > 0 && (issued & 31) == 0) {
+      win = win_next;
+      win_next = slab_of(issued + 32 + lane);
+    }
+    const int slab = __shfl_sync(0xffffffffu, win, issued & 31);
+    if (lane == 0) {
+      uint64_t* bar = &sm.full[warp][issued % kRing];
+      mbar_arrive_expect_tx(bar, kKv4Slab);
+      bulk_g2s(sm.ring[warp][issued % kRing],
+               a.c.pages + static_cast<size_t>(static_cast<unsigned>(slab)) * kKv4Slab, kKv4Slab, bar);
+    }
+    ++issued;
+  };
+  while (issued < kRing && issued < mine) issue();
+
+  int done = 0;
+  bool ok = true;
+  for (int fc = f0; fc < f1;) {
+    // ------------------------------------------------ one segment's share
+    const int si = seq_at(sm.cum, a.seqs, fc / H);
+    const int np = sm.cum[si + 1] - sm.cum[si], base = sm.cum[si] * H;
+    const int h = (fc - base) / np, seg0 = base + h * np, seg1 = seg0 + np;
+    const int fe = min(f1, seg1);
+    Kv4Seq s;
+    kv4_seq(a, si, s);
+    const int cols = s.n * rep;
+    uint32_t qf[NT][16];
+    float fac[NT][2], m[NT][2], l[NT][2], o[NT][8][4];
+    int seen[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int col = col0 + nt * 8 + g;
+      float qv[32], top = 0.f;
+      if (col < cols) {
+        const uint4* src = reinterpret_cast<const uint4*>(
+            static_cast<const Act*>(a.q) + (s.row0 + col / rep) * a.q_ld +
+            (h * rep + col % rep) * kHeadDim + 32 * c);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint4 raw = src[e];
+          const Act* v = reinterpret_cast<const Act*>(&raw);
+#pragma unroll
+          for (int u = 0; u < 8; ++u) qv[8 * e + u] = ActTraits<Act>::to_f(v[u]);
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 32; ++e) qv[e] = 0.f;
+      }
+#pragma unroll
+      for (int e = 0; e < 32; ++e) top = fmaxf(top, fabsf(qv[e]));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      // 2^-e of the row's largest exponent: the f16 copy is exact for values down
+      // to 2^-14 of it, and off by at most 2^-25 of it below
+      const int ex = min(max(static_cast<int>(__float_as_uint(top) >> 23) - 127, -100), 100);
+      const float down = exp2i(-ex);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) qf[nt][e] = pack_f16(qv[2 * e] * down, qv[2 * e + 1] * down);
+      const float mine_f = exp2i(ex) * a.scale * a.c.k_scale * 1.4426950408889634f;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        fac[nt][e] = __shfl_sync(0xffffffffu, mine_f, (2 * c + e) * 4);
+        const int cc = col0 + nt * 8 + 2 * c + e;
+        seen[nt][e] = cc < cols ? s.len - s.n + 1 + cc / rep : 0;
+        m[nt][e] = -INFINITY;
+        l[nt][e] = 0.f;
+      }
+#pragma unroll
+      for (int mt = 0; mt < 8; ++mt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[nt][mt][e] = 0.f;
+    }
+    // ------------------------------------------------------------- pages
+    for (; ok && done < mine && f0 + warp + kWarps * done < fe; ++done) {
+      const int slot = done % kRing, page = f0 + warp + kWarps * done - seg0;
+      const uint8_t* pg = sm.ring[warp][slot];
+      ok = __all_sync(0xffffffffu, mbar_wait(&sm.full[warp][slot], static_cast<uint32_t>(done / kRing) & 1u,
+                                             a.c.status, kStatusAttnRing));
+      if (!ok) break;
+      float x[NT][4];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[nt][e] = 0.f;
+      {
+        const int t0 = row_token(g), t1 = t0 + 8;
+        const uint4 k0 = *reinterpret_cast<const uint4*>(pg + t0 * 64 + c * 16);
+        const uint4 k1 = *reinterpret_cast<const uint4*>(pg + t1 * 64 + c * 16);
+        const uint32_t s0 = e4m3x2_to_f16x2(*reinterpret_cast<const uint16_t*>(pg + kKv4KScales + t0 * 8 + c * 2));
+        const uint32_t s1 = e4m3x2_to_f16x2(*reinterpret_cast<const uint16_t*>(pg + kKv4KScales + t1 * 8 + c * 2));
+        const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const uint32_t sc0 = __byte_perm(s0, 0, w < 2 ? 0x1010 : 0x3232);
+          const uint32_t sc1 = __byte_perm(s1, 0, w < 2 ? 0x1010 : 0x3232);
+          uint32_t r0[4], r1[4];
+          e2m1x8_to_f16x2x4(w0[w], r0);
+          e2m1x8_to_f16x2x4(w1[w], r1);
+#pragma unroll
+          for (int hf = 0; hf < 2; ++hf) {
+            const uint32_t af[4] = {hmul2(r0[2 * hf], sc0), hmul2(r1[2 * hf], sc1),
+                                    hmul2(r0[2 * hf + 1], sc0), hmul2(r1[2 * hf + 1], sc1)};
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+              mma_f16(x[nt], af, qf[nt][4 * w + 2 * hf], qf[nt][4 * w + 2 * hf + 1]);
+          }
+        }
+      }
+      const bool open = (page + 1) * kPageTokens <= s.len - s.n + 1;  // seen by every column
+      bool raise = false;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          x[nt][e] *= fac[nt][e & 1];
+          if (!open && page * kPageTokens + row_token(g) + (e >> 1) * 8 >= seen[nt][e & 1])
+            x[nt][e] = -INFINITY;
+          raise |= x[nt][e] > m[nt][e & 1] + kRaise;
+        }
+        if (d.scores) {
+          const int cc = col0 + nt * 8 + 2 * c;
+          if (cc < cols) {
+            float* to = d.scores + (static_cast<size_t>(seg0 + page) * kPageTokens + row_token(g)) * d.score_ld + cc;
+            *reinterpret_cast<float2*>(to) = make_float2(x[nt][0], x[nt][1]);
+            *reinterpret_cast<float2*>(to + 8 * d.score_ld) = make_float2(x[nt][2], x[nt][3]);
+          }
+        }
+      }
+      if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float top = fmaxf(x[nt][e], x[nt][e + 2]);
+#pragma unroll
+            for (int w = 4; w < 32; w <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+            const float mn = fmaxf(m[nt][e], top);
+            const float al = m[nt][e] == -INFINITY ? 0.f : ex2(m[nt][e] - mn);
+            m[nt][e] = mn;
+            l[nt][e] *= al;
+#pragma unroll
+            for (int mt = 0; mt < 8; ++mt) {
+              o[nt][mt][e] *= al;
+              o[nt][mt][e + 2] *= al;
+            }
+          }
+      }
+      uint32_t pf[NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const float r0 = m[nt][0] == -INFINITY ? 0.f : m[nt][0];
+        const float r1 = m[nt][1] == -INFINITY ? 0.f : m[nt][1];
+        const float p0 = ex2(x[nt][0] - r0), p1 = ex2(x[nt][1] - r1);
+        const float p2 = ex2(x[nt][2] - r0), p3 = ex2(x[nt][3] - r1);
+        l[nt][0] += p0 + p2;
+        l[nt][1] += p1 + p3;
+        pf[nt][0] = transpose8(pack_f16(p0, p1));
+        pf[nt][1] = transpose8(pack_f16(p2, p3));
+      }
+      // V: rows 2c, 2c + 1 (lo) and 2c + 8, 2c + 9 (hi), scale group g
+      {
+        const int ta = row_token(2 * c), tb = row_token(2 * c + 1);
+        const uint8_t* vp = pg + kKv4VCodes + g * 8;
+        const uint2 va = *reinterpret_cast<const uint2*>(vp + ta * 64);
+        const uint2 vb = *reinterpret_cast<const uint2*>(vp + tb * 64);
+        const uint2 vc = *reinterpret_cast<const uint2*>(vp + (ta + 8) * 64);
+        const uint2 vd = *reinterpret_cast<const uint2*>(vp + (tb + 8) * 64);
+        const uint8_t* sp = pg + kKv4VScales + g;
+        const uint32_t sab = e4m3x2_to_f16x2(static_cast<uint16_t>(sp[ta * 8] | sp[tb * 8] << 8));
+        const uint32_t scd = e4m3x2_to_f16x2(static_cast<uint16_t>(sp[(ta + 8) * 8] | sp[(tb + 8) * 8] << 8));
+        constexpr uint32_t kLow = 0x0F0F0F0Fu;
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          const uint32_t A = w ? va.y : va.x, B = w ? vb.y : vb.x, C = w ? vc.y : vc.x, D = w ? vd.y : vd.x;
+          uint32_t lo0[4], hi0[4], lo1[4], hi1[4];
+          e2m1x8_to_f16x2x4((A & kLow) | ((B << 4) & ~kLow), lo0);
+          e2m1x8_to_f16x2x4(((A >> 4) & kLow) | (B & ~kLow), hi0);
+          e2m1x8_to_f16x2x4((C & kLow) | ((D << 4) & ~kLow), lo1);
+          e2m1x8_to_f16x2x4(((C >> 4) & kLow) | (D & ~kLow), hi1);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t af[4] = {hmul2(lo0[e], sab), hmul2(hi0[e], sab), hmul2(lo1[e], scd),
+                                    hmul2(hi1[e], scd)};
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) mma_f16(o[nt][4 * w + e], af, pf[nt][0], pf[nt][1]);
+          }
+        }
+      }
+      // the slot's reads before the copy that refills it
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (issued < mine) issue();
+    }
+    // ------------------------------------- the warps' parts of the segment
+    const bool whole = fc == seg0 && fe == seg1;
+    const int seg = si * H + h;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float sum = l[nt][e];
+#pragma unroll
+        for (int w = 4; w < 32; w <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
+        if (g == 0) {
+          sm.ml[warp][2 * c + e][0] = m[nt][e];
+          sm.ml[warp][2 * c + e][1] = sum;
+        }
+#pragma unroll
+        for (int mt = 0; mt < 8; ++mt)
+          *reinterpret_cast<float2*>(&sm.o[warp][2 * c + e][16 * g + 2 * mt]) =
+              make_float2(o[nt][mt][e], o[nt][mt][e + 2]);
+      }
+      __syncthreads();
+      const size_t part = (static_cast<size_t>(b + seg) * d.groups + blockIdx.y) * NT * 8 + nt * 8;
+      const int dim = tid % kHeadDim;
+      for (int cl = tid / kHeadDim; cl < 8; cl += kWarps * 32 / kHeadDim) {
+        const int col = col0 + nt * 8 + cl;
+        if (col >= cols) break;
+        float M = -INFINITY, L = 0.f, O = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) M = fmaxf(M, sm.ml[w][cl][0]);
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+          const float mw = sm.ml[w][cl][0];
+          const float f = mw == -INFINITY ? 0.f : ex2(mw - M);
+          L = fmaf(f, sm.ml[w][cl][1], L);
+          O = fmaf(f, sm.o[w][cl][dim], O);
+        }
+        if (whole) {
+          static_cast<Act*>(a.out)[(s.row0 + col / rep) * a.out_ld + (h * rep + col % rep) * kHeadDim + dim] =
+              ActTraits<Act>::from_f(L != 0.f ? O / L * a.c.v_scale : 0.f);
+        } else {
+          d.part_o[(part + cl) * kHeadDim + dim] = O;
+        }
+        if ((!whole || d.scores) && dim == 0)
+          *reinterpret_cast<float2*>(d.part_ml + (part + cl) * 2) = make_float2(M, L);
+      }
+      __syncthreads();
+    }
+    fc = fe;
+  }
+  if (!ok)  // a copy did not land in time: wait (bounded) for those in flight
+    for (int i = done; i < issued; ++i)
+      mbar_wait(&sm.full[warp][i % kRing], static_cast<uint32_t>(i / kRing) & 1u, a.c.status, kStatusAttnRing);
+}
+
+constexpr int kJoinThreads = 256;
+
+// Joins the parts of the segments that cross ranges, and adds the
+// probabilities of every slot of this CTA's range to the running weights.
+template <typename Act, int NT>
+__global__ void __launch_bounds__(kJoinThreads) kv4_join_kernel(const DecodeArgs d) {
+  __shared__ int cum[kSeqChunk + 1];
+  __shared__ int sums[kJoinThreads / 32];
+  __shared__ float red_o[kJoinThreads / kHeadDim][kHeadDim];
+  __shared__ float red_l[kJoinThreads / kHeadDim];
+  __shared__ float2 ml[512];  // with weights: (m, 1 / l) of the segment's columns
+  const Kv4AttnArgs& a = d.a;
+  const int tid = threadIdx.x, b = blockIdx.x, H = a.c.kv_heads, rep = a.c.q_heads / H;
+  page_prefix<kJoinThreads>(a, cum, sums);
+  const int total = cum[a.seqs] * H;
+  pdl_wait();
+  const int ctas = ranges_of(total, d.ctas, kWarpsOf<NT>);
+  if (b >= ctas) return;
+  const int f0 = range_start(total, b, ctas), f1 = range_start(total, b + 1, ctas);
+  for (int fc = f0; fc < f1;) {
+    const int si = seq_at(cum, a.seqs, fc / H);
+    const int np = cum[si + 1] - cum[si], base = cum[si] * H;
+    const int h = (fc - base) / np, seg0 = base + h * np, seg1 = seg0 + np;
+    const int fe = min(f1, seg1), seg = si * H + h;
+    Kv4Seq s;
+    kv4_seq(a, si, s);
+    const int cols = s.n * rep;
+    const bool first = fc == seg0;  // the CTA that joins the segment's parts
+    const int b1 = range_of(total, seg1 - 1, ctas), b0 = first ? b : range_of(total, seg0, ctas);
+    // blockIdx.y: columns of the join, dealt out
+    if (first && b1 > b) {
+      const int dim = tid % kHeadDim, half = tid / kHeadDim;
+      for (int col = blockIdx.y; col < cols; col += gridDim.y) {
+        const int grp = col / (NT * 8), cl = col % (NT * 8);
+        auto part = [&](int bb) {
+          return (static_cast<size_t>(bb + seg) * d.groups + grp) * NT * 8 + cl;
+        };
+        float M = -INFINITY, L = 0.f, O = 0.f;
+        for (int bb = b; bb <= b1; ++bb) M = fmaxf(M, d.part_ml[part(bb) * 2]);
+        for (int bb = b + half; bb <= b1; bb += kJoinThreads / kHeadDim) {
+          const float2 p = *reinterpret_cast<const float2*>(d.part_ml + part(bb) * 2);
+          const float f = p.x == -INFINITY ? 0.f : ex2(p.x - M);
+          L = fmaf(f, p.y, L);
+          O = fmaf(f, d.part_o[part(bb) * kHeadDim + dim], O);
+        }
+        red_o[half][dim] = O;
+        if (dim == 0) red_l[half] = L;
+        __syncthreads();
+        if (half == 0) {
+#pragma unroll
+          for (int w = 1; w < kJoinThreads / kHeadDim; ++w) {
+            O += red_o[w][dim];
+            L += red_l[w];
+          }
+          static_cast<Act*>(a.out)[(s.row0 + col / rep) * a.out_ld + (h * rep + col % rep) * kHeadDim + dim] =
+              ActTraits<Act>::from_f(L != 0.f ? O / L * a.c.v_scale : 0.f);
+        }
+        __syncthreads();
+      }
+    }
+    if (d.scores) {
+      for (int col = tid; col < cols; col += kJoinThreads) {
+        const int grp = col / (NT * 8), cl = col % (NT * 8);
+        float M = -INFINITY, L = 0.f;
+        for (int pass = 0; pass < 2; ++pass)
+          for (int bb = b0; bb <= b1; ++bb) {
+            const float2 p = *reinterpret_cast<const float2*>(
+                d.part_ml + ((static_cast<size_t>(bb + seg) * d.groups + grp) * NT * 8 + cl) * 2);
+            if (pass == 0) M = fmaxf(M, p.x);
+            else if (p.x != -INFINITY) L = fmaf(ex2(p.x - M), p.y, L);
+          }
+        ml[col] = make_float2(M == -INFINITY ? 0.f : M, L > 0.f ? 1.f / L : 0.f);
+      }
+      __syncthreads();
+      const int lo = (fc - seg0) * kPageTokens + blockIdx.y * kJoinThreads;
+      for (int t = lo + tid; t < min((fe - seg0) * kPageTokens, s.len); t += gridDim.y * kJoinThreads) {
+        const float* x = d.scores + (static_cast<size_t>(seg0) * kPageTokens + t) * d.score_ld;
+        float sum = 0.f;
+        for (int col = 0; col < cols; col += 2) {
+          const float2 v = *reinterpret_cast<const float2*>(x + col);
+          sum = fmaf(ex2(v.x - ml[col].x), ml[col].y, sum);
+          if (col + 1 < cols) sum = fmaf(ex2(v.y - ml[col + 1].x), ml[col + 1].y, sum);
+        }
+        const int block = kv4_block(a.c, a.c.block_table, s.sid, t / kPageTokens);
+        if (block >= 0)
+          a.c.weights[kv4_slab_index(a.c, block, h) * kPageTokens + t % kPageTokens] += sum;
+      }
+      __syncthreads();
+    }
+    fc = fe;
+  }
+}
+
+int sm_count() {
+  static int n = [] {
+    int v = 0, dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess ||
+        cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || v < 1)
+      v = 148;
+    return v;
+  }();
+  return n;
+}
+
+// Sizes of one launch over `seqs` sequences.
+struct Plan {
+  int nt, groups, ctas, cols, score_ld;
+  long long pages;  // pages of all segments at most
+  size_t part_o, part_ml, scores;
+};
+
+Plan plan_of(int q_heads, int kv_heads, long long seqs, long long max_q, long long max_len,
+             bool weights, int sms) {
+  Plan p{};
+  const int rep = q_heads / kv_heads;
+  p.cols = static_cast<int>(max_q * rep);
+  p.nt = p.cols <= 8 ? 1 : 2;
+  p.groups = (p.cols + p.nt * 8 - 1) / (p.nt * 8);
+  const long long per = (max_len + kPageTokens - 1) / kPageTokens;
+  p.pages = seqs * per * kv_heads;
+  // a page a warp at least, as many CTAs as are resident at once at most
+  const int warps = p.nt == 1 ? kWarpsOf<1> : kWarpsOf<2>;
+  const long long want = (p.pages + warps - 1) / warps;
+  const long long most = static_cast<long long>(sms) * (p.nt == 1 ? kCtasPerSm<1> : kCtasPerSm<2>);
+  p.ctas = static_cast<int>(want < 1 ? 1 : want < most ? want : most);
+  p.score_ld = (p.cols + 1) & ~1;
+  auto up = [](size_t v) { return (v + 127) & ~static_cast<size_t>(127); };
+  const size_t rows = static_cast<size_t>(p.ctas + seqs * kv_heads) * p.groups * p.nt * 8;
+  p.part_o = up(rows * kHeadDim * 4);
+  p.part_ml = up(rows * 8);
+  p.scores = weights ? up(static_cast<size_t>(p.pages) * kPageTokens * p.score_ld * 4) : 0;
+  return p;
+}
+
+// Sequences a launch takes: the prefix in shared memory holds kSeqChunk, and
+// page numbers are 32-bit.
+long long chunk_of(int kv_heads, long long seqs, long long max_len) {
+  const long long per = (max_len + kPageTokens - 1) / kPageTokens * kv_heads;
+  long long n = per > 0 ? INT32_MAX / per : kSeqChunk;
+  n = n < kSeqChunk ? n : kSeqChunk;
+  return n < seqs ? n : seqs;
+}
+
+template <typename K>
+cudaError_t start(K kernel, dim3 grid, int threads, size_t smem, cudaStream_t s, const DecodeArgs& d) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, d);
+}
+
+template <typename Act, int NT>
+cudaError_t launch_nt(const DecodeArgs& d, cudaStream_t s) {
+  const size_t smem = sizeof(DecodeSmem<NT>);
+  cudaError_t e = cudaFuncSetAttribute(kv4_decode_kernel<Act, NT>,
+                                       cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  if (e != cudaSuccess) return e;
+  e = start(kv4_decode_kernel<Act, NT>, dim3(d.ctas, d.groups), kWarpsOf<NT> * 32, smem, s, d);
+  if (e != cudaSuccess) return e;
+  const int ys = d.cols_max < 8 ? d.cols_max : 8;
+  return start(kv4_join_kernel<Act, NT>, dim3(d.ctas, ys), kJoinThreads, 0, s, d);
+}
+
+}  // namespace
+
+size_t kv4_decode_scratch(int q_heads, int kv_heads, long long seqs, long long max_q,
+                          long long max_len, bool weights) {
+  const long long n = chunk_of(kv_heads, seqs, max_len);
+  if (n < 1) return 0;
+  const Plan p = plan_of(q_heads, kv_heads, n, max_q, max_len, weights, 148);
+  return p.part_o + p.part_ml + p.scores;
+}
+
+cudaError_t kv4_decode_launch(const Kv4AttnArgs& a, int act, cudaStream_t s) {
+  const long long n = chunk_of(a.c.kv_heads, a.seqs, a.max_len);
+  if (n < 1) return cudaErrorInvalidValue;
+  const int sms = sm_count() < 148 ? sm_count() : 148;  // as the scratch was sized
+  for (long long at = 0; at < a.seqs; at += n) {
+    DecodeArgs d{};
+    d.a = a;
+    d.a.seqs = static_cast<int>(a.seqs - at < n ? a.seqs - at : n);
+    d.a.sids = a.sids + at;
+    d.a.lens = a.lens + at;
+    if (a.q_starts) {
+      d.a.q_starts = a.q_starts + at;
+    } else {
+      d.a.q = static_cast<const uint8_t*>(a.q) + at * a.q_ld * 2;
+      d.a.out = static_cast<uint8_t*>(a.out) + at * a.out_ld * 2;
+    }
+    const Plan p = plan_of(a.c.q_heads, a.c.kv_heads, d.a.seqs, a.max_q, a.max_len,
+                           a.c.weights != nullptr, sms);
+    d.cols_max = p.cols;
+    d.groups = p.groups;
+    d.ctas = p.ctas;
+    d.score_ld = p.score_ld;
+    uint8_t* w = static_cast<uint8_t*>(a.scratch);
+    d.part_o = reinterpret_cast<float*>(w);
+    d.part_ml = reinterpret_cast<float*>(w + p.part_o);
+    d.scores = a.c.weights ? reinterpret_cast<float*>(w + p.part_o + p.part_ml) : nullptr;
+    const bool bf = act == DIAL_ACT_BF16;
+    const cudaError_t e = p.nt == 1 ? (bf ? launch_nt<__nv_bfloat16, 1>(d, s) : launch_nt<__half, 1>(d, s))
+                                    : (bf ? launch_nt<__nv_bfloat16, 2>(d, s) : launch_nt<__half, 2>(d, s));
+    if (e != cudaSuccess) return e;
+  }
+  return cudaSuccess;
+}
+
+}  // namespace dialb200

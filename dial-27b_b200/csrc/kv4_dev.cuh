@@ -4,7 +4,7 @@
 
 #include "attn_dev.cuh"
 #include "common.cuh"
-#include "kv4.h"
+#include "kv4_attn.h"
 
 namespace dialb200 {
 
@@ -92,6 +92,28 @@ __device__ __forceinline__ void kv4_decode(const uint8_t* slab, int codes_at, in
   v[1] = __high2float(ha) * s;
   v[2] = __low2float(hb) * s;
   v[3] = __high2float(hb) * s;
+}
+
+// A sequence of an attention call: its session, slots, first row and rows.
+struct Kv4Seq {
+  int sid, len, row0, n;
+};
+
+// The sequence's rows and slots; false (with the status recorded) for one
+// whose session, rows or length are out of range.
+__device__ __forceinline__ bool kv4_seq(const Kv4AttnArgs& a, int i,
+                                        Kv4Seq& s) {
+  s.sid = a.sids[i];
+  s.len = a.lens[i];
+  s.row0 = a.q_starts ? a.q_starts[i] : i;
+  const int end = a.q_starts ? a.q_starts[i + 1] : i + 1;
+  if (static_cast<unsigned>(s.sid) >= static_cast<unsigned>(a.c.sessions) || s.len < 0 ||
+      s.len > a.max_len || s.row0 < 0 || end < s.row0 || end > a.rows || end - s.row0 > a.max_q) {
+    set_status(a.c.status, kStatusBadArgs);
+    return false;
+  }
+  s.n = end - s.row0;
+  return true;
 }
 
 }  // namespace dialb200
