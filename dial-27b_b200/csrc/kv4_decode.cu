@@ -28,6 +28,7 @@
 // page's bytes at 4 heads a group) and the join turns them into probabilities
 // once m and l are known, one thread a slot, no atomics.
 #include <cmath>
+#include <type_traits>
 
 #include "kv4_attn.h"
 #include "kv4_dev.cuh"
@@ -40,6 +41,8 @@ namespace {
 template <int NT>
 constexpr int kWarpsOf = NT == 1 ? 8 : 4;
 template <int NT>
+constexpr bool kPair = NT == 1;  // two pages at once
+template <int NT>
 constexpr int kCtasPerSm = NT == 1 ? 2 : 3;
 constexpr int kRing = 4;           // pages in flight a warp
 constexpr int kSeqChunk = 1024;    // sequences a launch
@@ -48,10 +51,11 @@ constexpr int kColStride = kHeadDim + 4;
 
 struct DecodeArgs {
   Kv4AttnArgs a;
-  int cols_max;     // max_q * heads of a group
   int groups;       // column groups of NT * 8
   int ctas;         // ranges
   int score_ld;     // floats a slot in `scores`
+  int join_y;       // CTAs of the join that a segment's columns are dealt to
+  int4* desc;       // [ctas]: the segment that starts in a range and goes on
   float* part_o;    // [ctas + segments][groups][NT * 8][128]
   float* part_ml;   // [ctas + segments][groups][NT * 8][2]
   float* scores;    // [pages of all segments][16][score_ld] or null
@@ -182,7 +186,10 @@ __global__ void __launch_bounds__(kWarpsOf<NT> * 32, kCtasPerSm<NT>)
             make_uint4(0, 0, 0, 0);
   }
   const int ctas = ranges_of(total, d.ctas, kWarps);
-  if (b >= ctas) return;
+  if (b >= ctas) {
+    if (tid == 0 && blockIdx.y == 0) d.desc[b] = make_int4(-1, 0, 0, 0);
+    return;
+  }
   const int f0 = range_start(total, b, ctas), f1 = range_start(total, b + 1, ctas);
 
   // this warp's pages: f0 + warp + kWarps * i, i < mine; 32 slab numbers a window,
@@ -270,19 +277,30 @@ __global__ void __launch_bounds__(kWarpsOf<NT> * 32, kCtasPerSm<NT>)
         for (int e = 0; e < 4; ++e) o[nt][mt][e] = 0.f;
     }
     // ------------------------------------------------------------- pages
-    for (; ok && done < mine && f0 + warp + kWarps * done < fe; ++done) {
-      const int slot = done % kRing, page = f0 + warp + kWarps * done - seg0;
-      const uint8_t* pg = sm.ring[warp][slot];
-      ok = __all_sync(0xffffffffu, mbar_wait(&sm.full[warp][slot], static_cast<uint32_t>(done / kRing) & 1u,
-                                             a.c.status, kStatusAttnRing));
-      if (!ok) break;
-      float x[NT][4];
+    // U pages at once: their score chains (two a page, over even and odd MMA
+    // steps) and their exponentials overlap, one vote for all
+    auto step = [&](auto count) {
+      constexpr int U = decltype(count)::value;
+      float x[U][NT][4];
+      int page[U];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+      for (int u = 0; u < U; ++u) {
+        const int i = done + u, slot = i % kRing;
+        page[u] = f0 + warp + kWarps * i - seg0;
+        ok = ok && mbar_wait(&sm.full[warp][slot], static_cast<uint32_t>(i / kRing) & 1u, a.c.status,
+                             kStatusAttnRing);
+      }
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) return;
+      const int t0 = row_token(g), t1 = t0 + 8;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[nt][e] = 0.f;
-      {
-        const int t0 = row_token(g), t1 = t0 + 8;
+      for (int u = 0; u < U; ++u) {
+        const uint8_t* pg = sm.ring[warp][(done + u) % kRing];
+        float y[2][NT][4];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) y[0][nt][e] = y[1][nt][e] = 0.f;
         const uint4 k0 = *reinterpret_cast<const uint4*>(pg + t0 * 64 + c * 16);
         const uint4 k1 = *reinterpret_cast<const uint4*>(pg + t1 * 64 + c * 16);
         const uint32_t s0 = e4m3x2_to_f16x2(*reinterpret_cast<const uint16_t*>(pg + kKv4KScales + t0 * 8 + c * 2));
@@ -301,27 +319,34 @@ __global__ void __launch_bounds__(kWarpsOf<NT> * 32, kCtasPerSm<NT>)
                                     hmul2(r0[2 * hf + 1], sc0), hmul2(r1[2 * hf + 1], sc1)};
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
-              mma_f16(x[nt], af, qf[nt][4 * w + 2 * hf], qf[nt][4 * w + 2 * hf + 1]);
+              mma_f16(y[hf][nt], af, qf[nt][4 * w + 2 * hf], qf[nt][4 * w + 2 * hf + 1]);
           }
         }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[u][nt][e] = y[0][nt][e] + y[1][nt][e];
       }
-      const bool open = (page + 1) * kPageTokens <= s.len - s.n + 1;  // seen by every column
       bool raise = false;
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
+      for (int u = 0; u < U; ++u) {
+        const bool open = (page[u] + 1) * kPageTokens <= s.len - s.n + 1;  // seen by every column
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          x[nt][e] *= fac[nt][e & 1];
-          if (!open && page * kPageTokens + row_token(g) + (e >> 1) * 8 >= seen[nt][e & 1])
-            x[nt][e] = -INFINITY;
-          raise |= x[nt][e] > m[nt][e & 1] + kRaise;
-        }
-        if (d.scores) {
-          const int cc = col0 + nt * 8 + 2 * c;
-          if (cc < cols) {
-            float* to = d.scores + (static_cast<size_t>(seg0 + page) * kPageTokens + row_token(g)) * d.score_ld + cc;
-            *reinterpret_cast<float2*>(to) = make_float2(x[nt][0], x[nt][1]);
-            *reinterpret_cast<float2*>(to + 8 * d.score_ld) = make_float2(x[nt][2], x[nt][3]);
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            x[u][nt][e] *= fac[nt][e & 1];
+            if (!open && page[u] * kPageTokens + t0 + (e >> 1) * 8 >= seen[nt][e & 1])
+              x[u][nt][e] = -INFINITY;
+            raise |= x[u][nt][e] > m[nt][e & 1] + kRaise;
+          }
+          if (d.scores) {
+            const int cc = col0 + nt * 8 + 2 * c;
+            if (cc < cols) {
+              float* to = d.scores + (static_cast<size_t>(seg0 + page[u]) * kPageTokens + t0) * d.score_ld + cc;
+              *reinterpret_cast<float2*>(to) = make_float2(x[u][nt][0], x[u][nt][1]);
+              *reinterpret_cast<float2*>(to + 8 * d.score_ld) = make_float2(x[u][nt][2], x[u][nt][3]);
+            }
           }
         }
       }
@@ -330,7 +355,9 @@ __global__ void __launch_bounds__(kWarpsOf<NT> * 32, kCtasPerSm<NT>)
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            float top = fmaxf(x[nt][e], x[nt][e + 2]);
+            float top = fmaxf(x[0][nt][e], x[0][nt][e + 2]);
+#pragma unroll
+            for (int u = 1; u < U; ++u) top = fmaxf(top, fmaxf(x[u][nt][e], x[u][nt][e + 2]));
 #pragma unroll
             for (int w = 4; w < 32; w <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
             const float mn = fmaxf(m[nt][e], top);
@@ -344,21 +371,26 @@ __global__ void __launch_bounds__(kWarpsOf<NT> * 32, kCtasPerSm<NT>)
             }
           }
       }
-      uint32_t pf[NT][2];
+      uint32_t pf[U][NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         const float r0 = m[nt][0] == -INFINITY ? 0.f : m[nt][0];
         const float r1 = m[nt][1] == -INFINITY ? 0.f : m[nt][1];
-        const float p0 = ex2(x[nt][0] - r0), p1 = ex2(x[nt][1] - r1);
-        const float p2 = ex2(x[nt][2] - r0), p3 = ex2(x[nt][3] - r1);
-        l[nt][0] += p0 + p2;
-        l[nt][1] += p1 + p3;
-        pf[nt][0] = transpose8(pack_f16(p0, p1));
-        pf[nt][1] = transpose8(pack_f16(p2, p3));
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const float p0 = ex2(x[u][nt][0] - r0), p1 = ex2(x[u][nt][1] - r1);
+          const float p2 = ex2(x[u][nt][2] - r0), p3 = ex2(x[u][nt][3] - r1);
+          l[nt][0] += p0 + p2;
+          l[nt][1] += p1 + p3;
+          pf[u][nt][0] = transpose8(pack_f16(p0, p1));
+          pf[u][nt][1] = transpose8(pack_f16(p2, p3));
+        }
       }
-      // V: rows 2c, 2c + 1 (lo) and 2c + 8, 2c + 9 (hi), scale group g
-      {
-        const int ta = row_token(2 * c), tb = row_token(2 * c + 1);
+      // V: rows 2c, 2c + 1 and 2c + 8, 2c + 9 of the page, scale group g
+      const int ta = row_token(2 * c), tb = row_token(2 * c + 1);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const uint8_t* pg = sm.ring[warp][(done + u) % kRing];
         const uint8_t* vp = pg + kKv4VCodes + g * 8;
         const uint2 va = *reinterpret_cast<const uint2*>(vp + ta * 64);
         const uint2 vb = *reinterpret_cast<const uint2*>(vp + tb * 64);
@@ -381,14 +413,22 @@ __global__ void __launch_bounds__(kWarpsOf<NT> * 32, kCtasPerSm<NT>)
             const uint32_t af[4] = {hmul2(lo0[e], sab), hmul2(hi0[e], sab), hmul2(lo1[e], scd),
                                     hmul2(hi1[e], scd)};
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) mma_f16(o[nt][4 * w + e], af, pf[nt][0], pf[nt][1]);
+            for (int nt = 0; nt < NT; ++nt) mma_f16(o[nt][4 * w + e], af, pf[u][nt][0], pf[u][nt][1]);
           }
         }
       }
-      // the slot's reads before the copy that refills it
+      // the slots' reads before the copies that refill them
       fence_proxy_async_smem();
       __syncwarp();
-      if (issued < mine) issue();
+      done += U;
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (issued < mine) issue();
+    };
+    const int upto = fe - f0 > warp ? (fe - f0 - warp + kWarps - 1) / kWarps : 0;  // of `mine`
+    while (ok && done < upto) {
+      if (kPair<NT> && done + 1 < upto) step(std::integral_constant<int, 2>{});
+      else step(std::integral_constant<int, 1>{});
     }
     // ------------------------------------- the warps' parts of the segment
     const bool whole = fc == seg0 && fe == seg1;
@@ -436,6 +476,11 @@ __global__ void __launch_bounds__(kWarpsOf<NT> * 32, kCtasPerSm<NT>)
       }
       __syncthreads();
     }
+    // at most the last segment of a range starts in it and goes on
+    if (fe == f1 && tid == 0 && blockIdx.y == 0)
+      d.desc[b] = fc == seg0 && fe < seg1
+                      ? make_int4(seg, range_of(total, seg1 - 1, ctas) - b + 1, s.row0, cols)
+                      : make_int4(-1, 0, 0, 0);
     fc = fe;
   }
   if (!ok)  // a copy did not land in time: wait (bounded) for those in flight
@@ -443,25 +488,86 @@ __global__ void __launch_bounds__(kWarpsOf<NT> * 32, kCtasPerSm<NT>)
       mbar_wait(&sm.full[warp][i % kRing], static_cast<uint32_t>(i / kRing) & 1u, a.c.status, kStatusAttnRing);
 }
 
-constexpr int kJoinThreads = 256;
+constexpr int kJoinThreads = 256, kJoinWarps = kJoinThreads / 32;
 
-// Joins the parts of the segments that cross ranges, and adds the
-// probabilities of every slot of this CTA's range to the running weights.
+// max over a segment's parts of column `col`, and the sum l under it; one warp.
+__device__ __forceinline__ float2 join_ml(const float2* ml, size_t stride, int parts) {
+  const int lane = threadIdx.x & 31;
+  float M = -INFINITY, L = 0.f;
+  for (int p = lane; p < parts; p += 32) M = fmaxf(M, ml[p * stride].x);
+  M = warp_max(M);
+  for (int p = lane; p < parts; p += 32) {
+    const float2 v = ml[p * stride];
+    if (v.x != -INFINITY) L = fmaf(ex2(v.x - M), v.y, L);
+  }
+  return make_float2(M, warp_sum(L));
+}
+
+// blockIdx.y < d.join_y: joins the parts of the segment that starts in range
+// blockIdx.x and goes on in others, a column a CTA, parts over the warps.
+// blockIdx.y >= d.join_y (with weights): adds the probabilities of the slots of
+// range blockIdx.x to the running weights.
 template <typename Act, int NT>
 __global__ void __launch_bounds__(kJoinThreads) kv4_join_kernel(const DecodeArgs d) {
-  __shared__ int cum[kSeqChunk + 1];
-  __shared__ int sums[kJoinThreads / 32];
-  __shared__ float red_o[kJoinThreads / kHeadDim][kHeadDim];
-  __shared__ float red_l[kJoinThreads / kHeadDim];
-  __shared__ float2 ml[512];  // with weights: (m, 1 / l) of the segment's columns
   const Kv4AttnArgs& a = d.a;
-  const int tid = threadIdx.x, b = blockIdx.x, H = a.c.kv_heads, rep = a.c.q_heads / H;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, b = blockIdx.x;
+  const int H = a.c.kv_heads, rep = a.c.q_heads / H;
+  const size_t stride = static_cast<size_t>(d.groups) * NT * 8;  // columns of a part
+  if (blockIdx.y < d.join_y) {
+    __shared__ float4 red[kJoinWarps][kHeadDim / 4];
+    pdl_wait();
+    const int4 ds = d.desc[b];  // segment, its parts, first row, columns
+    if (ds.x < 0) return;
+    for (int col = blockIdx.y; col < ds.w; col += d.join_y) {
+      const size_t first = static_cast<size_t>(b + ds.x) * stride + col;
+      const float4* po = reinterpret_cast<const float4*>(d.part_o) + first * (kHeadDim / 4) + lane;
+      const float2* ml = reinterpret_cast<const float2*>(d.part_ml) + first;
+      constexpr int PRE = 4;  // parts a warp loads before the maximum is known
+      float4 pre[PRE];
+      float pm[PRE];
+#pragma unroll
+      for (int e = 0; e < PRE; ++e) {
+        const int p = warp + kJoinWarps * e;
+        pre[e] = p < ds.y ? po[p * stride * (kHeadDim / 4)] : make_float4(0.f, 0.f, 0.f, 0.f);
+        pm[e] = p < ds.y ? ml[p * stride].x : -INFINITY;
+      }
+      const float2 all = join_ml(ml, stride, ds.y);
+      float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
+      auto add = [&](const float4& v, float mp) {
+        const float f = mp == -INFINITY ? 0.f : ex2(mp - all.x);
+        O.x = fmaf(f, v.x, O.x);
+        O.y = fmaf(f, v.y, O.y);
+        O.z = fmaf(f, v.z, O.z);
+        O.w = fmaf(f, v.w, O.w);
+      };
+#pragma unroll
+      for (int e = 0; e < PRE; ++e) add(pre[e], pm[e]);
+#pragma unroll 4
+      for (int p = warp + kJoinWarps * PRE; p < ds.y; p += kJoinWarps)
+        add(po[p * stride * (kHeadDim / 4)], ml[p * stride].x);
+      red[warp][lane] = O;
+      __syncthreads();
+      if (tid < kHeadDim) {
+        float v = 0.f;
+#pragma unroll
+        for (int w = 0; w < kJoinWarps; ++w) v += reinterpret_cast<const float*>(red[w])[tid];
+        static_cast<Act*>(a.out)[(ds.z + col / rep) * a.out_ld + ((ds.x % H) * rep + col % rep) * kHeadDim + tid] =
+            ActTraits<Act>::from_f(all.y != 0.f ? v / all.y * a.c.v_scale : 0.f);
+      }
+      __syncthreads();
+    }
+    return;
+  }
+  __shared__ int cum[kSeqChunk + 1];
+  __shared__ int sums[kJoinWarps];
+  __shared__ float2 ml[kKv4DecodeCols];  // (m, 1 / l) of the segment's columns
   page_prefix<kJoinThreads>(a, cum, sums);
-  const int total = cum[a.seqs] * H;
   pdl_wait();
+  const int total = cum[a.seqs] * H;
   const int ctas = ranges_of(total, d.ctas, kWarpsOf<NT>);
   if (b >= ctas) return;
   const int f0 = range_start(total, b, ctas), f1 = range_start(total, b + 1, ctas);
+  const int y = blockIdx.y - d.join_y, ys = gridDim.y - d.join_y;
   for (int fc = f0; fc < f1;) {
     const int si = seq_at(cum, a.seqs, fc / H);
     const int np = cum[si + 1] - cum[si], base = cum[si] * H;
@@ -470,68 +576,34 @@ __global__ void __launch_bounds__(kJoinThreads) kv4_join_kernel(const DecodeArgs
     Kv4Seq s;
     kv4_seq(a, si, s);
     const int cols = s.n * rep;
-    const bool first = fc == seg0;  // the CTA that joins the segment's parts
-    const int b1 = range_of(total, seg1 - 1, ctas), b0 = first ? b : range_of(total, seg0, ctas);
-    // blockIdx.y: columns of the join, dealt out
-    if (first && b1 > b) {
-      const int dim = tid % kHeadDim, half = tid / kHeadDim;
-      for (int col = blockIdx.y; col < cols; col += gridDim.y) {
-        const int grp = col / (NT * 8), cl = col % (NT * 8);
-        auto part = [&](int bb) {
-          return (static_cast<size_t>(bb + seg) * d.groups + grp) * NT * 8 + cl;
-        };
-        float M = -INFINITY, L = 0.f, O = 0.f;
-        for (int bb = b; bb <= b1; ++bb) M = fmaxf(M, d.part_ml[part(bb) * 2]);
-        for (int bb = b + half; bb <= b1; bb += kJoinThreads / kHeadDim) {
-          const float2 p = *reinterpret_cast<const float2*>(d.part_ml + part(bb) * 2);
-          const float f = p.x == -INFINITY ? 0.f : ex2(p.x - M);
-          L = fmaf(f, p.y, L);
-          O = fmaf(f, d.part_o[part(bb) * kHeadDim + dim], O);
-        }
-        red_o[half][dim] = O;
-        if (dim == 0) red_l[half] = L;
-        __syncthreads();
-        if (half == 0) {
-#pragma unroll
-          for (int w = 1; w < kJoinThreads / kHeadDim; ++w) {
-            O += red_o[w][dim];
-            L += red_l[w];
-          }
-          static_cast<Act*>(a.out)[(s.row0 + col / rep) * a.out_ld + (h * rep + col % rep) * kHeadDim + dim] =
-              ActTraits<Act>::from_f(L != 0.f ? O / L * a.c.v_scale : 0.f);
-        }
-        __syncthreads();
-      }
+    const int b0 = range_of(total, seg0, ctas), b1 = range_of(total, seg1 - 1, ctas);
+    for (int col = warp; col < cols; col += kJoinWarps) {
+      const float2 v = join_ml(reinterpret_cast<const float2*>(d.part_ml) +
+                                   static_cast<size_t>(b0 + seg) * stride + col,
+                               stride, b1 - b0 + 1);
+      if (lane == 0) ml[col] = make_float2(v.x == -INFINITY ? 0.f : v.x, v.y > 0.f ? 1.f / v.y : 0.f);
     }
-    if (d.scores) {
-      for (int col = tid; col < cols; col += kJoinThreads) {
-        const int grp = col / (NT * 8), cl = col % (NT * 8);
-        float M = -INFINITY, L = 0.f;
-        for (int pass = 0; pass < 2; ++pass)
-          for (int bb = b0; bb <= b1; ++bb) {
-            const float2 p = *reinterpret_cast<const float2*>(
-                d.part_ml + ((static_cast<size_t>(bb + seg) * d.groups + grp) * NT * 8 + cl) * 2);
-            if (pass == 0) M = fmaxf(M, p.x);
-            else if (p.x != -INFINITY) L = fmaf(ex2(p.x - M), p.y, L);
-          }
-        ml[col] = make_float2(M == -INFINITY ? 0.f : M, L > 0.f ? 1.f / L : 0.f);
-      }
-      __syncthreads();
-      const int lo = (fc - seg0) * kPageTokens + blockIdx.y * kJoinThreads;
-      for (int t = lo + tid; t < min((fe - seg0) * kPageTokens, s.len); t += gridDim.y * kJoinThreads) {
-        const float* x = d.scores + (static_cast<size_t>(seg0) * kPageTokens + t) * d.score_ld;
-        float sum = 0.f;
-        for (int col = 0; col < cols; col += 2) {
-          const float2 v = *reinterpret_cast<const float2*>(x + col);
+    __syncthreads();
+    const int upto = min((fe - seg0) * kPageTokens, s.len);
+    for (int t = (fc - seg0) * kPageTokens + y * kJoinThreads + tid; t < upto; t += ys * kJoinThreads) {
+      const int block = kv4_block(a.c, a.c.block_table, s.sid, t / kPageTokens);
+      float* to = a.c.weights + kv4_slab_index(a.c, max(block, 0), h) * kPageTokens + t % kPageTokens;
+      const float old = *to;
+      const float* x = d.scores + (static_cast<size_t>(seg0) * kPageTokens + t) * d.score_ld;
+      float sum = 0.f;
+      int col = 0;
+      if ((d.score_ld & 3) == 0)
+        for (; col + 4 <= cols; col += 4) {
+          const float4 v = *reinterpret_cast<const float4*>(x + col);
           sum = fmaf(ex2(v.x - ml[col].x), ml[col].y, sum);
-          if (col + 1 < cols) sum = fmaf(ex2(v.y - ml[col + 1].x), ml[col + 1].y, sum);
+          sum = fmaf(ex2(v.y - ml[col + 1].x), ml[col + 1].y, sum);
+          sum = fmaf(ex2(v.z - ml[col + 2].x), ml[col + 2].y, sum);
+          sum = fmaf(ex2(v.w - ml[col + 3].x), ml[col + 3].y, sum);
         }
-        const int block = kv4_block(a.c, a.c.block_table, s.sid, t / kPageTokens);
-        if (block >= 0)
-          a.c.weights[kv4_slab_index(a.c, block, h) * kPageTokens + t % kPageTokens] += sum;
-      }
-      __syncthreads();
+      for (; col < cols; ++col) sum = fmaf(ex2(x[col] - ml[col].x), ml[col].y, sum);
+      if (block >= 0) *to = old + sum;
     }
+    __syncthreads();
     fc = fe;
   }
 }
@@ -551,7 +623,7 @@ int sm_count() {
 struct Plan {
   int nt, groups, ctas, cols, score_ld;
   long long pages;  // pages of all segments at most
-  size_t part_o, part_ml, scores;
+  size_t desc, part_o, part_ml, scores;
 };
 
 Plan plan_of(int q_heads, int kv_heads, long long seqs, long long max_q, long long max_len,
@@ -566,11 +638,13 @@ Plan plan_of(int q_heads, int kv_heads, long long seqs, long long max_q, long lo
   // a page a warp at least, as many CTAs as are resident at once at most
   const int warps = p.nt == 1 ? kWarpsOf<1> : kWarpsOf<2>;
   const long long want = (p.pages + warps - 1) / warps;
-  const long long most = static_cast<long long>(sms) * (p.nt == 1 ? kCtasPerSm<1> : kCtasPerSm<2>);
+  long long most = static_cast<long long>(sms) * (p.nt == 1 ? kCtasPerSm<1> : kCtasPerSm<2>) / p.groups;
+  if (most < sms / 4) most = sms / 4;
   p.ctas = static_cast<int>(want < 1 ? 1 : want < most ? want : most);
   p.score_ld = (p.cols + 1) & ~1;
   auto up = [](size_t v) { return (v + 127) & ~static_cast<size_t>(127); };
   const size_t rows = static_cast<size_t>(p.ctas + seqs * kv_heads) * p.groups * p.nt * 8;
+  p.desc = up(static_cast<size_t>(p.ctas) * sizeof(int4));
   p.part_o = up(rows * kHeadDim * 4);
   p.part_ml = up(rows * 8);
   p.scores = weights ? up(static_cast<size_t>(p.pages) * kPageTokens * p.score_ld * 4) : 0;
@@ -609,8 +683,7 @@ cudaError_t launch_nt(const DecodeArgs& d, cudaStream_t s) {
   if (e != cudaSuccess) return e;
   e = start(kv4_decode_kernel<Act, NT>, dim3(d.ctas, d.groups), kWarpsOf<NT> * 32, smem, s, d);
   if (e != cudaSuccess) return e;
-  const int ys = d.cols_max < 8 ? d.cols_max : 8;
-  return start(kv4_join_kernel<Act, NT>, dim3(d.ctas, ys), kJoinThreads, 0, s, d);
+  return start(kv4_join_kernel<Act, NT>, dim3(d.ctas, d.join_y + (d.scores ? 2 : 0)), kJoinThreads, 0, s, d);
 }
 
 }  // namespace
@@ -620,7 +693,7 @@ size_t kv4_decode_scratch(int q_heads, int kv_heads, long long seqs, long long m
   const long long n = chunk_of(kv_heads, seqs, max_len);
   if (n < 1) return 0;
   const Plan p = plan_of(q_heads, kv_heads, n, max_q, max_len, weights, 148);
-  return p.part_o + p.part_ml + p.scores;
+  return p.desc + p.part_o + p.part_ml + p.scores;
 }
 
 cudaError_t kv4_decode_launch(const Kv4AttnArgs& a, int act, cudaStream_t s) {
@@ -641,14 +714,15 @@ cudaError_t kv4_decode_launch(const Kv4AttnArgs& a, int act, cudaStream_t s) {
     }
     const Plan p = plan_of(a.c.q_heads, a.c.kv_heads, d.a.seqs, a.max_q, a.max_len,
                            a.c.weights != nullptr, sms);
-    d.cols_max = p.cols;
     d.groups = p.groups;
     d.ctas = p.ctas;
     d.score_ld = p.score_ld;
     uint8_t* w = static_cast<uint8_t*>(a.scratch);
-    d.part_o = reinterpret_cast<float*>(w);
-    d.part_ml = reinterpret_cast<float*>(w + p.part_o);
-    d.scores = a.c.weights ? reinterpret_cast<float*>(w + p.part_o + p.part_ml) : nullptr;
+    d.desc = reinterpret_cast<int4*>(w);
+    d.part_o = reinterpret_cast<float*>(w + p.desc);
+    d.part_ml = reinterpret_cast<float*>(w + p.desc + p.part_o);
+    d.scores = a.c.weights ? reinterpret_cast<float*>(w + p.desc + p.part_o + p.part_ml) : nullptr;
+    d.join_y = p.cols < 16 ? p.cols : 16;
     const bool bf = act == DIAL_ACT_BF16;
     const cudaError_t e = p.nt == 1 ? (bf ? launch_nt<__nv_bfloat16, 1>(d, s) : launch_nt<__half, 1>(d, s))
                                     : (bf ? launch_nt<__nv_bfloat16, 2>(d, s) : launch_nt<__half, 2>(d, s));
