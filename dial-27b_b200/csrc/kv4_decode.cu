@@ -41,13 +41,13 @@ namespace {
 template <int NT>
 constexpr int kWarpsOf = NT == 1 ? 8 : 4;
 template <int NT>
-constexpr bool kPair = NT == 1;  // two pages at once
+constexpr int kPages = NT == 1 ? 2 : 1;  // pages of a ring slot, taken at once
 template <int NT>
 constexpr int kCtasPerSm = NT == 1 ? 2 : 3;
 constexpr int kRing = 4;           // pages in flight a warp
-constexpr int kSeqChunk = 1024;    // sequences a launch
+constexpr int kSeqChunk = 512;     // sequences a launch
 constexpr float kRaise = 8.f;      // log2 headroom of a probability above 1
-constexpr int kColStride = kHeadDim + 4;
+constexpr int kColStride = kHeadDim + 8;
 
 struct DecodeArgs {
   Kv4AttnArgs a;
@@ -147,21 +147,49 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t v) {
 // row order in which a lane's 4 V tokens lie in both halves of a bank line.
 __device__ __forceinline__ int row_token(int r) { return r ^ ((r >> 1) & 1); }
 
+// Dim at place p of a part's row: the order in which the accumulators' lanes
+// reach shared memory without bank conflicts, kept up to the output.
+__device__ __forceinline__ int place_dim(int p) { return (p >> 1 & 7) * 16 + (p >> 4) * 2 + (p & 1); }
+
+// D = A B + C with the accumulator's first use: C zero.
+__device__ __forceinline__ void mma_f16_zero(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
+                                             uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 "
+      "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
+
+__device__ __forceinline__ void cp_async16(void* dst, const void* src, bool there) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src),
+               "r"(there ? 16 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
 template <int NT>
 struct DecodeSmem {
-  static constexpr int kWarps = kWarpsOf<NT>;
+  static constexpr int kWarps = kWarpsOf<NT>, kSlots = kRing / kPages<NT>;
   uint8_t ring[kWarps][kRing][kKv4Slab];
   float o[kWarps][8][kColStride];
+  uint8_t q[2][NT * 8][kHeadDim * 2];  // this segment's queries and the next one's
   float ml[kWarps][8][2];
-  uint64_t full[kWarps][kRing];
+  uint64_t full[kWarps][kSlots];
+  uint64_t merged;  // every warp has read the parts in o and ml
   int cum[kSeqChunk + 1];
   int sums[kWarps];
 };
 
-template <typename Act, int NT>
+// One segment's share of a range.
+struct Share {
+  Kv4Seq s;
+  int h, seg, seg0, seg1, end;  // kv head, number, first and last page, end of the share
+};
+
+template <typename Act, int NT, bool SCORES>
 __global__ void __launch_bounds__(kWarpsOf<NT> * 32, kCtasPerSm<NT>)
     kv4_decode_kernel(const DecodeArgs d) {
-  constexpr int kWarps = kWarpsOf<NT>;
+  constexpr int kWarps = kWarpsOf<NT>, U = kPages<NT>, kSlots = kRing / U;
   extern __shared__ __align__(128) uint8_t smem_raw[];
   DecodeSmem<NT>& sm = *reinterpret_cast<DecodeSmem<NT>*>(smem_raw);
   const Kv4AttnArgs& a = d.a;
@@ -171,7 +199,8 @@ __global__ void __launch_bounds__(kWarpsOf<NT> * 32, kCtasPerSm<NT>)
   pdl_wait();
   pdl_launch_dependents();
   if (lane == 0) {
-    for (int i = 0; i < kRing; ++i) mbar_init(&sm.full[warp][i], 1);
+    for (int i = 0; i < kSlots; ++i) mbar_init(&sm.full[warp][i], 1);
+    if (warp == 0) mbar_init(&sm.merged, kWarps);
     fence_mbar_init();
   }
   page_prefix<kWarps * 32>(a, sm.cum, sm.sums);
@@ -192,8 +221,9 @@ __global__ void __launch_bounds__(kWarpsOf<NT> * 32, kCtasPerSm<NT>)
   }
   const int f0 = range_start(total, b, ctas), f1 = range_start(total, b + 1, ctas);
 
-  // this warp's pages: f0 + warp + kWarps * i, i < mine; 32 slab numbers a window,
-  // the next window's loads a window ahead
+  // this warp's pages: f0 + warp + kWarps * i, i < mine; each lane holds the slab
+  // number of one page of a window of 32 and copies that page itself; the next
+  // window's table loads go out a window ahead
   const int mine = f1 - f0 > warp ? (f1 - f0 - warp + kWarps - 1) / kWarps : 0;
   auto slab_of = [&](int i) -> int {
     if (i >= mine) return 0;
@@ -203,54 +233,71 @@ __global__ void __launch_bounds__(kWarpsOf<NT> * 32, kCtasPerSm<NT>)
     return max(0, kv4_block(a.c, a.c.block_table, a.sids[s], r % np)) * H + r / np;
   };
   int win = slab_of(lane), win_next = slab_of(32 + lane), issued = 0;
-  auto issue = [&]() {  // warp-uniform
+  auto issue = [&]() {  // the next U pages into their slot; warp-uniform
     if (issued > 0 && (issued & 31) == 0) {
       win = win_next;
       win_next = slab_of(issued + 32 + lane);
     }
-    const int slab = __shfl_sync(0xffffffffu, win, issued & 31);
-    if (lane == 0) {
-      uint64_t* bar = &sm.full[warp][issued % kRing];
-      mbar_arrive_expect_tx(bar, kKv4Slab);
-      bulk_g2s(sm.ring[warp][issued % kRing],
-               a.c.pages + static_cast<size_t>(static_cast<unsigned>(slab)) * kKv4Slab, kKv4Slab, bar);
-    }
-    ++issued;
+    const int n = min(U, mine - issued), at = lane - (issued & 31);
+    uint64_t* bar = &sm.full[warp][issued / U % kSlots];
+    if (at == 0) mbar_arrive_expect_tx(bar, n * kKv4Slab);
+    if (at >= 0 && at < n)
+      bulk_g2s(sm.ring[warp][(issued + at) % kRing],
+               a.c.pages + static_cast<size_t>(static_cast<unsigned>(win)) * kKv4Slab, kKv4Slab, bar);
+    issued += n;
   };
   while (issued < kRing && issued < mine) issue();
 
-  int done = 0;
-  bool ok = true;
-  for (int fc = f0; fc < f1;) {
-    // ------------------------------------------------ one segment's share
-    const int si = seq_at(sm.cum, a.seqs, fc / H);
+  auto share_at = [&](int f) {
+    Share w;
+    const int si = seq_at(sm.cum, a.seqs, f / H);
     const int np = sm.cum[si + 1] - sm.cum[si], base = sm.cum[si] * H;
-    const int h = (fc - base) / np, seg0 = base + h * np, seg1 = seg0 + np;
-    const int fe = min(f1, seg1);
-    Kv4Seq s;
-    kv4_seq(a, si, s);
-    const int cols = s.n * rep;
+    w.h = (f - base) / np;
+    w.seg = si * H + w.h;
+    w.seg0 = base + w.h * np;
+    w.seg1 = w.seg0 + np;
+    w.end = min(f1, w.seg1);
+    kv4_seq(a, si, w.s);
+    return w;
+  };
+  auto load_q = [&](const Share& w, int buf) {
+    for (int e = tid; e < NT * 8 * 16; e += kWarps * 32) {
+      const int cl = e >> 4, col = col0 + cl, there = col < w.s.n * rep;
+      const int cc = there ? col : 0;
+      cp_async16(sm.q[buf][cl] + (e & 15) * 16,
+                 static_cast<const Act*>(a.q) + (w.s.row0 + cc / rep) * a.q_ld +
+                     (w.h * rep + cc % rep) * kHeadDim + (e & 15) * 8,
+                 there);
+    }
+  };
+
+  int done = 0, buf = 0;
+  uint32_t shares = 0;
+  bool ok = true;
+  Share w = share_at(f0);
+  load_q(w, 0);
+  cp_async_wait();
+  __syncthreads();
+  for (int fc = f0;; buf ^= 1, ++shares) {
+    // ------------------------------------------------ one segment's share
+    const int fe = w.end, cols = w.s.n * rep;
+    Share next = w;
+    if (fe < f1) {
+      next = share_at(fe);
+      load_q(next, buf ^ 1);
+    }
     uint32_t qf[NT][16];
-    float fac[NT][2], m[NT][2], l[NT][2], o[NT][8][4];
-    int seen[NT][2];
+    float fac[NT][2], m[NT][2], ref[NT][2], high[NT][2], l[NT][2], o[NT][8][4];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const int col = col0 + nt * 8 + g;
+      const uint4* src = reinterpret_cast<const uint4*>(sm.q[buf][nt * 8 + g] + 64 * c);
       float qv[32], top = 0.f;
-      if (col < cols) {
-        const uint4* src = reinterpret_cast<const uint4*>(
-            static_cast<const Act*>(a.q) + (s.row0 + col / rep) * a.q_ld +
-            (h * rep + col % rep) * kHeadDim + 32 * c);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const uint4 raw = src[e];
-          const Act* v = reinterpret_cast<const Act*>(&raw);
+      for (int e = 0; e < 4; ++e) {
+        const uint4 raw = src[e];
+        const Act* v = reinterpret_cast<const Act*>(&raw);
 #pragma unroll
-          for (int u = 0; u < 8; ++u) qv[8 * e + u] = ActTraits<Act>::to_f(v[u]);
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < 32; ++e) qv[e] = 0.f;
+        for (int u = 0; u < 8; ++u) qv[8 * e + u] = ActTraits<Act>::to_f(v[u]);
       }
 #pragma unroll
       for (int e = 0; e < 32; ++e) top = fmaxf(top, fabsf(qv[e]));
@@ -266,10 +313,8 @@ __global__ void __launch_bounds__(kWarpsOf<NT> * 32, kCtasPerSm<NT>)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         fac[nt][e] = __shfl_sync(0xffffffffu, mine_f, (2 * c + e) * 4);
-        const int cc = col0 + nt * 8 + 2 * c + e;
-        seen[nt][e] = cc < cols ? s.len - s.n + 1 + cc / rep : 0;
-        m[nt][e] = -INFINITY;
-        l[nt][e] = 0.f;
+        m[nt][e] = high[nt][e] = -INFINITY;
+        ref[nt][e] = l[nt][e] = 0.f;
       }
 #pragma unroll
       for (int mt = 0; mt < 8; ++mt)
@@ -277,92 +322,102 @@ __global__ void __launch_bounds__(kWarpsOf<NT> * 32, kCtasPerSm<NT>)
         for (int e = 0; e < 4; ++e) o[nt][mt][e] = 0.f;
     }
     // ------------------------------------------------------------- pages
-    // U pages at once: their score chains (two a page, over even and odd MMA
-    // steps) and their exponentials overlap, one vote for all
+    const int t0 = row_token(g), ta = row_token(2 * c), tb = row_token(2 * c + 1);
+    const int open_end = w.s.len - w.s.n + 1;  // slots every query sees
+    // N pages from `done` on, all of one slot: their score chains and
+    // exponentials overlap, and one vote does for all
     auto step = [&](auto count) {
-      constexpr int U = decltype(count)::value;
-      float x[U][NT][4];
-      int page[U];
+      constexpr int N = decltype(count)::value;
+      const int page0 = f0 + warp + kWarps * done - w.seg0;
+      const uint8_t* pg0 = sm.ring[warp][done % kRing];
+      // after a wait that ran out (status recorded) the rest is computed on
+      // whatever the slots hold, without more waiting
+      if (ok)
+        ok = mbar_wait(&sm.full[warp][done / U % kSlots], static_cast<uint32_t>(done / kRing) & 1u,
+                       a.c.status, kStatusAttnRing);
+      __syncwarp();
+      float x[N][NT][4];
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int i = done + u, slot = i % kRing;
-        page[u] = f0 + warp + kWarps * i - seg0;
-        ok = ok && mbar_wait(&sm.full[warp][slot], static_cast<uint32_t>(i / kRing) & 1u, a.c.status,
-                             kStatusAttnRing);
-      }
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) return;
-      const int t0 = row_token(g), t1 = t0 + 8;
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const uint8_t* pg = sm.ring[warp][(done + u) % kRing];
-        float y[2][NT][4];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) y[0][nt][e] = y[1][nt][e] = 0.f;
+      for (int u = 0; u < N; ++u) {
+        const uint8_t* pg = pg0 + u * kKv4Slab;
         const uint4 k0 = *reinterpret_cast<const uint4*>(pg + t0 * 64 + c * 16);
-        const uint4 k1 = *reinterpret_cast<const uint4*>(pg + t1 * 64 + c * 16);
+        const uint4 k1 = *reinterpret_cast<const uint4*>(pg + t0 * 64 + 512 + c * 16);
         const uint32_t s0 = e4m3x2_to_f16x2(*reinterpret_cast<const uint16_t*>(pg + kKv4KScales + t0 * 8 + c * 2));
-        const uint32_t s1 = e4m3x2_to_f16x2(*reinterpret_cast<const uint16_t*>(pg + kKv4KScales + t1 * 8 + c * 2));
+        const uint32_t s1 = e4m3x2_to_f16x2(*reinterpret_cast<const uint16_t*>(pg + kKv4KScales + t0 * 8 + 64 + c * 2));
         const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          const uint32_t sc0 = __byte_perm(s0, 0, w < 2 ? 0x1010 : 0x3232);
-          const uint32_t sc1 = __byte_perm(s1, 0, w < 2 ? 0x1010 : 0x3232);
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t sc0 = __byte_perm(s0, 0, i < 2 ? 0x1010 : 0x3232);
+          const uint32_t sc1 = __byte_perm(s1, 0, i < 2 ? 0x1010 : 0x3232);
           uint32_t r0[4], r1[4];
-          e2m1x8_to_f16x2x4(w0[w], r0);
-          e2m1x8_to_f16x2x4(w1[w], r1);
+          e2m1x8_to_f16x2x4(w0[i], r0);
+          e2m1x8_to_f16x2x4(w1[i], r1);
 #pragma unroll
           for (int hf = 0; hf < 2; ++hf) {
             const uint32_t af[4] = {hmul2(r0[2 * hf], sc0), hmul2(r1[2 * hf], sc1),
                                     hmul2(r0[2 * hf + 1], sc0), hmul2(r1[2 * hf + 1], sc1)};
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-              mma_f16(y[hf][nt], af, qf[nt][4 * w + 2 * hf], qf[nt][4 * w + 2 * hf + 1]);
-          }
-        }
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) x[u][nt][e] = y[0][nt][e] + y[1][nt][e];
-      }
-      bool raise = false;
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const bool open = (page[u] + 1) * kPageTokens <= s.len - s.n + 1;  // seen by every column
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            x[u][nt][e] *= fac[nt][e & 1];
-            if (!open && page[u] * kPageTokens + t0 + (e >> 1) * 8 >= seen[nt][e & 1])
-              x[u][nt][e] = -INFINITY;
-            raise |= x[u][nt][e] > m[nt][e & 1] + kRaise;
-          }
-          if (d.scores) {
-            const int cc = col0 + nt * 8 + 2 * c;
-            if (cc < cols) {
-              float* to = d.scores + (static_cast<size_t>(seg0 + page[u]) * kPageTokens + t0) * d.score_ld + cc;
-              *reinterpret_cast<float2*>(to) = make_float2(x[u][nt][0], x[u][nt][1]);
-              *reinterpret_cast<float2*>(to + 8 * d.score_ld) = make_float2(x[u][nt][2], x[u][nt][3]);
+            for (int nt = 0; nt < NT; ++nt) {
+              if (i == 0 && hf == 0) mma_f16_zero(x[u][nt], af, qf[nt][0], qf[nt][1]);
+              else mma_f16(x[u][nt], af, qf[nt][4 * i + 2 * hf], qf[nt][4 * i + 2 * hf + 1]);
             }
           }
         }
       }
+      if ((page0 + kWarps * (N - 1) + 1) * kPageTokens > open_end) {  // causal border or the end
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int cc = col0 + nt * 8 + 2 * c + e;
+            const int seen = cc < cols ? open_end + cc / rep : 0;
+#pragma unroll
+            for (int u = 0; u < N; ++u) {
+              const int t = (page0 + kWarps * u) * kPageTokens + t0;
+              if (t >= seen) x[u][nt][e] = -INFINITY;
+              if (t + 8 >= seen) x[u][nt][e + 2] = -INFINITY;
+            }
+          }
+      }
+      if constexpr (SCORES) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          const int cc = col0 + nt * 8 + 2 * c;
+          if (cc < cols)
+#pragma unroll
+            for (int u = 0; u < N; ++u) {
+              float* to = d.scores + (static_cast<size_t>(w.seg0 + page0 + kWarps * u) * kPageTokens + t0) * d.score_ld + cc;
+              *reinterpret_cast<float2*>(to) = make_float2(x[u][nt][0] * fac[nt][0], x[u][nt][1] * fac[nt][1]);
+              *reinterpret_cast<float2*>(to + 8 * d.score_ld) =
+                  make_float2(x[u][nt][2] * fac[nt][0], x[u][nt][3] * fac[nt][1]);
+            }
+        }
+      }
+      // `high` is (m + kRaise) / fac: the vote needs no scaled scores
+      float top[NT][2];
+      bool raise = false;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          top[nt][e] = fmaxf(x[0][nt][e], x[0][nt][e + 2]);
+#pragma unroll
+          for (int u = 1; u < N; ++u) top[nt][e] = fmaxf(top[nt][e], fmaxf(x[u][nt][e], x[u][nt][e + 2]));
+          raise |= top[nt][e] > high[nt][e];
+        }
       if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            float top = fmaxf(x[0][nt][e], x[0][nt][e + 2]);
+            float t = top[nt][e];
 #pragma unroll
-            for (int u = 1; u < U; ++u) top = fmaxf(top, fmaxf(x[u][nt][e], x[u][nt][e + 2]));
-#pragma unroll
-            for (int w = 4; w < 32; w <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
-            const float mn = fmaxf(m[nt][e], top);
+            for (int i = 4; i < 32; i <<= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, i));
+            const float mn = fmaxf(m[nt][e], t * fac[nt][e]);
             const float al = m[nt][e] == -INFINITY ? 0.f : ex2(m[nt][e] - mn);
             m[nt][e] = mn;
+            ref[nt][e] = mn == -INFINITY ? 0.f : mn;
+            high[nt][e] = __fdiv_rn(mn + kRaise, fac[nt][e]);
             l[nt][e] *= al;
 #pragma unroll
             for (int mt = 0; mt < 8; ++mt) {
@@ -371,38 +426,35 @@ __global__ void __launch_bounds__(kWarpsOf<NT> * 32, kCtasPerSm<NT>)
             }
           }
       }
-      uint32_t pf[U][NT][2];
+      uint32_t pf[N][NT][2];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        const float r0 = m[nt][0] == -INFINITY ? 0.f : m[nt][0];
-        const float r1 = m[nt][1] == -INFINITY ? 0.f : m[nt][1];
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const float p0 = ex2(x[u][nt][0] - r0), p1 = ex2(x[u][nt][1] - r1);
-          const float p2 = ex2(x[u][nt][2] - r0), p3 = ex2(x[u][nt][3] - r1);
+        for (int u = 0; u < N; ++u) {
+          const float p0 = ex2(fmaf(x[u][nt][0], fac[nt][0], -ref[nt][0]));
+          const float p1 = ex2(fmaf(x[u][nt][1], fac[nt][1], -ref[nt][1]));
+          const float p2 = ex2(fmaf(x[u][nt][2], fac[nt][0], -ref[nt][0]));
+          const float p3 = ex2(fmaf(x[u][nt][3], fac[nt][1], -ref[nt][1]));
           l[nt][0] += p0 + p2;
           l[nt][1] += p1 + p3;
           pf[u][nt][0] = transpose8(pack_f16(p0, p1));
           pf[u][nt][1] = transpose8(pack_f16(p2, p3));
         }
-      }
       // V: rows 2c, 2c + 1 and 2c + 8, 2c + 9 of the page, scale group g
-      const int ta = row_token(2 * c), tb = row_token(2 * c + 1);
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const uint8_t* pg = sm.ring[warp][(done + u) % kRing];
-        const uint8_t* vp = pg + kKv4VCodes + g * 8;
+      for (int u = 0; u < N; ++u) {
+        const uint8_t* vp = pg0 + u * kKv4Slab + kKv4VCodes + g * 8;
         const uint2 va = *reinterpret_cast<const uint2*>(vp + ta * 64);
         const uint2 vb = *reinterpret_cast<const uint2*>(vp + tb * 64);
-        const uint2 vc = *reinterpret_cast<const uint2*>(vp + (ta + 8) * 64);
-        const uint2 vd = *reinterpret_cast<const uint2*>(vp + (tb + 8) * 64);
-        const uint8_t* sp = pg + kKv4VScales + g;
+        const uint2 vc = *reinterpret_cast<const uint2*>(vp + ta * 64 + 512);
+        const uint2 vd = *reinterpret_cast<const uint2*>(vp + tb * 64 + 512);
+        const uint8_t* sp = pg0 + u * kKv4Slab + kKv4VScales + g;
         const uint32_t sab = e4m3x2_to_f16x2(static_cast<uint16_t>(sp[ta * 8] | sp[tb * 8] << 8));
-        const uint32_t scd = e4m3x2_to_f16x2(static_cast<uint16_t>(sp[(ta + 8) * 8] | sp[(tb + 8) * 8] << 8));
+        const uint32_t scd = e4m3x2_to_f16x2(static_cast<uint16_t>(sp[ta * 8 + 64] | sp[tb * 8 + 64] << 8));
         constexpr uint32_t kLow = 0x0F0F0F0Fu;
 #pragma unroll
-        for (int w = 0; w < 2; ++w) {
-          const uint32_t A = w ? va.y : va.x, B = w ? vb.y : vb.x, C = w ? vc.y : vc.x, D = w ? vd.y : vd.x;
+        for (int i = 0; i < 2; ++i) {
+          const uint32_t A = i ? va.y : va.x, B = i ? vb.y : vb.x, C = i ? vc.y : vc.x, D = i ? vd.y : vd.x;
           uint32_t lo0[4], hi0[4], lo1[4], hi1[4];
           e2m1x8_to_f16x2x4((A & kLow) | ((B << 4) & ~kLow), lo0);
           e2m1x8_to_f16x2x4(((A >> 4) & kLow) | (B & ~kLow), hi0);
@@ -413,79 +465,87 @@ __global__ void __launch_bounds__(kWarpsOf<NT> * 32, kCtasPerSm<NT>)
             const uint32_t af[4] = {hmul2(lo0[e], sab), hmul2(hi0[e], sab), hmul2(lo1[e], scd),
                                     hmul2(hi1[e], scd)};
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) mma_f16(o[nt][4 * w + e], af, pf[u][nt][0], pf[u][nt][1]);
+            for (int nt = 0; nt < NT; ++nt) mma_f16(o[nt][4 * i + e], af, pf[u][nt][0], pf[u][nt][1]);
           }
         }
       }
-      // the slots' reads before the copies that refill them
-      fence_proxy_async_smem();
-      __syncwarp();
-      done += U;
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (issued < mine) issue();
+      done += N;
+      if (done % U == 0 && issued < mine) {
+        // the slot's reads before the copies that refill it
+        fence_proxy_async_smem();
+        __syncwarp();
+        issue();
+      }
     };
     const int upto = fe - f0 > warp ? (fe - f0 - warp + kWarps - 1) / kWarps : 0;  // of `mine`
-    while (ok && done < upto) {
-      if (kPair<NT> && done + 1 < upto) step(std::integral_constant<int, 2>{});
+    while (done < upto) {
+      if (U == 2 && done % 2 == 0 && done + 1 < upto) step(std::integral_constant<int, U>{});
       else step(std::integral_constant<int, 1>{});
     }
     // ------------------------------------- the warps' parts of the segment
-    const bool whole = fc == seg0 && fe == seg1;
-    const int seg = si * H + h;
+    const bool whole = fc == w.seg0 && fe == w.seg1;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
+      // the parts before these have been read (the first wait passes at once)
+      const uint32_t turn = shares * NT + nt;
+      mbar_wait(&sm.merged, (turn & 1u) ^ 1u, a.c.status, kStatusAttnRing);
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         float sum = l[nt][e];
 #pragma unroll
-        for (int w = 4; w < 32; w <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
+        for (int i = 4; i < 32; i <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, i);
         if (g == 0) {
           sm.ml[warp][2 * c + e][0] = m[nt][e];
           sm.ml[warp][2 * c + e][1] = sum;
         }
 #pragma unroll
         for (int mt = 0; mt < 8; ++mt)
-          *reinterpret_cast<float2*>(&sm.o[warp][2 * c + e][16 * g + 2 * mt]) =
+          *reinterpret_cast<float2*>(&sm.o[warp][2 * c + e][16 * mt + 2 * g]) =
               make_float2(o[nt][mt][e], o[nt][mt][e + 2]);
       }
+      cp_async_wait();  // the next segment's queries, for the barrier to publish
       __syncthreads();
-      const size_t part = (static_cast<size_t>(b + seg) * d.groups + blockIdx.y) * NT * 8 + nt * 8;
-      const int dim = tid % kHeadDim;
+      const size_t part = (static_cast<size_t>(b + w.seg) * d.groups + blockIdx.y) * NT * 8 + nt * 8;
+      const int at = tid % kHeadDim, dim = place_dim(at);
       for (int cl = tid / kHeadDim; cl < 8; cl += kWarps * 32 / kHeadDim) {
         const int col = col0 + nt * 8 + cl;
         if (col >= cols) break;
         float M = -INFINITY, L = 0.f, O = 0.f;
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) M = fmaxf(M, sm.ml[w][cl][0]);
+        for (int i = 0; i < kWarps; ++i) M = fmaxf(M, sm.ml[i][cl][0]);
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-          const float mw = sm.ml[w][cl][0];
+        for (int i = 0; i < kWarps; ++i) {
+          const float mw = sm.ml[i][cl][0];
           const float f = mw == -INFINITY ? 0.f : ex2(mw - M);
-          L = fmaf(f, sm.ml[w][cl][1], L);
-          O = fmaf(f, sm.o[w][cl][dim], O);
+          L = fmaf(f, sm.ml[i][cl][1], L);
+          O = fmaf(f, sm.o[i][cl][at], O);
         }
-        if (whole) {
-          static_cast<Act*>(a.out)[(s.row0 + col / rep) * a.out_ld + (h * rep + col % rep) * kHeadDim + dim] =
+        if (whole)
+          static_cast<Act*>(a.out)[(w.s.row0 + col / rep) * a.out_ld + (w.h * rep + col % rep) * kHeadDim + dim] =
               ActTraits<Act>::from_f(L != 0.f ? O / L * a.c.v_scale : 0.f);
-        } else {
-          d.part_o[(part + cl) * kHeadDim + dim] = O;
-        }
-        if ((!whole || d.scores) && dim == 0)
+        else
+          d.part_o[(part + cl) * kHeadDim + at] = O;
+        if ((!whole || SCORES) && at == 0)
           *reinterpret_cast<float2*>(d.part_ml + (part + cl) * 2) = make_float2(M, L);
       }
-      __syncthreads();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.merged);
     }
-    // at most the last segment of a range starts in it and goes on
-    if (fe == f1 && tid == 0 && blockIdx.y == 0)
-      d.desc[b] = fc == seg0 && fe < seg1
-                      ? make_int4(seg, range_of(total, seg1 - 1, ctas) - b + 1, s.row0, cols)
-                      : make_int4(-1, 0, 0, 0);
+    if (fe == f1) {
+      // the only segment of the range that can start in it and go on
+      if (tid == 0 && blockIdx.y == 0)
+        d.desc[b] = fc == w.seg0 && fe < w.seg1
+                        ? make_int4(w.seg, range_of(total, w.seg1 - 1, ctas) - b + 1, w.s.row0, cols)
+                        : make_int4(-1, 0, 0, 0);
+      break;
+    }
     fc = fe;
+    w = next;
   }
-  if (!ok)  // a copy did not land in time: wait (bounded) for those in flight
-    for (int i = done; i < issued; ++i)
-      mbar_wait(&sm.full[warp][i % kRing], static_cast<uint32_t>(i / kRing) & 1u, a.c.status, kStatusAttnRing);
+  if (!ok)  // a copy did not land in time: wait (bounded) for each slot's last one
+    for (int i = 0, n = (mine + U - 1) / U; i < kSlots && i < n; ++i)
+      mbar_wait(&sm.full[warp][i], static_cast<uint32_t>((n - 1 - i) / kSlots) & 1u, a.c.status,
+                kStatusAttnRing);
 }
 
 constexpr int kJoinThreads = 256, kJoinWarps = kJoinThreads / 32;
@@ -551,7 +611,8 @@ __global__ void __launch_bounds__(kJoinThreads) kv4_join_kernel(const DecodeArgs
         float v = 0.f;
 #pragma unroll
         for (int w = 0; w < kJoinWarps; ++w) v += reinterpret_cast<const float*>(red[w])[tid];
-        static_cast<Act*>(a.out)[(ds.z + col / rep) * a.out_ld + ((ds.x % H) * rep + col % rep) * kHeadDim + tid] =
+        static_cast<Act*>(a.out)[(ds.z + col / rep) * a.out_ld + ((ds.x % H) * rep + col % rep) * kHeadDim +
+                                 place_dim(tid)] =
             ActTraits<Act>::from_f(all.y != 0.f ? v / all.y * a.c.v_scale : 0.f);
       }
       __syncthreads();
@@ -678,10 +739,10 @@ cudaError_t start(K kernel, dim3 grid, int threads, size_t smem, cudaStream_t s,
 template <typename Act, int NT>
 cudaError_t launch_nt(const DecodeArgs& d, cudaStream_t s) {
   const size_t smem = sizeof(DecodeSmem<NT>);
-  cudaError_t e = cudaFuncSetAttribute(kv4_decode_kernel<Act, NT>,
-                                       cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  auto kernel = d.scores ? kv4_decode_kernel<Act, NT, true> : kv4_decode_kernel<Act, NT, false>;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
   if (e != cudaSuccess) return e;
-  e = start(kv4_decode_kernel<Act, NT>, dim3(d.ctas, d.groups), kWarpsOf<NT> * 32, smem, s, d);
+  e = start(kernel, dim3(d.ctas, d.groups), kWarpsOf<NT> * 32, smem, s, d);
   if (e != cudaSuccess) return e;
   return start(kv4_join_kernel<Act, NT>, dim3(d.ctas, d.join_y + (d.scores ? 2 : 0)), kJoinThreads, 0, s, d);
 }
