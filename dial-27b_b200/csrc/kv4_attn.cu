@@ -1,12 +1,9 @@
-// Attention over the 4-bit KV cache.
+// Attention over the 4-bit KV cache: argument checks, the choice of kernel, and
+// the running weights of many queries.
 //
 //   o = sum_j p_j v_j,  p_j = exp(s_j - m) / l,  s_j = scale * q . k_j
 //
-// over the slots j a query sees.  One CTA of 8 warps per (query, query head,
-// sequence): warp w takes slots w, w + 8, ..., four dims a lane, with a running
-// maximum and sum; the warps' parts are merged in shared memory.  With running
-// weights a second kernel forms p_j again from each query's log-sum-exp, one
-// warp per (slot, kv head, sequence), so that no two warps add to one slot.
+// over the slots j a query sees.
 #include <cmath>
 
 #include "kv4_dev.cuh"
@@ -17,54 +14,7 @@ namespace {
 constexpr int kFewCols = 64;
 
 template <typename Act>
-__global__ void __launch_bounds__(256) kv4_attn_kernel(const Kv4AttnArgs a) {
-  __shared__ float part[8][kHeadDim + 2];
-  const int j = blockIdx.x, h = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  Kv4Seq s;
-  if (!kv4_seq(a, blockIdx.z, s) || j >= s.n) return;
-  const int seen = max(0, s.len - s.n + 1 + j), kvh = h / (a.c.q_heads / a.c.kv_heads);
-  const int row = s.row0 + j;
-  float q[4], o[4] = {0.f, 0.f, 0.f, 0.f}, m = -INFINITY, l = 0.f;
-  load4(static_cast<const Act*>(a.q) + row * a.q_ld + h * kHeadDim + lane * 4, q);
-  for (int t = warp; t < seen; t += 8) {
-    const int block = max(0, kv4_block(a.c, a.c.block_table, s.sid, t / kPageTokens));
-    const uint8_t* slab = a.c.pages + kv4_slab_index(a.c, block, kvh) * kKv4Slab;
-    float k[4], v[4];
-    kv4_decode(slab, 0, kKv4KScales, t % kPageTokens, lane, a.c.k_scale, k);
-    kv4_decode(slab, kKv4VCodes, kKv4VScales, t % kPageTokens, lane, a.c.v_scale, v);
-    const float sc =
-        warp_sum(fmaf(q[0], k[0], q[1] * k[1]) + fmaf(q[2], k[2], q[3] * k[3])) * a.scale;
-    const float mn = fmaxf(m, sc);
-    const float keep = m == -INFINITY ? 0.f : expf(m - mn), p = expf(sc - mn);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] = fmaf(o[e], keep, p * v[e]);
-    l = fmaf(l, keep, p);
-    m = mn;
-  }
-#pragma unroll
-  for (int e = 0; e < 4; ++e) part[warp][lane * 4 + e] = o[e];
-  if (lane == 0) {
-    part[warp][kHeadDim] = m;
-    part[warp][kHeadDim + 1] = l;
-  }
-  __syncthreads();
-  if (threadIdx.x < kHeadDim) {
-    float M = -INFINITY, L = 0.f, O = 0.f;
-    for (int w = 0; w < 8; ++w) M = fmaxf(M, part[w][kHeadDim]);
-    for (int w = 0; w < 8; ++w) {
-      const float f = part[w][kHeadDim] == -INFINITY ? 0.f : expf(part[w][kHeadDim] - M);
-      L = fmaf(f, part[w][kHeadDim + 1], L);
-      O = fmaf(f, part[w][threadIdx.x], O);
-    }
-    static_cast<Act*>(a.out)[row * a.out_ld + h * kHeadDim + threadIdx.x] =
-        ActTraits<Act>::from_f(seen > 0 ? O / L : 0.f);
-    if (a.c.weights && threadIdx.x == 0)
-      static_cast<float*>(a.scratch)[static_cast<size_t>(row) * a.c.q_heads + h] = M + logf(L);
-  }
-}
-
-template <typename Act>
-__global__ void __launch_bounds__(256) kv4_weights_kernel(const Kv4AttnArgs a) {
+__global__ void __launch_bounds__(256) kv4_weights_kernel(const Kv4AttnArgs a, const float* lse) {
   const int t = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   const int kvh = blockIdx.y, rep = a.c.q_heads / a.c.kv_heads;
   Kv4Seq s;
@@ -81,20 +31,19 @@ __global__ void __launch_bounds__(256) kv4_weights_kernel(const Kv4AttnArgs a) {
       load4(static_cast<const Act*>(a.q) + row * a.q_ld + h * kHeadDim + lane * 4, q);
       const float sc =
           warp_sum(fmaf(q[0], k[0], q[1] * k[1]) + fmaf(q[2], k[2], q[3] * k[3])) * a.scale;
-      sum += expf(sc - static_cast<const float*>(a.scratch)[row * a.c.q_heads + h]);
+      sum += exp2f(sc * 1.4426950408889634f - lse[row * a.c.q_heads + h]);
     }
   if (lane == 0 && block >= 0) a.c.weights[si * kPageTokens + t % kPageTokens] += sum;
 }
 
-template <typename Act>
-cudaError_t launch(const Kv4AttnArgs& a, cudaStream_t s) {
-  kv4_attn_kernel<Act><<<dim3(a.max_q, a.c.q_heads, a.seqs), 256, 0, s>>>(a);
-  cudaError_t e = cudaGetLastError();
-  if (e == cudaSuccess && a.c.weights) {
-    kv4_weights_kernel<Act><<<dim3((a.max_len + 7) / 8, a.c.kv_heads, a.seqs), 256, 0, s>>>(a);
-    e = cudaGetLastError();
-  }
-  return e;
+cudaError_t launch(const Kv4AttnArgs& a, int act, cudaStream_t s) {
+  if (a.max_q * (a.c.q_heads / a.c.kv_heads) <= kFewCols) return kv4_decode_launch(a, act, s);
+  cudaError_t e = kv4_prefill_launch(a, act, s);
+  if (e != cudaSuccess || !a.c.weights) return e;
+  const dim3 grid((a.max_len + 7) / 8, a.c.kv_heads, a.seqs);
+  if (act == DIAL_ACT_BF16) kv4_weights_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(a, kv4_prefill_lse(a));
+  else kv4_weights_kernel<__half><<<grid, 256, 0, s>>>(a, kv4_prefill_lse(a));
+  return cudaGetLastError();
 }
 
 }  // namespace
@@ -111,7 +60,7 @@ extern "C" int64_t dial_b200_kv4_attention_scratch_bytes(const dial_b200_kv4_sha
   if (max_q * (sh->q_heads / sh->kv_heads) <= kFewCols)
     return static_cast<int64_t>(kv4_decode_scratch(sh->q_heads, sh->kv_heads, seqs, max_q, max_len,
                                                    with_weights != 0));
-  return with_weights ? rows * sh->q_heads * 4 : 0;
+  return static_cast<int64_t>(kv4_prefill_scratch(sh->q_heads, rows, with_weights != 0));
 }
 
 extern "C" int dial_b200_kv4_attention(const dial_b200_kv4_shape* sh, const void* q, int64_t q_ld,
@@ -163,9 +112,7 @@ extern "C" int dial_b200_kv4_attention(const dial_b200_kv4_shape* sh, const void
   a.scale = sh->softmax_scale > 0.f ? sh->softmax_scale : 1.f / sqrtf(static_cast<float>(kHeadDim));
   if ((rc = kv4_ready(&a.c, err, n)) != DIAL_OK) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const cudaError_t e = a.max_q * (sh->q_heads / sh->kv_heads) <= kFewCols
-                            ? kv4_decode_launch(a, sh->act, s)
-                        : sh->act == DIAL_ACT_BF16 ? launch<__nv_bfloat16>(a, s) : launch<__half>(a, s);
+  const cudaError_t e = launch(a, sh->act, s);
   if (e != cudaSuccess)
     return kv4_fail(err, n, DIAL_ERR_CUDA, "kv4 attention launch failed: %s", cudaGetErrorString(e));
   return DIAL_OK;

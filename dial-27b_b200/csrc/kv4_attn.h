@@ -25,4 +25,11 @@ size_t kv4_decode_scratch(int q_heads, int kv_heads, long long seqs, long long m
                           long long max_len, bool weights);
 cudaError_t kv4_decode_launch(const Kv4AttnArgs& a, int act, cudaStream_t s);
 
+// Many queries a sequence: tcgen05, 256 (query, head) rows over each key block
+// (kv4_prefill.cu).  With weights it leaves each row's log-sum-exp, base 2, in
+// scratch at kv4_prefill_lse.
+size_t kv4_prefill_scratch(int q_heads, long long rows, bool weights);
+float* kv4_prefill_lse(const Kv4AttnArgs& a);
+cudaError_t kv4_prefill_launch(const Kv4AttnArgs& a, int act, cudaStream_t s);
+
 }  // namespace dialb200

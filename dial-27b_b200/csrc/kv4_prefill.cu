@@ -1,0 +1,823 @@
+// Attention of many queries over the 4-bit KV cache on the 5th-generation
+// tensor cores (prompts, chunks of prompts).
+//
+// Tensor-bound: 4 * 128 FLOP a (query, head, slot) against 144 bytes a slot and
+// kv head, which 256 rows share.  A row is a (query, head of the group) pair, so
+// that a tile of 128 rows uses one kv head whatever the group's size, and a CTA
+// takes two tiles over the same keys.  Its 13 warps:
+//   0-3, 4-7  one row of tile 0 / 1 a thread: the row's queries into shared
+//             memory (f16 after an exact power-of-two scale), softmax, output
+//   8-11      codes -> f16 operands: registers one block ahead, e2m1 * e4m3
+//             (exact in f16), 128-byte swizzled tiles, K and V double-buffered
+//   12        tcgen05.mma: S_t = Q_t K^T into TMEM, O_t += P_t V with P from TMEM
+// P (f16) takes the upper half of its own S: the thread reads the upper 64
+// scores, then the lower 64 for the maximum alone, writes the upper half's P,
+// reads the lower half again and writes its P.  S_t of block j + 1 is issued right
+// after P V of block j, so one tile's softmax runs beside the other's MMAs.
+// The exponent's reference moves only when a score exceeds it by 2^8, so O in
+// TMEM is rarely rescaled.
+//
+// Work split: the 128-key blocks of all items (sequence, kv head, pair of tiles)
+// laid end to end, one range a CTA, cut at an item's border where one is near; the
+// parts of items that cross ranges are added by kv4_prefill_join_kernel.
+#include <cmath>
+
+#include "kv4_attn.h"
+#include "kv4_dev.cuh"
+
+namespace dialb200 {
+namespace {
+
+constexpr int kRows = 128;                  // rows of a tile
+constexpr int kKeys = 128;                  // keys of a block
+constexpr int kThreads = 13 * 32;
+constexpr int kSeqChunk = 512;              // sequences a launch
+constexpr int kTile = 128 * 128 * 2;        // f16 tile: two 64-column halves
+constexpr int kHalf = kTile / 2;
+constexpr int kOffQ = 0;                    // [2]
+constexpr int kOffK = 2 * kTile;            // [2]
+constexpr int kOffV = 4 * kTile;            // [2]
+constexpr int kOffMisc = 6 * kTile;
+constexpr float kRaise = 8.f;               // log2 headroom of a probability above 1
+constexpr int kStatusKv4Prefill = 0x601;
+
+struct Misc {
+  uint64_t kfull[2], kfree[2], vfull[2], vfree[2];  // by buffer
+  uint64_t qfull[2], sfull[2], pready[2], odone[2], fin;  // by tile
+  uint32_t tmem;
+  int failed;
+  long long cum[kSeqChunk + 1];  // blocks of one kv head of the sequences before
+  long long cut[2];
+};
+constexpr int kSmemBytes = kOffMisc + sizeof(Misc) + 1024;
+
+struct PrefillArgs {
+  Kv4AttnArgs a;
+  int ctas;
+  // [ctas]: (sequence, kv head, pair) of the item that starts in a range and
+  // goes on, or -1; and whether the item the range begins inside ends in it
+  int4* desc;
+  float* part_o;    // [2 * ctas][256][128]
+  float2* part_ml;  // [2 * ctas][256]
+  float* lse;       // [rows][q_heads], base 2; null without weights
+};
+
+// ------------------------------------------------------------ tcgen05 forms
+constexpr uint32_t idesc(bool b_mn_major) {  // f16 x f16 -> f32, M = N = 128
+  return (1u << 4) | ((b_mn_major ? 1u : 0u) << 16) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
+}
+// K-major operand: 128-byte rows, 128-byte swizzle, 8-row groups 1 KB apart.
+__device__ __forceinline__ uint64_t kmajor_desc(uint32_t saddr) {
+  return static_cast<uint64_t>((saddr >> 4) & 0x3FFFu) | (1ull << 16) | (64ull << 32) |
+         (1ull << 46) | (2ull << 61);
+}
+// MN-major operand (keys x dims, dims contiguous): 64-dim halves kHalf apart.
+__device__ __forceinline__ uint64_t mnmajor_desc(uint32_t saddr) {
+  return static_cast<uint64_t>((saddr >> 4) & 0x3FFFu) | (static_cast<uint64_t>(kHalf >> 4) << 16) |
+         (64ull << 32) | (1ull << 46) | (2ull << 61);
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t da, uint64_t db, uint32_t id, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+      "l"(da), "l"(db), "r"(id), "r"(acc));
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t ta, uint64_t db, uint32_t id, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
+      "r"(ta), "l"(db), "r"(id), "r"(acc));
+}
+__device__ __forceinline__ void commit(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
+                   smem_u32(bar))
+               : "memory");
+}
+__device__ __forceinline__ void fence_before() {
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+}
+__device__ __forceinline__ void fence_after() {
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+}
+__device__ __forceinline__ void ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+#define KV4_R32(v)                                                                              \
+  "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), \
+      "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]),  \
+      "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), \
+      "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), \
+      "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+// 32 columns of the thread's TMEM lane, without the wait.
+__device__ __forceinline__ void ld32(uint32_t taddr, uint32_t* v) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, "
+      "%12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, "
+      "%30, %31}, [%32];"
+      : KV4_R32(v)
+      : "r"(taddr));
+}
+__device__ __forceinline__ void st32(uint32_t taddr, const uint32_t* v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, "
+      "%12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, "
+      "%30, %31, %32};" ::"r"(taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
+      "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]),
+      "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]),
+      "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]),
+      "r"(v[30]), "r"(v[31]));
+}
+__device__ __forceinline__ void st16(uint32_t taddr, const uint32_t* v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, "
+      "%12, %13, %14, %15, %16};" ::"r"(taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
+      "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]));
+}
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
+  const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+// (x0, x1) * f + c, and a + b, on pairs.
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+  return static_cast<uint64_t>(__float_as_uint(lo)) | static_cast<uint64_t>(__float_as_uint(hi)) << 32;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ float lo_of(uint64_t v) { return __uint_as_float(static_cast<uint32_t>(v)); }
+__device__ __forceinline__ float hi_of(uint64_t v) { return __uint_as_float(static_cast<uint32_t>(v >> 32)); }
+
+// --------------------------------------------------------------- work items
+// Key blocks that tile T (128 rows) of the sequence sees.
+__device__ __forceinline__ int tile_blocks(const Kv4Seq& s, int rep, int T) {
+  const long long all = static_cast<long long>(s.n) * rep, r0 = static_cast<long long>(T) * kRows;
+  if (r0 >= all) return 0;
+  const long long last = (r0 + kRows - 1 < all ? r0 + kRows - 1 : all - 1) / rep;
+  const long long seen = s.len - s.n + 1 + last;
+  return seen > 0 ? static_cast<int>((seen + kKeys - 1) / kKeys) : 0;
+}
+// Blocks of the pair of tiles tp: the later tile sees the most.
+__device__ __forceinline__ int pair_blocks(const Kv4Seq& s, int rep, int tp) {
+  return max(tile_blocks(s, rep, 2 * tp), tile_blocks(s, rep, 2 * tp + 1));
+}
+__device__ __forceinline__ int pairs_of(const Kv4Seq& s, int rep) {
+  return static_cast<int>((static_cast<long long>(s.n) * rep + 2 * kRows - 1) / (2 * kRows));
+}
+
+// One item's share of a range: blocks j0 .. j1 - 1 of the item's nb.
+struct Share {
+  Kv4Seq s;
+  int i, h, tp, nb, j0, j1;
+  int blocks[2];     // of the two tiles
+  long long start;   // the item's first block among all
+};
+
+__device__ __forceinline__ long long cut_at(long long total, int b, int ctas) {
+  return total * b / ctas;
+}
+
+// The item that holds block f (f < total); warp-collective.
+__device__ Share item_at(const Kv4AttnArgs& a, const long long* cum, long long f) {
+  const int lane = threadIdx.x & 31, H = a.c.kv_heads, rep = a.c.q_heads / H;
+  int lo = 0, hi = a.seqs;  // cum[lo] * H <= f < cum[hi] * H
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (cum[mid] * H <= f) lo = mid;
+    else hi = mid;
+  }
+  Share w;
+  w.i = lo;
+  kv4_seq(a, lo, w.s);
+  const long long per = cum[lo + 1] - cum[lo];
+  long long r = f - cum[lo] * H;
+  w.h = static_cast<int>(r / per);
+  r -= w.h * per;
+  w.start = f - r;
+  w.tp = 0;
+  w.nb = 1;
+  for (int tp = 0; tp < pairs_of(w.s, rep); tp += 32) {  // the pair whose blocks hold r
+    int v = pair_blocks(w.s, rep, tp + lane);
+    const int own = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, v, o);
+      if (lane >= o) v += u;
+    }
+    const unsigned past = __ballot_sync(0xffffffffu, v > r);
+    if (past) {
+      const int at = __ffs(past) - 1;
+      w.tp = tp + at;
+      w.nb = __shfl_sync(0xffffffffu, own, at);
+      w.start += __shfl_sync(0xffffffffu, v, at) - w.nb;
+      break;
+    }
+    const int all = __shfl_sync(0xffffffffu, v, 31);
+    r -= all;
+    w.start += all;
+  }
+  return w;
+}
+
+// The share of [f, end) that begins at f in item w.
+__device__ __forceinline__ void set_share(const Kv4AttnArgs& a, Share& w, long long f, long long end) {
+  const int rep = a.c.q_heads / a.c.kv_heads;
+  w.j0 = static_cast<int>(f - w.start);
+  w.j1 = static_cast<int>(min(static_cast<long long>(w.nb), end - w.start));
+  w.blocks[0] = tile_blocks(w.s, rep, 2 * w.tp);
+  w.blocks[1] = tile_blocks(w.s, rep, 2 * w.tp + 1);
+}
+
+// The item after w, which is not the last.
+__device__ __forceinline__ void next_item(const Kv4AttnArgs& a, const long long* cum, Share& w) {
+  const int rep = a.c.q_heads / a.c.kv_heads;
+  w.start += w.nb;
+  do {
+    if (++w.tp >= pairs_of(w.s, rep)) {
+      w.tp = 0;
+      if (++w.h >= a.c.kv_heads) {
+        w.h = 0;
+        do ++w.i;
+        while (cum[w.i + 1] == cum[w.i]);
+        kv4_seq(a, w.i, w.s);
+      }
+    }
+    w.nb = pair_blocks(w.s, rep, w.tp);
+  } while (w.nb == 0);
+}
+
+__device__ void work_prefix(const Kv4AttnArgs& a, long long* cum) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  const int rep = a.c.q_heads / a.c.kv_heads;
+  for (int i = warp; i < a.seqs; i += warps) {
+    Kv4Seq s;
+    long long sum = 0;
+    if (kv4_seq(a, i, s))
+      for (int tp = lane; tp < pairs_of(s, rep); tp += 32) sum += pair_blocks(s, rep, tp);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0) cum[i + 1] = sum;
+  }
+  if (threadIdx.x == 0) cum[0] = 0;
+  __syncthreads();
+  if (warp == 0) {
+    long long carry = 0;
+    for (int i0 = 1; i0 <= a.seqs; i0 += 32) {
+      long long v = i0 + lane <= a.seqs ? cum[i0 + lane] : 0;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long u = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += u;
+      }
+      if (i0 + lane <= a.seqs) cum[i0 + lane] = v + carry;
+      carry += __shfl_sync(0xffffffffu, v, 31);
+    }
+  }
+  __syncthreads();
+}
+
+template <typename Act>
+__global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const PrefillArgs d) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~static_cast<uintptr_t>(1023));
+  Misc& sm = *reinterpret_cast<Misc*>(smem + kOffMisc);
+  const Kv4AttnArgs& a = d.a;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, b = blockIdx.x;
+  const int H = a.c.kv_heads, rep = a.c.q_heads / H;
+  if (tid == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sm.kfull[i], 4);
+      mbar_init(&sm.vfull[i], 4);
+      mbar_init(&sm.kfree[i], 1);
+      mbar_init(&sm.vfree[i], 1);
+      mbar_init(&sm.qfull[i], 4);
+      mbar_init(&sm.pready[i], 4);
+      mbar_init(&sm.sfull[i], 1);
+      mbar_init(&sm.odone[i], 1);
+    }
+    mbar_init(&sm.fin, 1);
+    sm.failed = 0;
+    fence_mbar_init();
+  }
+  if (warp == 12) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&sm.tmem)));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  pdl_wait();
+  pdl_launch_dependents();
+  work_prefix(a, sm.cum);
+  const long long total = sm.cum[a.seqs] * H;
+  // queries that see no slot: zeros
+  for (int i = b; i < a.seqs; i += d.ctas) {
+    Kv4Seq s;
+    if (!kv4_seq(a, i, s)) continue;
+    for (int r = 0; r < min(s.n, s.n - s.len); ++r) {
+      for (int e = tid * 8; e < a.c.q_heads * kHeadDim; e += kThreads * 8)
+        *reinterpret_cast<uint4*>(static_cast<Act*>(a.out) + (s.row0 + r) * a.out_ld + e) =
+            make_uint4(0, 0, 0, 0);
+      if (d.lse)
+        for (int e = tid; e < a.c.q_heads; e += kThreads)
+          d.lse[static_cast<size_t>(s.row0 + r) * a.c.q_heads + e] = INFINITY;
+    }
+  }
+  const int ctas = static_cast<int>(min(static_cast<long long>(d.ctas), total));
+  if (warp < 2 && b < ctas) {
+    // this CTA's two cuts; one within an eighth of a range of an item's border
+    // moves there
+    const int which = b + warp;
+    long long f = cut_at(total, which, ctas);
+    if (which > 0 && which < ctas) {
+      const Share w = item_at(a, sm.cum, f);
+      const long long tol = total / ctas / 8;
+      if (f - w.start <= tol) f = w.start;
+      else if (w.start + w.nb - f <= tol) f = w.start + w.nb;
+    }
+    if (lane == 0) sm.cut[warp] = f;
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = sm.tmem;
+  const long long f0 = b < ctas ? sm.cut[0] : 0, f1 = b < ctas ? sm.cut[1] : 0;
+  auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
+    if (mbar_try_wait(bar, parity)) return true;
+    if (*reinterpret_cast<volatile int*>(&sm.failed)) return false;
+    if (mbar_wait(bar, parity, a.c.status, kStatusKv4Prefill)) return true;
+    *reinterpret_cast<volatile int*>(&sm.failed) = 1;
+    return false;
+  };
+
+  if (f0 >= f1) {
+    if (tid == 0) d.desc[b] = make_int4(-1, 0, 0, -1);
+  } else if (warp < 8) {
+    // ------------------------------------------- queries, softmax and output
+    const int t = warp >> 2, quarter = warp & 3, r = quarter * 32 + lane;
+    const uint32_t lane_off = static_cast<uint32_t>(32 * quarter) << 16;
+    const uint32_t tS = tmem + t * 128 + lane_off, tO = tmem + 256 + t * 128 + lane_off;
+    uint8_t* q_row = smem + kOffQ + t * kTile + (r >> 3) * 1024 + (r & 7) * 128;
+    uint32_t sphase = 0, ophase = 0;
+    Share w = item_at(a, sm.cum, f0);
+    bool ok = true;
+    int first = -1;  // the item the range begins inside: 1 if it ends in the range, 0 if not
+    for (long long f = f0;;) {
+      set_share(a, w, f, f1);
+      if (f == f0) first = w.j0 == 0 ? -1 : w.j1 == w.nb;
+      const long long R = (static_cast<long long>(w.tp) * 2 + t) * kRows + r;
+      const bool live = R < static_cast<long long>(w.s.n) * rep;
+      const int j = live ? static_cast<int>(R / rep) : 0, head = w.h * rep + (live ? static_cast<int>(R % rep) : 0);
+      const int seen = live ? max(0, w.s.len - w.s.n + 1 + j) : 0;
+      const int last = min(w.j1, w.blocks[t]);
+      float m = -INFINITY, ref = 0.f, fac = 0.f;
+      uint64_t l2 = 0;
+      if (w.j0 < last) {
+        // the row's queries: f16 after 2^-e of its largest exponent
+        float top = 0.f;
+        const uint4* src = reinterpret_cast<const uint4*>(static_cast<const Act*>(a.q) + (w.s.row0 + j) * a.q_ld +
+                                                          head * kHeadDim);
+        if (live)
+#pragma unroll 4
+          for (int e = 0; e < 16; ++e) {
+            const uint4 raw = src[e];
+            const Act* v = reinterpret_cast<const Act*>(&raw);
+#pragma unroll
+            for (int u = 0; u < 8; ++u) top = fmaxf(top, fabsf(ActTraits<Act>::to_f(v[u])));
+          }
+        const int ex = min(max(static_cast<int>(__float_as_uint(top) >> 23) - 127, -100), 100);
+        const float down = exp2i(-ex);
+        fac = exp2i(ex) * a.scale * a.c.k_scale * 1.4426950408889634f;
+#pragma unroll 4
+        for (int e = 0; e < 16; ++e) {
+          const uint4 raw = live ? src[e] : make_uint4(0, 0, 0, 0);
+          const Act* v = reinterpret_cast<const Act*>(&raw);
+          uint32_t o[4];
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+            o[u] = pack_f16(ActTraits<Act>::to_f(v[2 * u]) * down, ActTraits<Act>::to_f(v[2 * u + 1]) * down);
+          *reinterpret_cast<uint4*>(q_row + (e >> 3) * kHalf + (((e & 7) ^ (r & 7)) << 4)) =
+              make_uint4(o[0], o[1], o[2], o[3]);
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.qfull[t]);
+      }
+      const uint64_t fac2 = pair(fac, fac);
+      for (int kb = w.j0; kb < last; ++kb) {
+        ok = __all_sync(0xffffffffu, ok && wait(&sm.sfull[t], sphase & 1u));
+        if (!ok) break;
+        ++sphase;
+        fence_after();
+        uint32_t v[64];
+        ld32(tS, v);
+        ld32(tS + 32, v + 32);
+        ld_wait();
+        // slots of the block that the row sees; a warp's rows share most blocks whole
+        const int open = seen - kb * kKeys;
+        const bool border = __any_sync(0xffffffffu, open < kKeys);
+        float top = -INFINITY;
+        if (border) {
+#pragma unroll
+          for (int e = 0; e < 64; ++e)
+            if (e < open) top = fmaxf(top, __uint_as_float(v[e]));
+        } else {
+#pragma unroll
+          for (int e = 0; e < 64; ++e) top = fmaxf(top, __uint_as_float(v[e]));
+        }
+        __syncwarp();  // tcgen05.ld and .st are warp-collective
+        ld32(tS + 64, v);
+        ld32(tS + 96, v + 32);
+        ld_wait();
+        if (border) {
+#pragma unroll
+          for (int e = 0; e < 64; ++e) {
+            if (e + 64 >= open) v[e] = 0xFF800000u;  // -inf
+            top = fmaxf(top, __uint_as_float(v[e]));
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 64; ++e) top = fmaxf(top, __uint_as_float(v[e]));
+        }
+        top *= fac;
+        if (__any_sync(0xffffffffu, top > m + kRaise)) {
+          const float mn = fmaxf(m, top);
+          const float al = m == -INFINITY ? 0.f : ex2(m - mn);
+          m = mn;
+          ref = mn == -INFINITY ? 0.f : mn;
+          l2 = pair(lo_of(l2) * al, hi_of(l2) * al);
+          if (kb > w.j0) {  // S of this block was issued after P V of the one before
+#pragma unroll
+            for (int cb = 0; cb < 4; ++cb) {
+              uint32_t o[32];
+              ld32(tO + cb * 32, o);
+              ld_wait();
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * al);
+              st32(tO + cb * 32, o);
+            }
+          }
+        }
+        __syncwarp();
+        const uint64_t off2 = pair(-ref, -ref);
+        auto probs = [&](uint32_t to) {  // v: 64 scores -> 32 columns of P
+#pragma unroll
+          for (int hf = 0; hf < 2; ++hf) {
+            uint32_t p[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              const int i = 32 * hf + 2 * e;
+              const uint64_t x = fma2(pair(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), fac2, off2);
+              const float p0 = ex2(lo_of(x)), p1 = ex2(hi_of(x));
+              l2 = add2(l2, pair(p0, p1));
+              p[e] = pack_f16(p0, p1);
+            }
+            st16(to + 16 * hf, p);
+          }
+        };
+        probs(tS + 96);  // keys 64 .. 127
+        ld32(tS, v);
+        ld32(tS + 32, v + 32);
+        ld_wait();
+        if (border) {
+#pragma unroll
+          for (int e = 0; e < 64; ++e)
+            if (e >= open) v[e] = 0xFF800000u;
+        }
+        __syncwarp();
+        probs(tS + 64);  // keys 0 .. 63
+        st_wait();
+        fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.pready[t]);
+      }
+      // ------------------------------------------------------------ output
+      const bool whole = w.j0 == 0 && w.j1 == w.nb;
+      const int slot = 2 * b + (w.j0 == 0 ? 1 : 0);
+      const float l = lo_of(l2) + hi_of(l2);
+      if (ok && w.j0 < last) {
+        ok = __all_sync(0xffffffffu, wait(&sm.odone[t], ophase & 1u));
+        ++ophase;
+        if (ok) {
+          fence_after();
+          const float inv = l != 0.f ? a.c.v_scale / l : 0.f;
+          Act* dst = static_cast<Act*>(a.out) + (w.s.row0 + j) * a.out_ld + head * kHeadDim;
+          float* part = d.part_o + (static_cast<size_t>(slot) * 2 * kRows + t * kRows + r) * kHeadDim;
+#pragma unroll
+          for (int cb = 0; cb < 4; ++cb) {
+            uint32_t o[32];
+            ld32(tO + cb * 32, o);
+            ld_wait();
+            if (live && whole) {
+              uint4 out[4];
+              Act* h = reinterpret_cast<Act*>(out);
+#pragma unroll
+              for (int e = 0; e < 32; ++e)
+                h[e] = ActTraits<Act>::from_f(l != 0.f ? __uint_as_float(o[e]) * inv : 0.f);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) reinterpret_cast<uint4*>(dst + cb * 32)[e] = out[e];
+            } else if (live) {
+#pragma unroll
+              for (int e = 0; e < 8; ++e)
+                reinterpret_cast<uint4*>(part + cb * 32)[e] =
+                    make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+            }
+            __syncwarp();
+          }
+          fence_before();
+        }
+      }
+      if (live) {
+        if (!whole)
+          d.part_ml[static_cast<size_t>(slot) * 2 * kRows + t * kRows + r] = make_float2(l > 0.f || l != l ? m : -INFINITY, l);
+        else if (d.lse)
+          d.lse[static_cast<size_t>(w.s.row0 + j) * a.c.q_heads + head] = l > 0.f ? m + log2f(l) : INFINITY;
+      }
+      f = w.start + w.j1;
+      if (f >= f1 || !ok) {
+        // the only item of the range that can start in it and go on
+        if (tid == 0)
+          d.desc[b] = w.j0 == 0 && w.j1 < w.nb ? make_int4(w.i, w.h, w.tp, first) : make_int4(-1, 0, 0, first);
+        break;
+      }
+      next_item(a, sm.cum, w);
+    }
+  } else if (warp < 12) {
+    // ------------------------------------------------- codes to f16 operands
+    // 4 lanes a token: lane q of a token holds dims 32q .. 32q + 31 (two scale
+    // groups); a warp's load covers 8 tokens, 4 loads a warp and block
+    const int dw = warp - 8, q = lane & 3, tok = lane >> 2;
+    const bool swap = (q & 2) != 0;
+    uint4 kc[4], vc[4];
+    uint32_t ks[4], vs[4];
+    Share w = item_at(a, sm.cum, f0);
+    set_share(a, w, f0, f1);
+    auto load = [&](int kb) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int key = kb * kKeys + dw * 32 + e * 8 + tok;
+        const bool there = key < w.s.len;
+        const int block = there ? max(0, kv4_block(a.c, a.c.block_table, w.s.sid, key / kPageTokens)) : 0;
+        const uint8_t* slab = a.c.pages + kv4_slab_index(a.c, block, w.h) * kKv4Slab;
+        const int tt = key % kPageTokens;
+        kc[e] = *reinterpret_cast<const uint4*>(slab + tt * 64 + q * 16);
+        vc[e] = *reinterpret_cast<const uint4*>(slab + kKv4VCodes + tt * 64 + q * 16);
+        // slots past the end may hold anything: scale 0
+        ks[e] = there ? *reinterpret_cast<const uint16_t*>(slab + kKv4KScales + tt * 8 + q * 2) : 0u;
+        vs[e] = there ? *reinterpret_cast<const uint16_t*>(slab + kKv4VScales + tt * 8 + q * 2) : 0u;
+      }
+    };
+    auto store = [&](uint8_t* tile, const uint4 (&c)[4], const uint32_t (&s)[4]) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int row = dw * 32 + e * 8 + tok;
+        const uint32_t sc = e4m3x2_to_f16x2(static_cast<uint16_t>(s[e]));
+        const uint32_t first = __byte_perm(sc, 0, swap ? 0x3232 : 0x1010);
+        const uint32_t second = __byte_perm(sc, 0, swap ? 0x1010 : 0x3232);
+        uint8_t* to = tile + (q >> 1) * kHalf + row * 128;
+        // lanes of the upper half take their words two on: no two lanes of a
+        // quarter warp meet in a bank
+        const uint32_t words[4] = {swap ? c[e].z : c[e].x, swap ? c[e].w : c[e].y,
+                                   swap ? c[e].x : c[e].z, swap ? c[e].y : c[e].w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          uint32_t o[4];
+          e2m1x8_to_f16x2x4(words[i], o);
+          const uint32_t sx = i < 2 ? first : second;
+          const int chunk = (q & 1) * 4 + (swap ? i ^ 2 : i);
+          *reinterpret_cast<uint4*>(to + ((chunk ^ (row & 7)) << 4)) =
+              make_uint4(hmul2(o[0], sx), hmul2(o[1], sx), hmul2(o[2], sx), hmul2(o[3], sx));
+        }
+      }
+    };
+    load(w.j0);
+    uint32_t n = 0;
+    for (long long f = f0;; ) {
+      for (int kb = w.j0; kb < w.j1; ++kb, ++n) {
+        const int buf = n & 1;
+        const uint32_t turn = (n >> 1) & 1u;
+        if (!__all_sync(0xffffffffu, wait(&sm.kfree[buf], turn ^ 1u))) goto done;
+        store(smem + kOffK + buf * kTile, kc, ks);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.kfull[buf]);
+        if (!__all_sync(0xffffffffu, wait(&sm.vfree[buf], turn ^ 1u))) goto done;
+        store(smem + kOffV + buf * kTile, vc, vs);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.vfull[buf]);
+        if (kb + 1 < w.j1) load(kb + 1);
+      }
+      f = w.start + w.j1;
+      if (f >= f1) break;
+      next_item(a, sm.cum, w);
+      set_share(a, w, f, f1);
+      load(w.j0);
+    }
+  done:;
+  } else {
+    // ------------------------------------------------------------------ MMA
+    Share w = item_at(a, sm.cum, f0);
+    const uint32_t sq = smem_u32(smem + kOffQ), sk = smem_u32(smem + kOffK), sv = smem_u32(smem + kOffV);
+    uint32_t n = 0, qphase[2] = {0, 0}, pphase[2] = {0, 0};
+    bool ok = true;
+    for (long long f = f0; ok;) {
+      set_share(a, w, f, f1);
+      if (lane == 0) {
+        auto issue_s = [&](int t, uint32_t kb_n) {
+          const uint32_t k0 = sk + (kb_n & 1) * kTile, q0 = sq + t * kTile;
+#pragma unroll
+          for (int i = 0; i < kHeadDim / 16; ++i) {
+            const uint32_t off = (i >> 2) * kHalf + (i & 3) * 32;
+            mma_ss(tmem + t * 128, kmajor_desc(q0 + off), kmajor_desc(k0 + off), idesc(false), i > 0 ? 1u : 0u);
+          }
+          commit(&sm.sfull[t]);
+        };
+        const int last[2] = {min(w.j1, w.blocks[0]), min(w.j1, w.blocks[1])};
+        for (int t = 0; t < 2; ++t)
+          if (w.j0 < last[t]) ok = ok && wait(&sm.qfull[t], qphase[t]++ & 1u);
+        ok = ok && wait(&sm.kfull[n & 1], (n >> 1) & 1u);
+        if (ok) {
+          fence_after();
+          for (int t = 0; t < 2; ++t)
+            if (w.j0 < last[t]) issue_s(t, n);
+          commit(&sm.kfree[n & 1]);
+        }
+        for (int kb = w.j0; kb < w.j1 && ok; ++kb, ++n) {
+          ok = wait(&sm.vfull[n & 1], (n >> 1) & 1u);
+          const bool more = kb + 1 < w.j1;
+          for (int t = 0; t < 2 && ok; ++t) {
+            if (kb < last[t]) {
+              ok = wait(&sm.pready[t], pphase[t]++ & 1u);
+              if (!ok) break;
+              fence_after();
+              const uint32_t v0 = sv + (n & 1) * kTile;
+#pragma unroll
+              for (int i = 0; i < kKeys / 16; ++i)
+                mma_ts(tmem + 256 + t * 128, tmem + t * 128 + 64 + i * 8, mnmajor_desc(v0 + i * 2048), idesc(true),
+                       (kb > w.j0 || i > 0) ? 1u : 0u);
+              if (kb + 1 == last[t]) commit(&sm.odone[t]);
+            }
+            if (kb + 1 < last[t]) {
+              ok = wait(&sm.kfull[(n + 1) & 1], ((n + 1) >> 1) & 1u);
+              if (!ok) break;
+              fence_after();
+              issue_s(t, n + 1);
+            }
+          }
+          if (ok) {
+            commit(&sm.vfree[n & 1]);
+            if (more) commit(&sm.kfree[(n + 1) & 1]);
+          }
+        }
+      }
+      ok = __all_sync(0xffffffffu, ok);
+      f = w.start + w.j1;
+      if (f >= f1) break;
+      next_item(a, sm.cum, w);
+    }
+    if (lane == 0) {
+      commit(&sm.fin);  // nothing may still write TMEM when it is freed
+      mbar_wait(&sm.fin, 0, a.c.status, kStatusKv4Prefill);
+    }
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  if (warp == 12)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+}
+
+// Adds the parts of the item that starts in range blockIdx.x and goes on in
+// others: one warp a row, parts in order.
+template <typename Act>
+__global__ void __launch_bounds__(256) kv4_prefill_join_kernel(const PrefillArgs d) {
+  const Kv4AttnArgs& a = d.a;
+  const int b = blockIdx.x, lane = threadIdx.x & 31, row = blockIdx.y * 8 + (threadIdx.x >> 5);
+  const int rep = a.c.q_heads / a.c.kv_heads;
+  pdl_wait();
+  const int4 it = d.desc[b];
+  if (it.x < 0) return;
+  Kv4Seq s;
+  kv4_seq(a, it.x, s);
+  const long long R = static_cast<long long>(it.z) * 2 * kRows + row;
+  if (R >= static_cast<long long>(s.n) * rep) return;
+  // the ranges after this one that go on with the item, up to the one it ends in
+  int parts = 1;
+  for (;; parts += 32) {
+    const bool end = b + parts + lane >= d.ctas || d.desc[b + parts + lane].w != 0;
+    const unsigned ends = __ballot_sync(0xffffffffu, end);
+    if (ends) {
+      parts += __ffs(ends);
+      break;
+    }
+  }
+  float M = -INFINITY, L = 0.f;
+  float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
+  auto slot = [&](int p) { return static_cast<size_t>(p == 0 ? 2 * b + 1 : 2 * (b + p)) * 2 * kRows + row; };
+  for (int p = 0; p < parts; ++p) M = fmaxf(M, d.part_ml[slot(p)].x);
+  for (int p = 0; p < parts; ++p) {
+    const float2 ml = d.part_ml[slot(p)];
+    if (ml.x == -INFINITY) continue;
+    const float f = ex2(ml.x - M);
+    const float4 v = reinterpret_cast<const float4*>(d.part_o)[slot(p) * (kHeadDim / 4) + lane];
+    L = fmaf(f, ml.y, L);
+    O.x = fmaf(f, v.x, O.x);
+    O.y = fmaf(f, v.y, O.y);
+    O.z = fmaf(f, v.z, O.z);
+    O.w = fmaf(f, v.w, O.w);
+  }
+  const int j = static_cast<int>(R / rep), head = it.y * rep + static_cast<int>(R % rep);
+  const float inv = L != 0.f ? a.c.v_scale / L : 0.f;
+  const float o[4] = {O.x * inv, O.y * inv, O.z * inv, O.w * inv};
+  store4(static_cast<Act*>(a.out) + (s.row0 + j) * a.out_ld + head * kHeadDim + lane * 4, o);
+  if (d.lse && lane == 0)
+    d.lse[static_cast<size_t>(s.row0 + j) * a.c.q_heads + head] = L > 0.f ? M + log2f(L) : INFINITY;
+}
+
+int range_count() {
+  static int n = [] {
+    int v = 0, dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess ||
+        cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || v < 1 || v > 148)
+      v = 148;
+    return v;
+  }();
+  return n;
+}
+
+constexpr size_t kDescBytes = 148 * 16 + 128 - (148 * 16) % 128;
+constexpr size_t kPartBytes = 2ull * 148 * 2 * kRows * kHeadDim * 4;
+constexpr size_t kMlBytes = 2ull * 148 * 2 * kRows * 8;
+
+template <typename K>
+cudaError_t start(K kernel, dim3 grid, int threads, size_t smem, cudaStream_t s, const PrefillArgs& d) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, d);
+}
+
+template <typename Act>
+cudaError_t launch(const PrefillArgs& d, cudaStream_t s) {
+  cudaError_t e = cudaFuncSetAttribute(kv4_prefill_kernel<Act>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+  if (e != cudaSuccess) return e;
+  e = start(kv4_prefill_kernel<Act>, dim3(d.ctas), kThreads, kSmemBytes, s, d);
+  if (e != cudaSuccess) return e;
+  return start(kv4_prefill_join_kernel<Act>, dim3(d.ctas, 2 * kRows / 8), 256, 0, s, d);
+}
+
+}  // namespace
+
+size_t kv4_prefill_scratch(int q_heads, long long rows, bool weights) {
+  return kDescBytes + kPartBytes + kMlBytes + (weights ? static_cast<size_t>(rows) * q_heads * 4 : 0);
+}
+
+float* kv4_prefill_lse(const Kv4AttnArgs& a) {
+  return reinterpret_cast<float*>(static_cast<uint8_t*>(a.scratch) + kDescBytes + kPartBytes + kMlBytes);
+}
+
+cudaError_t kv4_prefill_launch(const Kv4AttnArgs& a, int act, cudaStream_t s) {
+  for (int at = 0; at < a.seqs; at += kSeqChunk) {
+    PrefillArgs d{};
+    d.a = a;
+    d.a.seqs = a.seqs - at < kSeqChunk ? a.seqs - at : kSeqChunk;
+    d.a.sids = a.sids + at;
+    d.a.lens = a.lens + at;
+    if (a.q_starts) d.a.q_starts = a.q_starts + at;
+    d.ctas = range_count();
+    uint8_t* w = static_cast<uint8_t*>(a.scratch);
+    d.desc = reinterpret_cast<int4*>(w);
+    d.part_o = reinterpret_cast<float*>(w + kDescBytes);
+    d.part_ml = reinterpret_cast<float2*>(w + kDescBytes + kPartBytes);
+    d.lse = a.c.weights ? kv4_prefill_lse(a) : nullptr;
+    const cudaError_t e = act == DIAL_ACT_BF16 ? launch<__nv_bfloat16>(d, s) : launch<__half>(d, s);
+    if (e != cudaSuccess) return e;
+  }
+  return cudaSuccess;
+}
+
+}  // namespace dialb200
