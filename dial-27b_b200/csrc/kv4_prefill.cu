@@ -18,8 +18,9 @@
 // TMEM is rarely rescaled.
 //
 // Work split: the 128-key blocks of all items (sequence, kv head, pair of tiles)
-// laid end to end, one range a CTA, cut at an item's border where one is near; the
-// parts of items that cross ranges are added by kv4_prefill_join_kernel.
+// laid end to end, one range a CTA, an item counted as kPad blocks more for its
+// start and output; the parts of items that cross ranges are added by
+// kv4_prefill_join_kernel.
 #include <cmath>
 
 #include "kv4_attn.h"
@@ -31,6 +32,7 @@ namespace {
 constexpr int kRows = 128;                  // rows of a tile
 constexpr int kKeys = 128;                  // keys of a block
 constexpr int kThreads = 13 * 32;
+constexpr int kPad = 2;                     // an item's own cost, in blocks
 constexpr int kSeqChunk = 512;              // sequences a launch
 constexpr int kTile = 128 * 128 * 2;        // f16 tile: two 64-column halves
 constexpr int kHalf = kTile / 2;
@@ -46,8 +48,9 @@ struct Misc {
   uint64_t qfull[2], sfull[2], pready[2], odone[2], fin;  // by tile
   uint32_t tmem;
   int failed;
-  long long cum[kSeqChunk + 1];  // blocks of one kv head of the sequences before
+  long long cum[kSeqChunk + 1];  // cost of one kv head of the sequences before
   long long cut[2];
+  alignas(16) unsigned char share[8][2][96];  // of the softmax warps: this item and the next
 };
 constexpr int kSmemBytes = kOffMisc + sizeof(Misc) + 1024;
 
@@ -99,7 +102,28 @@ __device__ __forceinline__ void fence_before() {
 __device__ __forceinline__ void fence_after() {
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 }
-__device__ __forceinline__ void ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// The wait for the tcgen05.ld before it; naming the registers keeps their uses
+// behind it.
+#define KV4_RW32(v)                                                                              \
+  "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), \
+      "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]),   \
+      "+r"(v[15]), "+r"(v[16]), "+r"(v[17]), "+r"(v[18]), "+r"(v[19]), "+r"(v[20]), "+r"(v[21]),  \
+      "+r"(v[22]), "+r"(v[23]), "+r"(v[24]), "+r"(v[25]), "+r"(v[26]), "+r"(v[27]), "+r"(v[28]),  \
+      "+r"(v[29]), "+r"(v[30]), "+r"(v[31])
+__device__ __forceinline__ void ld_wait(uint32_t* v) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" : KV4_RW32(v)::"memory");
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ void cp_async16(void* dst, const void* src, bool there) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src),
+               "r"(there ? 16 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 __device__ __forceinline__ void st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 #define KV4_R32(v)                                                                              \
@@ -117,16 +141,16 @@ __device__ __forceinline__ void ld32(uint32_t taddr, uint32_t* v) {
       : KV4_R32(v)
       : "r"(taddr));
 }
-__device__ __forceinline__ void st32(uint32_t taddr, const uint32_t* v) {
+// 16 columns, waited for.
+__device__ __forceinline__ void ld16(uint32_t taddr, uint32_t* v) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, "
-      "%12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, "
-      "%30, %31, %32};" ::"r"(taddr),
-      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
-      "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]),
-      "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]),
-      "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]),
-      "r"(v[30]), "r"(v[31]));
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, "
+      "%12, %13, %14, %15}, [%16];\n\ttcgen05.wait::ld.sync.aligned;"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]),
+        "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]),
+        "=r"(v[14]), "=r"(v[15])
+      : "r"(taddr)
+      : "memory");
 }
 __device__ __forceinline__ void st16(uint32_t taddr, const uint32_t* v) {
   asm volatile(
@@ -167,21 +191,24 @@ __device__ __forceinline__ float lo_of(uint64_t v) { return __uint_as_float(stat
 __device__ __forceinline__ float hi_of(uint64_t v) { return __uint_as_float(static_cast<uint32_t>(v >> 32)); }
 
 // --------------------------------------------------------------- work items
-// Key blocks that tile T (128 rows) of the sequence sees.
-__device__ __forceinline__ int tile_blocks(const Kv4Seq& s, int rep, int T) {
-  const long long all = static_cast<long long>(s.n) * rep, r0 = static_cast<long long>(T) * kRows;
+// Key blocks that tile T (128 rows) of the sequence sees.  n * rep < 2^29.
+__device__ __forceinline__ int tile_blocks(const Kv4Seq& s, unsigned rep, int T) {
+  const int all = s.n * static_cast<int>(rep), r0 = T * kRows;
   if (r0 >= all) return 0;
-  const long long last = (r0 + kRows - 1 < all ? r0 + kRows - 1 : all - 1) / rep;
-  const long long seen = s.len - s.n + 1 + last;
-  return seen > 0 ? static_cast<int>((seen + kKeys - 1) / kKeys) : 0;
+  const int last = static_cast<int>(static_cast<unsigned>(min(r0 + kRows, all) - 1) / rep);
+  const int seen = s.len - s.n + 1 + last;
+  return seen > 0 ? (seen + kKeys - 1) / kKeys : 0;
 }
-// Blocks of the pair of tiles tp: the later tile sees the most.
-__device__ __forceinline__ int pair_blocks(const Kv4Seq& s, int rep, int tp) {
-  return max(tile_blocks(s, rep, 2 * tp), tile_blocks(s, rep, 2 * tp + 1));
+// Blocks of the pair of tiles tp: its last row sees the most.
+__device__ __forceinline__ int pair_blocks(const Kv4Seq& s, unsigned rep, int tp) {
+  const int t1 = 2 * tp + 1;
+  return tile_blocks(s, rep, t1 * kRows < s.n * static_cast<int>(rep) ? t1 : t1 - 1);
 }
 __device__ __forceinline__ int pairs_of(const Kv4Seq& s, int rep) {
-  return static_cast<int>((static_cast<long long>(s.n) * rep + 2 * kRows - 1) / (2 * kRows));
+  return (s.n * rep + 2 * kRows - 1) / (2 * kRows);
 }
+// An item's length in the order of work.
+__device__ __forceinline__ int item_cost(int blocks) { return blocks > 0 ? blocks + kPad : 0; }
 
 // One item's share of a range: blocks j0 .. j1 - 1 of the item's nb.
 struct Share {
@@ -191,11 +218,7 @@ struct Share {
   long long start;   // the item's first block among all
 };
 
-__device__ __forceinline__ long long cut_at(long long total, int b, int ctas) {
-  return total * b / ctas;
-}
-
-// The item that holds block f (f < total); warp-collective.
+// The item that holds place f of the order of work (f < total); warp-collective.
 __device__ Share item_at(const Kv4AttnArgs& a, const long long* cum, long long f) {
   const int lane = threadIdx.x & 31, H = a.c.kv_heads, rep = a.c.q_heads / H;
   int lo = 0, hi = a.seqs;  // cum[lo] * H <= f < cum[hi] * H
@@ -215,8 +238,8 @@ __device__ Share item_at(const Kv4AttnArgs& a, const long long* cum, long long f
   w.tp = 0;
   w.nb = 1;
   for (int tp = 0; tp < pairs_of(w.s, rep); tp += 32) {  // the pair whose blocks hold r
-    int v = pair_blocks(w.s, rep, tp + lane);
-    const int own = v;
+    const int own = pair_blocks(w.s, rep, tp + lane);
+    int v = item_cost(own);
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int u = __shfl_up_sync(0xffffffffu, v, o);
@@ -227,7 +250,7 @@ __device__ Share item_at(const Kv4AttnArgs& a, const long long* cum, long long f
       const int at = __ffs(past) - 1;
       w.tp = tp + at;
       w.nb = __shfl_sync(0xffffffffu, own, at);
-      w.start += __shfl_sync(0xffffffffu, v, at) - w.nb;
+      w.start += __shfl_sync(0xffffffffu, v, at) - item_cost(w.nb);
       break;
     }
     const int all = __shfl_sync(0xffffffffu, v, 31);
@@ -240,8 +263,8 @@ __device__ Share item_at(const Kv4AttnArgs& a, const long long* cum, long long f
 // The share of [f, end) that begins at f in item w.
 __device__ __forceinline__ void set_share(const Kv4AttnArgs& a, Share& w, long long f, long long end) {
   const int rep = a.c.q_heads / a.c.kv_heads;
-  w.j0 = static_cast<int>(f - w.start);
-  w.j1 = static_cast<int>(min(static_cast<long long>(w.nb), end - w.start));
+  w.j0 = max(0, static_cast<int>(f - w.start) - kPad);
+  w.j1 = static_cast<int>(min(static_cast<long long>(w.nb), end - w.start - kPad));
   w.blocks[0] = tile_blocks(w.s, rep, 2 * w.tp);
   w.blocks[1] = tile_blocks(w.s, rep, 2 * w.tp + 1);
 }
@@ -249,7 +272,7 @@ __device__ __forceinline__ void set_share(const Kv4AttnArgs& a, Share& w, long l
 // The item after w, which is not the last.
 __device__ __forceinline__ void next_item(const Kv4AttnArgs& a, const long long* cum, Share& w) {
   const int rep = a.c.q_heads / a.c.kv_heads;
-  w.start += w.nb;
+  w.start += item_cost(w.nb);
   do {
     if (++w.tp >= pairs_of(w.s, rep)) {
       w.tp = 0;
@@ -271,7 +294,7 @@ __device__ void work_prefix(const Kv4AttnArgs& a, long long* cum) {
     Kv4Seq s;
     long long sum = 0;
     if (kv4_seq(a, i, s))
-      for (int tp = lane; tp < pairs_of(s, rep); tp += 32) sum += pair_blocks(s, rep, tp);
+      for (int tp = lane; tp < pairs_of(s, rep); tp += 32) sum += item_cost(pair_blocks(s, rep, tp));
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (lane == 0) cum[i + 1] = sum;
@@ -341,15 +364,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const PrefillA
   }
   const int ctas = static_cast<int>(min(static_cast<long long>(d.ctas), total));
   if (warp < 2 && b < ctas) {
-    // this CTA's two cuts; one within an eighth of a range of an item's border
-    // moves there
-    const int which = b + warp;
-    long long f = cut_at(total, which, ctas);
-    if (which > 0 && which < ctas) {
+    // this CTA's two cuts, none before an item's first block
+    long long f = total * (b + warp) / ctas;
+    if (f < total) {
       const Share w = item_at(a, sm.cum, f);
-      const long long tol = total / ctas / 8;
-      if (f - w.start <= tol) f = w.start;
-      else if (w.start + w.nb - f <= tol) f = w.start + w.nb;
+      if (f - w.start <= kPad) f = w.start;
     }
     if (lane == 0) sm.cut[warp] = f;
   }
@@ -373,54 +392,89 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const PrefillA
     const int t = warp >> 2, quarter = warp & 3, r = quarter * 32 + lane;
     const uint32_t lane_off = static_cast<uint32_t>(32 * quarter) << 16;
     const uint32_t tS = tmem + t * 128 + lane_off, tO = tmem + 256 + t * 128 + lane_off;
-    uint8_t* q_row = smem + kOffQ + t * kTile + (r >> 3) * 1024 + (r & 7) * 128;
+    uint8_t* q_tile = smem + kOffQ + t * kTile;
+    uint8_t* q_row = q_tile + r * 128;
     uint32_t sphase = 0, ophase = 0;
-    Share w = item_at(a, sm.cum, f0);
-    bool ok = true;
-    int first = -1;  // the item the range begins inside: 1 if it ends in the range, 0 if not
-    for (long long f = f0;;) {
+    // kept in shared memory: registers are for the scores
+    static_assert(sizeof(Share) <= sizeof(sm.share[0][0]), "a share's place");
+    Share* cur = reinterpret_cast<Share*>(sm.share[warp][0]);
+    Share* next = reinterpret_cast<Share*>(sm.share[warp][1]);
+    {
+      Share w = item_at(a, sm.cum, f0);
+      set_share(a, w, f0, f1);
+      if (lane == 0) *cur = w;
+      __syncwarp();
+    }
+    auto find_next = [&](long long f) {
+      Share w = *cur;
+      next_item(a, sm.cum, w);
       set_share(a, w, f, f1);
-      if (f == f0) first = w.j0 == 0 ? -1 : w.j1 == w.nb;
-      const long long R = (static_cast<long long>(w.tp) * 2 + t) * kRows + r;
-      const bool live = R < static_cast<long long>(w.s.n) * rep;
-      const int j = live ? static_cast<int>(R / rep) : 0, head = w.h * rep + (live ? static_cast<int>(R % rep) : 0);
+      if (lane == 0) *next = w;
+      __syncwarp();
+    };
+    bool ok = true, fetched = false;
+    // whether the item the range begins inside ends in it (1) or not (0)
+    const int first = cur->j0 == 0 ? -1 : cur->j1 == cur->nb;
+    // the warp's 32 rows of the tile's queries, raw, where their f16 form will be
+    auto fetch_q = [&](const Share& x) {
+      const int R = (2 * x.tp + t) * kRows + r;
+      const bool mine = R < x.s.n * rep;
+      const int j = mine ? R / rep : 0;
+      long long at = (x.s.row0 + j) * a.q_ld + (x.h * rep + (mine ? R - j * rep : 0)) * kHeadDim;
+      if (!mine) at = -1;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int row = 2 * e + (lane >> 4), c = lane & 15;
+        const long long from = __shfl_sync(0xffffffffu, at, row);
+        cp_async16(q_tile + (c >> 3) * kHalf + (quarter * 32 + row) * 128 + (((c & 7) ^ (row & 7)) << 4),
+                   static_cast<const Act*>(a.q) + (from < 0 ? 0 : from) + c * 8, from >= 0);
+      }
+    };
+    for (;;) {
+      const Share& w = *cur;
+      const int R = (2 * w.tp + t) * kRows + r;
+      const bool live = R < w.s.n * rep;
+      const int j = live ? R / rep : 0, head = w.h * rep + (live ? R - j * rep : 0);
       const int seen = live ? max(0, w.s.len - w.s.n + 1 + j) : 0;
-      const int last = min(w.j1, w.blocks[t]);
+      const int begin = w.j0, last = min(w.j1, w.blocks[t]);
+      const long long f = w.start + kPad + w.j1;
       float m = -INFINITY, ref = 0.f, fac = 0.f;
       uint64_t l2 = 0;
-      if (w.j0 < last) {
-        // the row's queries: f16 after 2^-e of its largest exponent
+      if (begin < last) {
+        if (!fetched) fetch_q(w);
+        cp_async_wait();
+        __syncwarp();
+        // f16 after 2^-e of the row's largest exponent: exact for values down to
+        // 2^-14 of it, and off by at most 2^-25 of it below
         float top = 0.f;
-        const uint4* src = reinterpret_cast<const uint4*>(static_cast<const Act*>(a.q) + (w.s.row0 + j) * a.q_ld +
-                                                          head * kHeadDim);
-        if (live)
-#pragma unroll 4
-          for (int e = 0; e < 16; ++e) {
-            const uint4 raw = src[e];
-            const Act* v = reinterpret_cast<const Act*>(&raw);
 #pragma unroll
-            for (int u = 0; u < 8; ++u) top = fmaxf(top, fabsf(ActTraits<Act>::to_f(v[u])));
-          }
+        for (int e = 0; e < 16; ++e) {
+          const uint4 raw = *reinterpret_cast<const uint4*>(q_row + (e >> 3) * kHalf + (((e & 7) ^ (r & 7)) << 4));
+          const Act* v = reinterpret_cast<const Act*>(&raw);
+#pragma unroll
+          for (int u = 0; u < 8; ++u) top = fmaxf(top, fabsf(ActTraits<Act>::to_f(v[u])));
+        }
         const int ex = min(max(static_cast<int>(__float_as_uint(top) >> 23) - 127, -100), 100);
         const float down = exp2i(-ex);
         fac = exp2i(ex) * a.scale * a.c.k_scale * 1.4426950408889634f;
-#pragma unroll 4
+#pragma unroll
         for (int e = 0; e < 16; ++e) {
-          const uint4 raw = live ? src[e] : make_uint4(0, 0, 0, 0);
+          uint4* at = reinterpret_cast<uint4*>(q_row + (e >> 3) * kHalf + (((e & 7) ^ (r & 7)) << 4));
+          const uint4 raw = *at;
           const Act* v = reinterpret_cast<const Act*>(&raw);
           uint32_t o[4];
 #pragma unroll
           for (int u = 0; u < 4; ++u)
             o[u] = pack_f16(ActTraits<Act>::to_f(v[2 * u]) * down, ActTraits<Act>::to_f(v[2 * u + 1]) * down);
-          *reinterpret_cast<uint4*>(q_row + (e >> 3) * kHalf + (((e & 7) ^ (r & 7)) << 4)) =
-              make_uint4(o[0], o[1], o[2], o[3]);
+          *at = make_uint4(o[0], o[1], o[2], o[3]);
         }
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&sm.qfull[t]);
       }
+      fetched = false;
       const uint64_t fac2 = pair(fac, fac);
-      for (int kb = w.j0; kb < last; ++kb) {
+      for (int kb = begin; kb < last; ++kb) {
         ok = __all_sync(0xffffffffu, ok && wait(&sm.sfull[t], sphase & 1u));
         if (!ok) break;
         ++sphase;
@@ -428,54 +482,57 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const PrefillA
         uint32_t v[64];
         ld32(tS, v);
         ld32(tS + 32, v + 32);
-        ld_wait();
-        // slots of the block that the row sees; a warp's rows share most blocks whole
+        // slots of the block that the row sees; most blocks are whole for a warp
         const int open = seen - kb * kKeys;
         const bool border = __any_sync(0xffffffffu, open < kKeys);
-        float top = -INFINITY;
-        if (border) {
+        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        auto half = [&](int keys) {  // the scores in v: the mask, and their maximum
+          if (border) {
 #pragma unroll
-          for (int e = 0; e < 64; ++e)
-            if (e < open) top = fmaxf(top, __uint_as_float(v[e]));
-        } else {
+            for (int e = 0; e < 64; ++e)
+              if (e + keys >= open) v[e] = 0xFF800000u;  // -inf
+          }
 #pragma unroll
-          for (int e = 0; e < 64; ++e) top = fmaxf(top, __uint_as_float(v[e]));
-        }
-        __syncwarp();  // tcgen05.ld and .st are warp-collective
+          for (int e = 0; e < 64; e += 8)
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+              top[u] = max3(top[u], __uint_as_float(v[e + 2 * u]), __uint_as_float(v[e + 2 * u + 1]));
+          __syncwarp();  // tcgen05.ld and .st are warp-collective
+        };
+        ld_wait(v);
+        ld_wait(v + 32);
+        half(0);
         ld32(tS + 64, v);
         ld32(tS + 96, v + 32);
-        ld_wait();
-        if (border) {
-#pragma unroll
-          for (int e = 0; e < 64; ++e) {
-            if (e + 64 >= open) v[e] = 0xFF800000u;  // -inf
-            top = fmaxf(top, __uint_as_float(v[e]));
-          }
-        } else {
-#pragma unroll
-          for (int e = 0; e < 64; ++e) top = fmaxf(top, __uint_as_float(v[e]));
+        ld_wait(v);
+        ld_wait(v + 32);
+        half(64);
+        if (kb + 1 == last && f < f1) {
+          // the tile's queries are read: the next item's may take their place
+          find_next(f);
+          fetched = next->j0 < min(next->j1, next->blocks[t]);
+          if (fetched) fetch_q(*next);
         }
-        top *= fac;
-        if (__any_sync(0xffffffffu, top > m + kRaise)) {
-          const float mn = fmaxf(m, top);
+        const float all = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * fac;
+        if (__any_sync(0xffffffffu, all > m + kRaise)) {
+          const float mn = fmaxf(m, all);
           const float al = m == -INFINITY ? 0.f : ex2(m - mn);
           m = mn;
           ref = mn == -INFINITY ? 0.f : mn;
           l2 = pair(lo_of(l2) * al, hi_of(l2) * al);
-          if (kb > w.j0) {  // S of this block was issued after P V of the one before
+          if (kb > begin) {  // S of this block was issued after P V of the one before
+#pragma unroll 1
+            for (int cb = 0; cb < 8; ++cb) {
+              uint32_t o[16];
+              ld16(tO + cb * 16, o);
 #pragma unroll
-            for (int cb = 0; cb < 4; ++cb) {
-              uint32_t o[32];
-              ld32(tO + cb * 32, o);
-              ld_wait();
-#pragma unroll
-              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * al);
-              st32(tO + cb * 32, o);
+              for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * al);
+              st16(tO + cb * 16, o);
             }
           }
         }
-        __syncwarp();
         const uint64_t off2 = pair(-ref, -ref);
+        __syncwarp();
         auto probs = [&](uint32_t to) {  // v: 64 scores -> 32 columns of P
 #pragma unroll
           for (int hf = 0; hf < 2; ++hf) {
@@ -494,13 +551,14 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const PrefillA
         probs(tS + 96);  // keys 64 .. 127
         ld32(tS, v);
         ld32(tS + 32, v + 32);
-        ld_wait();
+        ld_wait(v);
+        ld_wait(v + 32);
         if (border) {
 #pragma unroll
           for (int e = 0; e < 64; ++e)
             if (e >= open) v[e] = 0xFF800000u;
+          __syncwarp();
         }
-        __syncwarp();
         probs(tS + 64);  // keys 0 .. 63
         st_wait();
         fence_before();
@@ -520,26 +578,31 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const PrefillA
           Act* dst = static_cast<Act*>(a.out) + (w.s.row0 + j) * a.out_ld + head * kHeadDim;
           float* part = d.part_o + (static_cast<size_t>(slot) * 2 * kRows + t * kRows + r) * kHeadDim;
 #pragma unroll
-          for (int cb = 0; cb < 4; ++cb) {
-            uint32_t o[32];
-            ld32(tO + cb * 32, o);
-            ld_wait();
+          for (int cb = 0; cb < 2; ++cb) {
+            uint32_t o[64];
+            ld32(tO + cb * 64, o);
+            ld32(tO + cb * 64 + 32, o + 32);
+            ld_wait(o);
+            ld_wait(o + 32);
             if (live && whole) {
-              uint4 out[4];
-              Act* h = reinterpret_cast<Act*>(out);
 #pragma unroll
-              for (int e = 0; e < 32; ++e)
-                h[e] = ActTraits<Act>::from_f(l != 0.f ? __uint_as_float(o[e]) * inv : 0.f);
+              for (int e = 0; e < 8; ++e) {
+                uint4 out;
+                Act* h = reinterpret_cast<Act*>(&out);
 #pragma unroll
-              for (int e = 0; e < 4; ++e) reinterpret_cast<uint4*>(dst + cb * 32)[e] = out[e];
+                for (int u = 0; u < 8; ++u)
+                  h[u] = ActTraits<Act>::from_f(l != 0.f ? __uint_as_float(o[8 * e + u]) * inv : 0.f);
+                reinterpret_cast<uint4*>(dst)[cb * 8 + e] = out;
+              }
             } else if (live) {
 #pragma unroll
-              for (int e = 0; e < 8; ++e)
-                reinterpret_cast<uint4*>(part + cb * 32)[e] =
+              for (int e = 0; e < 16; ++e)
+                reinterpret_cast<uint4*>(part)[cb * 16 + e] =
                     make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
             }
             __syncwarp();
           }
+          __syncwarp();
           fence_before();
         }
       }
@@ -549,15 +612,20 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const PrefillA
         else if (d.lse)
           d.lse[static_cast<size_t>(w.s.row0 + j) * a.c.q_heads + head] = l > 0.f ? m + log2f(l) : INFINITY;
       }
-      f = w.start + w.j1;
       if (f >= f1 || !ok) {
         // the only item of the range that can start in it and go on
         if (tid == 0)
           d.desc[b] = w.j0 == 0 && w.j1 < w.nb ? make_int4(w.i, w.h, w.tp, first) : make_int4(-1, 0, 0, first);
         break;
       }
-      next_item(a, sm.cum, w);
+      if (w.j0 >= last) {  // nothing of this item for the tile: the next is not known yet
+        find_next(f);
+      }
+      Share* was = cur;
+      cur = next;
+      next = was;
     }
+    cp_async_wait();
   } else if (warp < 12) {
     // ------------------------------------------------- codes to f16 operands
     // 4 lanes a token: lane q of a token holds dims 32q .. 32q + 31 (two scale
@@ -566,21 +634,41 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const PrefillA
     const bool swap = (q & 2) != 0;
     uint4 kc[4], vc[4];
     uint32_t ks[4], vs[4];
+    // the block whose page numbers are being fetched: its item, slots, slabs
     Share w = item_at(a, sm.cum, f0);
     set_share(a, w, f0, f1);
-    auto load = [&](int kb) {
+    int kb = w.j0, slab[4], left = 0;
+    bool more = true;
+    auto fetch_pages = [&]() {  // of block kb, then on to the next block
+      if (!more) return;
+      left = w.s.len - kb * kKeys;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const int key = kb * kKeys + dw * 32 + e * 8 + tok;
-        const bool there = key < w.s.len;
-        const int block = there ? max(0, kv4_block(a.c, a.c.block_table, w.s.sid, key / kPageTokens)) : 0;
-        const uint8_t* slab = a.c.pages + kv4_slab_index(a.c, block, w.h) * kKv4Slab;
-        const int tt = key % kPageTokens;
-        kc[e] = *reinterpret_cast<const uint4*>(slab + tt * 64 + q * 16);
-        vc[e] = *reinterpret_cast<const uint4*>(slab + kKv4VCodes + tt * 64 + q * 16);
+        const int at = dw * 32 + e * 8 + tok;
+        const int block =
+            at < left ? max(0, kv4_block(a.c, a.c.block_table, w.s.sid, (kb * kKeys + at) / kPageTokens)) : 0;
+        slab[e] = block * H + w.h;
+      }
+      if (++kb >= w.j1) {
+        const long long f = w.start + kPad + w.j1;
+        more = f < f1;
+        if (more) {
+          next_item(a, sm.cum, w);
+          set_share(a, w, f, f1);
+          kb = w.j0;
+        }
+      }
+    };
+    auto load = [&]() {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int at = dw * 32 + e * 8 + tok, tt = at % kPageTokens;
+        const uint8_t* src = a.c.pages + static_cast<size_t>(static_cast<unsigned>(slab[e])) * kKv4Slab;
+        kc[e] = *reinterpret_cast<const uint4*>(src + tt * 64 + q * 16);
+        vc[e] = *reinterpret_cast<const uint4*>(src + kKv4VCodes + tt * 64 + q * 16);
         // slots past the end may hold anything: scale 0
-        ks[e] = there ? *reinterpret_cast<const uint16_t*>(slab + kKv4KScales + tt * 8 + q * 2) : 0u;
-        vs[e] = there ? *reinterpret_cast<const uint16_t*>(slab + kKv4VScales + tt * 8 + q * 2) : 0u;
+        ks[e] = at < left ? *reinterpret_cast<const uint16_t*>(src + kKv4KScales + tt * 8 + q * 2) : 0u;
+        vs[e] = at < left ? *reinterpret_cast<const uint16_t*>(src + kKv4VScales + tt * 8 + q * 2) : 0u;
       }
     };
     auto store = [&](uint8_t* tile, const uint4 (&c)[4], const uint32_t (&s)[4]) {
@@ -606,31 +694,26 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const PrefillA
         }
       }
     };
-    load(w.j0);
-    uint32_t n = 0;
-    for (long long f = f0;; ) {
-      for (int kb = w.j0; kb < w.j1; ++kb, ++n) {
-        const int buf = n & 1;
-        const uint32_t turn = (n >> 1) & 1u;
-        if (!__all_sync(0xffffffffu, wait(&sm.kfree[buf], turn ^ 1u))) goto done;
-        store(smem + kOffK + buf * kTile, kc, ks);
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sm.kfull[buf]);
-        if (!__all_sync(0xffffffffu, wait(&sm.vfree[buf], turn ^ 1u))) goto done;
-        store(smem + kOffV + buf * kTile, vc, vs);
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sm.vfull[buf]);
-        if (kb + 1 < w.j1) load(kb + 1);
-      }
-      f = w.start + w.j1;
-      if (f >= f1) break;
-      next_item(a, sm.cum, w);
-      set_share(a, w, f, f1);
-      load(w.j0);
+    fetch_pages();
+    load();
+    for (uint32_t n = 0;; ++n) {
+      const bool again = more;
+      fetch_pages();  // of the block after this one
+      const int buf = n & 1;
+      const uint32_t turn = (n >> 1) & 1u;
+      if (!__all_sync(0xffffffffu, wait(&sm.kfree[buf], turn ^ 1u))) break;
+      store(smem + kOffK + buf * kTile, kc, ks);
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.kfull[buf]);
+      if (!__all_sync(0xffffffffu, wait(&sm.vfree[buf], turn ^ 1u))) break;
+      store(smem + kOffV + buf * kTile, vc, vs);
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.vfull[buf]);
+      if (!again) break;
+      load();
     }
-  done:;
   } else {
     // ------------------------------------------------------------------ MMA
     Share w = item_at(a, sm.cum, f0);
@@ -688,7 +771,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const PrefillA
         }
       }
       ok = __all_sync(0xffffffffu, ok);
-      f = w.start + w.j1;
+      f = w.start + kPad + w.j1;
       if (f >= f1) break;
       next_item(a, sm.cum, w);
     }
