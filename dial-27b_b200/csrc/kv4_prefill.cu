@@ -14,8 +14,8 @@
 // scores, then the lower 64 for the maximum alone, writes the upper half's P,
 // reads the lower half again and writes its P.  S_t of block j + 1 is issued right
 // after P V of block j, so one tile's softmax runs beside the other's MMAs.
-// The exponent's reference moves only when a score exceeds it by 2^8, so O in
-// TMEM is rarely rescaled.
+// The exponent's reference moves only when a score exceeds it by 2^8: a block is
+// taken in one pass, without its maximum first, and O in TMEM is rarely rescaled.
 //
 // Work split: the 128-key blocks of all items (sequence, kv head, pair of tiles)
 // laid end to end, one range a CTA, an item counted as kPad blocks more for its
@@ -96,6 +96,13 @@ __device__ __forceinline__ void commit(uint64_t* bar) {
                    smem_u32(bar))
                : "memory");
 }
+// One lane of the warp, the same on every call.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(p));
+  return p != 0;
+}
 __device__ __forceinline__ void fence_before() {
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
 }
@@ -141,16 +148,20 @@ __device__ __forceinline__ void ld32(uint32_t taddr, uint32_t* v) {
       : KV4_R32(v)
       : "r"(taddr));
 }
-// 16 columns, waited for.
 __device__ __forceinline__ void ld16(uint32_t taddr, uint32_t* v) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, "
-      "%12, %13, %14, %15}, [%16];\n\ttcgen05.wait::ld.sync.aligned;"
+      "%12, %13, %14, %15}, [%16];"
       : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]),
         "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]),
         "=r"(v[14]), "=r"(v[15])
-      : "r"(taddr)
-      : "memory");
+      : "r"(taddr));
+}
+__device__ __forceinline__ void ld_wait16(uint32_t* v) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]),
+                 "+r"(v[7]), "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]),
+                 "+r"(v[13]), "+r"(v[14]), "+r"(v[15])::"memory");
 }
 __device__ __forceinline__ void st16(uint32_t taddr, const uint32_t* v) {
   asm volatile(
@@ -324,7 +335,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const PrefillA
                                              ~static_cast<uintptr_t>(1023));
   Misc& sm = *reinterpret_cast<Misc*>(smem + kOffMisc);
   const Kv4AttnArgs& a = d.a;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, b = blockIdx.x;
+  const int tid = threadIdx.x, lane = tid & 31, b = blockIdx.x;
+  const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);  // known to be one value a warp
   const int H = a.c.kv_heads, rep = a.c.q_heads / H;
   if (tid == 0) {
     for (int i = 0; i < 2; ++i) {
@@ -380,7 +392,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const PrefillA
   auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
     if (mbar_try_wait(bar, parity)) return true;
     if (*reinterpret_cast<volatile int*>(&sm.failed)) return false;
-    if (mbar_wait(bar, parity, a.c.status, kStatusKv4Prefill)) return true;
+    if (mbar_wait_sleep(bar, parity, a.c.status, kStatusKv4Prefill)) return true;
     *reinterpret_cast<volatile int*>(&sm.failed) = 1;
     return false;
   };
@@ -479,43 +491,59 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const PrefillA
         if (!ok) break;
         ++sphase;
         fence_after();
-        uint32_t v[64];
-        ld32(tS, v);
-        ld32(tS + 32, v + 32);
-        // slots of the block that the row sees; most blocks are whole for a warp
-        const int open = seen - kb * kKeys;
-        const bool border = __any_sync(0xffffffffu, open < kKeys);
-        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-        auto half = [&](int keys) {  // the scores in v: the mask, and their maximum
-          if (border) {
+        const int open = seen - kb * kKeys;  // slots of the block that the row sees
+        if (__any_sync(0xffffffffu, open < kKeys)) {  // few blocks are not whole: masked in place
+#pragma unroll 1
+          for (int c = 0; c < 8; ++c) {
+            uint32_t x[16];
+            ld16(tS + 16 * c, x);
+            ld_wait16(x);
 #pragma unroll
-            for (int e = 0; e < 64; ++e)
-              if (e + keys >= open) v[e] = 0xFF800000u;  // -inf
+            for (int e = 0; e < 16; ++e)
+              if (e + 16 * c >= open) x[e] = 0xFF800000u;  // -inf
+            __syncwarp();  // tcgen05.ld and .st are warp-collective
+            st16(tS + 16 * c, x);
           }
-#pragma unroll
-          for (int e = 0; e < 64; e += 8)
-#pragma unroll
-            for (int u = 0; u < 4; ++u)
-              top[u] = max3(top[u], __uint_as_float(v[e + 2 * u]), __uint_as_float(v[e + 2 * u + 1]));
-          __syncwarp();  // tcgen05.ld and .st are warp-collective
-        };
-        ld_wait(v);
-        ld_wait(v + 32);
-        half(0);
-        ld32(tS + 64, v);
-        ld32(tS + 96, v + 32);
-        ld_wait(v);
-        ld_wait(v + 32);
-        half(64);
-        if (kb + 1 == last && f < f1) {
-          // the tile's queries are read: the next item's may take their place
-          find_next(f);
-          fetched = next->j0 < min(next->j1, next->blocks[t]);
-          if (fetched) fetch_q(*next);
+          st_wait();
         }
-        const float all = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * fac;
-        if (__any_sync(0xffffffffu, all > m + kRaise)) {
-          const float mn = fmaxf(m, all);
+        // the probabilities under the reference so far, 16 scores at a time, the
+        // load of one chunk beside the work on the other; where one would exceed
+        // 2^kRaise the reference moves to the row's maximum and all is done again
+        uint32_t p[64];
+        uint64_t sum0, sum1;
+        float top;
+        auto probs = [&]() {
+          const uint64_t off2 = pair(-ref, -ref);
+          uint32_t x[16], y[16];
+          float t0 = -INFINITY, t1 = -INFINITY;
+          sum0 = sum1 = 0;
+          auto chunk = [&](const uint32_t* v, uint32_t* to) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const uint64_t z = fma2(pair(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])), fac2, off2);
+              if (e & 1) t1 = max3(t1, lo_of(z), hi_of(z));
+              else t0 = max3(t0, lo_of(z), hi_of(z));
+              const float p0 = ex2(lo_of(z)), p1 = ex2(hi_of(z));
+              if (e & 1) sum1 = add2(sum1, pair(p0, p1));
+              else sum0 = add2(sum0, pair(p0, p1));
+              to[e] = pack_f16(p0, p1);
+            }
+          };
+          ld16(tS, x);
+#pragma unroll
+          for (int c = 0; c < 8; c += 2) {
+            ld_wait16(x);
+            ld16(tS + 16 * c + 16, y);
+            chunk(x, p + 8 * c);
+            ld_wait16(y);
+            if (c < 6) ld16(tS + 16 * c + 32, x);
+            chunk(y, p + 8 * c + 8);
+          }
+          top = fmaxf(t0, t1);
+        };
+        probs();
+        if (__any_sync(0xffffffffu, top > kRaise || (m == -INFINITY && top > -INFINITY))) {
+          const float mn = fmaxf(m, top + ref);
           const float al = m == -INFINITY ? 0.f : ex2(m - mn);
           m = mn;
           ref = mn == -INFINITY ? 0.f : mn;
@@ -525,41 +553,25 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const PrefillA
             for (int cb = 0; cb < 8; ++cb) {
               uint32_t o[16];
               ld16(tO + cb * 16, o);
+              ld_wait16(o);
 #pragma unroll
               for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * al);
+              __syncwarp();
               st16(tO + cb * 16, o);
             }
           }
+          probs();
         }
-        const uint64_t off2 = pair(-ref, -ref);
+        l2 = add2(l2, add2(sum0, sum1));
+        if (kb + 1 == last && f < f1) {
+          // the tile's queries are read: the next item's may take their place
+          find_next(f);
+          fetched = next->j0 < min(next->j1, next->blocks[t]);
+          if (fetched) fetch_q(*next);
+        }
         __syncwarp();
-        auto probs = [&](uint32_t to) {  // v: 64 scores -> 32 columns of P
 #pragma unroll
-          for (int hf = 0; hf < 2; ++hf) {
-            uint32_t p[16];
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              const int i = 32 * hf + 2 * e;
-              const uint64_t x = fma2(pair(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), fac2, off2);
-              const float p0 = ex2(lo_of(x)), p1 = ex2(hi_of(x));
-              l2 = add2(l2, pair(p0, p1));
-              p[e] = pack_f16(p0, p1);
-            }
-            st16(to + 16 * hf, p);
-          }
-        };
-        probs(tS + 96);  // keys 64 .. 127
-        ld32(tS, v);
-        ld32(tS + 32, v + 32);
-        ld_wait(v);
-        ld_wait(v + 32);
-        if (border) {
-#pragma unroll
-          for (int e = 0; e < 64; ++e)
-            if (e >= open) v[e] = 0xFF800000u;
-          __syncwarp();
-        }
-        probs(tS + 64);  // keys 0 .. 63
+        for (int c = 0; c < 4; ++c) st16(tS + 16 * c, p + 16 * c);
         st_wait();
         fence_before();
         __syncwarp();
@@ -716,69 +728,83 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const PrefillA
     }
   } else {
     // ------------------------------------------------------------------ MMA
+    // the whole warp runs this, on values that are the same in all its lanes, and
+    // one lane issues: operands stay in uniform registers
     Share w = item_at(a, sm.cum, f0);
-    const uint32_t sq = smem_u32(smem + kOffQ), sk = smem_u32(smem + kOffK), sv = smem_u32(smem + kOffV);
+    const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+    const uint64_t dq = kmajor_desc(smem_u32(smem + kOffQ)), dk = kmajor_desc(smem_u32(smem + kOffK)),
+                   dv = mnmajor_desc(smem_u32(smem + kOffV));
+    const bool leader = elect_one();
     uint32_t n = 0, qphase[2] = {0, 0}, pphase[2] = {0, 0};
+    auto all_wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)) != 0; };
+    auto issue_s = [&](int t, uint32_t kn) {
+      const uint64_t k0 = dk + (kn & 1) * (kTile >> 4), q0 = dq + t * (kTile >> 4);
+      if (leader) {
+#pragma unroll
+        for (int i = 0; i < kHeadDim / 16; ++i) {
+          const uint64_t off = ((i >> 2) * kHalf + (i & 3) * 32) >> 4;
+          mma_ss(tm + t * 128, q0 + off, k0 + off, idesc(false), i > 0 ? 1u : 0u);
+        }
+        commit(&sm.sfull[t]);
+      }
+      __syncwarp();
+    };
     bool ok = true;
     for (long long f = f0; ok;) {
       set_share(a, w, f, f1);
-      if (lane == 0) {
-        auto issue_s = [&](int t, uint32_t kb_n) {
-          const uint32_t k0 = sk + (kb_n & 1) * kTile, q0 = sq + t * kTile;
+      const int j0 = __shfl_sync(0xffffffffu, w.j0, 0), j1 = __shfl_sync(0xffffffffu, w.j1, 0);
+      const int last0 = min(j1, __shfl_sync(0xffffffffu, w.blocks[0], 0));
+      const int last1 = min(j1, __shfl_sync(0xffffffffu, w.blocks[1], 0));
+      if (j0 < last0) ok = ok && all_wait(&sm.qfull[0], qphase[0]++ & 1u);
+      if (j0 < last1) ok = ok && all_wait(&sm.qfull[1], qphase[1]++ & 1u);
+      ok = ok && all_wait(&sm.kfull[n & 1], (n >> 1) & 1u);
+      if (!ok) break;
+      fence_after();
+      if (j0 < last0) issue_s(0, n);
+      if (j0 < last1) issue_s(1, n);
+      if (leader) commit(&sm.kfree[n & 1]);
+      for (int kb = j0; kb < j1; ++kb, ++n) {
+        ok = all_wait(&sm.vfull[n & 1], (n >> 1) & 1u);
+        const uint64_t v0 = dv + (n & 1) * (kTile >> 4);
 #pragma unroll
-          for (int i = 0; i < kHeadDim / 16; ++i) {
-            const uint32_t off = (i >> 2) * kHalf + (i & 3) * 32;
-            mma_ss(tmem + t * 128, kmajor_desc(q0 + off), kmajor_desc(k0 + off), idesc(false), i > 0 ? 1u : 0u);
-          }
-          commit(&sm.sfull[t]);
-        };
-        const int last[2] = {min(w.j1, w.blocks[0]), min(w.j1, w.blocks[1])};
-        for (int t = 0; t < 2; ++t)
-          if (w.j0 < last[t]) ok = ok && wait(&sm.qfull[t], qphase[t]++ & 1u);
-        ok = ok && wait(&sm.kfull[n & 1], (n >> 1) & 1u);
-        if (ok) {
-          fence_after();
-          for (int t = 0; t < 2; ++t)
-            if (w.j0 < last[t]) issue_s(t, n);
-          commit(&sm.kfree[n & 1]);
-        }
-        for (int kb = w.j0; kb < w.j1 && ok; ++kb, ++n) {
-          ok = wait(&sm.vfull[n & 1], (n >> 1) & 1u);
-          const bool more = kb + 1 < w.j1;
-          for (int t = 0; t < 2 && ok; ++t) {
-            if (kb < last[t]) {
-              ok = wait(&sm.pready[t], pphase[t]++ & 1u);
-              if (!ok) break;
-              fence_after();
-              const uint32_t v0 = sv + (n & 1) * kTile;
+        for (int t = 0; t < 2; ++t) {
+          const int last = t == 0 ? last0 : last1;
+          if (kb < last && ok) {
+            ok = all_wait(&sm.pready[t], pphase[t]++ & 1u);
+            if (!ok) break;
+            fence_after();
+            if (leader) {
 #pragma unroll
               for (int i = 0; i < kKeys / 16; ++i)
-                mma_ts(tmem + 256 + t * 128, tmem + t * 128 + 64 + i * 8, mnmajor_desc(v0 + i * 2048), idesc(true),
-                       (kb > w.j0 || i > 0) ? 1u : 0u);
-              if (kb + 1 == last[t]) commit(&sm.odone[t]);
+                mma_ts(tm + 256 + t * 128, tm + t * 128 + i * 8, v0 + (i * 2048 >> 4), idesc(true),
+                       (kb > j0 || i > 0) ? 1u : 0u);
+              if (kb + 1 == last) commit(&sm.odone[t]);
             }
-            if (kb + 1 < last[t]) {
-              ok = wait(&sm.kfull[(n + 1) & 1], ((n + 1) >> 1) & 1u);
-              if (!ok) break;
-              fence_after();
-              issue_s(t, n + 1);
-            }
+            __syncwarp();
           }
-          if (ok) {
-            commit(&sm.vfree[n & 1]);
-            if (more) commit(&sm.kfree[(n + 1) & 1]);
+          if (kb + 1 < last && ok) {
+            ok = all_wait(&sm.kfull[(n + 1) & 1], ((n + 1) >> 1) & 1u);
+            if (!ok) break;
+            fence_after();
+            issue_s(t, n + 1);
           }
         }
+        if (!ok) break;
+        if (leader) {
+          commit(&sm.vfree[n & 1]);
+          if (kb + 1 < j1) commit(&sm.kfree[(n + 1) & 1]);
+        }
+        __syncwarp();
       }
-      ok = __all_sync(0xffffffffu, ok);
-      f = w.start + kPad + w.j1;
+      f = w.start + kPad + j1;
       if (f >= f1) break;
       next_item(a, sm.cum, w);
     }
-    if (lane == 0) {
+    if (leader) {
       commit(&sm.fin);  // nothing may still write TMEM when it is freed
       mbar_wait(&sm.fin, 0, a.c.status, kStatusKv4Prefill);
     }
+    __syncwarp();
   }
   fence_before();
   __syncthreads();
