@@ -1,5 +1,4 @@
-// Attention over the 4-bit KV cache: argument checks, the choice of kernel, and
-// the running weights of many queries.
+// Attention over the 4-bit KV cache: argument checks and the choice of kernel.
 //
 //   o = sum_j p_j v_j,  p_j = exp(s_j - m) / l,  s_j = scale * q . k_j
 //
@@ -13,37 +12,17 @@ namespace {
 
 constexpr int kFewCols = 64;
 
-template <typename Act>
-__global__ void __launch_bounds__(256) kv4_weights_kernel(const Kv4AttnArgs a, const float* lse) {
-  const int t = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  const int kvh = blockIdx.y, rep = a.c.q_heads / a.c.kv_heads;
-  Kv4Seq s;
-  if (!kv4_seq(a, blockIdx.z, s) || t >= s.len) return;
-  const int block = kv4_block(a.c, a.c.block_table, s.sid, t / kPageTokens);
-  const size_t si = kv4_slab_index(a.c, max(block, 0), kvh);
-  float k[4], sum = 0.f;
-  kv4_decode(a.c.pages + si * kKv4Slab, 0, kKv4KScales, t % kPageTokens, lane, a.c.k_scale, k);
-  for (int j = max(0, t - (s.len - s.n)); j < s.n; ++j)
-    for (int r = 0; r < rep; ++r) {
-      const int h = kvh * rep + r;
-      const size_t row = s.row0 + j;
-      float q[4];
-      load4(static_cast<const Act*>(a.q) + row * a.q_ld + h * kHeadDim + lane * 4, q);
-      const float sc =
-          warp_sum(fmaf(q[0], k[0], q[1] * k[1]) + fmaf(q[2], k[2], q[3] * k[3])) * a.scale;
-      sum += exp2f(sc * 1.4426950408889634f - lse[row * a.c.q_heads + h]);
-    }
-  if (lane == 0 && block >= 0) a.c.weights[si * kPageTokens + t % kPageTokens] += sum;
+// Scratch of the attention of many queries; that of their weights follows.
+size_t rows_part(int q_heads, long long rows) {
+  return (kv4_prefill_scratch(q_heads, rows, true) + 127) & ~static_cast<size_t>(127);
 }
 
 cudaError_t launch(const Kv4AttnArgs& a, int act, cudaStream_t s) {
   if (a.max_q * (a.c.q_heads / a.c.kv_heads) <= kFewCols) return kv4_decode_launch(a, act, s);
-  cudaError_t e = kv4_prefill_launch(a, act, s);
+  const cudaError_t e = kv4_prefill_launch(a, act, s);
   if (e != cudaSuccess || !a.c.weights) return e;
-  const dim3 grid((a.max_len + 7) / 8, a.c.kv_heads, a.seqs);
-  if (act == DIAL_ACT_BF16) kv4_weights_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(a, kv4_prefill_lse(a));
-  else kv4_weights_kernel<__half><<<grid, 256, 0, s>>>(a, kv4_prefill_lse(a));
-  return cudaGetLastError();
+  return kv4_colsum_launch(a, kv4_prefill_rows(a),
+                           static_cast<uint8_t*>(a.scratch) + rows_part(a.c.q_heads, a.rows), s);
 }
 
 }  // namespace
@@ -60,7 +39,9 @@ extern "C" int64_t dial_b200_kv4_attention_scratch_bytes(const dial_b200_kv4_sha
   if (max_q * (sh->q_heads / sh->kv_heads) <= kFewCols)
     return static_cast<int64_t>(kv4_decode_scratch(sh->q_heads, sh->kv_heads, seqs, max_q, max_len,
                                                    with_weights != 0));
-  return static_cast<int64_t>(kv4_prefill_scratch(sh->q_heads, rows, with_weights != 0));
+  if (!with_weights) return static_cast<int64_t>(kv4_prefill_scratch(sh->q_heads, rows, false));
+  return static_cast<int64_t>(rows_part(sh->q_heads, rows) +
+                              kv4_colsum_scratch(sh->q_heads, sh->kv_heads, seqs, max_q, max_len));
 }
 
 extern "C" int dial_b200_kv4_attention(const dial_b200_kv4_shape* sh, const void* q, int64_t q_ld,

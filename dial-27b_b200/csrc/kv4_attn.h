@@ -26,10 +26,22 @@ size_t kv4_decode_scratch(int q_heads, int kv_heads, long long seqs, long long m
 cudaError_t kv4_decode_launch(const Kv4AttnArgs& a, int act, cudaStream_t s);
 
 // Many queries a sequence: tcgen05, 256 (query, head) rows over each key block
-// (kv4_prefill.cu).  With weights it leaves each row's log-sum-exp, base 2, in
-// scratch at kv4_prefill_lse.
+// (kv4_prefill.cu).  With weights it leaves in scratch, for every row and head,
+// the f16 queries, their scale to base-2 scores and the log-sum-exp.
+struct Kv4Rows {
+  uint16_t* q16;  // [rows][q_heads][128]
+  float* fac;     // [rows][q_heads]
+  float* lse;     // [rows][q_heads], base 2
+};
+constexpr int kKv4RowBytes = 128 * 2 + 4 + 4;
 size_t kv4_prefill_scratch(int q_heads, long long rows, bool weights);
-float* kv4_prefill_lse(const Kv4AttnArgs& a);
+Kv4Rows kv4_prefill_rows(const Kv4AttnArgs& a);
 cudaError_t kv4_prefill_launch(const Kv4AttnArgs& a, int act, cudaStream_t s);
+
+// The running weights of those queries (kv4_colsum.cu); `scratch` of its own.
+size_t kv4_colsum_scratch(int q_heads, int kv_heads, long long seqs, long long max_q,
+                          long long max_len);
+cudaError_t kv4_colsum_launch(const Kv4AttnArgs& a, const Kv4Rows& rows, void* scratch,
+                              cudaStream_t s);
 
 }  // namespace dialb200
