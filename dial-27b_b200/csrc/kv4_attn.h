@@ -27,11 +27,11 @@ cudaError_t kv4_decode_launch(const Kv4AttnArgs& a, int act, cudaStream_t s);
 
 // Many queries a sequence: tcgen05, 256 (query, head) rows over each key block
 // (kv4_prefill.cu).  With weights it leaves in scratch, for every row and head,
-// the f16 queries, their scale to base-2 scores and the log-sum-exp.
+// the f16 queries, their scale to base-2 scores and minus the log-sum-exp.
 struct Kv4Rows {
   uint16_t* q16;  // [rows][q_heads][128]
   float* fac;     // [rows][q_heads]
-  float* lse;     // [rows][q_heads], base 2
+  float* off;     // [rows][q_heads], minus the log-sum-exp, base 2
 };
 constexpr int kKv4RowBytes = 128 * 2 + 4 + 4;
 size_t kv4_prefill_scratch(int q_heads, long long rows, bool weights);

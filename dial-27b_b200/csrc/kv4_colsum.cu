@@ -11,8 +11,9 @@
 // Items: a 128-key block of a (sequence, kv head) and up to kChunk tiles of 128 rows
 // that see it, dealt to the CTAs in turn.  Warps 0-3 and 4-7 take tiles in turn
 // and leave a sum for each key; kv4_colsum_add_kernel adds an item's sums to the
-// weights in a fixed order.  Warps 8-11: K codes -> f16 once an item, query tiles
-// by cp.async into three buffers; warp 12: tcgen05.mma into four TMEM buffers.
+// weights in a fixed order.  Warps 8-11: K codes -> f16 once an item (loaded during
+// the item before), query tiles and their constants by cp.async into four buffers;
+// warp 12: tcgen05.mma into four TMEM buffers.
 #include "kv4_attn.h"
 #include "kv4_tc.cuh"
 
@@ -22,7 +23,7 @@ namespace {
 constexpr int kThreads = 13 * 32;
 constexpr int kSeqChunk = 512;  // sequences a launch
 constexpr int kChunk = 32;      // query tiles of an item at most
-constexpr int kQBufs = 3, kSBufs = 4;
+constexpr int kQBufs = 4, kSBufs = 4;
 constexpr int kOffK = 0;                     // [2]
 constexpr int kOffQ = 2 * kTile;             // [kQBufs]
 constexpr int kOffMisc = (2 + kQBufs) * kTile;
@@ -33,7 +34,7 @@ struct Misc {
   uint32_t tmem;
   int failed;
   alignas(16) float fac[kQBufs][128];
-  alignas(16) float off[kQBufs][128];   // -lse
+  alignas(16) float off[kQBufs][128];
   alignas(16) int seen[kQBufs][128];    // slots the row sees
   long long cum[kSeqChunk + 1];         // items of one kv head of the sequences before
 };
@@ -45,6 +46,10 @@ struct ColsumArgs {
   float* part;  // [seqs][kv_heads][kb_max][chunks][2][128]
   int kb_max, chunks;
 };
+
+__device__ __forceinline__ void cp_async4(void* dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
 
 struct Item {
   Kv4Seq s;
@@ -217,21 +222,23 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_colsum_kernel(const ColsumArg
   } else if (warp < 12) {
     // --------------------------------------------- K codes and query tiles
     const int dw = warp - 8, q = lane & 3, tok = lane >> 2, row = dw * 32 + lane;
-    uint32_t n = 0, items = 0;
-    int pending = -1;  // buffer whose copies are in flight
+    constexpr uint32_t kAhead = 2;         // tiles in flight behind the one being issued
+    uint32_t n = 0, landed = 0, items = 0;  // tiles issued and handed on
     bool ok = true;
-    auto landed = [&]() {
-      if (pending < 0) return;
+    auto hand_on = [&]() {
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&sm.qfull[pending]);
-      pending = -1;
+      if (lane == 0) mbar_arrive(&sm.qfull[landed % kQBufs]);
+      ++landed;
     };
-    for (long long f = blockIdx.x; f < total && ok; f += gridDim.x) {
-      const Item w = item_at(d, sm.cum, f);
-      if (w.t1 <= w.t0) continue;
-      uint4 kc[4];
-      uint32_t ks[4];
+    uint4 kc[4];
+    uint32_t ks[4];
+    auto next_item = [&](long long& f, Item& w) {  // the next with tiles, and its codes
+      for (; f < total; f += gridDim.x) {
+        w = item_at(d, sm.cum, f);
+        if (w.t1 > w.t0) break;
+      }
+      if (f >= total) return;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int key = w.kb * 128 + dw * 32 + e * 8 + tok, tt = key % kPageTokens;
@@ -239,49 +246,65 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_colsum_kernel(const ColsumArg
         const int block = there ? max(0, kv4_block(a.c, a.c.block_table, w.s.sid, key / kPageTokens)) : 0;
         const uint8_t* slab = a.c.pages + kv4_slab_index(a.c, block, w.h) * kKv4Slab;
         kc[e] = *reinterpret_cast<const uint4*>(slab + tt * 64 + q * 16);
+        // slots past the end may hold anything: scale 0
         ks[e] = there ? *reinterpret_cast<const uint16_t*>(slab + kKv4KScales + tt * 8 + q * 2) : 0u;
       }
+    };
+    long long f = blockIdx.x;
+    Item w;
+    next_item(f, w);
+    while (f < total) {
       const int kbuf = items & 1;
-      ok = wait(&sm.kfree[kbuf], (items >> 1 & 1u) ^ 1u);
+      const uint32_t turn = (items >> 1 & 1u) ^ 1u;
+      if (!__all_sync(0xffffffffu, mbar_try_wait(&sm.kfree[kbuf], turn))) {
+        // the buffer's MMAs may need tiles that are still held back here
+        cp_async_wait();
+        while (landed < n) hand_on();
+      }
+      ok = wait(&sm.kfree[kbuf], turn);
       if (!ok) break;
       codes_to_tile(smem + kOffK + kbuf * kTile, dw, kc, ks);
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&sm.kfull[kbuf]);
       ++items;
-      for (int T = w.t0; T < w.t1; ++T, ++n) {
+      const Item cur = w;
+      f += gridDim.x;
+      next_item(f, w);
+      for (int T = cur.t0; T < cur.t1; ++T, ++n) {
         const uint32_t qb = n % kQBufs;
         ok = wait(&sm.qfree[qb], (n / kQBufs & 1u) ^ 1u);
         if (!ok) break;
         const int R = T * 128 + row;
-        const bool live = R < w.s.n * rep;
+        const bool live = R < cur.s.n * rep;
         const int j = live ? R / rep : 0;
-        const size_t at = static_cast<size_t>(w.s.row0 + j) * a.c.q_heads + w.h * rep + (live ? R - j * rep : 0);
+        const long long at = live ? static_cast<long long>(cur.s.row0 + j) * a.c.q_heads + cur.h * rep + (R - j * rep) : -1;
         uint8_t* tile = smem + kOffQ + qb * kTile;
-        const long long mine = live ? static_cast<long long>(at) : -1;
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           const int rr = 2 * e + (lane >> 4), c = lane & 15;
-          const long long from = __shfl_sync(0xffffffffu, mine, rr);
+          const long long from = __shfl_sync(0xffffffffu, at, rr);
           cp_async16(tile + (c >> 3) * kHalf + (dw * 32 + rr) * 128 + (((c & 7) ^ (rr & 7)) << 4),
                      d.r.q16 + (from < 0 ? 0 : from) * kHeadDim + c * 8, from >= 0);
         }
-        sm.fac[qb][row] = live ? d.r.fac[at] : 0.f;
-        sm.off[qb][row] = live ? -d.r.lse[at] : -INFINITY;
-        sm.seen[qb][row] = live ? w.s.len - w.s.n + 1 + j : 0;
-        asm volatile("cp.async.commit_group;" ::: "memory");
-        if (pending >= 0) {
-          asm volatile("cp.async.wait_group 1;" ::: "memory");
-          landed();
+        if (live) {
+          cp_async4(&sm.fac[qb][row], d.r.fac + at);
+          cp_async4(&sm.off[qb][row], d.r.off + at);
+        } else {
+          sm.fac[qb][row] = 0.f;
+          sm.off[qb][row] = -INFINITY;
         }
-        pending = qb;
+        sm.seen[qb][row] = live ? cur.s.len - cur.s.n + 1 + j : 0;
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        if (n - landed >= kAhead) {
+          asm volatile("cp.async.wait_group %0;" ::"n"(kAhead) : "memory");
+          hand_on();
+        }
       }
-      if (pending >= 0) {  // the item's last tile does not wait for the next item
-        cp_async_wait();
-        landed();
-      }
+      if (!ok) break;
     }
     cp_async_wait();
+    while (landed < n) hand_on();
   } else {
     // ------------------------------------------------------------------ MMA
     const uint32_t tm = __shfl_sync(0xffffffffu, sm.tmem, 0);

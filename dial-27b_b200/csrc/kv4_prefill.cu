@@ -61,10 +61,10 @@ struct PrefillArgs {
   float* part_o;    // [2 * ctas][256][128]
   float2* part_ml;  // [2 * ctas][256]
   // with weights (else null), for every row and head: the queries as f16, their
-  // scale to base-2 scores, and the log-sum-exp, base 2
+  // scale to base-2 scores, and minus the log-sum-exp, base 2
   uint16_t* q16;
   float* fac;
-  float* lse;
+  float* off;
 };
 
 // --------------------------------------------------------------- work items
@@ -235,9 +235,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const PrefillA
       for (int e = tid * 8; e < a.c.q_heads * kHeadDim; e += kThreads * 8)
         *reinterpret_cast<uint4*>(static_cast<Act*>(a.out) + (s.row0 + r) * a.out_ld + e) =
             make_uint4(0, 0, 0, 0);
-      if (d.lse)
+      if (d.off)
         for (int e = tid; e < a.c.q_heads; e += kThreads)
-          d.lse[static_cast<size_t>(s.row0 + r) * a.c.q_heads + e] = INFINITY;
+          d.off[static_cast<size_t>(s.row0 + r) * a.c.q_heads + e] = -INFINITY;
     }
   }
   const int ctas = static_cast<int>(min(static_cast<long long>(d.ctas), total));
@@ -335,7 +335,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const PrefillA
         const int ex = min(max(static_cast<int>(__float_as_uint(top) >> 23) - 127, -100), 100);
         const float down = exp2i(-ex);
         fac = exp2i(ex) * a.scale * a.c.k_scale * 1.4426950408889634f;
-        const bool keep_q = d.lse && live && begin == 0;
+        const bool keep_q = d.off && live && begin == 0;
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           uint4* at = reinterpret_cast<uint4*>(q_row + (e >> 3) * kHalf + (((e & 7) ^ (r & 7)) << 4));
@@ -491,8 +491,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const PrefillA
       if (live) {
         if (!whole)
           d.part_ml[static_cast<size_t>(slot) * 2 * kRows + t * kRows + r] = make_float2(l > 0.f || l != l ? m : -INFINITY, l);
-        else if (d.lse)
-          d.lse[static_cast<size_t>(w.s.row0 + j) * a.c.q_heads + head] = l > 0.f ? m + log2f(l) : INFINITY;
+        else if (d.off)
+          d.off[static_cast<size_t>(w.s.row0 + j) * a.c.q_heads + head] = l > 0.f ? -(m + log2f(l)) : -INFINITY;
       }
       if (f >= f1 || !ok) {
         // the only item of the range that can start in it and go on
@@ -702,8 +702,8 @@ __global__ void __launch_bounds__(256) kv4_prefill_join_kernel(const PrefillArgs
   const float inv = L != 0.f ? a.c.v_scale / L : 0.f;
   const float o[4] = {O.x * inv, O.y * inv, O.z * inv, O.w * inv};
   store4(static_cast<Act*>(a.out) + (s.row0 + j) * a.out_ld + head * kHeadDim + lane * 4, o);
-  if (d.lse && lane == 0)
-    d.lse[static_cast<size_t>(s.row0 + j) * a.c.q_heads + head] = L > 0.f ? M + log2f(L) : INFINITY;
+  if (d.off && lane == 0)
+    d.off[static_cast<size_t>(s.row0 + j) * a.c.q_heads + head] = L > 0.f ? -(M + log2f(L)) : -INFINITY;
 }
 
 int range_count() {
@@ -757,7 +757,7 @@ Kv4Rows kv4_prefill_rows(const Kv4AttnArgs& a) {
   const size_t n = static_cast<size_t>(a.rows) * a.c.q_heads;
   r.q16 = reinterpret_cast<uint16_t*>(w);
   r.fac = reinterpret_cast<float*>(w + n * kHeadDim * 2);
-  r.lse = r.fac + n;
+  r.off = r.fac + n;
   return r;
 }
 
@@ -778,7 +778,7 @@ cudaError_t kv4_prefill_launch(const Kv4AttnArgs& a, int act, cudaStream_t s) {
       const Kv4Rows r = kv4_prefill_rows(a);
       d.q16 = r.q16;
       d.fac = r.fac;
-      d.lse = r.lse;
+      d.off = r.off;
     }
     const cudaError_t e = act == DIAL_ACT_BF16 ? launch<__nv_bfloat16>(d, s) : launch<__half>(d, s);
     if (e != cudaSuccess) return e;

@@ -183,10 +183,11 @@ def test_attention_few_queries(cuda, heads, weights):
 
 
 @pytest.mark.parametrize("queries,lens", [(16, (16, 40)), (33, (33, 90)), (64, (64, 257)),
-                                          (129, (129, 400)), (200, (150, 200))])
+                                          (129, (129, 400)), (200, (150, 200)), (20, (20, 2000)),
+                                          (40, (700, 1300))])
 @pytest.mark.parametrize("heads", [(8, 2), (5, 1), (2, 2)])
 def test_attention_prompts(cuda, queries, lens, heads):
-    c = Cache(13, 4, 416, *heads)
+    c = Cache(13, 4, max(lens) + 16, *heads)
     check_attention(c, cuda, [(2, lens[1], queries), (0, lens[0], queries), (3, 7, 3)],
                     spare_rows=1, stride=64)
 
