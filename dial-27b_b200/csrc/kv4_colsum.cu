@@ -23,19 +23,19 @@ namespace {
 constexpr int kThreads = 13 * 32;
 constexpr int kSeqChunk = 512;  // sequences a launch
 constexpr int kChunk = 32;      // query tiles of an item at most
-constexpr int kQBufs = 4, kSBufs = 4;
+constexpr int kQBufs = 4, kSBufs = 4, kCBufs = 8;  // query tiles, scores, constants
 constexpr int kOffK = 0;                     // [2]
 constexpr int kOffQ = 2 * kTile;             // [kQBufs]
 constexpr int kOffMisc = (2 + kQBufs) * kTile;
 constexpr int kStatusKv4Colsum = 0x602;
 
 struct Misc {
-  uint64_t kfull[2], kfree[2], qfull[kQBufs], qfree[kQBufs], sfull[kSBufs], sfree[kSBufs], fin;
+  uint64_t kfull[2], kfree[2], qfull[kQBufs], qfree[kQBufs], sfull[kSBufs], sfree[kSBufs], cfull[kCBufs], cfree[kCBufs], fin;
   uint32_t tmem;
   int failed;
-  alignas(16) float fac[kQBufs][128];
-  alignas(16) float off[kQBufs][128];
-  alignas(16) int seen[kQBufs][128];    // slots the row sees
+  alignas(16) float fac[kCBufs][128];
+  alignas(16) float off[kCBufs][128];
+  alignas(16) int seen[kCBufs][128];    // slots the row sees
   long long cum[kSeqChunk + 1];         // items of one kv head of the sequences before
 };
 constexpr int kSmemBytes = kOffMisc + sizeof(Misc) + 1024;
@@ -112,11 +112,15 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_colsum_kernel(const ColsumArg
     }
     for (int i = 0; i < kQBufs; ++i) {
       mbar_init(&sm.qfull[i], 4);
-      mbar_init(&sm.qfree[i], 5);  // the MMA, and four warps that read its constants
+      mbar_init(&sm.qfree[i], 1);
     }
     for (int i = 0; i < kSBufs; ++i) {
       mbar_init(&sm.sfull[i], 1);
       mbar_init(&sm.sfree[i], 4);
+    }
+    for (int i = 0; i < kCBufs; ++i) {
+      mbar_init(&sm.cfull[i], 4);
+      mbar_init(&sm.cfree[i], 4);
     }
     mbar_init(&sm.fin, 1);
     sm.failed = 0;
@@ -172,48 +176,58 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_colsum_kernel(const ColsumArg
       bool ok = true;
       for (int T = w.t0; T < w.t1; ++T, ++n) {
         if ((n & 1u) != static_cast<uint32_t>(grp)) continue;
-        const uint32_t sb = n % kSBufs, qb = n % kQBufs;
-        ok = ok && wait(&sm.qfull[qb], n / kQBufs & 1u) && wait(&sm.sfull[sb], n / kSBufs & 1u);
+        const uint32_t sb = n % kSBufs, cb = n % kCBufs;
+        ok = ok && wait(&sm.cfull[cb], n / kCBufs & 1u) && wait(&sm.sfull[sb], n / kSBufs & 1u);
         if (!ok) continue;
         fence_after();
         const uint32_t tS = sm.tmem + sb * 128 + lane_off;
-        uint32_t x[32], y[32];
+        const float *fc = sm.fac[cb], *of = sm.off[cb];
         // every row of the tile sees the whole block
-        const bool open = w.s.len - w.s.n + 1 + T * 128 / rep >= (w.kb + 1) * 128;
-        ld32(tS, x);
-        ld_wait(x);
-        auto add = [&](const uint32_t* v, int c0) {
-          const ulonglong2* fc = reinterpret_cast<const ulonglong2*>(sm.fac[qb] + c0);
-          const ulonglong2* of = reinterpret_cast<const ulonglong2*>(sm.off[qb] + c0);
+        if (w.s.len - w.s.n + 1 + T * 128 / rep >= (w.kb + 1) * 128) {
+          uint32_t x[32], y[32];
+          auto add = [&](const uint32_t* v, int c0) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {  // 4 columns
-            const ulonglong2 f2 = fc[e], o2 = of[e];
-            uint64_t z0 = fma2(pair(__uint_as_float(v[4 * e]), __uint_as_float(v[4 * e + 1])), f2.x, o2.x);
-            uint64_t z1 = fma2(pair(__uint_as_float(v[4 * e + 2]), __uint_as_float(v[4 * e + 3])), f2.y, o2.y);
-            if (!open) {
-              const int4 see = *reinterpret_cast<const int4*>(sm.seen[qb] + c0 + 4 * e);
-              z0 = pair(key < see.x ? lo_of(z0) : -INFINITY, key < see.y ? hi_of(z0) : -INFINITY);
-              z1 = pair(key < see.z ? lo_of(z1) : -INFINITY, key < see.w ? hi_of(z1) : -INFINITY);
+            for (int e = 0; e < 32; e += 4) {
+              const ulonglong2 f2 = *reinterpret_cast<const ulonglong2*>(fc + c0 + e);
+              const ulonglong2 o2 = *reinterpret_cast<const ulonglong2*>(of + c0 + e);
+              const uint64_t z0 = fma2(pair(__uint_as_float(v[e]), __uint_as_float(v[e + 1])), f2.x, o2.x);
+              const uint64_t z1 = fma2(pair(__uint_as_float(v[e + 2]), __uint_as_float(v[e + 3])), f2.y, o2.y);
+              s0 = add2(s0, pair(ex2(lo_of(z0)), ex2(hi_of(z0))));
+              s1 = add2(s1, pair(ex2(lo_of(z1)), ex2(hi_of(z1))));
             }
-            s0 = add2(s0, pair(ex2(lo_of(z0)), ex2(hi_of(z0))));
-            s1 = add2(s1, pair(ex2(lo_of(z1)), ex2(hi_of(z1))));
-          }
-          __syncwarp();
-        };
-#pragma unroll 1
-        for (int c = 0; c < 4; c += 2) {
-          ld32(tS + 32 * c + 32, y);
-          add(x, 32 * c);
+          };
+          ld32(tS, x);
+          ld_wait(x);
+          ld32(tS + 32, y);
+          add(x, 0);
           ld_wait(y);
-          if (c == 0) ld32(tS + 64, x);
-          add(y, 32 * c + 32);
-          if (c == 0) ld_wait(x);
+          ld32(tS + 64, x);
+          add(y, 32);
+          ld_wait(x);
+          ld32(tS + 96, y);
+          add(x, 64);
+          ld_wait(y);
+          add(y, 96);
+        } else {
+#pragma unroll 1
+          for (int c = 0; c < 128; c += 16) {
+            uint32_t x[16];
+            ld16(tS + c, x);
+            ld_wait16(x);
+#pragma unroll
+            for (int e = 0; e < 16; e += 2) {
+              const float z0 = fmaf(__uint_as_float(x[e]), fc[c + e], of[c + e]);
+              const float z1 = fmaf(__uint_as_float(x[e + 1]), fc[c + e + 1], of[c + e + 1]);
+              s0 = add2(s0, pair(key < sm.seen[cb][c + e] ? ex2(z0) : 0.f, key < sm.seen[cb][c + e + 1] ? ex2(z1) : 0.f));
+            }
+            __syncwarp();
+          }
         }
         fence_before();
         __syncwarp();
         if (lane == 0) {
           mbar_arrive(&sm.sfree[sb]);
-          mbar_arrive(&sm.qfree[qb]);
+          mbar_arrive(&sm.cfree[cb]);
         }
       }
       const uint64_t s = add2(s0, s1);
@@ -228,7 +242,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_colsum_kernel(const ColsumArg
     auto hand_on = [&]() {
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&sm.qfull[landed % kQBufs]);
+      if (lane == 0) {
+        mbar_arrive(&sm.qfull[landed % kQBufs]);
+        mbar_arrive(&sm.cfull[landed % kCBufs]);
+      }
       ++landed;
     };
     uint4 kc[4];
@@ -272,8 +289,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_colsum_kernel(const ColsumArg
       f += gridDim.x;
       next_item(f, w);
       for (int T = cur.t0; T < cur.t1; ++T, ++n) {
-        const uint32_t qb = n % kQBufs;
-        ok = wait(&sm.qfree[qb], (n / kQBufs & 1u) ^ 1u);
+        const uint32_t qb = n % kQBufs, cb = n % kCBufs;
+        ok = wait(&sm.qfree[qb], (n / kQBufs & 1u) ^ 1u) && wait(&sm.cfree[cb], (n / kCBufs & 1u) ^ 1u);
         if (!ok) break;
         const int R = T * 128 + row;
         const bool live = R < cur.s.n * rep;
@@ -288,13 +305,13 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_colsum_kernel(const ColsumArg
                      d.r.q16 + (from < 0 ? 0 : from) * kHeadDim + c * 8, from >= 0);
         }
         if (live) {
-          cp_async4(&sm.fac[qb][row], d.r.fac + at);
-          cp_async4(&sm.off[qb][row], d.r.off + at);
+          cp_async4(&sm.fac[cb][row], d.r.fac + at);
+          cp_async4(&sm.off[cb][row], d.r.off + at);
         } else {
-          sm.fac[qb][row] = 0.f;
-          sm.off[qb][row] = -INFINITY;
+          sm.fac[cb][row] = 0.f;
+          sm.off[cb][row] = -INFINITY;
         }
-        sm.seen[qb][row] = live ? cur.s.len - cur.s.n + 1 + j : 0;
+        sm.seen[cb][row] = live ? cur.s.len - cur.s.n + 1 + j : 0;
         asm volatile("cp.async.commit_group;" ::: "memory");
         if (n - landed >= kAhead) {
           asm volatile("cp.async.wait_group %0;" ::"n"(kAhead) : "memory");
