@@ -61,6 +61,8 @@ extern "C" int dial_b200_kv4_attention(const dial_b200_kv4_shape* sh, const void
   if (rows < 0 || rows > (1 << 26) || max_q < 0 || max_q > (1 << 24))
     return kv4_fail(err, n, DIAL_ERR_INVALID, "rows %lld / max_q %lld out of range",
                     (long long)rows, (long long)max_q);
+  if (rows * sh->q_heads > INT32_MAX)
+    return kv4_fail(err, n, DIAL_ERR_INVALID, "rows %lld times q_heads out of range", (long long)rows);
   if (!q_starts && rows != seqs)
     return kv4_fail(err, n, DIAL_ERR_INVALID, "without q_starts rows %lld must equal seqs %lld",
                     (long long)rows, (long long)seqs);

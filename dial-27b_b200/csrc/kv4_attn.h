@@ -29,9 +29,9 @@ cudaError_t kv4_decode_launch(const Kv4AttnArgs& a, int act, cudaStream_t s);
 // (kv4_prefill.cu).  With weights it leaves in scratch, for every row and head,
 // the f16 queries, their scale to base-2 scores and minus the log-sum-exp.
 struct Kv4Rows {
-  uint16_t* q16;  // [rows][q_heads][128]
-  float* fac;     // [rows][q_heads]
-  float* off;     // [rows][q_heads], minus the log-sum-exp, base 2
+  uint16_t* q16;  // [kv_heads][rows][heads of a group][128]
+  float* fac;     // [kv_heads][rows][heads of a group]
+  float* off;     // the same, minus the log-sum-exp, base 2
 };
 constexpr int kKv4RowBytes = 128 * 2 + 4 + 4;
 size_t kv4_prefill_scratch(int q_heads, long long rows, bool weights);

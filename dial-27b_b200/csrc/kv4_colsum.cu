@@ -8,29 +8,33 @@
 // by the exponentials (16 a clock and SM).  S^T = K Q^T has a key in every TMEM
 // lane, so a thread adds up its own key's row and nothing is exchanged.
 //
-// Items: a 128-key block of a (sequence, kv head) and up to kChunk tiles of 128 rows
-// that see it, dealt to the CTAs in turn.  Warps 0-3 and 4-7 take tiles in turn
-// and leave a sum for each key; kv4_colsum_add_kernel adds an item's sums to the
-// weights in a fixed order.  Warps 8-11: K codes -> f16 once an item (loaded during
-// the item before), query tiles and their constants by cp.async into four buffers;
-// warp 12: tcgen05.mma into four TMEM buffers.
+// Items: two 128-key blocks of a (sequence, kv head), so that a query tile fetched
+// from L2 serves 256 keys, and up to kChunk tiles of 128 rows that see them, dealt
+// to the CTAs in turn.  Warps 0-3 and 4-7 add up a key block each and leave a sum
+// for each key; kv4_colsum_add_kernel adds the sums to the weights in a fixed order.
+// Warps 8-11: K codes -> f16 once an item, loaded during the item before; warp 12:
+// query tiles by TMA into four buffers, and their constants; warp 13: tcgen05.mma
+// into four TMEM buffers.
+#include <cuda.h>
+
 #include "kv4_attn.h"
 #include "kv4_tc.cuh"
 
 namespace dialb200 {
 namespace {
 
-constexpr int kThreads = 13 * 32;
+constexpr int kThreads = 14 * 32;
 constexpr int kSeqChunk = 512;  // sequences a launch
+constexpr int kKeys = 256;      // of an item
 constexpr int kChunk = 32;      // query tiles of an item at most
 constexpr int kQBufs = 4, kSBufs = 4, kCBufs = 8;  // query tiles, scores, constants
-constexpr int kOffK = 0;                     // [2]
+constexpr int kOffK = 0;                     // [2], the item's two key blocks
 constexpr int kOffQ = 2 * kTile;             // [kQBufs]
 constexpr int kOffMisc = (2 + kQBufs) * kTile;
 constexpr int kStatusKv4Colsum = 0x602;
 
 struct Misc {
-  uint64_t kfull[2], kfree[2], qfull[kQBufs], qfree[kQBufs], sfull[kSBufs], sfree[kSBufs], cfull[kCBufs], cfree[kCBufs], fin;
+  uint64_t kfull, kfree, qfull[kQBufs], qfree[kQBufs], sfull[kSBufs], sfree[kSBufs], cfull[kCBufs], cfree[kCBufs], fin;
   uint32_t tmem;
   int failed;
   alignas(16) float fac[kCBufs][128];
@@ -43,12 +47,16 @@ constexpr int kSmemBytes = kOffMisc + sizeof(Misc) + 1024;
 struct ColsumArgs {
   Kv4AttnArgs a;
   Kv4Rows r;
-  float* part;  // [seqs][kv_heads][kb_max][chunks][2][128]
+  float* part;  // [seqs][kv_heads][kb_max][chunks][256]
   int kb_max, chunks;
 };
 
-__device__ __forceinline__ void cp_async4(void* dst, const void* src) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+__device__ __forceinline__ void tma2d(void* dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, "
+      "{%2, %3}], [%4];" ::"r"(smem_u32(dst)),
+      "l"(map), "r"(x), "r"(y), "r"(smem_u32(bar))
+      : "memory");
 }
 
 struct Item {
@@ -58,18 +66,18 @@ struct Item {
 };
 
 __device__ __forceinline__ int tiles_of(const Kv4Seq& s, int rep) { return (s.n * rep + 127) / 128; }
-__device__ __forceinline__ int blocks_of(const Kv4Seq& s) { return s.n > 0 ? (s.len + 127) / 128 : 0; }
+__device__ __forceinline__ int blocks_of(const Kv4Seq& s) { return s.n > 0 ? (s.len + kKeys - 1) / kKeys : 0; }
 __device__ __forceinline__ int chunks_of(const Kv4Seq& s, int rep) { return (tiles_of(s, rep) + kChunk - 1) / kChunk; }
 
-// Tiles of chunk c that see key block kb: t1 <= t0 for none.
+// Tiles of chunk c that see the keys from kb * kKeys on: t1 <= t0 for none.
 __device__ __forceinline__ void tiles_seeing(const Kv4Seq& s, int rep, int kb, int c, int& t0, int& t1) {
-  const int first = max(0, kb * 128 - (s.len - s.n));  // the first query that sees the block
+  const int first = max(0, kb * kKeys - (s.len - s.n));  // the first query that does
   t0 = static_cast<int>(static_cast<unsigned>(first * rep) / 128u) + c * kChunk;
   t1 = min(t0 + kChunk, tiles_of(s, rep));
 }
 
 __device__ __forceinline__ size_t part_at(const ColsumArgs& d, int i, int h, int kb, int c) {
-  return ((((static_cast<size_t>(i) * d.a.c.kv_heads + h) * d.kb_max + kb) * d.chunks + c) * 2) * 128;
+  return (((static_cast<size_t>(i) * d.a.c.kv_heads + h) * d.kb_max + kb) * d.chunks + c) * kKeys;
 }
 
 // Item f of all (cum: items of a kv head of the sequences before).
@@ -96,7 +104,17 @@ __device__ __forceinline__ Item item_at(const ColsumArgs& d, const long long* cu
   return w;
 }
 
-__global__ void __launch_bounds__(kThreads, 1) kv4_colsum_kernel(const ColsumArgs d) {
+// The first item from f on (in steps of the grid) that has tiles.
+__device__ __forceinline__ long long next_with_tiles(const ColsumArgs& d, const long long* cum, long long f,
+                                                     long long total) {
+  for (; f < total; f += gridDim.x) {
+    const Item w = item_at(d, cum, f);
+    if (w.t1 > w.t0) break;
+  }
+  return f;
+}
+
+__global__ void __launch_bounds__(kThreads, 1) kv4_colsum_kernel(const __grid_constant__ CUtensorMap q_map, const ColsumArgs d) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
@@ -106,12 +124,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_colsum_kernel(const ColsumArg
   const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
   const int H = a.c.kv_heads, rep = a.c.q_heads / H;
   if (tid == 0) {
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&sm.kfull[i], 4);
-      mbar_init(&sm.kfree[i], 1);
-    }
+    mbar_init(&sm.kfull, 4);
+    mbar_init(&sm.kfree, 1);
     for (int i = 0; i < kQBufs; ++i) {
-      mbar_init(&sm.qfull[i], 4);
+      mbar_init(&sm.qfull[i], 1);
       mbar_init(&sm.qfree[i], 1);
     }
     for (int i = 0; i < kSBufs; ++i) {
@@ -119,14 +135,14 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_colsum_kernel(const ColsumArg
       mbar_init(&sm.sfree[i], 4);
     }
     for (int i = 0; i < kCBufs; ++i) {
-      mbar_init(&sm.cfull[i], 4);
-      mbar_init(&sm.cfree[i], 4);
+      mbar_init(&sm.cfull[i], 1);
+      mbar_init(&sm.cfree[i], 8);
     }
     mbar_init(&sm.fin, 1);
     sm.failed = 0;
     fence_mbar_init();
   }
-  if (warp == 12) {
+  if (warp == 13) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&sm.tmem)));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
@@ -171,19 +187,18 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_colsum_kernel(const ColsumArg
     uint32_t n = 0;  // tiles so far
     for (long long f = blockIdx.x; f < total; f += gridDim.x) {
       const Item w = item_at(d, sm.cum, f);
-      const int key = w.kb * 128 + r;
+      const int key0 = w.kb * kKeys + grp * 128, key = key0 + r;
       uint64_t s0 = 0, s1 = 0;
       bool ok = true;
       for (int T = w.t0; T < w.t1; ++T, ++n) {
-        if ((n & 1u) != static_cast<uint32_t>(grp)) continue;
-        const uint32_t sb = n % kSBufs, cb = n % kCBufs;
-        ok = ok && wait(&sm.cfull[cb], n / kCBufs & 1u) && wait(&sm.sfull[sb], n / kSBufs & 1u);
+        const uint32_t sb = n % 2 * 2 + grp, cb = n % kCBufs;
+        ok = ok && wait(&sm.cfull[cb], n / kCBufs & 1u) && wait(&sm.sfull[sb], n / 2 & 1u);
         if (!ok) continue;
         fence_after();
         const uint32_t tS = sm.tmem + sb * 128 + lane_off;
         const float *fc = sm.fac[cb], *of = sm.off[cb];
-        // every row of the tile sees the whole block
-        if (w.s.len - w.s.n + 1 + T * 128 / rep >= (w.kb + 1) * 128) {
+        // every row of the tile is there and sees the whole block
+        if ((T + 1) * 128 <= w.s.n * rep && w.s.len - w.s.n + 1 + T * 128 / rep >= key0 + 128) {
           uint32_t x[32], y[32];
           auto add = [&](const uint32_t* v, int c0) {
 #pragma unroll
@@ -231,97 +246,79 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_colsum_kernel(const ColsumArg
         }
       }
       const uint64_t s = add2(s0, s1);
-      d.part[w.part + grp * 128 + r] = w.t1 > w.t0 ? lo_of(s) + hi_of(s) : 0.f;
+      if (w.t1 > w.t0) d.part[w.part + grp * 128 + r] = lo_of(s) + hi_of(s);
     }
   } else if (warp < 12) {
-    // --------------------------------------------- K codes and query tiles
-    const int dw = warp - 8, q = lane & 3, tok = lane >> 2, row = dw * 32 + lane;
-    constexpr uint32_t kAhead = 2;         // tiles in flight behind the one being issued
-    uint32_t n = 0, landed = 0, items = 0;  // tiles issued and handed on
-    bool ok = true;
-    auto hand_on = [&]() {
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(&sm.qfull[landed % kQBufs]);
-        mbar_arrive(&sm.cfull[landed % kCBufs]);
-      }
-      ++landed;
-    };
-    uint4 kc[4];
-    uint32_t ks[4];
-    auto next_item = [&](long long& f, Item& w) {  // the next with tiles, and its codes
-      for (; f < total; f += gridDim.x) {
-        w = item_at(d, sm.cum, f);
-        if (w.t1 > w.t0) break;
-      }
-      if (f >= total) return;
+    // ------------------------------------------------------- K codes, once an item
+    const int dw = warp - 8, q = lane & 3, tok = lane >> 2;
+    uint4 kc[2][4];
+    uint32_t ks[2][4], items = 0;
+    auto fetch = [&](const Item& w) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int key = w.kb * 128 + dw * 32 + e * 8 + tok, tt = key % kPageTokens;
+      for (int i = 0; i < 8; ++i) {
+        const int g = i >> 2, e = i & 3, key = w.kb * kKeys + g * 128 + dw * 32 + e * 8 + tok, tt = key % kPageTokens;
         const bool there = key < w.s.len;
         const int block = there ? max(0, kv4_block(a.c, a.c.block_table, w.s.sid, key / kPageTokens)) : 0;
         const uint8_t* slab = a.c.pages + kv4_slab_index(a.c, block, w.h) * kKv4Slab;
-        kc[e] = *reinterpret_cast<const uint4*>(slab + tt * 64 + q * 16);
+        kc[g][e] = *reinterpret_cast<const uint4*>(slab + tt * 64 + q * 16);
         // slots past the end may hold anything: scale 0
-        ks[e] = there ? *reinterpret_cast<const uint16_t*>(slab + kKv4KScales + tt * 8 + q * 2) : 0u;
+        ks[g][e] = there ? *reinterpret_cast<const uint16_t*>(slab + kKv4KScales + tt * 8 + q * 2) : 0u;
       }
     };
-    long long f = blockIdx.x;
-    Item w;
-    next_item(f, w);
-    while (f < total) {
-      const int kbuf = items & 1;
-      const uint32_t turn = (items >> 1 & 1u) ^ 1u;
-      if (!__all_sync(0xffffffffu, mbar_try_wait(&sm.kfree[kbuf], turn))) {
-        // the buffer's MMAs may need tiles that are still held back here
-        cp_async_wait();
-        while (landed < n) hand_on();
-      }
-      ok = wait(&sm.kfree[kbuf], turn);
-      if (!ok) break;
-      codes_to_tile(smem + kOffK + kbuf * kTile, dw, kc, ks);
+    long long f = next_with_tiles(d, sm.cum, blockIdx.x, total);
+    if (f < total) fetch(item_at(d, sm.cum, f));
+    for (; f < total; ++items) {
+      if (!wait(&sm.kfree, (items & 1u) ^ 1u)) break;
+      codes_to_tile(smem + kOffK, dw, kc[0], ks[0]);
+      codes_to_tile(smem + kOffK + kTile, dw, kc[1], ks[1]);
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&sm.kfull[kbuf]);
-      ++items;
-      const Item cur = w;
-      f += gridDim.x;
-      next_item(f, w);
-      for (int T = cur.t0; T < cur.t1; ++T, ++n) {
-        const uint32_t qb = n % kQBufs, cb = n % kCBufs;
-        ok = wait(&sm.qfree[qb], (n / kQBufs & 1u) ^ 1u) && wait(&sm.cfree[cb], (n / kCBufs & 1u) ^ 1u);
-        if (!ok) break;
-        const int R = T * 128 + row;
-        const bool live = R < cur.s.n * rep;
-        const int j = live ? R / rep : 0;
-        const long long at = live ? static_cast<long long>(cur.s.row0 + j) * a.c.q_heads + cur.h * rep + (R - j * rep) : -1;
-        uint8_t* tile = smem + kOffQ + qb * kTile;
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int rr = 2 * e + (lane >> 4), c = lane & 15;
-          const long long from = __shfl_sync(0xffffffffu, at, rr);
-          cp_async16(tile + (c >> 3) * kHalf + (dw * 32 + rr) * 128 + (((c & 7) ^ (rr & 7)) << 4),
-                     d.r.q16 + (from < 0 ? 0 : from) * kHeadDim + c * 8, from >= 0);
-        }
-        if (live) {
-          cp_async4(&sm.fac[cb][row], d.r.fac + at);
-          cp_async4(&sm.off[cb][row], d.r.off + at);
-        } else {
-          sm.fac[cb][row] = 0.f;
-          sm.off[cb][row] = -INFINITY;
-        }
-        sm.seen[cb][row] = live ? cur.s.len - cur.s.n + 1 + j : 0;
-        asm volatile("cp.async.commit_group;" ::: "memory");
-        if (n - landed >= kAhead) {
-          asm volatile("cp.async.wait_group %0;" ::"n"(kAhead) : "memory");
-          hand_on();
-        }
-      }
-      if (!ok) break;
+      if (lane == 0) mbar_arrive(&sm.kfull);
+      f = next_with_tiles(d, sm.cum, f + gridDim.x, total);
+      if (f < total) fetch(item_at(d, sm.cum, f));
     }
-    cp_async_wait();
-    while (landed < n) hand_on();
+  } else if (warp == 12) {
+    // ------------------------------------- query tiles (TMA) and their constants
+    uint32_t n = 0, issued = 0;
+    bool ok = true;
+    for (long long f = blockIdx.x; f < total && ok; f += gridDim.x) {
+      const Item w = item_at(d, sm.cum, f);
+      const int y0 = (w.h * a.rows + w.s.row0) * rep;  // the sequence's first row of the kv head
+      for (int T = w.t0; T < w.t1; ++T, ++n) {
+        const uint32_t qb = n % kQBufs, cb = n % kCBufs;
+        float fv[4], ov[4];
+        int sv[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int R = T * 128 + e * 32 + lane;
+          const bool live = R < w.s.n * rep;
+          fv[e] = live ? d.r.fac[y0 + R] : 0.f;
+          ov[e] = live ? d.r.off[y0 + R] : -INFINITY;
+          sv[e] = live ? w.s.len - w.s.n + 1 + R / rep : 0;
+        }
+        ok = wait(&sm.qfree[qb], (n / kQBufs & 1u) ^ 1u);
+        if (!ok) break;
+        if (lane == 0) {
+          mbar_arrive_expect_tx(&sm.qfull[qb], kTile);
+          tma2d(smem + kOffQ + qb * kTile, &q_map, 0, y0 + T * 128, &sm.qfull[qb]);
+          tma2d(smem + kOffQ + qb * kTile + kHalf, &q_map, 64, y0 + T * 128, &sm.qfull[qb]);
+        }
+        ++issued;
+        ok = wait(&sm.cfree[cb], (n / kCBufs & 1u) ^ 1u);
+        if (!ok) break;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          sm.fac[cb][e * 32 + lane] = fv[e];
+          sm.off[cb][e * 32 + lane] = ov[e];
+          sm.seen[cb][e * 32 + lane] = sv[e];
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.cfull[cb]);
+      }
+    }
+    // every copy has landed before the block ends
+    for (uint32_t i = issued > kQBufs ? issued - kQBufs : 0; i < issued; ++i)
+      mbar_wait(&sm.qfull[i % kQBufs], i / kQBufs & 1u, a.c.status, kStatusKv4Colsum);
   } else {
     // ------------------------------------------------------------------ MMA
     const uint32_t tm = __shfl_sync(0xffffffffu, sm.tmem, 0);
@@ -333,24 +330,30 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_colsum_kernel(const ColsumArg
       const Item w = item_at(d, sm.cum, f);
       const int t0 = __shfl_sync(0xffffffffu, w.t0, 0), t1 = __shfl_sync(0xffffffffu, w.t1, 0);
       if (t1 <= t0) continue;
-      const uint32_t kbuf = items & 1;
-      ok = wait(&sm.kfull[kbuf], items >> 1 & 1u);
-      const uint64_t k0 = dk + kbuf * (kTile >> 4);
+      ok = wait(&sm.kfull, items & 1u);
       for (int T = t0; T < t1 && ok; ++T, ++n) {
-        const uint32_t qb = n % kQBufs, sb = n % kSBufs;
-        ok = wait(&sm.qfull[qb], n / kQBufs & 1u) && wait(&sm.sfree[sb], (n / kSBufs & 1u) ^ 1u);
-        if (!ok) break;
-        fence_after();
+        const uint32_t qb = n % kQBufs;
+        ok = wait(&sm.qfull[qb], n / kQBufs & 1u);
         const uint64_t q0 = dq + qb * (kTile >> 4);
-        if (leader) {
 #pragma unroll
-          for (int i = 0; i < kHeadDim / 16; ++i) {
-            const uint64_t off = ((i >> 2) * kHalf + (i & 3) * 32) >> 4;
-            mma_ss(tm + sb * 128, k0 + off, q0 + off, idesc(false), i > 0 ? 1u : 0u);
+        for (int g = 0; g < 2; ++g) {
+          const uint32_t sb = n % 2 * 2 + g;
+          ok = ok && wait(&sm.sfree[sb], (n / 2 & 1u) ^ 1u);
+          if (!ok) break;
+          fence_after();
+          if (leader) {
+#pragma unroll
+            for (int i = 0; i < kHeadDim / 16; ++i) {
+              const uint64_t off = ((i >> 2) * kHalf + (i & 3) * 32) >> 4;
+              mma_ss(tm + sb * 128, dk + g * (kTile >> 4) + off, q0 + off, idesc(false), i > 0 ? 1u : 0u);
+            }
+            commit(&sm.sfull[sb]);
           }
-          commit(&sm.sfull[sb]);
+          __syncwarp();
+        }
+        if (ok && leader) {
           commit(&sm.qfree[qb]);
-          if (T + 1 == t1) commit(&sm.kfree[kbuf]);
+          if (T + 1 == t1) commit(&sm.kfree);
         }
         __syncwarp();
       }
@@ -365,15 +368,15 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_colsum_kernel(const ColsumArg
   fence_before();
   __syncthreads();
   fence_after();
-  if (warp == 12)
+  if (warp == 13)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(sm.tmem));
 }
 
-// weights of a key block: its items' sums in order, one thread a slot.
-__global__ void __launch_bounds__(128) kv4_colsum_add_kernel(const ColsumArgs d) {
+// weights of 256 keys: their items' sums in order, one thread a slot.
+__global__ void __launch_bounds__(kKeys) kv4_colsum_add_kernel(const ColsumArgs d) {
   const Kv4AttnArgs& a = d.a;
   const int kb = blockIdx.x, h = blockIdx.y, i = blockIdx.z, rep = a.c.q_heads / a.c.kv_heads;
-  const int key = kb * 128 + threadIdx.x;
+  const int key = kb * kKeys + threadIdx.x;
   pdl_wait();
   Kv4Seq s;
   if (!kv4_seq(a, i, s) || s.n == 0 || key >= s.len) return;
@@ -382,15 +385,14 @@ __global__ void __launch_bounds__(128) kv4_colsum_add_kernel(const ColsumArgs d)
     int t0, t1;
     tiles_seeing(s, rep, kb, c, t0, t1);
     if (t1 <= t0) break;
-    const float* p = d.part + part_at(d, i, h, kb, c) + threadIdx.x;
-    sum += p[0] + p[128];
+    sum += d.part[part_at(d, i, h, kb, c) + threadIdx.x];
   }
   const int block = kv4_block(a.c, a.c.block_table, s.sid, key / kPageTokens);
   if (block >= 0) a.c.weights[kv4_slab_index(a.c, block, h) * kPageTokens + key % kPageTokens] += sum;
 }
 
-template <typename K>
-cudaError_t start(K kernel, dim3 grid, int threads, size_t smem, cudaStream_t s, const ColsumArgs& d) {
+template <typename K, typename... Args>
+cudaError_t start(K kernel, dim3 grid, int threads, size_t smem, cudaStream_t s, const Args&... args) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(threads);
@@ -401,7 +403,36 @@ cudaError_t start(K kernel, dim3 grid, int threads, size_t smem, cudaStream_t s,
   at.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &at;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, d);
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
+                                   const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                   const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                   CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiledFn encode_fn() {
+  static EncodeTiledFn fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q{};
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      return static_cast<EncodeTiledFn>(nullptr);
+    return reinterpret_cast<EncodeTiledFn>(p);
+  }();
+  return fn;
+}
+
+// The f16 queries as rows of 128, boxes of 128 rows by 64 dims; rows past the end
+// read as zeros.
+bool q_map_of(const Kv4Rows& r, uint64_t rows, CUtensorMap* m) {
+  EncodeTiledFn enc = encode_fn();
+  if (!enc) return false;
+  const cuuint64_t dims[2] = {kHeadDim, rows}, strides[1] = {kHeadDim * 2};
+  const cuuint32_t box[2] = {64, 128}, one[2] = {1, 1};
+  return enc(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, r.q16, dims, strides, box, one,
+             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 long long chunks_max(int rep, long long max_q) {
@@ -414,13 +445,15 @@ long long chunks_max(int rep, long long max_q) {
 size_t kv4_colsum_scratch(int q_heads, int kv_heads, long long seqs, long long max_q,
                           long long max_len) {
   const long long n = seqs < kSeqChunk ? seqs : kSeqChunk;
-  return static_cast<size_t>(n) * kv_heads * ((max_len + 127) / 128) * chunks_max(q_heads / kv_heads, max_q) * 2 *
-         128 * sizeof(float);
+  return static_cast<size_t>(n) * kv_heads * ((max_len + kKeys - 1) / kKeys) * chunks_max(q_heads / kv_heads, max_q) *
+         kKeys * sizeof(float);
 }
 
 cudaError_t kv4_colsum_launch(const Kv4AttnArgs& a, const Kv4Rows& rows, void* scratch,
                               cudaStream_t s) {
   if (a.max_len == 0) return cudaSuccess;
+  CUtensorMap map;
+  if (!q_map_of(rows, static_cast<uint64_t>(a.rows) * a.c.q_heads, &map)) return cudaErrorNotSupported;
   cudaError_t e = cudaFuncSetAttribute(kv4_colsum_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
   for (int at = 0; at < a.seqs && e == cudaSuccess; at += kSeqChunk) {
     ColsumArgs d{};
@@ -431,11 +464,11 @@ cudaError_t kv4_colsum_launch(const Kv4AttnArgs& a, const Kv4Rows& rows, void* s
     if (a.q_starts) d.a.q_starts = a.q_starts + at;
     d.r = rows;
     d.part = static_cast<float*>(scratch);
-    d.kb_max = (a.max_len + 127) / 128;
+    d.kb_max = (a.max_len + kKeys - 1) / kKeys;
     d.chunks = static_cast<int>(chunks_max(a.c.q_heads / a.c.kv_heads, a.max_q));
-    e = start(kv4_colsum_kernel, dim3(148), kThreads, kSmemBytes, s, d);
+    e = start(kv4_colsum_kernel, dim3(148), kThreads, kSmemBytes, s, map, d);
     if (e == cudaSuccess)
-      e = start(kv4_colsum_add_kernel, dim3(d.kb_max, a.c.kv_heads, d.a.seqs), 128, 0, s, d);
+      e = start(kv4_colsum_add_kernel, dim3(d.kb_max, a.c.kv_heads, d.a.seqs), kKeys, 0, s, d);
   }
   return e;
 }

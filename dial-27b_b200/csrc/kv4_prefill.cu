@@ -67,6 +67,12 @@ struct PrefillArgs {
   float* off;
 };
 
+// Place of (row, query head) in the arrays that the weights' kernel reads.
+__device__ __forceinline__ size_t row_at(const Kv4AttnArgs& a, int row, int head) {
+  const int rep = a.c.q_heads / a.c.kv_heads, h = head / rep;
+  return (static_cast<size_t>(h) * a.rows + row) * rep + (head - h * rep);
+}
+
 // --------------------------------------------------------------- work items
 // Key blocks that tile T (128 rows) of the sequence sees.  n * rep < 2^29.
 __device__ __forceinline__ int tile_blocks(const Kv4Seq& s, unsigned rep, int T) {
@@ -237,7 +243,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const PrefillA
             make_uint4(0, 0, 0, 0);
       if (d.off)
         for (int e = tid; e < a.c.q_heads; e += kThreads)
-          d.off[static_cast<size_t>(s.row0 + r) * a.c.q_heads + e] = -INFINITY;
+          d.off[row_at(a, s.row0 + r, e)] = -INFINITY;
     }
   }
   const int ctas = static_cast<int>(min(static_cast<long long>(d.ctas), total));
@@ -347,9 +353,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const PrefillA
             o[u] = pack_f16(ActTraits<Act>::to_f(v[2 * u]) * down, ActTraits<Act>::to_f(v[2 * u + 1]) * down);
           *at = make_uint4(o[0], o[1], o[2], o[3]);
           if (keep_q)
-            reinterpret_cast<uint4*>(d.q16 + (static_cast<size_t>(w.s.row0 + j) * a.c.q_heads + head) * kHeadDim)[e] = *at;
+            reinterpret_cast<uint4*>(d.q16 + row_at(a, w.s.row0 + j, head) * kHeadDim)[e] = *at;
         }
-        if (keep_q) d.fac[static_cast<size_t>(w.s.row0 + j) * a.c.q_heads + head] = fac;
+        if (keep_q) d.fac[row_at(a, w.s.row0 + j, head)] = fac;
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&sm.qfull[t]);
@@ -492,7 +498,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const PrefillA
         if (!whole)
           d.part_ml[static_cast<size_t>(slot) * 2 * kRows + t * kRows + r] = make_float2(l > 0.f || l != l ? m : -INFINITY, l);
         else if (d.off)
-          d.off[static_cast<size_t>(w.s.row0 + j) * a.c.q_heads + head] = l > 0.f ? -(m + log2f(l)) : -INFINITY;
+          d.off[row_at(a, w.s.row0 + j, head)] = l > 0.f ? -(m + log2f(l)) : -INFINITY;
       }
       if (f >= f1 || !ok) {
         // the only item of the range that can start in it and go on
@@ -703,7 +709,7 @@ __global__ void __launch_bounds__(256) kv4_prefill_join_kernel(const PrefillArgs
   const float o[4] = {O.x * inv, O.y * inv, O.z * inv, O.w * inv};
   store4(static_cast<Act*>(a.out) + (s.row0 + j) * a.out_ld + head * kHeadDim + lane * 4, o);
   if (d.off && lane == 0)
-    d.off[static_cast<size_t>(s.row0 + j) * a.c.q_heads + head] = L > 0.f ? -(M + log2f(L)) : -INFINITY;
+    d.off[row_at(a, s.row0 + j, head)] = L > 0.f ? -(M + log2f(L)) : -INFINITY;
 }
 
 int range_count() {
