@@ -18,6 +18,7 @@
 #include <cuda.h>
 
 #include "kv4_attn.h"
+#include "kv4_launch.h"
 #include "kv4_tc.cuh"
 
 namespace dialb200 {
@@ -391,21 +392,6 @@ __global__ void __launch_bounds__(kKeys) kv4_colsum_add_kernel(const ColsumArgs 
   if (block >= 0) a.c.weights[kv4_slab_index(a.c, block, h) * kPageTokens + key % kPageTokens] += sum;
 }
 
-template <typename K, typename... Args>
-cudaError_t start(K kernel, dim3 grid, int threads, size_t smem, cudaStream_t s, const Args&... args) {
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = s;
-  cudaLaunchAttribute at{};
-  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &at;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, args...);
-}
-
 using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
                                    const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
                                    const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
@@ -454,7 +440,7 @@ cudaError_t kv4_colsum_launch(const Kv4AttnArgs& a, const Kv4Rows& rows, void* s
   if (a.max_len == 0) return cudaSuccess;
   CUtensorMap map;
   if (!q_map_of(rows, static_cast<uint64_t>(a.rows) * a.c.q_heads, &map)) return cudaErrorNotSupported;
-  cudaError_t e = cudaFuncSetAttribute(kv4_colsum_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+  cudaError_t e = kv4_allow_smem<kv4_colsum_kernel>(kSmemBytes);
   for (int at = 0; at < a.seqs && e == cudaSuccess; at += kSeqChunk) {
     ColsumArgs d{};
     d.a = a;
@@ -466,9 +452,9 @@ cudaError_t kv4_colsum_launch(const Kv4AttnArgs& a, const Kv4Rows& rows, void* s
     d.part = static_cast<float*>(scratch);
     d.kb_max = (a.max_len + kKeys - 1) / kKeys;
     d.chunks = static_cast<int>(chunks_max(a.c.q_heads / a.c.kv_heads, a.max_q));
-    e = start(kv4_colsum_kernel, dim3(148), kThreads, kSmemBytes, s, map, d);
+    e = kv4_start(kv4_colsum_kernel, dim3(148), kThreads, kSmemBytes, s, map, d);
     if (e == cudaSuccess)
-      e = start(kv4_colsum_add_kernel, dim3(d.kb_max, a.c.kv_heads, d.a.seqs), kKeys, 0, s, d);
+      e = kv4_start(kv4_colsum_add_kernel, dim3(d.kb_max, a.c.kv_heads, d.a.seqs), kKeys, 0, s, d);
   }
   return e;
 }

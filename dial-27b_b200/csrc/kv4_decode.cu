@@ -32,6 +32,7 @@
 
 #include "kv4_attn.h"
 #include "kv4_dev.cuh"
+#include "kv4_launch.h"
 
 namespace dialb200 {
 namespace {
@@ -46,6 +47,7 @@ template <int NT>
 constexpr int kCtasPerSm = NT == 1 ? 2 : 3;
 constexpr int kRing = 4;           // pages in flight a warp
 constexpr int kSeqChunk = 512;     // sequences a launch
+constexpr int kOneLen = 512;       // slots up to which a CTA takes a whole segment
 constexpr float kRaise = 8.f;      // log2 headroom of a probability above 1
 constexpr int kColStride = kHeadDim + 8;
 
@@ -53,6 +55,8 @@ struct DecodeArgs {
   Kv4AttnArgs a;
   int groups;       // column groups of NT * 8
   int ctas;         // ranges
+  int one;          // every CTA takes one whole segment: ctas = segments, no join
+  int pages_max;    // of a sequence
   int score_ld;     // floats a slot in `scores`
   int join_y;       // CTAs of the join that a segment's columns are dealt to
   int4* desc;       // [ctas]: the segment that starts in a range and goes on
@@ -61,9 +65,10 @@ struct DecodeArgs {
   float* scores;    // [pages of all segments][16][score_ld] or null
 };
 
-// cum[i]: pages of the sequences before i; the block's threads share the scan.
+// cum[i]: pages of the sequences before first + i of `seqs`; the block's threads
+// share the scan.
 template <int THREADS>
-__device__ __forceinline__ void page_prefix(const Kv4AttnArgs& a, int* cum, int* sums) {
+__device__ __forceinline__ void page_prefix(const Kv4AttnArgs& a, int first, int seqs, int* cum, int* sums) {
   constexpr int PER = kSeqChunk / THREADS;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   int v[PER], total = 0;
@@ -72,7 +77,7 @@ __device__ __forceinline__ void page_prefix(const Kv4AttnArgs& a, int* cum, int*
     const int i = tid * PER + e;
     Kv4Seq s;
     v[e] = 0;
-    if (i < a.seqs && kv4_seq(a, i, s) && s.n > 0) v[e] = (s.len + kPageTokens - 1) / kPageTokens;
+    if (i < seqs && kv4_seq(a, first + i, s) && s.n > 0) v[e] = (s.len + kPageTokens - 1) / kPageTokens;
     total += v[e];
   }
   int run = total;
@@ -88,10 +93,10 @@ __device__ __forceinline__ void page_prefix(const Kv4AttnArgs& a, int* cum, int*
 #pragma unroll
   for (int e = 0; e < PER; ++e) {
     const int i = tid * PER + e;
-    if (i <= a.seqs) cum[i] = before;
+    if (i <= seqs) cum[i] = before;
     before += v[e];
   }
-  if (tid == THREADS - 1 && a.seqs == kSeqChunk) cum[kSeqChunk] = before;
+  if (tid == THREADS - 1 && seqs == kSeqChunk) cum[kSeqChunk] = before;
   __syncthreads();
 }
 
@@ -174,11 +179,34 @@ struct DecodeSmem {
   float o[kWarps][8][kColStride];
   uint8_t q[2][NT * 8][kHeadDim * 2];  // this segment's queries and the next one's
   float ml[kWarps][8][2];
+  float2 fin[NT * 8];  // (m, 1 / l) of the only segment
   uint64_t full[kWarps][kSlots];
   uint64_t merged;  // every warp has read the parts in o and ml
   int cum[kSeqChunk + 1];
   int sums[kWarps];
 };
+
+// The probabilities of slot t (scores x, the columns' (m, 1 / l) in ml) into its
+// running weight.
+__device__ __forceinline__ void add_weight(const DecodeArgs& d, const Kv4Seq& s, int h, int t, const float* x,
+                                           const float2* ml, int cols) {
+  const Kv4AttnArgs& a = d.a;
+  const int block = kv4_block(a.c, a.c.block_table, s.sid, t / kPageTokens);
+  float* to = a.c.weights + kv4_slab_index(a.c, max(block, 0), h) * kPageTokens + t % kPageTokens;
+  const float old = *to;
+  float sum = 0.f;
+  int col = 0;
+  if ((d.score_ld & 3) == 0)
+    for (; col + 4 <= cols; col += 4) {
+      const float4 v = *reinterpret_cast<const float4*>(x + col);
+      sum = fmaf(ex2(v.x - ml[col].x), ml[col].y, sum);
+      sum = fmaf(ex2(v.y - ml[col + 1].x), ml[col + 1].y, sum);
+      sum = fmaf(ex2(v.z - ml[col + 2].x), ml[col + 2].y, sum);
+      sum = fmaf(ex2(v.w - ml[col + 3].x), ml[col + 3].y, sum);
+    }
+  for (; col < cols; ++col) sum = fmaf(ex2(x[col] - ml[col].x), ml[col].y, sum);
+  if (block >= 0) *to = old + sum;
+}
 
 // One segment's share of a range.
 struct Share {
@@ -203,23 +231,35 @@ __global__ void __launch_bounds__(kWarpsOf<NT> * 32, kCtasPerSm<NT>)
     if (warp == 0) mbar_init(&sm.merged, kWarps);
     fence_mbar_init();
   }
-  page_prefix<kWarps * 32>(a, sm.cum, sm.sums);
-  const int total = sm.cum[a.seqs] * H;
-  // sequences without a slot: zeros
-  for (int i = b; i < a.seqs; i += d.ctas) {
+  // sequences of this CTA's work: all of the call, or one
+  const int si0 = d.one ? b / H : 0, seqs = d.one ? 1 : a.seqs, b_of = d.one ? b - si0 * H : b;
+  if (d.one) {
     Kv4Seq s;
-    if (sm.cum[i + 1] != sm.cum[i] || !kv4_seq(a, i, s) || blockIdx.y != 0) continue;
+    if (tid == 0) {
+      sm.cum[0] = 0;
+      sm.cum[1] = kv4_seq(a, si0, s) && s.n > 0 ? (s.len + kPageTokens - 1) / kPageTokens : 0;
+    }
+    __syncthreads();
+  } else {
+    page_prefix<kWarps * 32>(a, 0, seqs, sm.cum, sm.sums);
+  }
+  const int total = sm.cum[seqs] * H;
+  // sequences without a slot: zeros
+  for (int i = b_of; i < seqs; i += d.ctas) {
+    Kv4Seq s;
+    if (sm.cum[i + 1] != sm.cum[i] || !kv4_seq(a, si0 + i, s) || blockIdx.y != 0) continue;
     for (int r = 0; r < s.n; ++r)
       for (int e = tid * 8; e < a.c.q_heads * kHeadDim; e += kWarps * 32 * 8)
         *reinterpret_cast<uint4*>(static_cast<Act*>(a.out) + (s.row0 + r) * a.out_ld + e) =
             make_uint4(0, 0, 0, 0);
   }
-  const int ctas = ranges_of(total, d.ctas, kWarps);
-  if (b >= ctas) {
-    if (tid == 0 && blockIdx.y == 0) d.desc[b] = make_int4(-1, 0, 0, 0);
+  const int ctas = d.one ? (total > 0 ? H : 0) : ranges_of(total, d.ctas, kWarps);
+  if (b_of >= ctas) {
+    if (tid == 0 && blockIdx.y == 0 && !d.one) d.desc[b] = make_int4(-1, 0, 0, 0);
     return;
   }
-  const int f0 = range_start(total, b, ctas), f1 = range_start(total, b + 1, ctas);
+  // with one segment a CTA the ranges are the sequence's kv heads
+  const int f0 = range_start(total, b_of, ctas), f1 = range_start(total, b_of + 1, ctas);
 
   // this warp's pages: f0 + warp + kWarps * i, i < mine; each lane holds the slab
   // number of one page of a window of 32 and copies that page itself; the next
@@ -228,9 +268,9 @@ __global__ void __launch_bounds__(kWarpsOf<NT> * 32, kCtasPerSm<NT>)
   auto slab_of = [&](int i) -> int {
     if (i >= mine) return 0;
     const int f = f0 + warp + kWarps * i;
-    const int s = seq_at(sm.cum, a.seqs, f / H);
+    const int s = seq_at(sm.cum, seqs, f / H);
     const int np = sm.cum[s + 1] - sm.cum[s], r = f - sm.cum[s] * H;
-    return max(0, kv4_block(a.c, a.c.block_table, a.sids[s], r % np)) * H + r / np;
+    return max(0, kv4_block(a.c, a.c.block_table, a.sids[si0 + s], r % np)) * H + r / np;
   };
   int win = slab_of(lane), win_next = slab_of(32 + lane), issued = 0;
   auto issue = [&]() {  // the next U pages into their slot; warp-uniform
@@ -250,14 +290,14 @@ __global__ void __launch_bounds__(kWarpsOf<NT> * 32, kCtasPerSm<NT>)
 
   auto share_at = [&](int f) {
     Share w;
-    const int si = seq_at(sm.cum, a.seqs, f / H);
+    const int si = seq_at(sm.cum, seqs, f / H);
     const int np = sm.cum[si + 1] - sm.cum[si], base = sm.cum[si] * H;
     w.h = (f - base) / np;
     w.seg = si * H + w.h;
     w.seg0 = base + w.h * np;
     w.seg1 = w.seg0 + np;
     w.end = min(f1, w.seg1);
-    kv4_seq(a, si, w.s);
+    kv4_seq(a, si0 + si, w.s);
     return w;
   };
   auto load_q = [&](const Share& w, int buf) {
@@ -271,6 +311,8 @@ __global__ void __launch_bounds__(kWarpsOf<NT> * 32, kCtasPerSm<NT>)
     }
   };
 
+  // scores of the sequences before this CTA's (one segment a CTA)
+  const size_t score0 = static_cast<size_t>(si0) * H * d.pages_max * kPageTokens;
   int done = 0, buf = 0;
   uint32_t shares = 0;
   bool ok = true;
@@ -386,7 +428,7 @@ __global__ void __launch_bounds__(kWarpsOf<NT> * 32, kCtasPerSm<NT>)
           if (cc < cols)
 #pragma unroll
             for (int u = 0; u < N; ++u) {
-              float* to = d.scores + (static_cast<size_t>(w.seg0 + page0 + kWarps * u) * kPageTokens + t0) * d.score_ld + cc;
+              float* to = d.scores + (score0 + static_cast<size_t>(w.seg0 + page0 + kWarps * u) * kPageTokens + t0) * d.score_ld + cc;
               *reinterpret_cast<float2*>(to) = make_float2(x[u][nt][0] * fac[nt][0], x[u][nt][1] * fac[nt][1]);
               *reinterpret_cast<float2*>(to + 8 * d.score_ld) =
                   make_float2(x[u][nt][2] * fac[nt][0], x[u][nt][3] * fac[nt][1]);
@@ -525,12 +567,22 @@ __global__ void __launch_bounds__(kWarpsOf<NT> * 32, kCtasPerSm<NT>)
               ActTraits<Act>::from_f(L != 0.f ? O / L * a.c.v_scale : 0.f);
         else
           d.part_o[(part + cl) * kHeadDim + at] = O;
-        if ((!whole || SCORES) && at == 0)
+        if (SCORES && at == 0 && d.one)
+          sm.fin[nt * 8 + cl] = make_float2(M == -INFINITY ? 0.f : M, L > 0.f ? 1.f / L : 0.f);
+        else if ((!whole || SCORES) && at == 0)
           *reinterpret_cast<float2*>(d.part_ml + (part + cl) * 2) = make_float2(M, L);
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&sm.merged);
     }
+    if (SCORES && d.one) {  // this CTA's scores, all of the segment's columns
+      __syncthreads();
+      for (int t = tid; t < w.s.len; t += kWarps * 32)
+        add_weight(d, w.s, w.h, t, d.scores + (score0 + static_cast<size_t>(w.seg0) * kPageTokens + t) * d.score_ld,
+                   sm.fin, cols);
+      break;
+    }
+    if (d.one) break;
     if (fe == f1) {
       // the only segment of the range that can start in it and go on
       if (tid == 0 && blockIdx.y == 0)
@@ -622,7 +674,7 @@ __global__ void __launch_bounds__(kJoinThreads) kv4_join_kernel(const DecodeArgs
   __shared__ int cum[kSeqChunk + 1];
   __shared__ int sums[kJoinWarps];
   __shared__ float2 ml[kKv4DecodeCols];  // (m, 1 / l) of the segment's columns
-  page_prefix<kJoinThreads>(a, cum, sums);
+  page_prefix<kJoinThreads>(a, 0, a.seqs, cum, sums);
   pdl_wait();
   const int total = cum[a.seqs] * H;
   const int ctas = ranges_of(total, d.ctas, kWarpsOf<NT>);
@@ -647,22 +699,7 @@ __global__ void __launch_bounds__(kJoinThreads) kv4_join_kernel(const DecodeArgs
     __syncthreads();
     const int upto = min((fe - seg0) * kPageTokens, s.len);
     for (int t = (fc - seg0) * kPageTokens + y * kJoinThreads + tid; t < upto; t += ys * kJoinThreads) {
-      const int block = kv4_block(a.c, a.c.block_table, s.sid, t / kPageTokens);
-      float* to = a.c.weights + kv4_slab_index(a.c, max(block, 0), h) * kPageTokens + t % kPageTokens;
-      const float old = *to;
-      const float* x = d.scores + (static_cast<size_t>(seg0) * kPageTokens + t) * d.score_ld;
-      float sum = 0.f;
-      int col = 0;
-      if ((d.score_ld & 3) == 0)
-        for (; col + 4 <= cols; col += 4) {
-          const float4 v = *reinterpret_cast<const float4*>(x + col);
-          sum = fmaf(ex2(v.x - ml[col].x), ml[col].y, sum);
-          sum = fmaf(ex2(v.y - ml[col + 1].x), ml[col + 1].y, sum);
-          sum = fmaf(ex2(v.z - ml[col + 2].x), ml[col + 2].y, sum);
-          sum = fmaf(ex2(v.w - ml[col + 3].x), ml[col + 3].y, sum);
-        }
-      for (; col < cols; ++col) sum = fmaf(ex2(x[col] - ml[col].x), ml[col].y, sum);
-      if (block >= 0) *to = old + sum;
+      add_weight(d, s, h, t, d.scores + (static_cast<size_t>(seg0) * kPageTokens + t) * d.score_ld, ml, cols);
     }
     __syncthreads();
     fc = fe;
@@ -682,7 +719,8 @@ int sm_count() {
 
 // Sizes of one launch over `seqs` sequences.
 struct Plan {
-  int nt, groups, ctas, cols, score_ld;
+  int nt, groups, ctas, cols, score_ld, pages_max;
+  bool one;
   long long pages;  // pages of all segments at most
   size_t desc, part_o, part_ml, scores;
 };
@@ -697,14 +735,20 @@ Plan plan_of(int q_heads, int kv_heads, long long seqs, long long max_q, long lo
   const long long per = (max_len + kPageTokens - 1) / kPageTokens;
   p.pages = seqs * per * kv_heads;
   // a page a warp at least, as many CTAs as are resident at once at most
+  p.pages_max = static_cast<int>(per);
+  // Short sequences: a CTA for each segment, which nothing has to join.  A
+  // segment of kOneLen slots takes one CTA about as long as the join of ranges
+  // (3 us) and its launch; the weights of several column groups need the join.
+  p.one = max_len <= kOneLen && !(weights && p.groups > 1);
   const int warps = p.nt == 1 ? kWarpsOf<1> : kWarpsOf<2>;
   const long long want = (p.pages + warps - 1) / warps;
   long long most = static_cast<long long>(sms) * (p.nt == 1 ? kCtasPerSm<1> : kCtasPerSm<2>) / p.groups;
   if (most < sms / 4) most = sms / 4;
   p.ctas = static_cast<int>(want < 1 ? 1 : want < most ? want : most);
+  if (p.one) p.ctas = static_cast<int>(seqs * kv_heads);
   p.score_ld = (p.cols + 1) & ~1;
   auto up = [](size_t v) { return (v + 127) & ~static_cast<size_t>(127); };
-  const size_t rows = static_cast<size_t>(p.ctas + seqs * kv_heads) * p.groups * p.nt * 8;
+  const size_t rows = p.one ? 0 : static_cast<size_t>(p.ctas + seqs * kv_heads) * p.groups * p.nt * 8;
   p.desc = up(static_cast<size_t>(p.ctas) * sizeof(int4));
   p.part_o = up(rows * kHeadDim * 4);
   p.part_ml = up(rows * 8);
@@ -721,30 +765,21 @@ long long chunk_of(int kv_heads, long long seqs, long long max_len) {
   return n < seqs ? n : seqs;
 }
 
-template <typename K>
-cudaError_t start(K kernel, dim3 grid, int threads, size_t smem, cudaStream_t s, const DecodeArgs& d) {
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = s;
-  cudaLaunchAttribute at{};
-  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &at;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, d);
-}
-
 template <typename Act, int NT>
 cudaError_t launch_nt(const DecodeArgs& d, cudaStream_t s) {
   const size_t smem = sizeof(DecodeSmem<NT>);
-  auto kernel = d.scores ? kv4_decode_kernel<Act, NT, true> : kv4_decode_kernel<Act, NT, false>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-  if (e != cudaSuccess) return e;
-  e = start(kernel, dim3(d.ctas, d.groups), kWarpsOf<NT> * 32, smem, s, d);
-  if (e != cudaSuccess) return e;
-  return start(kv4_join_kernel<Act, NT>, dim3(d.ctas, d.join_y + (d.scores ? 2 : 0)), kJoinThreads, 0, s, d);
+  cudaError_t e;
+  if (d.scores) {
+    e = kv4_allow_smem<kv4_decode_kernel<Act, NT, true>>(smem);
+    if (e == cudaSuccess)
+      e = kv4_start(kv4_decode_kernel<Act, NT, true>, dim3(d.ctas, d.groups), kWarpsOf<NT> * 32, smem, s, d);
+  } else {
+    e = kv4_allow_smem<kv4_decode_kernel<Act, NT, false>>(smem);
+    if (e == cudaSuccess)
+      e = kv4_start(kv4_decode_kernel<Act, NT, false>, dim3(d.ctas, d.groups), kWarpsOf<NT> * 32, smem, s, d);
+  }
+  if (e != cudaSuccess || d.one) return e;
+  return kv4_start(kv4_join_kernel<Act, NT>, dim3(d.ctas, d.join_y + (d.scores ? 2 : 0)), kJoinThreads, 0, s, d);
 }
 
 }  // namespace
@@ -777,6 +812,8 @@ cudaError_t kv4_decode_launch(const Kv4AttnArgs& a, int act, cudaStream_t s) {
                            a.c.weights != nullptr, sms);
     d.groups = p.groups;
     d.ctas = p.ctas;
+    d.one = p.one;
+    d.pages_max = p.pages_max;
     d.score_ld = p.score_ld;
     uint8_t* w = static_cast<uint8_t*>(a.scratch);
     d.desc = reinterpret_cast<int4*>(w);

@@ -24,6 +24,7 @@
 #include <cmath>
 
 #include "kv4_attn.h"
+#include "kv4_launch.h"
 #include "kv4_tc.cuh"
 
 namespace dialb200 {
@@ -727,28 +728,13 @@ constexpr size_t kDescBytes = 148 * 16 + 128 - (148 * 16) % 128;
 constexpr size_t kPartBytes = 2ull * 148 * 2 * kRows * kHeadDim * 4;
 constexpr size_t kMlBytes = 2ull * 148 * 2 * kRows * 8;
 
-template <typename K>
-cudaError_t start(K kernel, dim3 grid, int threads, size_t smem, cudaStream_t s, const PrefillArgs& d) {
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = s;
-  cudaLaunchAttribute at{};
-  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &at;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, d);
-}
-
 template <typename Act>
 cudaError_t launch(const PrefillArgs& d, cudaStream_t s) {
-  cudaError_t e = cudaFuncSetAttribute(kv4_prefill_kernel<Act>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+  cudaError_t e = kv4_allow_smem<kv4_prefill_kernel<Act>>(kSmemBytes);
   if (e != cudaSuccess) return e;
-  e = start(kv4_prefill_kernel<Act>, dim3(d.ctas), kThreads, kSmemBytes, s, d);
+  e = kv4_start(kv4_prefill_kernel<Act>, dim3(d.ctas), kThreads, kSmemBytes, s, d);
   if (e != cudaSuccess) return e;
-  return start(kv4_prefill_join_kernel<Act>, dim3(d.ctas, 2 * kRows / 8), 256, 0, s, d);
+  return kv4_start(kv4_prefill_join_kernel<Act>, dim3(d.ctas, 2 * kRows / 8), 256, 0, s, d);
 }
 
 }  // namespace

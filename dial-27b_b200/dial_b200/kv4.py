@@ -11,7 +11,9 @@ reference's cache (llama3/cache.rs:9-265) holds the activation dtype and slides
 instead.
 
 Every op runs on the current stream of its tensors' device, allocates only its
-results and, unless given, its scratch, and does not synchronise.
+results and, unless given, its scratch, and does not synchronise.  A call
+captured into a graph keeps the scratch it was given (or allocated from the
+capture's pool): two graphs that may run at the same time need two.
 """
 
 from __future__ import annotations
@@ -63,55 +65,67 @@ def _bad(msg: str):
     raise DialError(DIAL_ERR_INVALID, msg)
 
 
-def _need(name: str, t, dtype, shape, dev) -> int:
-    """Address of a contiguous tensor of this dtype, shape and device (None in
-    `shape`: any size); 0 for no tensor."""
+def _need(name: str, t, dtype, shape, idx: int) -> int:
+    """Address of a contiguous tensor of this dtype and shape on device `idx`;
+    0 for no tensor."""
     if t is None:
         return 0
-    if t.dtype != dtype or t.device != dev or not t.is_contiguous() or t.dim() != len(shape) or any(
-            w is not None and w != g for w, g in zip(shape, t.shape)):
-        _bad(f"{name}: expected a contiguous {dtype} tensor {tuple(shape)} on {dev}, got {t.dtype} "
-             f"{tuple(t.shape)} on {t.device}{'' if t.is_contiguous() else ', not contiguous'}")
-    return t.data_ptr()
+    if (t.dtype is dtype and t.shape == shape and t.is_contiguous()
+            and t.get_device() == idx):
+        return t.data_ptr()
+    _bad(f"{name}: expected a contiguous {dtype} tensor {tuple(shape)} on device {idx}, got {t.dtype} "
+         f"{tuple(t.shape)} on {t.device}{'' if t.is_contiguous() else ', not contiguous'}")
 
 
-def _rows(name: str, t, dtype, width: int, rows, dev) -> int:
-    """Address of row-major rows of at least `width` elements, any row stride."""
-    if (t.dtype != dtype or t.device != dev or t.dim() != 2 or t.shape[1] != width
-            or (rows is not None and t.shape[0] != rows) or (t.shape[1] > 1 and t.stride(1) != 1)):
-        _bad(f"{name}: expected {dtype} rows [{'rows' if rows is None else rows}, {width}] on {dev}, "
-             f"got {t.dtype} {tuple(t.shape)} strides {t.stride()} on {t.device}")
-    return t.data_ptr()
+def _table(name: str, t, width: int, idx: int):
+    """Address and rows of a block table [sessions, width]."""
+    if (t.dtype is torch.int32 and t.dim() == 2 and t.shape[1] == width and t.is_contiguous()
+            and t.get_device() == idx):
+        return t.data_ptr(), t.shape[0]
+    _bad(f"{name}: expected a contiguous int32 tensor [sessions, {width}] on device {idx}, got "
+         f"{t.dtype} {tuple(t.shape)} on {t.device}{'' if t.is_contiguous() else ', not contiguous'}")
 
 
-def _ld(t) -> int:
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+def _rows(name: str, t, dtype, rows, width: int, idx: int):
+    """Address and row stride of rows of `width` elements (rows None: any number)."""
+    if (t.dtype is dtype and t.dim() == 2 and t.shape[1] == width
+            and (rows is None or t.shape[0] == rows) and t.stride(1) == 1
+            and t.get_device() == idx):
+        return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else max(t.stride(0), width)
+    _bad(f"{name}: expected {dtype} rows [{'rows' if rows is None else rows}, {width}] on device {idx}, "
+         f"got {t.dtype} {tuple(t.shape)} strides {t.stride()} on {t.device}")
 
 
-def _pool(sh: Kv4Shape, cache: Kv4Cache, dev):
-    n, h = sh.num_blocks, sh.kv_heads
-    return (_need("pages", cache.pages, torch.uint8, (n, h, SLAB_BYTES), dev),
-            _need("weights", cache.weights, torch.float32, (n, h, PAGE_TOKENS), dev),
-            _need("positions", cache.positions, torch.int32, (n, h, PAGE_TOKENS), dev))
-
-
-def _launch(name: str, dev, *args):
-    if dev.type != "cuda":
-        _bad(f"{name}: tensors must be on a CUDA device, got {dev}")
-    stream = torch.cuda.current_stream(dev).cuda_stream
-    if torch.cuda.current_device() == dev.index:
+def _launch(name: str, idx: int, *args):
+    """The call on the current stream of device `idx`, which is made current."""
+    if idx < 0:
+        _bad(f"{name}: tensors must be on a CUDA device")
+    stream = _raw_stream(idx)
+    if _current_device() == idx:
         call(name, *args, stream)
     else:
-        with torch.cuda.device(dev):
+        with torch.cuda.device(idx):
             call(name, *args, stream)
 
 
-def _scratch(given, nbytes: int, dev):
+def _raw_stream(idx: int) -> int:
+    return torch._C._cuda_getCurrentRawStream(idx)
+
+
+def _current_device() -> int:
+    return torch._C._cuda_getDevice()
+
+
+def _scratch(given, nbytes: int, like):
+    """Address of the scratch, and what keeps it alive during the call."""
     if given is None:
-        return torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    if given.device != dev or not given.is_contiguous() or given.numel() * given.element_size() < nbytes:
-        _bad(f"scratch: expected {nbytes} contiguous bytes on {dev}")
-    return given
+        if not nbytes:
+            return 0, None
+        given = torch.empty(nbytes, dtype=torch.uint8, device=like.device)
+    elif (given.get_device() != like.get_device() or not given.is_contiguous()
+          or given.numel() * given.element_size() < nbytes):
+        _bad(f"scratch: expected {nbytes} contiguous bytes on {like.device}")
+    return given.data_ptr(), given
 
 
 def kv4_append(sh: Kv4Shape, cache: Kv4Cache, qkv, block_table, sids, slots, positions=None,
@@ -120,25 +134,27 @@ def kv4_append(sh: Kv4Shape, cache: Kv4Cache, qkv, block_table, sids, slots, pos
     padding row), with RMSNorm if the norm weights are given and RoPE at
     positions[m] if cos and sin are; returns q after both [rows, q_heads * 128]
     (in q_out if given; None with want_q=False)."""
-    dev, dt = qkv.device, _DTYPE[sh.act]
-    width = (sh.q_heads + 2 * sh.kv_heads) * HEAD_DIM
+    idx, dt, i32 = qkv.get_device(), _DTYPE[sh.act], torch.int32
+    H, Q, nb = sh.kv_heads, sh.q_heads, sh.num_blocks
     rows = qkv.shape[0]
-    p_qkv = _rows("qkv", qkv, dt, width, None, dev)
+    p_qkv, ld = _rows("qkv", qkv, dt, None, (Q + 2 * H) * HEAD_DIM, idx)
+    p_q = ld_q = 0
     if q_out is None and want_q:
-        q_out = torch.empty(rows, sh.q_heads * HEAD_DIM, dtype=dt, device=dev)
-    p_q = _rows("q_out", q_out, dt, sh.q_heads * HEAD_DIM, rows, dev) if q_out is not None else 0
-    i32 = torch.int32
-    _launch("dial_b200_kv4_append", dev, C.byref(sh), p_qkv, _ld(qkv),
-            _need("q_norm_w", q_norm_w, dt, (HEAD_DIM,), dev),
-            _need("k_norm_w", k_norm_w, dt, (HEAD_DIM,), dev),
-            _need("cos", cos, dt, (sh.max_pos, HEAD_DIM // 2), dev),
-            _need("sin", sin, dt, (sh.max_pos, HEAD_DIM // 2), dev),
-            *_pool(sh, cache, dev),
-            _need("block_table", block_table, i32, (None, sh.max_blocks), dev),
-            block_table.shape[0], _need("sids", sids, i32, (rows,), dev),
-            _need("slots", slots, i32, (rows,), dev),
-            _need("positions", positions, i32, (rows,), dev), p_q,
-            _ld(q_out) if q_out is not None else 0, rows)
+        q_out = torch.empty(rows, Q * HEAD_DIM, dtype=dt, device=qkv.device)
+    if q_out is not None:
+        p_q, ld_q = _rows("q_out", q_out, dt, rows, Q * HEAD_DIM, idx)
+    p_bt, sessions = _table("block_table", block_table, sh.max_blocks, idx)
+    one = (rows,)
+    _launch("dial_b200_kv4_append", idx, C.byref(sh), p_qkv, ld,
+            _need("q_norm_w", q_norm_w, dt, (HEAD_DIM,), idx),
+            _need("k_norm_w", k_norm_w, dt, (HEAD_DIM,), idx),
+            _need("cos", cos, dt, (sh.max_pos, HEAD_DIM // 2), idx),
+            _need("sin", sin, dt, (sh.max_pos, HEAD_DIM // 2), idx),
+            _need("pages", cache.pages, torch.uint8, (nb, H, SLAB_BYTES), idx),
+            _need("weights", cache.weights, torch.float32, (nb, H, PAGE_TOKENS), idx),
+            _need("positions pool", cache.positions, i32, (nb, H, PAGE_TOKENS), idx), p_bt, sessions,
+            _need("sids", sids, i32, one, idx), _need("slots", slots, i32, one, idx),
+            _need("positions", positions, i32, one, idx), p_q, ld_q, rows)
     return q_out
 
 
@@ -146,17 +162,18 @@ def kv4_read(sh: Kv4Shape, cache: Kv4Cache, block_table, sids, lens, count: int,
     """The values that slots first[i] + j (default j), j < count, of session
     sids[i] stand for: k and v [seqs, count, kv_heads, 128] in the activation
     dtype, zeros at and past lens[i]."""
-    dev, i32 = sids.device, torch.int32
+    idx, i32, H = sids.get_device(), torch.int32, sh.kv_heads
     n = sids.shape[0]
     if count < 0:
         _bad(f"count {count} is negative")
-    k = torch.empty(n, count, sh.kv_heads, HEAD_DIM, dtype=_DTYPE[sh.act], device=dev)
-    v = torch.empty_like(k)
-    _launch("dial_b200_kv4_read", dev, C.byref(sh), _pool(sh, cache, dev)[0],
-            _need("block_table", block_table, i32, (None, sh.max_blocks), dev),
-            block_table.shape[0], _need("sids", sids, i32, (n,), dev),
-            _need("first", first, i32, (n,), dev), _need("lens", lens, i32, (n,), dev), n, count,
-            k.data_ptr(), v.data_ptr())
+    kv = torch.empty(2, n, count, H, HEAD_DIM, dtype=_DTYPE[sh.act], device=sids.device)
+    k, v = kv.unbind(0)
+    p_bt, sessions = _table("block_table", block_table, sh.max_blocks, idx)
+    one = (n,)
+    _launch("dial_b200_kv4_read", idx, C.byref(sh),
+            _need("pages", cache.pages, torch.uint8, (sh.num_blocks, H, SLAB_BYTES), idx), p_bt,
+            sessions, _need("sids", sids, i32, one, idx), _need("first", first, i32, one, idx),
+            _need("lens", lens, i32, one, idx), n, count, k.data_ptr(), v.data_ptr())
     return k, v
 
 
@@ -174,23 +191,23 @@ def kv4_attention(sh: Kv4Shape, cache: Kv4Cache, q, block_table, sids, lens, max
     lens[i] - 1 of session sids[i].  max_q and max_len bound the queries and
     slots of a sequence.  accumulate adds each slot's probabilities to
     cache.weights.  Returns out [rows, q_heads * 128]."""
-    dev, dt, i32 = q.device, _DTYPE[sh.act], torch.int32
-    rows, n, width = q.shape[0], sids.shape[0], sh.q_heads * HEAD_DIM
-    p_q = _rows("q", q, dt, width, None, dev)
+    idx, dt, i32 = q.get_device(), _DTYPE[sh.act], torch.int32
+    H, rows, n, width = sh.kv_heads, q.shape[0], sids.shape[0], sh.q_heads * HEAD_DIM
+    p_q, ld = _rows("q", q, dt, None, width, idx)
     if out is None:
-        # rows that no sequence names are left as they were: none here
-        out = torch.empty(rows, width, dtype=dt, device=dev)
-    p_out = _rows("out", out, dt, width, rows, dev)
-    pages, weights, _ = _pool(sh, cache, dev)
-    if accumulate and not weights:
-        _bad("accumulate needs a cache with weights")
-    buf = _scratch(scratch, attention_scratch_bytes(sh, n, rows, max_q, max_len, accumulate), dev)
-    _launch("dial_b200_kv4_attention", dev, C.byref(sh), p_q, _ld(q), pages,
-            weights if accumulate else 0,
-            _need("block_table", block_table, i32, (None, sh.max_blocks), dev),
-            block_table.shape[0], _need("sids", sids, i32, (n,), dev),
-            _need("lens", lens, i32, (n,), dev), _need("q_starts", q_starts, i32, (n + 1,), dev), n,
-            rows, max_q, max_len, p_out, _ld(out), buf.data_ptr() if buf is not None else 0)
+        out = torch.empty(rows, width, dtype=dt, device=q.device)
+    p_out, ld_out = _rows("out", out, dt, rows, width, idx)
+    p_w = 0
+    if accumulate:
+        p_w = _need("weights", cache.weights, torch.float32, (sh.num_blocks, H, PAGE_TOKENS), idx)
+        if not p_w:
+            _bad("accumulate needs a cache with weights")
+    p_bt, sessions = _table("block_table", block_table, sh.max_blocks, idx)
+    p_s, keep = _scratch(scratch, attention_scratch_bytes(sh, n, rows, max_q, max_len, accumulate), q)
+    _launch("dial_b200_kv4_attention", idx, C.byref(sh), p_q, ld,
+            _need("pages", cache.pages, torch.uint8, (sh.num_blocks, H, SLAB_BYTES), idx), p_w, p_bt,
+            sessions, _need("sids", sids, i32, (n,), idx), _need("lens", lens, i32, (n,), idx),
+            _need("q_starts", q_starts, i32, (n + 1,), idx), n, rows, max_q, max_len, p_out, ld_out, p_s)
     return out
 
 
@@ -203,19 +220,20 @@ def kv4_evict(sh: Kv4Shape, cache: Kv4Cache, block_table, sids, lens, max_len: i
     """Cut the sessions to their `keep` most attended entries, kv head by kv
     head; entries newer than (newest position - recent) come first.  In place,
     or into the pages of dst_table.  Returns the new lengths [seqs]."""
-    dev, i32 = sids.device, torch.int32
+    idx, i32, H, nb = sids.get_device(), torch.int32, sh.kv_heads, sh.num_blocks
     n = sids.shape[0]
-    pages, weights, positions = _pool(sh, cache, dev)
-    if lens_out is None:
-        lens_out = torch.empty(n, dtype=i32, device=dev)
-    sessions = block_table.shape[0]
+    one, slots = (n,), (nb, H, PAGE_TOKENS)
     if keep < 0 or max_len < 0:
         _bad(f"keep {keep} / max_len {max_len} is negative")
-    buf = _scratch(scratch, evict_scratch_bytes(sh, n, max_len, keep), dev)
-    _launch("dial_b200_kv4_evict", dev, C.byref(sh), pages, weights, positions,
-            _need("block_table", block_table, i32, (None, sh.max_blocks), dev),
-            _need("dst_table", dst_table, i32, (sessions, sh.max_blocks), dev), sessions,
-            _need("sids", sids, i32, (n,), dev), _need("lens", lens, i32, (n,), dev),
-            _need("lens_out", lens_out, i32, (n,), dev), n, max_len, keep, recent,
-            buf.data_ptr() if buf is not None else 0)
+    if lens_out is None:
+        lens_out = torch.empty(n, dtype=i32, device=sids.device)
+    p_bt, sessions = _table("block_table", block_table, sh.max_blocks, idx)
+    p_s, alive = _scratch(scratch, evict_scratch_bytes(sh, n, max_len, keep), sids)
+    _launch("dial_b200_kv4_evict", idx, C.byref(sh),
+            _need("pages", cache.pages, torch.uint8, (nb, H, SLAB_BYTES), idx),
+            _need("weights", cache.weights, torch.float32, slots, idx),
+            _need("positions pool", cache.positions, i32, slots, idx), p_bt,
+            _need("dst_table", dst_table, i32, (sessions, sh.max_blocks), idx), sessions,
+            _need("sids", sids, i32, one, idx), _need("lens", lens, i32, one, idx),
+            _need("lens_out", lens_out, i32, one, idx), n, max_len, keep, recent, p_s)
     return lens_out
