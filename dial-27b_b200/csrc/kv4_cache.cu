@@ -4,8 +4,10 @@
 #include <atomic>
 #include <cstdarg>
 #include <cstdio>
+#include <type_traits>
 
 #include "kv4_dev.cuh"
+#include "kv4_launch.h"
 
 namespace dialb200 {
 namespace {
@@ -30,88 +32,175 @@ struct AppendArgs {
   float eps;
 };
 
-// RMSNorm and RoPE of the head held four dims a lane, each step rounded to the
-// activation dtype (the decode op's steps).  The sum of squares is exact in 64
-// bits, so that a value next to a code's border falls on one side of it
-// whatever the order of the sum.
+// Packed pairs of the activation dtype, each operation rounded once (never
+// contracted).
 template <typename Act>
-__device__ __forceinline__ void norm_rope64(float (&x)[4], const Act* w, float eps, const Act* cos,
-                                            const Act* sin, int lane) {
-  using AT = ActTraits<Act>;
-  if (w) {
-    double ss = 0.;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) ss = fma(static_cast<double>(x[e]), static_cast<double>(x[e]), ss);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    const float m = AT::round(static_cast<float>(sqrt(ss / kHeadDim + static_cast<double>(eps))));
-    float wv[4];
-    load4(w + lane * 4, wv);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) x[e] = AT::round(AT::round(__fdiv_rn(x[e], m)) * wv[e]);
+struct Pair;
+template <>
+struct Pair<__nv_bfloat16> {
+  using T = __nv_bfloat162;
+  static __device__ __forceinline__ T of(float lo, float hi) { return __floats2bfloat162_rn(lo, hi); }
+  static __device__ __forceinline__ T mul(T a, T b) { return __hmul2_rn(a, b); }
+  static __device__ __forceinline__ T add(T a, T b) { return __hadd2_rn(a, b); }
+};
+template <>
+struct Pair<__half> {
+  using T = __half2;
+  static __device__ __forceinline__ T of(float lo, float hi) { return __floats2half2_rn(lo, hi); }
+  static __device__ __forceinline__ T mul(T a, T b) { return __hmul2_rn(a, b); }
+  static __device__ __forceinline__ T add(T a, T b) { return __hadd2_rn(a, b); }
+};
+
+// A head held four dims a lane (dims 4 * lane ..), as two pairs.
+template <typename Act>
+struct Head {
+  typename Pair<Act>::T v[2];
+  __device__ __forceinline__ void load(const Act* p, int lane) {
+    *reinterpret_cast<uint2*>(v) = *reinterpret_cast<const uint2*>(p + lane * 4);
   }
-  if (cos) {
-    float c[4], s[4];
-    load4(cos + (lane & 15) * 4, c);
-    load4(sin + (lane & 15) * 4, s);
-    const bool first = lane < 16;
+  __device__ __forceinline__ void store(Act* p, int lane) const {
+    *reinterpret_cast<uint2*>(p + lane * 4) = *reinterpret_cast<const uint2*>(v);
+  }
+  __device__ __forceinline__ void floats(float (&x)[4]) const {
+    const Act* h = reinterpret_cast<const Act*>(v);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float other = __shfl_xor_sync(0xffffffffu, x[e], 16);
-      const float x1 = first ? x[e] : other, x2 = first ? other : x[e];
-      x[e] = first ? AT::round(AT::round(x1 * c[e]) - AT::round(x2 * s[e]))
-                   : AT::round(AT::round(x1 * s[e]) + AT::round(x2 * c[e]));
+    for (int e = 0; e < 4; ++e) x[e] = ActTraits<Act>::to_f(h[e]);
+  }
+};
+
+// act(sqrt(sum x^2 / 128 + eps)) of the warp's head, as from an exact sum: the f32
+// form (off by less than 2^-20: 9 roundings of the sum, halved by the root, and 3
+// more) unless a border of the dtype lies within 2^-19 of it, else 64 bits.
+template <typename Act>
+__device__ __forceinline__ float rms_of(const float (&x)[4], float eps) {
+  using AT = ActTraits<Act>;
+  const float ss = warp_sum(fmaf(x[0], x[0], x[1] * x[1]) + fmaf(x[2], x[2], x[3] * x[3]));
+  const float m = __fsqrt_rn(ss * (1.f / kHeadDim) + eps);
+  const float lo = AT::round(m * (1.f - 0x1p-19f)), hi = AT::round(m * (1.f + 0x1p-19f));
+  // sums near the ends of f32's range lose more than that
+  if (lo == hi && ss > 1e-30f && ss < 1e37f) return lo;
+  double sum = 0.;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) sum = fma(static_cast<double>(x[e]), static_cast<double>(x[e]), sum);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  return AT::round(static_cast<float>(sqrt(sum / kHeadDim + static_cast<double>(eps))));
+}
+
+// act(x / m).  A quotient of two bf16 values is never within 2^-17 of the middle of
+// two bf16 values, so a product with 1 / m rounds as the quotient does; f16's
+// quotients come as near as 2^-23 and are divided.
+template <typename Act>
+__device__ __forceinline__ void divide(const float (&x)[4], float m, typename Pair<Act>::T (&v)[2]) {
+  float q[4];
+  if (std::is_same<Act, __nv_bfloat16>::value && m > 1e-37f && m < 1e37f) {
+    const float inv = __frcp_rn(m);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) q[e] = x[e] * inv;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) q[e] = __fdiv_rn(x[e], m);
+  }
+  v[0] = Pair<Act>::of(q[0], q[1]);
+  v[1] = Pair<Act>::of(q[2], q[3]);
+}
+
+// RMSNorm and RoPE, each step rounded to the activation dtype (the decode op's
+// steps).  rope: cos, and sin with the sign of the lane's half.
+template <typename Act>
+__device__ __forceinline__ void norm_rope(Head<Act>& x, const Head<Act>& w, const Head<Act>& c, const Head<Act>& s,
+                                          float eps, bool norm, bool rope) {
+  using P = Pair<Act>;
+  if (norm) {
+    float f[4];
+    x.floats(f);
+    divide<Act>(f, rms_of<Act>(f, eps), x.v);
+    x.v[0] = P::mul(x.v[0], w.v[0]);
+    x.v[1] = P::mul(x.v[1], w.v[1]);
+  }
+  if (rope) {
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const uint32_t own = *reinterpret_cast<const uint32_t*>(&x.v[e]);
+      const uint32_t far = __shfl_xor_sync(0xffffffffu, own, 16);
+      x.v[e] = P::add(P::mul(x.v[e], c.v[e]), P::mul(*reinterpret_cast<const typename P::T*>(&far), s.v[e]));
     }
   }
 }
 
-// One warp per (row, head unit): unit u < kv_heads is a kv head (k and v),
-// the others query heads.
-template <typename Act>
+// One CTA for a row and a share (blockIdx.y) of its head units: unit u < kv_heads is a
+// kv head (k and v), the others query heads.  A warp's norm weights, cos and sin
+// serve all its heads.
+// Bound by the bytes for long prompts (2048 rows of 32 + 16 heads: 17 us, 2.6 TB/s with
+// the rows in L2), by latency for a token.
+template <typename Act, int U>
 __global__ void __launch_bounds__(256) kv4_append_kernel(const AppendArgs a) {
-  const int lane = threadIdx.x & 31;
-  const long long item = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5);
-  if (item >= static_cast<long long>(a.rows) * a.units) return;
-  const int m = static_cast<int>(item / a.units), u = static_cast<int>(item % a.units);
+  const int lane = threadIdx.x & 31, m = blockIdx.x;
+  pdl_wait();
+  pdl_launch_dependents();
   const int slot = a.slots[m];
   if (slot < 0) return;
   const int sid = a.sids[m], pos = a.pos ? a.pos[m] : 0;
   const int page = slot / kPageTokens, t = slot % kPageTokens;
-  if (static_cast<unsigned>(sid) >= static_cast<unsigned>(a.c.sessions) ||
-      page >= a.c.max_blocks ||
-      (a.cos && static_cast<unsigned>(pos) >= static_cast<unsigned>(a.max_pos))) {
-    if (lane == 0) set_status(a.c.status, kStatusBadArgs);
+  const bool norm = a.q_norm_w != nullptr, rope = a.cos != nullptr;
+  if (static_cast<unsigned>(sid) >= static_cast<unsigned>(a.c.sessions) || page >= a.c.max_blocks ||
+      (rope && static_cast<unsigned>(pos) >= static_cast<unsigned>(a.max_pos))) {
+    if (threadIdx.x == 0) set_status(a.c.status, kStatusBadArgs);
     return;
   }
   const Act* row = static_cast<const Act*>(a.qkv) + m * a.qkv_ld;
-  const size_t rope = static_cast<size_t>(pos) * (kHeadDim / 2);
-  const Act* cos = a.cos ? static_cast<const Act*>(a.cos) + rope : nullptr;
-  const Act* sin = a.cos ? static_cast<const Act*>(a.sin) + rope : nullptr;
-  float x[4];
-  if (u >= a.c.kv_heads) {
-    const int h = u - a.c.kv_heads;
-    load4(row + h * kHeadDim + lane * 4, x);
-    norm_rope64(x, static_cast<const Act*>(a.q_norm_w), a.eps, cos, sin, lane);
-    store4(static_cast<Act*>(a.q_out) + m * a.q_out_ld + h * kHeadDim + lane * 4, x);
-    return;
+  Head<Act> qw{}, kw{}, c{}, s{};
+  if (norm) {
+    qw.load(static_cast<const Act*>(a.q_norm_w), lane);
+    kw.load(static_cast<const Act*>(a.k_norm_w), lane);
   }
+  if (rope) {
+    const size_t at = static_cast<size_t>(pos) * (kHeadDim / 2);
+    c.load(static_cast<const Act*>(a.cos) + at, lane & 15);
+    s.load(static_cast<const Act*>(a.sin) + at, lane & 15);
+    if (lane < 16) {  // dims below 64: x c - far s; above: x c + far s
+      s.v[0] = __hneg2(s.v[0]);
+      s.v[1] = __hneg2(s.v[1]);
+    }
+  }
+  const int step = gridDim.y * 8, H = a.c.kv_heads, Q = a.c.q_heads;
   const int block = kv4_block(a.c, a.c.block_table, sid, page);
-  if (block < 0) return;
-  const size_t si = kv4_slab_index(a.c, block, u);
-  uint8_t* slab = a.c.pages + si * kKv4Slab;
-  uint32_t codes, scale;
-  load4(row + (a.c.q_heads + u) * kHeadDim + lane * 4, x);
-  norm_rope64(x, static_cast<const Act*>(a.k_norm_w), a.eps, cos, sin, lane);
-  kv4_encode(x, a.c.k_scale, codes, scale);
-  *reinterpret_cast<uint16_t*>(slab + t * 64 + lane * 2) = static_cast<uint16_t>(codes);
-  if ((lane & 3) == 0) slab[kKv4KScales + t * 8 + (lane >> 2)] = static_cast<uint8_t>(scale);
-  load4(row + (a.c.q_heads + a.c.kv_heads + u) * kHeadDim + lane * 4, x);
-  kv4_encode(x, a.c.v_scale, codes, scale);
-  *reinterpret_cast<uint16_t*>(slab + kKv4VCodes + t * 64 + lane * 2) =
-      static_cast<uint16_t>(codes);
-  if ((lane & 3) == 0) slab[kKv4VScales + t * 8 + (lane >> 2)] = static_cast<uint8_t>(scale);
-  if (lane == 0 && a.c.weights) a.c.weights[si * kPageTokens + t] = 0.f;
-  if (lane == 1 && a.c.positions) a.c.positions[si * kPageTokens + t] = pos;
+  for (int u0 = blockIdx.y * 8 + (threadIdx.x >> 5); u0 < a.units; u0 += U * step) {
+    Head<Act> x[U];  // U heads in flight; a kv head's v is loaded at its turn
+#pragma unroll
+    for (int e = 0; e < U; ++e) {
+      const int u = u0 + e * step;
+      if (u < a.units) x[e].load(row + (u < H ? Q + u : u - H) * kHeadDim, lane);
+    }
+#pragma unroll
+    for (int e = 0; e < U; ++e) {
+      const int u = u0 + e * step;
+      if (u >= a.units) break;
+      if (u >= H) {
+        norm_rope(x[e], qw, c, s, a.eps, norm, rope);
+        x[e].store(static_cast<Act*>(a.q_out) + m * a.q_out_ld + (u - H) * kHeadDim, lane);
+        continue;
+      }
+      Head<Act> y;
+      y.load(row + (Q + H + u) * kHeadDim, lane);
+      norm_rope(x[e], kw, c, s, a.eps, norm, rope);
+      if (block < 0) continue;
+      const size_t si = kv4_slab_index(a.c, block, u);
+      uint8_t* slab = a.c.pages + si * kKv4Slab;
+      uint32_t codes, scale;
+      float f[4];
+      x[e].floats(f);
+      kv4_encode(f, a.c.k_scale, codes, scale);
+      *reinterpret_cast<uint16_t*>(slab + t * 64 + lane * 2) = static_cast<uint16_t>(codes);
+      if ((lane & 3) == 0) slab[kKv4KScales + t * 8 + (lane >> 2)] = static_cast<uint8_t>(scale);
+      y.floats(f);
+      kv4_encode(f, a.c.v_scale, codes, scale);
+      *reinterpret_cast<uint16_t*>(slab + kKv4VCodes + t * 64 + lane * 2) = static_cast<uint16_t>(codes);
+      if ((lane & 3) == 0) slab[kKv4VScales + t * 8 + (lane >> 2)] = static_cast<uint8_t>(scale);
+      if (lane == 0 && a.c.weights) a.c.weights[si * kPageTokens + t] = 0.f;
+      if (lane == 1 && a.c.positions) a.c.positions[si * kPageTokens + t] = pos;
+    }
+  }
 }
 
 struct ReadArgs {
@@ -121,36 +210,69 @@ struct ReadArgs {
   const int32_t* lens;
   void* k_out;
   void* v_out;
-  int seqs, count;
+  unsigned rows;  // seqs * count
+  int count;
 };
 
-// One warp per (sequence, slot, kv head).
-template <typename Act>
+// Lanes 0-15 of a warp take k and 16-31 v, 8 dims each: 4 bytes of codes in, 16 bytes
+// out, so that its stores are whole lines.  HEADS: a warp takes rows (slots) and goes
+// over their kv heads, which shares a row's table look-ups; else one (slot, kv head).
+template <typename Act, bool HEADS>
 __global__ void __launch_bounds__(256) kv4_read_kernel(const ReadArgs a) {
-  const int lane = threadIdx.x & 31;
-  const long long item = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5);
-  const int H = a.c.kv_heads;
-  if (item >= static_cast<long long>(a.seqs) * a.count * H) return;
-  const int h = static_cast<int>(item % H);
-  const long long r = item / H;
-  const int i = static_cast<int>(r / a.count);
-  const long long slot = (a.first ? a.first[i] : 0) + r % a.count;
-  const int sid = a.sids[i];
-  float k[4] = {0.f, 0.f, 0.f, 0.f}, v[4] = {0.f, 0.f, 0.f, 0.f};
-  if (slot >= 0 && slot < a.lens[i]) {
-    if (static_cast<unsigned>(sid) >= static_cast<unsigned>(a.c.sessions) ||
-        slot >= static_cast<long long>(a.c.max_blocks) * kPageTokens) {
+  const int lane = threadIdx.x & 31, part = lane >> 4, l = lane & 15;
+  const unsigned H = a.c.kv_heads;
+  pdl_wait();
+  pdl_launch_dependents();
+  const float mult = part ? a.c.v_scale : a.c.k_scale;
+  const int codes_at = (part ? kKv4VCodes : 0) + l * 4;
+  const int scales_at = (part ? kKv4VScales : kKv4KScales) + (l >> 1);
+  const unsigned unit = blockIdx.x * 8 + (threadIdx.x >> 5);
+#pragma unroll
+  for (unsigned e = 0; e < (HEADS ? 2u : 1u); ++e) {
+    const unsigned row = HEADS ? unit * 2 + e : unit / H;
+    if (row >= a.rows) return;
+    const unsigned h0 = HEADS ? 0 : unit - row * H, h1 = HEADS ? H : h0 + 1;
+    const unsigned i = row / static_cast<unsigned>(a.count);
+    const int sid = a.sids[i];
+    const long long slot = (a.first ? a.first[i] : 0) + static_cast<long long>(row - i * a.count);
+    const bool there = slot >= 0 && slot < a.lens[i];
+    if (there && (static_cast<unsigned>(sid) >= static_cast<unsigned>(a.c.sessions) ||
+                  slot >= static_cast<long long>(a.c.max_blocks) * kPageTokens)) {
       if (lane == 0) set_status(a.c.status, kStatusBadArgs);
-      return;
+      continue;
     }
-    const int t = static_cast<int>(slot % kPageTokens);
-    const int block = max(0, kv4_block(a.c, a.c.block_table, sid, static_cast<int>(slot / kPageTokens)));
-    const uint8_t* slab = a.c.pages + kv4_slab_index(a.c, block, h) * kKv4Slab;
-    kv4_decode(slab, 0, kKv4KScales, t, lane, a.c.k_scale, k);
-    kv4_decode(slab, kKv4VCodes, kKv4VScales, t, lane, a.c.v_scale, v);
+    const int t = there ? static_cast<int>(slot % kPageTokens) : 0;
+    const int block = there ? max(0, kv4_block(a.c, a.c.block_table, sid, static_cast<int>(slot / kPageTokens))) : 0;
+    const uint8_t* slab = a.c.pages + kv4_slab_index(a.c, block, 0) * kKv4Slab;
+    Act* out = static_cast<Act*>(part ? a.v_out : a.k_out) + static_cast<size_t>(row) * H * kHeadDim + l * 8;
+#pragma unroll 4
+    for (unsigned h = h0; h < h1; ++h) {
+      uint32_t w = 0, sc = 0;
+      if (there) {
+        w = *reinterpret_cast<const uint32_t*>(slab + h * kKv4Slab + codes_at + t * 64);
+        sc = slab[h * kKv4Slab + scales_at + t * 8];
+      }
+      const float f = e4m3_value(sc) * mult;
+      uint32_t o[4];
+      e2m1x8_to_f16x2x4(w, o);
+      uint4 r;
+      typename Pair<Act>::T* p = reinterpret_cast<typename Pair<Act>::T*>(&r);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&o[q]));
+        p[q] = Pair<Act>::of(v.x * f, v.y * f);
+      }
+      *reinterpret_cast<uint4*>(out + static_cast<size_t>(h) * kHeadDim) = r;
+    }
   }
-  store4(static_cast<Act*>(a.k_out) + item * kHeadDim + lane * 4, k);
-  store4(static_cast<Act*>(a.v_out) + item * kHeadDim + lane * 4, v);
+}
+
+template <typename Act>
+cudaError_t launch_read(const ReadArgs& a, cudaStream_t s) {
+  const long long units = static_cast<long long>(a.rows) * a.c.kv_heads;
+  if (units <= 148 * 16)  // few: every (slot, kv head) a warp of its own
+    return kv4_start(kv4_read_kernel<Act, false>, dim3(static_cast<unsigned>((units + 7) / 8)), 256, 0, s, a);
+  return kv4_start(kv4_read_kernel<Act, true>, dim3((a.rows + 15) / 16), 256, 0, s, a);
 }
 
 cudaError_t kv4_status_word(int** word) {
@@ -290,16 +412,19 @@ extern "C" int dial_b200_kv4_append(const dial_b200_kv4_shape* sh, const void* q
   a.units = sh->kv_heads + (q_out ? sh->q_heads : 0);
   a.max_pos = sh->max_pos;
   a.eps = sh->eps;
-  const long long grid = (rows * a.units + 7) / 8;
-  if (grid > INT32_MAX)
-    return kv4_fail(err, n, DIAL_ERR_INVALID, "rows %lld times heads out of range", (long long)rows);
   if ((rc = kv4_ready(&a.c, err, n)) != DIAL_OK) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (sh->act == DIAL_ACT_BF16)
-    kv4_append_kernel<__nv_bfloat16><<<static_cast<unsigned>(grid), 256, 0, s>>>(a);
-  else
-    kv4_append_kernel<__half><<<static_cast<unsigned>(grid), 256, 0, s>>>(a);
-  const cudaError_t e = cudaGetLastError();
+  cudaError_t e;
+  const int most = (a.units + 7) / 8;
+  if (rows * most <= 1184) {  // a head a warp while the GPU's 148 SMs have room for more CTAs
+    const dim3 grid(static_cast<unsigned>(rows), most);
+    e = sh->act == DIAL_ACT_BF16 ? kv4_start(kv4_append_kernel<__nv_bfloat16, 1>, grid, 256, 0, s, a)
+                                 : kv4_start(kv4_append_kernel<__half, 1>, grid, 256, 0, s, a);
+  } else {  // a row a CTA, three of a warp's heads in flight
+    const dim3 grid(static_cast<unsigned>(rows), 1);
+    e = sh->act == DIAL_ACT_BF16 ? kv4_start(kv4_append_kernel<__nv_bfloat16, 3>, grid, 256, 0, s, a)
+                                 : kv4_start(kv4_append_kernel<__half, 3>, grid, 256, 0, s, a);
+  }
   if (e != cudaSuccess)
     return kv4_fail(err, n, DIAL_ERR_CUDA, "kv4 append launch failed: %s", cudaGetErrorString(e));
   return DIAL_OK;
@@ -315,8 +440,8 @@ extern "C" int dial_b200_kv4_read(const dial_b200_kv4_shape* sh, const void* pag
   if (rc != DIAL_OK) return rc;
   if (!sids || !lens || !k_out || !v_out)
     return kv4_fail(err, n, DIAL_ERR_INVALID, "null pointer argument");
-  if (!aligned(k_out, 8) || !aligned(v_out, 8))
-    return kv4_fail(err, n, DIAL_ERR_INVALID, "k_out and v_out must be 8-byte aligned");
+  if (!aligned(k_out, 16) || !aligned(v_out, 16))
+    return kv4_fail(err, n, DIAL_ERR_INVALID, "k_out and v_out must be 16-byte aligned");
   if (seqs < 0 || seqs > (1 << 20) || count < 0 || count > INT32_MAX / 2)
     return kv4_fail(err, n, DIAL_ERR_INVALID, "seqs %lld / count %lld out of range",
                     (long long)seqs, (long long)count);
@@ -326,19 +451,14 @@ extern "C" int dial_b200_kv4_read(const dial_b200_kv4_shape* sh, const void* pag
   a.lens = lens;
   a.k_out = k_out;
   a.v_out = v_out;
-  a.seqs = static_cast<int>(seqs);
-  a.count = static_cast<int>(count);
-  if (seqs * count > (1LL << 31) * 8 / sh->kv_heads - 8)
+  if (seqs * count > INT32_MAX / sh->kv_heads)
     return kv4_fail(err, n, DIAL_ERR_INVALID, "seqs %lld times count %lld out of range",
                     (long long)seqs, (long long)count);
-  const long long grid = (seqs * count * sh->kv_heads + 7) / 8;
+  a.rows = static_cast<unsigned>(seqs * count);
+  a.count = static_cast<int>(count);
   if ((rc = kv4_ready(&a.c, err, n)) != DIAL_OK) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (sh->act == DIAL_ACT_BF16)
-    kv4_read_kernel<__nv_bfloat16><<<static_cast<unsigned>(grid), 256, 0, s>>>(a);
-  else
-    kv4_read_kernel<__half><<<static_cast<unsigned>(grid), 256, 0, s>>>(a);
-  const cudaError_t e = cudaGetLastError();
+  const cudaError_t e = sh->act == DIAL_ACT_BF16 ? launch_read<__nv_bfloat16>(a, s) : launch_read<__half>(a, s);
   if (e != cudaSuccess)
     return kv4_fail(err, n, DIAL_ERR_CUDA, "kv4 read launch failed: %s", cudaGetErrorString(e));
   return DIAL_OK;

@@ -749,7 +749,7 @@ Plan plan_of(int q_heads, int kv_heads, long long seqs, long long max_q, long lo
   p.score_ld = (p.cols + 1) & ~1;
   auto up = [](size_t v) { return (v + 127) & ~static_cast<size_t>(127); };
   const size_t rows = p.one ? 0 : static_cast<size_t>(p.ctas + seqs * kv_heads) * p.groups * p.nt * 8;
-  p.desc = up(static_cast<size_t>(p.ctas) * sizeof(int4));
+  p.desc = p.one ? 0 : up(static_cast<size_t>(p.ctas) * sizeof(int4));
   p.part_o = up(rows * kHeadDim * 4);
   p.part_ml = up(rows * 8);
   p.scores = weights ? up(static_cast<size_t>(p.pages) * kPageTokens * p.score_ld * 4) : 0;

@@ -47,15 +47,12 @@ __device__ __forceinline__ uint32_t e2m1x2_of(float lo, float hi) {
   return r;
 }
 
-// Two e2m1 codes (one byte) to f16x2, exact.
-__device__ __forceinline__ uint32_t e2m1x2_to_f16x2(uint32_t byte) {
-  uint32_t r;
-  asm("{\n\t.reg .b8 b;\n\t"
-      "cvt.u8.u32 b, %1;\n\t"
-      "cvt.rn.f16x2.e2m1x2 %0, b;\n\t}"
-      : "=r"(r)
-      : "r"(byte));
-  return r;
+// x / s correctly rounded, with y = 1 / s correctly rounded: the remainder of x y
+// is exact, and its product with y corrects the last place (Markstein).  Quotients
+// that overflow are divided.
+__device__ __forceinline__ float quotient(float x, float s, float y) {
+  const float q = x * y;
+  return fabsf(q) < 1e30f ? fmaf(fmaf(-q, s, x), y, q) : __fdiv_rn(x, s);
 }
 
 // Four values (dims 4 * lane ..) of a 128-dim row quantised by its warp: the
@@ -70,28 +67,15 @@ __device__ __forceinline__ void kv4_encode(const float (&x)[4], float mult, uint
   }
   amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
   amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-  scale = e4m3_of(__fdiv_rn(__fdiv_rn(amax, 6.f), mult));
+  scale = e4m3_of(__fdiv_rn(quotient(amax, 6.f, 1.f / 6.f), mult));
   const float s = e4m3_value(scale) * mult;
   codes = 0;
   if (s > 0.f) {
+    const float y = __frcp_rn(s);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = __fdiv_rn(v[e], s);
+    for (int e = 0; e < 4; ++e) v[e] = quotient(v[e], s, y);
     codes = e2m1x2_of(v[0], v[1]) | e2m1x2_of(v[2], v[3]) << 8;
   }
-}
-
-// The four values of the lane's dims (4 * lane ..) of token t of a slab's k
-// or v part; mult is the multiplier beside the e4m3 scales.
-__device__ __forceinline__ void kv4_decode(const uint8_t* slab, int codes_at, int scales_at, int t,
-                                           int lane, float mult, float (&v)[4]) {
-  const uint32_t c = *reinterpret_cast<const uint16_t*>(slab + codes_at + t * 64 + lane * 2);
-  const float s = e4m3_value(slab[scales_at + t * 8 + (lane >> 2)]) * mult;
-  const uint32_t a = e2m1x2_to_f16x2(c & 0xFFu), b = e2m1x2_to_f16x2(c >> 8);
-  const __half2 ha = *reinterpret_cast<const __half2*>(&a), hb = *reinterpret_cast<const __half2*>(&b);
-  v[0] = __low2float(ha) * s;
-  v[1] = __high2float(ha) * s;
-  v[2] = __low2float(hb) * s;
-  v[3] = __high2float(hb) * s;
 }
 
 // A sequence of an attention call: its session, slots, first row and rows.

@@ -19,6 +19,7 @@ capture's pool): two graphs that may run at the same time need two.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 from dataclasses import dataclass
 
 import torch
@@ -65,33 +66,32 @@ def _bad(msg: str):
     raise DialError(DIAL_ERR_INVALID, msg)
 
 
-def _need(name: str, t, dtype, shape, idx: int) -> int:
-    """Address of a contiguous tensor of this dtype and shape on device `idx`;
-    0 for no tensor."""
+def _need(name: str, t, dtype, numel: int, idx: int) -> int:
+    """Address of a contiguous tensor of this dtype and size on device `idx`; 0 for
+    no tensor."""
     if t is None:
         return 0
-    if (t.dtype is dtype and t.shape == shape and t.is_contiguous()
-            and t.get_device() == idx):
+    if t.dtype is dtype and t.numel() == numel and t.is_contiguous() and t.get_device() == idx:
         return t.data_ptr()
-    _bad(f"{name}: expected a contiguous {dtype} tensor {tuple(shape)} on device {idx}, got {t.dtype} "
-         f"{tuple(t.shape)} on {t.device}{'' if t.is_contiguous() else ', not contiguous'}")
+    _bad(f"{name}: expected a contiguous {dtype} tensor of {numel} elements on device {idx}, got "
+         f"{t.dtype} {tuple(t.shape)} on {t.device}{'' if t.is_contiguous() else ', not contiguous'}")
 
 
 def _table(name: str, t, width: int, idx: int):
     """Address and rows of a block table [sessions, width]."""
-    if (t.dtype is torch.int32 and t.dim() == 2 and t.shape[1] == width and t.is_contiguous()
+    if (t.dtype is torch.int32 and t.dim() == 2 and t.size(1) == width and t.is_contiguous()
             and t.get_device() == idx):
-        return t.data_ptr(), t.shape[0]
+        return t.data_ptr(), t.size(0)
     _bad(f"{name}: expected a contiguous int32 tensor [sessions, {width}] on device {idx}, got "
          f"{t.dtype} {tuple(t.shape)} on {t.device}{'' if t.is_contiguous() else ', not contiguous'}")
 
 
 def _rows(name: str, t, dtype, rows, width: int, idx: int):
     """Address and row stride of rows of `width` elements (rows None: any number)."""
-    if (t.dtype is dtype and t.dim() == 2 and t.shape[1] == width
-            and (rows is None or t.shape[0] == rows) and t.stride(1) == 1
+    if (t.dtype is dtype and t.dim() == 2 and t.size(1) == width
+            and (rows is None or t.size(0) == rows) and t.stride(1) == 1
             and t.get_device() == idx):
-        return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else max(t.stride(0), width)
+        return t.data_ptr(), t.stride(0) if t.size(0) > 1 else max(t.stride(0), width)
     _bad(f"{name}: expected {dtype} rows [{'rows' if rows is None else rows}, {width}] on device {idx}, "
          f"got {t.dtype} {tuple(t.shape)} strides {t.stride()} on {t.device}")
 
@@ -136,25 +136,25 @@ def kv4_append(sh: Kv4Shape, cache: Kv4Cache, qkv, block_table, sids, slots, pos
     (in q_out if given; None with want_q=False)."""
     idx, dt, i32 = qkv.get_device(), _DTYPE[sh.act], torch.int32
     H, Q, nb = sh.kv_heads, sh.q_heads, sh.num_blocks
-    rows = qkv.shape[0]
+    rows = qkv.size(0)
     p_qkv, ld = _rows("qkv", qkv, dt, None, (Q + 2 * H) * HEAD_DIM, idx)
     p_q = ld_q = 0
-    if q_out is None and want_q:
-        q_out = torch.empty(rows, Q * HEAD_DIM, dtype=dt, device=qkv.device)
     if q_out is not None:
         p_q, ld_q = _rows("q_out", q_out, dt, rows, Q * HEAD_DIM, idx)
+    elif want_q:
+        q_out = torch.empty(rows, Q * HEAD_DIM, dtype=dt, device=qkv.device)
+        p_q, ld_q = q_out.data_ptr(), Q * HEAD_DIM
     p_bt, sessions = _table("block_table", block_table, sh.max_blocks, idx)
-    one = (rows,)
+    slabs, rope = nb * H, sh.max_pos * (HEAD_DIM // 2)
     _launch("dial_b200_kv4_append", idx, C.byref(sh), p_qkv, ld,
-            _need("q_norm_w", q_norm_w, dt, (HEAD_DIM,), idx),
-            _need("k_norm_w", k_norm_w, dt, (HEAD_DIM,), idx),
-            _need("cos", cos, dt, (sh.max_pos, HEAD_DIM // 2), idx),
-            _need("sin", sin, dt, (sh.max_pos, HEAD_DIM // 2), idx),
-            _need("pages", cache.pages, torch.uint8, (nb, H, SLAB_BYTES), idx),
-            _need("weights", cache.weights, torch.float32, (nb, H, PAGE_TOKENS), idx),
-            _need("positions pool", cache.positions, i32, (nb, H, PAGE_TOKENS), idx), p_bt, sessions,
-            _need("sids", sids, i32, one, idx), _need("slots", slots, i32, one, idx),
-            _need("positions", positions, i32, one, idx), p_q, ld_q, rows)
+            _need("q_norm_w", q_norm_w, dt, HEAD_DIM, idx),
+            _need("k_norm_w", k_norm_w, dt, HEAD_DIM, idx),
+            _need("cos", cos, dt, rope, idx), _need("sin", sin, dt, rope, idx),
+            _need("pages", cache.pages, torch.uint8, slabs * SLAB_BYTES, idx),
+            _need("weights", cache.weights, torch.float32, slabs * PAGE_TOKENS, idx),
+            _need("positions pool", cache.positions, i32, slabs * PAGE_TOKENS, idx), p_bt, sessions,
+            _need("sids", sids, i32, rows, idx), _need("slots", slots, i32, rows, idx),
+            _need("positions", positions, i32, rows, idx), p_q, ld_q, rows)
     return q_out
 
 
@@ -163,22 +163,27 @@ def kv4_read(sh: Kv4Shape, cache: Kv4Cache, block_table, sids, lens, count: int,
     sids[i] stand for: k and v [seqs, count, kv_heads, 128] in the activation
     dtype, zeros at and past lens[i]."""
     idx, i32, H = sids.get_device(), torch.int32, sh.kv_heads
-    n = sids.shape[0]
+    n = sids.numel()
     if count < 0:
         _bad(f"count {count} is negative")
-    kv = torch.empty(2, n, count, H, HEAD_DIM, dtype=_DTYPE[sh.act], device=sids.device)
-    k, v = kv.unbind(0)
+    k = torch.empty(n, count, H, HEAD_DIM, dtype=_DTYPE[sh.act], device=sids.device)
+    v = torch.empty_like(k)
     p_bt, sessions = _table("block_table", block_table, sh.max_blocks, idx)
-    one = (n,)
     _launch("dial_b200_kv4_read", idx, C.byref(sh),
-            _need("pages", cache.pages, torch.uint8, (sh.num_blocks, H, SLAB_BYTES), idx), p_bt,
-            sessions, _need("sids", sids, i32, one, idx), _need("first", first, i32, one, idx),
-            _need("lens", lens, i32, one, idx), n, count, k.data_ptr(), v.data_ptr())
+            _need("pages", cache.pages, torch.uint8, sh.num_blocks * H * SLAB_BYTES, idx), p_bt,
+            sessions, _need("sids", sids, i32, n, idx), _need("first", first, i32, n, idx),
+            _need("lens", lens, i32, n, idx), n, count, k.data_ptr(), v.data_ptr())
     return k, v
 
 
 def attention_scratch_bytes(sh: Kv4Shape, seqs: int, rows: int, max_q: int, max_len: int,
                             accumulate: bool = False) -> int:
+    return _attention_scratch(sh.q_heads, sh.kv_heads, seqs, rows, max_q, max_len, bool(accumulate))
+
+
+@functools.lru_cache(maxsize=1024)
+def _attention_scratch(q_heads, kv_heads, seqs, rows, max_q, max_len, accumulate) -> int:
+    sh = make_shape(q_heads, kv_heads, 1, 1)  # the size goes by the heads alone
     return int(lib.dial_b200_kv4_attention_scratch_bytes(C.byref(sh), seqs, rows, max_q, max_len,
                                                          int(accumulate)))
 
@@ -192,26 +197,35 @@ def kv4_attention(sh: Kv4Shape, cache: Kv4Cache, q, block_table, sids, lens, max
     slots of a sequence.  accumulate adds each slot's probabilities to
     cache.weights.  Returns out [rows, q_heads * 128]."""
     idx, dt, i32 = q.get_device(), _DTYPE[sh.act], torch.int32
-    H, rows, n, width = sh.kv_heads, q.shape[0], sids.shape[0], sh.q_heads * HEAD_DIM
+    H, rows, n, width = sh.kv_heads, q.size(0), sids.numel(), sh.q_heads * HEAD_DIM
+    slabs = sh.num_blocks * H
     p_q, ld = _rows("q", q, dt, None, width, idx)
     if out is None:
         out = torch.empty(rows, width, dtype=dt, device=q.device)
-    p_out, ld_out = _rows("out", out, dt, rows, width, idx)
+        p_out, ld_out = out.data_ptr(), width
+    else:
+        p_out, ld_out = _rows("out", out, dt, rows, width, idx)
     p_w = 0
     if accumulate:
-        p_w = _need("weights", cache.weights, torch.float32, (sh.num_blocks, H, PAGE_TOKENS), idx)
+        p_w = _need("weights", cache.weights, torch.float32, slabs * PAGE_TOKENS, idx)
         if not p_w:
             _bad("accumulate needs a cache with weights")
     p_bt, sessions = _table("block_table", block_table, sh.max_blocks, idx)
     p_s, keep = _scratch(scratch, attention_scratch_bytes(sh, n, rows, max_q, max_len, accumulate), q)
     _launch("dial_b200_kv4_attention", idx, C.byref(sh), p_q, ld,
-            _need("pages", cache.pages, torch.uint8, (sh.num_blocks, H, SLAB_BYTES), idx), p_w, p_bt,
-            sessions, _need("sids", sids, i32, (n,), idx), _need("lens", lens, i32, (n,), idx),
-            _need("q_starts", q_starts, i32, (n + 1,), idx), n, rows, max_q, max_len, p_out, ld_out, p_s)
+            _need("pages", cache.pages, torch.uint8, slabs * SLAB_BYTES, idx), p_w, p_bt,
+            sessions, _need("sids", sids, i32, n, idx), _need("lens", lens, i32, n, idx),
+            _need("q_starts", q_starts, i32, n + 1, idx), n, rows, max_q, max_len, p_out, ld_out, p_s)
     return out
 
 
 def evict_scratch_bytes(sh: Kv4Shape, seqs: int, max_len: int, keep: int) -> int:
+    return _evict_scratch(sh.kv_heads, seqs, max_len, keep)
+
+
+@functools.lru_cache(maxsize=1024)
+def _evict_scratch(kv_heads, seqs, max_len, keep) -> int:
+    sh = make_shape(kv_heads, kv_heads, 1, 1)
     return int(lib.dial_b200_kv4_evict_scratch_bytes(C.byref(sh), seqs, max_len, keep))
 
 
@@ -221,8 +235,7 @@ def kv4_evict(sh: Kv4Shape, cache: Kv4Cache, block_table, sids, lens, max_len: i
     head; entries newer than (newest position - recent) come first.  In place,
     or into the pages of dst_table.  Returns the new lengths [seqs]."""
     idx, i32, H, nb = sids.get_device(), torch.int32, sh.kv_heads, sh.num_blocks
-    n = sids.shape[0]
-    one, slots = (n,), (nb, H, PAGE_TOKENS)
+    n, slots = sids.numel(), nb * H * PAGE_TOKENS
     if keep < 0 or max_len < 0:
         _bad(f"keep {keep} / max_len {max_len} is negative")
     if lens_out is None:
@@ -230,10 +243,10 @@ def kv4_evict(sh: Kv4Shape, cache: Kv4Cache, block_table, sids, lens, max_len: i
     p_bt, sessions = _table("block_table", block_table, sh.max_blocks, idx)
     p_s, alive = _scratch(scratch, evict_scratch_bytes(sh, n, max_len, keep), sids)
     _launch("dial_b200_kv4_evict", idx, C.byref(sh),
-            _need("pages", cache.pages, torch.uint8, (nb, H, SLAB_BYTES), idx),
+            _need("pages", cache.pages, torch.uint8, nb * H * SLAB_BYTES, idx),
             _need("weights", cache.weights, torch.float32, slots, idx),
             _need("positions pool", cache.positions, i32, slots, idx), p_bt,
-            _need("dst_table", dst_table, i32, (sessions, sh.max_blocks), idx), sessions,
-            _need("sids", sids, i32, one, idx), _need("lens", lens, i32, one, idx),
-            _need("lens_out", lens_out, i32, one, idx), n, max_len, keep, recent, p_s)
+            _need("dst_table", dst_table, i32, sessions * sh.max_blocks, idx), sessions,
+            _need("sids", sids, i32, n, idx), _need("lens", lens, i32, n, idx),
+            _need("lens_out", lens_out, i32, n, idx), n, max_len, keep, recent, p_s)
     return lens_out

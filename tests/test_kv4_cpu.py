@@ -49,7 +49,7 @@ CASES = [("append", APPEND, c) for c in POOL + [
     ({"qkv_ld": 47 * 128}, "must hold their heads"), ({"qkv_ld": 48 * 128 + 2}, "8-byte"),
     ({"qkv": P + 4}, "8-byte"), ({"q_ld": 100}, "must hold"), ({"kn": P + 2}, "8-byte aligned")]]
 CASES += [("read", READ, c) for c in POOL + [
-    ({"lens": None}, "null pointer"), ({"k": None}, "null pointer"), ({"v": P + 4}, "8-byte"),
+    ({"lens": None}, "null pointer"), ({"k": None}, "null pointer"), ({"v": P + 8}, "16-byte"),
     ({"count": -1}, "out of range"), ({"seqs": -1}, "out of range"),
     ({"seqs": 1 << 20, "count": 1 << 20}, "out of range")]]
 CASES += [("attention", ATTN, c) for c in POOL + [
