@@ -51,39 +51,43 @@ struct Pair<__half> {
   static __device__ __forceinline__ T add(T a, T b) { return __hadd2_rn(a, b); }
 };
 
-// A head held four dims a lane (dims 4 * lane ..), as two pairs.
+// A head held by 16 lanes, eight dims each (dims 8 * l ..), as four pairs.
 template <typename Act>
 struct Head {
-  typename Pair<Act>::T v[2];
-  __device__ __forceinline__ void load(const Act* p, int lane) {
-    *reinterpret_cast<uint2*>(v) = *reinterpret_cast<const uint2*>(p + lane * 4);
+  typename Pair<Act>::T v[4];
+  __device__ __forceinline__ void load(const Act* p, int l) {
+    *reinterpret_cast<uint4*>(v) = *reinterpret_cast<const uint4*>(p + l * 8);
   }
-  __device__ __forceinline__ void store(Act* p, int lane) const {
-    *reinterpret_cast<uint2*>(p + lane * 4) = *reinterpret_cast<const uint2*>(v);
+  __device__ __forceinline__ void store(Act* p, int l) const {
+    *reinterpret_cast<uint4*>(p + l * 8) = *reinterpret_cast<const uint4*>(v);
   }
-  __device__ __forceinline__ void floats(float (&x)[4]) const {
+  __device__ __forceinline__ void floats(float (&x)[8]) const {
     const Act* h = reinterpret_cast<const Act*>(v);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) x[e] = ActTraits<Act>::to_f(h[e]);
+    for (int e = 0; e < 8; ++e) x[e] = ActTraits<Act>::to_f(h[e]);
   }
 };
 
-// act(sqrt(sum x^2 / 128 + eps)) of the warp's head, as from an exact sum: the f32
+// act(sqrt(sum x^2 / 128 + eps)) of each half warp's head, as from an exact sum: the f32
 // form (off by less than 2^-20: 9 roundings of the sum, halved by the root, and 3
 // more) unless a border of the dtype lies within 2^-19 of it, else 64 bits.
 template <typename Act>
-__device__ __forceinline__ float rms_of(const float (&x)[4], float eps) {
+__device__ __forceinline__ float rms_of(const float (&x)[8], float eps) {
   using AT = ActTraits<Act>;
-  const float ss = warp_sum(fmaf(x[0], x[0], x[1] * x[1]) + fmaf(x[2], x[2], x[3] * x[3]));
+  float ss = fmaf(x[0], x[0], x[1] * x[1]) + fmaf(x[2], x[2], x[3] * x[3]);
+  ss += fmaf(x[4], x[4], x[5] * x[5]) + fmaf(x[6], x[6], x[7] * x[7]);
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
   const float m = __fsqrt_rn(ss * (1.f / kHeadDim) + eps);
   const float lo = AT::round(m * (1.f - 0x1p-19f)), hi = AT::round(m * (1.f + 0x1p-19f));
   // sums near the ends of f32's range lose more than that
-  if (lo == hi && ss > 1e-30f && ss < 1e37f) return lo;
+  const bool near = !(lo == hi && ss > 1e-30f && ss < 1e37f);
+  if (!__any_sync(0xffffffffu, near)) return lo;
   double sum = 0.;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) sum = fma(static_cast<double>(x[e]), static_cast<double>(x[e]), sum);
+  for (int e = 0; e < 8; ++e) sum = fma(static_cast<double>(x[e]), static_cast<double>(x[e]), sum);
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   return AT::round(static_cast<float>(sqrt(sum / kHeadDim + static_cast<double>(eps))));
 }
 
@@ -91,114 +95,141 @@ __device__ __forceinline__ float rms_of(const float (&x)[4], float eps) {
 // two bf16 values, so a product with 1 / m rounds as the quotient does; f16's
 // quotients come as near as 2^-23 and are divided.
 template <typename Act>
-__device__ __forceinline__ void divide(const float (&x)[4], float m, typename Pair<Act>::T (&v)[2]) {
-  float q[4];
+__device__ __forceinline__ void divide(const float (&x)[8], float m, typename Pair<Act>::T (&v)[4]) {
+  float q[8];
   if (std::is_same<Act, __nv_bfloat16>::value && m > 1e-37f && m < 1e37f) {
     const float inv = __frcp_rn(m);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) q[e] = x[e] * inv;
+    for (int e = 0; e < 8; ++e) q[e] = x[e] * inv;
   } else {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) q[e] = __fdiv_rn(x[e], m);
+    for (int e = 0; e < 8; ++e) q[e] = __fdiv_rn(x[e], m);
   }
-  v[0] = Pair<Act>::of(q[0], q[1]);
-  v[1] = Pair<Act>::of(q[2], q[3]);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] = Pair<Act>::of(q[2 * e], q[2 * e + 1]);
 }
 
 // RMSNorm and RoPE, each step rounded to the activation dtype (the decode op's
-// steps).  rope: cos, and sin with the sign of the lane's half.
+// steps); sin has the sign of the lane's half of the dims.
 template <typename Act>
 __device__ __forceinline__ void norm_rope(Head<Act>& x, const Head<Act>& w, const Head<Act>& c, const Head<Act>& s,
                                           float eps, bool norm, bool rope) {
   using P = Pair<Act>;
   if (norm) {
-    float f[4];
+    float f[8];
     x.floats(f);
     divide<Act>(f, rms_of<Act>(f, eps), x.v);
-    x.v[0] = P::mul(x.v[0], w.v[0]);
-    x.v[1] = P::mul(x.v[1], w.v[1]);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x.v[e] = P::mul(x.v[e], w.v[e]);
   }
   if (rope) {
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
+    for (int e = 0; e < 4; ++e) {
       const uint32_t own = *reinterpret_cast<const uint32_t*>(&x.v[e]);
-      const uint32_t far = __shfl_xor_sync(0xffffffffu, own, 16);
+      const uint32_t far = __shfl_xor_sync(0xffffffffu, own, 8);
       x.v[e] = P::add(P::mul(x.v[e], c.v[e]), P::mul(*reinterpret_cast<const typename P::T*>(&far), s.v[e]));
     }
   }
 }
 
-// One CTA for a row and a share (blockIdx.y) of its head units: unit u < kv_heads is a
-// kv head (k and v), the others query heads.  A warp's norm weights, cos and sin
-// serve all its heads.
-// Bound by the bytes for long prompts (2048 rows of 32 + 16 heads: 17 us, 2.6 TB/s with
-// the rows in L2), by latency for a token.
+// The lane's eight values quantised: four code bytes, and the scale code of its
+// 16-dim group (two lanes).
+__device__ __forceinline__ void encode8(const float (&x)[8], float mult, uint32_t& codes, uint32_t& scale) {
+  float v[8], amax = 0.f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    v[e] = isnan(x[e]) ? 0.f : x[e];
+    amax = fmaxf(amax, fabsf(v[e]));
+  }
+  amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+  scale = e4m3_of(__fdiv_rn(quotient(amax, 6.f, 1.f / 6.f), mult));
+  const float s = e4m3_value(scale) * mult;
+  codes = 0;
+  if (s > 0.f) {
+    const float y = __frcp_rn(s);
+#pragma unroll
+    for (int e = 0; e < 8; e += 2)
+      codes |= e2m1x2_of(quotient(v[e], s, y), quotient(v[e + 1], s, y)) << (4 * e);
+  }
+}
+
+// A CTA for a row and a share (blockIdx.y) of its head units, a half warp a unit: unit
+// u < kv_heads is a kv head (k and v), the others query heads.  A warp's norm weights,
+// cos and sin serve all its units, U of which are loaded at once.
+// Bound by instructions for long prompts (about half of them the quantisation), by
+// latency for a token.
 template <typename Act, int U>
 __global__ void __launch_bounds__(256) kv4_append_kernel(const AppendArgs a) {
-  const int lane = threadIdx.x & 31, m = blockIdx.x;
+  const int lane = threadIdx.x & 31, l = lane & 15, m = blockIdx.x;
   pdl_wait();
   pdl_launch_dependents();
-  const int slot = a.slots[m];
-  if (slot < 0) return;
-  const int sid = a.sids[m], pos = a.pos ? a.pos[m] : 0;
-  const int page = slot / kPageTokens, t = slot % kPageTokens;
+  const Act* row = static_cast<const Act*>(a.qkv) + m * a.qkv_ld;
+  const int step = gridDim.y * 16, H = a.c.kv_heads, Q = a.c.q_heads;
+  const int u0 = (blockIdx.y * 8 + (threadIdx.x >> 5)) * 2 + (lane >> 4);
   const bool norm = a.q_norm_w != nullptr, rope = a.cos != nullptr;
+  // the first units' loads beside the look-ups
+  Head<Act> x[U], y{};
+  auto fetch = [&](int base) {
+#pragma unroll
+    for (int e = 0; e < U; ++e) {
+      const int u = base + e * step;
+      x[e] = Head<Act>{};
+      if (u < a.units) x[e].load(row + (u < H ? Q + u : u - H) * kHeadDim, l);
+    }
+    if (base < H && base < a.units) y.load(row + (Q + H + base) * kHeadDim, l);
+  };
+  fetch(u0);
+  const int slot = a.slots[m], sid = a.sids[m], pos = a.pos ? a.pos[m] : 0;
+  if (slot < 0) return;
+  const int page = slot / kPageTokens, t = slot % kPageTokens;
   if (static_cast<unsigned>(sid) >= static_cast<unsigned>(a.c.sessions) || page >= a.c.max_blocks ||
       (rope && static_cast<unsigned>(pos) >= static_cast<unsigned>(a.max_pos))) {
     if (threadIdx.x == 0) set_status(a.c.status, kStatusBadArgs);
     return;
   }
-  const Act* row = static_cast<const Act*>(a.qkv) + m * a.qkv_ld;
+  const int block = kv4_block(a.c, a.c.block_table, sid, page);
   Head<Act> qw{}, kw{}, c{}, s{};
   if (norm) {
-    qw.load(static_cast<const Act*>(a.q_norm_w), lane);
-    kw.load(static_cast<const Act*>(a.k_norm_w), lane);
+    qw.load(static_cast<const Act*>(a.q_norm_w), l);
+    kw.load(static_cast<const Act*>(a.k_norm_w), l);
   }
   if (rope) {
     const size_t at = static_cast<size_t>(pos) * (kHeadDim / 2);
-    c.load(static_cast<const Act*>(a.cos) + at, lane & 15);
-    s.load(static_cast<const Act*>(a.sin) + at, lane & 15);
-    if (lane < 16) {  // dims below 64: x c - far s; above: x c + far s
-      s.v[0] = __hneg2(s.v[0]);
-      s.v[1] = __hneg2(s.v[1]);
+    c.load(static_cast<const Act*>(a.cos) + at, l & 7);
+    s.load(static_cast<const Act*>(a.sin) + at, l & 7);
+    if (l < 8) {  // dims below 64: x c - far s; above: x c + far s
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s.v[e] = __hneg2(s.v[e]);
     }
   }
-  const int step = gridDim.y * 8, H = a.c.kv_heads, Q = a.c.q_heads;
-  const int block = kv4_block(a.c, a.c.block_table, sid, page);
-  for (int u0 = blockIdx.y * 8 + (threadIdx.x >> 5); u0 < a.units; u0 += U * step) {
-    Head<Act> x[U];  // U heads in flight; a kv head's v is loaded at its turn
+  for (int base = u0; base - (lane >> 4) < a.units; base += U * step) {  // warp-uniform
+    if (base != u0) fetch(base);
 #pragma unroll
     for (int e = 0; e < U; ++e) {
-      const int u = u0 + e * step;
-      if (u < a.units) x[e].load(row + (u < H ? Q + u : u - H) * kHeadDim, lane);
-    }
-#pragma unroll
-    for (int e = 0; e < U; ++e) {
-      const int u = u0 + e * step;
-      if (u >= a.units) break;
-      if (u >= H) {
-        norm_rope(x[e], qw, c, s, a.eps, norm, rope);
-        x[e].store(static_cast<Act*>(a.q_out) + m * a.q_out_ld + (u - H) * kHeadDim, lane);
-        continue;
-      }
-      Head<Act> y;
-      y.load(row + (Q + H + u) * kHeadDim, lane);
-      norm_rope(x[e], kw, c, s, a.eps, norm, rope);
-      if (block < 0) continue;
+      const int u = base + e * step;
+      const bool kv = u < H && u < a.units;
+      const bool some_kv = __any_sync(0xffffffffu, kv);
+      if (e > 0 && kv) y.load(row + (Q + H + u) * kHeadDim, l);
+      norm_rope(x[e], u < H ? kw : qw, c, s, a.eps, norm, rope);
+      if (!kv && u < a.units) x[e].store(static_cast<Act*>(a.q_out) + m * a.q_out_ld + (u - H) * kHeadDim, l);
+      if (!some_kv) continue;
+      uint32_t kc, ks, vc, vs;
+      float f[8];
+      x[e].floats(f);
+      encode8(f, a.c.k_scale, kc, ks);
+      y.floats(f);
+      encode8(f, a.c.v_scale, vc, vs);
+      if (!kv || block < 0) continue;
       const size_t si = kv4_slab_index(a.c, block, u);
       uint8_t* slab = a.c.pages + si * kKv4Slab;
-      uint32_t codes, scale;
-      float f[4];
-      x[e].floats(f);
-      kv4_encode(f, a.c.k_scale, codes, scale);
-      *reinterpret_cast<uint16_t*>(slab + t * 64 + lane * 2) = static_cast<uint16_t>(codes);
-      if ((lane & 3) == 0) slab[kKv4KScales + t * 8 + (lane >> 2)] = static_cast<uint8_t>(scale);
-      y.floats(f);
-      kv4_encode(f, a.c.v_scale, codes, scale);
-      *reinterpret_cast<uint16_t*>(slab + kKv4VCodes + t * 64 + lane * 2) = static_cast<uint16_t>(codes);
-      if ((lane & 3) == 0) slab[kKv4VScales + t * 8 + (lane >> 2)] = static_cast<uint8_t>(scale);
-      if (lane == 0 && a.c.weights) a.c.weights[si * kPageTokens + t] = 0.f;
-      if (lane == 1 && a.c.positions) a.c.positions[si * kPageTokens + t] = pos;
+      *reinterpret_cast<uint32_t*>(slab + t * 64 + l * 4) = kc;
+      *reinterpret_cast<uint32_t*>(slab + kKv4VCodes + t * 64 + l * 4) = vc;
+      if ((l & 1) == 0) {
+        slab[kKv4KScales + t * 8 + (l >> 1)] = static_cast<uint8_t>(ks);
+        slab[kKv4VScales + t * 8 + (l >> 1)] = static_cast<uint8_t>(vs);
+      }
+      if (l == 1 && a.c.weights) a.c.weights[si * kPageTokens + t] = 0.f;
+      if (l == 3 && a.c.positions) a.c.positions[si * kPageTokens + t] = pos;
     }
   }
 }
@@ -270,7 +301,7 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const ReadArgs a) {
 template <typename Act>
 cudaError_t launch_read(const ReadArgs& a, cudaStream_t s) {
   const long long units = static_cast<long long>(a.rows) * a.c.kv_heads;
-  if (units <= 148 * 16)  // few: every (slot, kv head) a warp of its own
+  if (a.rows <= 148 * 64)  // few: every (slot, kv head) a warp of its own
     return kv4_start(kv4_read_kernel<Act, false>, dim3(static_cast<unsigned>((units + 7) / 8)), 256, 0, s, a);
   return kv4_start(kv4_read_kernel<Act, true>, dim3((a.rows + 15) / 16), 256, 0, s, a);
 }
@@ -390,12 +421,12 @@ extern "C" int dial_b200_kv4_append(const dial_b200_kv4_shape* sh, const void* q
   if (rows < 0 || rows > (1 << 26))
     return kv4_fail(err, n, DIAL_ERR_INVALID, "rows %lld outside [0, 2^26]", (long long)rows);
   const int64_t width = (sh->q_heads + 2LL * sh->kv_heads) * kHeadDim;
-  if (qkv_ld < width || qkv_ld % 4 != 0 || !aligned(qkv, 8) || (q_out && !aligned(q_out, 8)) ||
-      (q_out && (q_out_ld < 1LL * sh->q_heads * kHeadDim || q_out_ld % 4 != 0)))
+  if (qkv_ld < width || qkv_ld % 8 != 0 || !aligned(qkv, 16) || (q_out && !aligned(q_out, 16)) ||
+      (q_out && (q_out_ld < 1LL * sh->q_heads * kHeadDim || q_out_ld % 8 != 0)))
     return kv4_fail(err, n, DIAL_ERR_INVALID,
-                    "qkv and q_out rows must hold their heads and start on 8-byte boundaries");
-  if (!aligned(q_norm_w, 8) || !aligned(k_norm_w, 8) || !aligned(cos, 8) || !aligned(sin, 8))
-    return kv4_fail(err, n, DIAL_ERR_INVALID, "norm weights and RoPE tables must be 8-byte aligned");
+                    "qkv and q_out rows must hold their heads and start on 16-byte boundaries");
+  if (!aligned(q_norm_w, 16) || !aligned(k_norm_w, 16) || !aligned(cos, 16) || !aligned(sin, 16))
+    return kv4_fail(err, n, DIAL_ERR_INVALID, "norm weights and RoPE tables must be 16-byte aligned");
   if (rows == 0) return DIAL_OK;
   a.qkv = qkv;
   a.q_norm_w = q_norm_w;
@@ -415,12 +446,12 @@ extern "C" int dial_b200_kv4_append(const dial_b200_kv4_shape* sh, const void* q
   if ((rc = kv4_ready(&a.c, err, n)) != DIAL_OK) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   cudaError_t e;
-  const int most = (a.units + 7) / 8;
-  if (rows * most <= 1184) {  // a head a warp while the GPU's 148 SMs have room for more CTAs
+  const int most = (a.units + 15) / 16;
+  if (rows * most <= 1184) {  // a unit a half warp while the GPU's 148 SMs have room for more CTAs
     const dim3 grid(static_cast<unsigned>(rows), most);
     e = sh->act == DIAL_ACT_BF16 ? kv4_start(kv4_append_kernel<__nv_bfloat16, 1>, grid, 256, 0, s, a)
                                  : kv4_start(kv4_append_kernel<__half, 1>, grid, 256, 0, s, a);
-  } else {  // a row a CTA, three of a warp's heads in flight
+  } else {  // a row a CTA, three of a half warp's units in flight
     const dim3 grid(static_cast<unsigned>(rows), 1);
     e = sh->act == DIAL_ACT_BF16 ? kv4_start(kv4_append_kernel<__nv_bfloat16, 3>, grid, 256, 0, s, a)
                                  : kv4_start(kv4_append_kernel<__half, 3>, grid, 256, 0, s, a);

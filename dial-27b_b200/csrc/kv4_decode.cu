@@ -406,7 +406,16 @@ __global__ void __launch_bounds__(kWarpsOf<NT> * 32, kCtasPerSm<NT>)
           }
         }
       }
+      uint32_t there[N][2];  // V scales to keep: slots past the end may hold anything
+#pragma unroll
+      for (int u = 0; u < N; ++u) there[u][0] = there[u][1] = 0xFFFFFFFFu;
       if ((page0 + kWarps * (N - 1) + 1) * kPageTokens > open_end) {  // causal border or the end
+#pragma unroll
+        for (int u = 0; u < N; ++u) {
+          const int left = w.s.len - (page0 + kWarps * u) * kPageTokens;
+          there[u][0] = (ta < left ? 0xFFFFu : 0u) | (tb < left ? 0xFFFF0000u : 0u);
+          there[u][1] = (ta + 8 < left ? 0xFFFFu : 0u) | (tb + 8 < left ? 0xFFFF0000u : 0u);
+        }
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -491,8 +500,8 @@ __global__ void __launch_bounds__(kWarpsOf<NT> * 32, kCtasPerSm<NT>)
         const uint2 vc = *reinterpret_cast<const uint2*>(vp + ta * 64 + 512);
         const uint2 vd = *reinterpret_cast<const uint2*>(vp + tb * 64 + 512);
         const uint8_t* sp = pg0 + u * kKv4Slab + kKv4VScales + g;
-        const uint32_t sab = e4m3x2_to_f16x2(static_cast<uint16_t>(sp[ta * 8] | sp[tb * 8] << 8));
-        const uint32_t scd = e4m3x2_to_f16x2(static_cast<uint16_t>(sp[ta * 8 + 64] | sp[tb * 8 + 64] << 8));
+        const uint32_t sab = e4m3x2_to_f16x2(static_cast<uint16_t>(sp[ta * 8] | sp[tb * 8] << 8)) & there[u][0];
+        const uint32_t scd = e4m3x2_to_f16x2(static_cast<uint16_t>(sp[ta * 8 + 64] | sp[tb * 8 + 64] << 8)) & there[u][1];
         constexpr uint32_t kLow = 0x0F0F0F0Fu;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {

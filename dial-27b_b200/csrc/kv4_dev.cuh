@@ -55,29 +55,6 @@ __device__ __forceinline__ float quotient(float x, float s, float y) {
   return fabsf(q) < 1e30f ? fmaf(fmaf(-q, s, x), y, q) : __fdiv_rn(x, s);
 }
 
-// Four values (dims 4 * lane ..) of a 128-dim row quantised by its warp: the
-// two code bytes, and the scale code of the lane's 16-dim group (4 lanes).
-__device__ __forceinline__ void kv4_encode(const float (&x)[4], float mult, uint32_t& codes,
-                                           uint32_t& scale) {
-  float v[4], amax = 0.f;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    v[e] = isnan(x[e]) ? 0.f : x[e];
-    amax = fmaxf(amax, fabsf(v[e]));
-  }
-  amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-  amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-  scale = e4m3_of(__fdiv_rn(quotient(amax, 6.f, 1.f / 6.f), mult));
-  const float s = e4m3_value(scale) * mult;
-  codes = 0;
-  if (s > 0.f) {
-    const float y = __frcp_rn(s);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = quotient(v[e], s, y);
-    codes = e2m1x2_of(v[0], v[1]) | e2m1x2_of(v[2], v[3]) << 8;
-  }
-}
-
 // A sequence of an attention call: its session, slots, first row and rows.
 struct Kv4Seq {
   int sid, len, row0, n;

@@ -19,7 +19,7 @@ namespace dialb200 {
 namespace {
 
 constexpr int kSelectThreads = 1024, kSelectWarps = kSelectThreads / 32;
-constexpr int kStaged = 48 * 1024;  // keys that shared memory holds (4 bytes each)
+constexpr int kStaged = 24 * 1024;  // slots whose keys and positions fit shared memory
 
 struct EvictArgs {
   Kv4Cache c;
@@ -68,7 +68,7 @@ __device__ __forceinline__ int block_before(int v, int* warp_sums, int& total) {
 // every pass reads the weights again.
 template <bool STAGED>
 __global__ void __launch_bounds__(kSelectThreads) kv4_select_kernel(const EvictArgs a) {
-  extern __shared__ uint32_t keys[];  // STAGED: [max_len]
+  extern __shared__ uint32_t keys[];  // STAGED: [max_len], and the positions after it
   __shared__ uint32_t safe_bits[STAGED ? kStaged / 32 : 1];
   __shared__ int hist[256];
   __shared__ int sums[32];
@@ -99,12 +99,17 @@ __global__ void __launch_bounds__(kSelectThreads) kv4_select_kernel(const EvictA
   if (tid == 0) newest = INT32_MIN;
   __syncthreads();
   // keys, and the newest position
+  int32_t* staged_pos = reinterpret_cast<int32_t*>(keys) + a.max_len;
   int top = INT32_MIN;
-#pragma unroll 4
+#pragma unroll 8
   for (int s = tid; s < n; s += kSelectThreads) {
     const size_t at = index(s);
-    if (a.recent > 0) top = max(top, a.c.positions[at]);
-    if (STAGED) keys[s] = weight_key(a.c.weights[at]);
+    const int p = a.recent > 0 ? a.c.positions[at] : 0;
+    if (STAGED) {
+      keys[s] = weight_key(a.c.weights[at]);
+      staged_pos[s] = p;
+    }
+    top = max(top, p);
   }
   if (a.recent > 0) {
     top = __reduce_max_sync(0xffffffffu, top);
@@ -113,14 +118,17 @@ __global__ void __launch_bounds__(kSelectThreads) kv4_select_kernel(const EvictA
     top = newest;
   }
   const long long bar = a.recent > 0 ? static_cast<long long>(top) - a.recent : INT64_MAX;
-  auto is_new = [&](size_t at) { return a.recent > 0 && static_cast<long long>(a.c.positions[at]) > bar; };
+  auto is_new = [&](int s) {
+    return a.recent > 0 && static_cast<long long>(STAGED ? staged_pos[s] : a.c.positions[index(s)]) > bar;
+  };
+  __syncthreads();
   // runs of 32 slots, in order over the warps: warp w takes runs w * per ..
   const int runs = (n + 31) / 32, per = (runs + kSelectWarps - 1) / kSelectWarps;
   const int run0 = min(warp * per, runs), run1 = min(run0 + per, runs);
   int protects = 0;
   for (int r = run0; r < run1; ++r) {
     const int s = r * 32 + lane;
-    const uint32_t bits = __ballot_sync(0xffffffffu, s < n && is_new(index(min(s, n - 1))));
+    const uint32_t bits = __ballot_sync(0xffffffffu, s < n && is_new(min(s, n - 1)));
     if (STAGED && lane == 0) safe_bits[r] = bits;
     if (lane == 0) protects += __popc(bits);
   }
@@ -129,7 +137,7 @@ __global__ void __launch_bounds__(kSelectThreads) kv4_select_kernel(const EvictA
   protects = all;
   auto key_of = [&](int s) { return STAGED ? keys[s] : weight_key(a.c.weights[index(s)]); };
   auto safe = [&](int s) {
-    return STAGED ? (safe_bits[s >> 5] >> (s & 31) & 1u) != 0 : is_new(index(s));
+    return STAGED ? (safe_bits[s >> 5] >> (s & 31) & 1u) != 0 : is_new(s);
   };
   // the class whose entries compete for `want` places
   const bool cls = protects >= a.keep;
@@ -138,10 +146,20 @@ __global__ void __launch_bounds__(kSelectThreads) kv4_select_kernel(const EvictA
   for (int shift = 24; shift >= 0; shift -= 8) {
     if (tid < 256) hist[tid] = 0;
     __syncthreads();
-    for (int s = tid; s < n; s += kSelectThreads) {
-      const uint32_t key = key_of(s);
-      if ((shift == 24 || key >> (shift + 8) == prefix >> (shift + 8)) && safe(s) == cls)
-        atomicAdd(&hist[key >> shift & 255u], 1);
+    for (int r = warp; r < runs; r += kSelectWarps) {
+      const int s = r * 32 + lane;
+      uint32_t digit = 256;  // none
+      if (s < n) {
+        const uint32_t key = key_of(s);
+        if ((shift == 24 || key >> (shift + 8) == prefix >> (shift + 8)) && safe(s) == cls)
+          digit = key >> shift & 255u;
+      }
+      if (shift == 24) {  // weights share their sign and exponent: one addition for the lanes that do
+        const uint32_t same = __match_any_sync(0xffffffffu, digit);
+        if (digit < 256 && lane == __ffs(same) - 1) atomicAdd(&hist[digit], __popc(same));
+      } else if (digit < 256) {
+        atomicAdd(&hist[digit], 1);
+      }
     }
     __syncthreads();
     // entries with a higher digit, from the top down: warp 0, eight digits a lane
@@ -321,9 +339,9 @@ extern "C" int dial_b200_kv4_evict(const dial_b200_kv4_shape* sh, void* pages, f
   const dim3 grid(sh->kv_heads, a.seqs);
   cudaError_t e;
   if (max_len <= kStaged) {
-    e = kv4_allow_smem<kv4_select_kernel<true>>(kStaged * 4);
+    e = kv4_allow_smem<kv4_select_kernel<true>>(kStaged * 8);
     if (e == cudaSuccess)
-      e = kv4_start(kv4_select_kernel<true>, grid, kSelectThreads, static_cast<size_t>(max_len) * 4, s, a);
+      e = kv4_start(kv4_select_kernel<true>, grid, kSelectThreads, static_cast<size_t>(max_len) * 8, s, a);
   } else {
     e = kv4_start(kv4_select_kernel<false>, grid, kSelectThreads, 0, s, a);
   }

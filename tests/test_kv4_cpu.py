@@ -46,8 +46,8 @@ CASES = [("append", APPEND, c) for c in POOL + [
     ({"qkv": None}, "null pointer"), ({"slots": None}, "null pointer"), ({"qn": None}, "go in pairs"),
     ({"cos": None}, "go in pairs"), ({"pos": None}, "need positions"),
     ({"sh": dict(max_pos=0)}, "max_pos 0"), ({"sh": dict(eps=-1.0)}, "eps"), ({"rows": -1}, "rows -1"),
-    ({"qkv_ld": 47 * 128}, "must hold their heads"), ({"qkv_ld": 48 * 128 + 2}, "8-byte"),
-    ({"qkv": P + 4}, "8-byte"), ({"q_ld": 100}, "must hold"), ({"kn": P + 2}, "8-byte aligned")]]
+    ({"qkv_ld": 47 * 128}, "must hold their heads"), ({"qkv_ld": 48 * 128 + 4}, "16-byte"),
+    ({"qkv": P + 8}, "16-byte"), ({"q_ld": 100}, "must hold"), ({"kn": P + 8}, "16-byte aligned")]]
 CASES += [("read", READ, c) for c in POOL + [
     ({"lens": None}, "null pointer"), ({"k": None}, "null pointer"), ({"v": P + 8}, "16-byte"),
     ({"count": -1}, "out of range"), ({"seqs": -1}, "out of range"),

@@ -210,6 +210,22 @@ def test_attention_of_dominant_and_equal_scores(cuda):
     check_attention(c, cuda, [(0, 1000, 70), (1, 517, 40)], q_scale=30.0)
 
 
+@pytest.mark.parametrize("queries", [1, 5, 40])
+def test_attention_ignores_what_lies_past_the_end(cuda, queries):
+    """Slots past a sequence's end, in its last page and in the pages after it, hold
+    bytes that would decode to NaN."""
+    c = Cache(18, 3, 400, 8, 2)
+    lens = [300, 41, 129]
+    for s, n in enumerate(lens):
+        for slot in range(n, c.max_blocks * PAGE):
+            b, o = c.table[s, slot // PAGE], slot % PAGE
+            for part, w in ((0, 64), (1024, 64), (2048, 8), (2176, 8)):
+                c.pages[b, :, part + w * o:part + w * (o + 1)] = 0xFF
+    check_attention(c, cuda, [(s, n, min(n, queries)) for s, n in enumerate(lens)])
+    check_attention(c, cuda, [(s, n, min(n, queries)) for s, n in enumerate(lens)], weights=False,
+                    max_len=400)
+
+
 def test_attention_scale_of_the_shape(cuda):
     from dial_b200 import kv4
 
