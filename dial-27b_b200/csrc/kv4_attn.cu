@@ -36,12 +36,15 @@ extern "C" int64_t dial_b200_kv4_attention_scratch_bytes(const dial_b200_kv4_sha
   if (!sh || sh->q_heads < 1 || sh->kv_heads < 1 || sh->q_heads % sh->kv_heads != 0 || seqs < 0 || rows < 0 || max_q < 0 ||
       max_len < 0)
     return -1;
-  if (max_q * (sh->q_heads / sh->kv_heads) <= kFewCols)
-    return static_cast<int64_t>(kv4_decode_scratch(sh->q_heads, sh->kv_heads, seqs, max_q, max_len,
-                                                   with_weights != 0));
-  if (!with_weights) return static_cast<int64_t>(kv4_prefill_scratch(sh->q_heads, rows, false));
-  return static_cast<int64_t>(rows_part(sh->q_heads, rows) +
-                              kv4_colsum_scratch(sh->q_heads, sh->kv_heads, seqs, max_q, max_len));
+  // enough for every call within the sizes, whichever kernels it takes
+  const int rep = sh->q_heads / sh->kv_heads;
+  const int64_t few = max_q < kFewCols / rep ? max_q : kFewCols / rep;
+  const size_t a = kv4_decode_scratch(sh->q_heads, sh->kv_heads, seqs, few, max_len, with_weights != 0);
+  if (max_q * rep <= kFewCols) return static_cast<int64_t>(a);
+  const size_t b = with_weights ? rows_part(sh->q_heads, rows) +
+                                      kv4_colsum_scratch(sh->q_heads, sh->kv_heads, seqs, max_q, max_len)
+                                : kv4_prefill_scratch(sh->q_heads, rows, false);
+  return static_cast<int64_t>(a > b ? a : b);
 }
 
 extern "C" int dial_b200_kv4_attention(const dial_b200_kv4_shape* sh, const void* q, int64_t q_ld,

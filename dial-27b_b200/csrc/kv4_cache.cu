@@ -366,7 +366,7 @@ int kv4_cache_of(const dial_b200_kv4_shape* sh, const void* pages, float* weight
                     sh->kv_heads);
   // slabs and pages of a sequence are counted in 32 bits
   if (sh->max_blocks < 1 || sh->num_blocks < 1 || sh->max_blocks > (1 << 26) ||
-      1LL * sh->max_blocks * sh->kv_heads > INT32_MAX ||
+      (1LL * sh->max_blocks + 64) * sh->kv_heads > INT32_MAX ||
       1LL * sh->num_blocks * sh->kv_heads > INT32_MAX)
     return kv4_fail(err, n, DIAL_ERR_INVALID, "max_blocks %d / num_blocks %d out of range",
                     sh->max_blocks, sh->num_blocks);

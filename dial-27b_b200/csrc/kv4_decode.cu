@@ -46,10 +46,18 @@ constexpr int kPages = NT == 1 ? 2 : 1;  // pages of a ring slot, taken at once
 template <int NT>
 constexpr int kCtasPerSm = NT == 1 ? 2 : 3;
 constexpr int kRing = 4;           // pages in flight a warp
-constexpr int kSeqChunk = 512;     // sequences a launch
+constexpr int kSeqChunk = 256;     // sequences a launch
+constexpr int kSegPad = 20;        // a segment's own cost (its start, and the merge of its parts), in pages
+constexpr int kInfo = 6;           // sequences of a range kept in shared memory
 constexpr int kOneLen = 512;       // slots up to which a CTA takes a whole segment
 constexpr float kRaise = 8.f;      // log2 headroom of a probability above 1
 constexpr int kColStride = kHeadDim + 8;
+
+// A range's share of a segment, for its weights.
+struct Rec {
+  int seg, seg0, page0, page1;  // segment, its first page, the share's pages in it
+  int sid, h, len, cols;
+};
 
 struct DecodeArgs {
   Kv4AttnArgs a;
@@ -59,25 +67,31 @@ struct DecodeArgs {
   int pages_max;    // of a sequence
   int score_ld;     // floats a slot in `scores`
   int join_y;       // CTAs of the join that a segment's columns are dealt to
-  int4* desc;       // [ctas]: the segment that starts in a range and goes on
+  // [ctas]: the segment that starts in a range and goes on (or -1), its first row
+  // and columns; and of the segment that the range begins inside (if it does)
+  // whether it ends there: 1 yes, 0 no, -1 the range begins with a segment
+  int4* desc;
+  int rec_ld;       // records a range can have
+  int* rec_n;       // [ctas], with weights
+  Rec* rec;         // [ctas][rec_ld]
   float* part_o;    // [ctas + segments][groups][NT * 8][128]
   float* part_ml;   // [ctas + segments][groups][NT * 8][2]
   float* scores;    // [pages of all segments][16][score_ld] or null
 };
 
-// cum[i]: pages of the sequences before first + i of `seqs`; the block's threads
-// share the scan.
+// cum[i]: pages of the sequences before i; the block's threads share the scan, and
+// each keeps its sequences in `s`.
 template <int THREADS>
-__device__ __forceinline__ void page_prefix(const Kv4AttnArgs& a, int first, int seqs, int* cum, int* sums) {
+__device__ __forceinline__ void page_prefix(const Kv4AttnArgs& a, int* cum, int* sums,
+                                            Kv4Seq (&s)[kSeqChunk / THREADS]) {
   constexpr int PER = kSeqChunk / THREADS;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, seqs = a.seqs;
   int v[PER], total = 0;
 #pragma unroll
   for (int e = 0; e < PER; ++e) {
     const int i = tid * PER + e;
-    Kv4Seq s;
     v[e] = 0;
-    if (i < seqs && kv4_seq(a, first + i, s) && s.n > 0) v[e] = (s.len + kPageTokens - 1) / kPageTokens;
+    if (i < seqs && kv4_seq(a, i, s[e]) && s[e].n > 0) v[e] = (s[e].len + kPageTokens - 1) / kPageTokens;
     total += v[e];
   }
   int run = total;
@@ -116,14 +130,21 @@ __device__ __forceinline__ int seq_at(const int* cum, int seqs, int fp) {
 __device__ __forceinline__ int ranges_of(int total, int ctas, int warps) {
   return min(ctas, (total + warps - 1) / warps);
 }
-// Range of pages (over all segments) of CTA b, and the CTA whose range holds f.
-__device__ __forceinline__ int range_start(int total, int b, int ctas) {
-  return static_cast<int>(static_cast<long long>(total) * b / ctas);
-}
-__device__ __forceinline__ int range_of(int total, int f, int ctas) {
-  int b = static_cast<int>(static_cast<long long>(f) * ctas / total);
-  while (b + 1 < ctas && range_start(total, b + 1, ctas) <= f) ++b;
-  return b;
+// First page (over all segments) of range b of `ctas`.  Ranges are equal in cost, a
+// segment's own counted before its first page; a cut inside that falls on the page.
+// Costs are below 2^31 (chunk_of).
+__device__ __forceinline__ int range_start(const int* cum, int seqs, int H, int b, int ctas) {
+  if (b >= ctas) return cum[seqs] * H;
+  const unsigned all = H * (cum[seqs] + kSegPad * seqs);
+  const int x = static_cast<int>(static_cast<double>(static_cast<unsigned long long>(all) * b) / ctas);
+  int lo = 0, hi = seqs;  // cost before sequence lo <= x < cost before sequence hi
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (H * (cum[mid] + kSegPad * mid) <= x) lo = mid;
+    else hi = mid;
+  }
+  const int np = cum[lo + 1] - cum[lo], r = x - H * (cum[lo] + kSegPad * lo), h = r / (np + kSegPad);
+  return cum[lo] * H + h * np + max(0, r - h * (np + kSegPad) - kSegPad);
 }
 
 __device__ __forceinline__ float ex2(float x) {
@@ -182,16 +203,17 @@ struct DecodeSmem {
   float2 fin[NT * 8];  // (m, 1 / l) of the only segment
   uint64_t full[kWarps][kSlots];
   uint64_t merged;  // every warp has read the parts in o and ml
+  Kv4Seq info[kInfo];  // the range's first sequences
   int cum[kSeqChunk + 1];
   int sums[kWarps];
 };
 
 // The probabilities of slot t (scores x, the columns' (m, 1 / l) in ml) into its
 // running weight.
-__device__ __forceinline__ void add_weight(const DecodeArgs& d, const Kv4Seq& s, int h, int t, const float* x,
+__device__ __forceinline__ void add_weight(const DecodeArgs& d, int sid, int h, int t, const float* x,
                                            const float2* ml, int cols) {
   const Kv4AttnArgs& a = d.a;
-  const int block = kv4_block(a.c, a.c.block_table, s.sid, t / kPageTokens);
+  const int block = kv4_block(a.c, a.c.block_table, sid, t / kPageTokens);
   float* to = a.c.weights + kv4_slab_index(a.c, max(block, 0), h) * kPageTokens + t % kPageTokens;
   const float old = *to;
   float sum = 0.f;
@@ -214,6 +236,13 @@ struct Share {
   int h, seg, seg0, seg1, end;  // kv head, number, first and last page, end of the share
 };
 
+template <typename Act>
+__device__ __forceinline__ void zero_rows(const Kv4AttnArgs& a, const Kv4Seq& s, int tid, int threads) {
+  for (int r = 0; r < s.n; ++r)
+    for (int e = tid * 8; e < a.c.q_heads * kHeadDim; e += threads * 8)
+      *reinterpret_cast<uint4*>(static_cast<Act*>(a.out) + (s.row0 + r) * a.out_ld + e) = make_uint4(0, 0, 0, 0);
+}
+
 template <typename Act, int NT, bool SCORES>
 __global__ void __launch_bounds__(kWarpsOf<NT> * 32, kCtasPerSm<NT>)
     kv4_decode_kernel(const DecodeArgs d) {
@@ -233,50 +262,73 @@ __global__ void __launch_bounds__(kWarpsOf<NT> * 32, kCtasPerSm<NT>)
   }
   // sequences of this CTA's work: all of the call, or one
   const int si0 = d.one ? b / H : 0, seqs = d.one ? 1 : a.seqs, b_of = d.one ? b - si0 * H : b;
+  Kv4Seq own[kSeqChunk / (kWarps * 32)];
+  int f0, f1, first_seq = 0;
   if (d.one) {
-    Kv4Seq s;
+    const bool good = kv4_seq(a, si0, own[0]);
+    const int np = good && own[0].n > 0 ? (own[0].len + kPageTokens - 1) / kPageTokens : 0;
     if (tid == 0) {
       sm.cum[0] = 0;
-      sm.cum[1] = kv4_seq(a, si0, s) && s.n > 0 ? (s.len + kPageTokens - 1) / kPageTokens : 0;
+      sm.cum[1] = np;
+      sm.info[0] = own[0];
     }
-    __syncthreads();
+    f0 = b_of * np;
+    f1 = f0 + np;
+    if (good && np == 0 && b_of == 0 && blockIdx.y == 0) zero_rows<Act>(a, own[0], tid, kWarps * 32);
   } else {
-    page_prefix<kWarps * 32>(a, 0, seqs, sm.cum, sm.sums);
+    page_prefix<kWarps * 32>(a, sm.cum, sm.sums, own);
+    const int ctas = ranges_of(sm.cum[seqs] * H, d.ctas, kWarps);
+    f0 = range_start(sm.cum, seqs, H, min(b, ctas), ctas);
+    f1 = range_start(sm.cum, seqs, H, min(b + 1, ctas), ctas);
+    first_seq = f0 < f1 ? seq_at(sm.cum, seqs, f0 / H) : 0;
+#pragma unroll
+    for (int e = 0; e < kSeqChunk / (kWarps * 32); ++e) {
+      const int i = tid * (kSeqChunk / (kWarps * 32)) + e;
+      if (i >= first_seq && i < min(seqs, first_seq + kInfo)) sm.info[i - first_seq] = own[e];
+    }
+    // sequences without a slot: zeros
+    for (int i = b; i < seqs; i += d.ctas) {
+      Kv4Seq s;
+      if (sm.cum[i + 1] == sm.cum[i] && blockIdx.y == 0 && kv4_seq(a, i, s)) zero_rows<Act>(a, s, tid, kWarps * 32);
+    }
+    if (f0 == f1 && tid == 0 && blockIdx.y == 0) {
+      d.desc[b] = make_int4(-1, 0, 0, -1);
+      if (SCORES) d.rec_n[b] = 0;
+    }
   }
-  const int total = sm.cum[seqs] * H;
-  // sequences without a slot: zeros
-  for (int i = b_of; i < seqs; i += d.ctas) {
-    Kv4Seq s;
-    if (sm.cum[i + 1] != sm.cum[i] || !kv4_seq(a, si0 + i, s) || blockIdx.y != 0) continue;
-    for (int r = 0; r < s.n; ++r)
-      for (int e = tid * 8; e < a.c.q_heads * kHeadDim; e += kWarps * 32 * 8)
-        *reinterpret_cast<uint4*>(static_cast<Act*>(a.out) + (s.row0 + r) * a.out_ld + e) =
-            make_uint4(0, 0, 0, 0);
-  }
-  const int ctas = d.one ? (total > 0 ? H : 0) : ranges_of(total, d.ctas, kWarps);
-  if (b_of >= ctas) {
-    if (tid == 0 && blockIdx.y == 0 && !d.one) d.desc[b] = make_int4(-1, 0, 0, 0);
-    return;
-  }
-  // with one segment a CTA the ranges are the sequence's kv heads
-  const int f0 = range_start(total, b_of, ctas), f1 = range_start(total, b_of + 1, ctas);
+  if (f0 == f1) return;
+  __syncthreads();
+  auto seq_info = [&](int i, Kv4Seq& s) {
+    if (i - first_seq < kInfo) s = sm.info[i - first_seq];
+    else kv4_seq(a, i, s);
+  };
 
   // this warp's pages: f0 + warp + kWarps * i, i < mine; each lane holds the slab
   // number of one page of a window of 32 and copies that page itself; the next
   // window's table loads go out a window ahead
   const int mine = f1 - f0 > warp ? (f1 - f0 - warp + kWarps - 1) / kWarps : 0;
-  auto slab_of = [&](int i) -> int {
-    if (i >= mine) return 0;
-    const int f = f0 + warp + kWarps * i;
+  // table entry of the warp's page i, and its kv head
+  auto entry_of = [&](int i, int& h) -> const int32_t* {
+    const int f = f0 + warp + kWarps * min(i, max(mine - 1, 0));
     const int s = seq_at(sm.cum, seqs, f / H);
     const int np = sm.cum[s + 1] - sm.cum[s], r = f - sm.cum[s] * H;
-    return max(0, kv4_block(a.c, a.c.block_table, a.sids[si0 + s], r % np)) * H + r / np;
+    Kv4Seq q;
+    seq_info(s, q);
+    h = r / np;
+    return a.c.block_table + static_cast<size_t>(q.sid) * a.c.max_blocks + (r - h * np);
   };
-  int win = slab_of(lane), win_next = slab_of(32 + lane), issued = 0;
+  auto slab_of = [&](int block, int h) -> int {
+    if (static_cast<unsigned>(block) >= static_cast<unsigned>(a.c.num_blocks)) {
+      set_status(a.c.status, kStatusBadArgs);
+      block = 0;
+    }
+    return block * H + h;
+  };
+  int win = 0, block_next = 0, head_next = 0, issued = 0;
   auto issue = [&]() {  // the next U pages into their slot; warp-uniform
     if (issued > 0 && (issued & 31) == 0) {
-      win = win_next;
-      win_next = slab_of(issued + 32 + lane);
+      win = slab_of(block_next, head_next);
+      block_next = *entry_of(issued + 32 + lane, head_next);
     }
     const int n = min(U, mine - issued), at = lane - (issued & 31);
     uint64_t* bar = &sm.full[warp][issued / U % kSlots];
@@ -286,8 +338,6 @@ __global__ void __launch_bounds__(kWarpsOf<NT> * 32, kCtasPerSm<NT>)
                a.c.pages + static_cast<size_t>(static_cast<unsigned>(win)) * kKv4Slab, kKv4Slab, bar);
     issued += n;
   };
-  while (issued < kRing && issued < mine) issue();
-
   auto share_at = [&](int f) {
     Share w;
     const int si = seq_at(sm.cum, seqs, f / H);
@@ -297,7 +347,7 @@ __global__ void __launch_bounds__(kWarpsOf<NT> * 32, kCtasPerSm<NT>)
     w.seg0 = base + w.h * np;
     w.seg1 = w.seg0 + np;
     w.end = min(f1, w.seg1);
-    kv4_seq(a, si0 + si, w.s);
+    seq_info(si, w.s);
     return w;
   };
   auto load_q = [&](const Share& w, int buf) {
@@ -318,8 +368,19 @@ __global__ void __launch_bounds__(kWarpsOf<NT> * 32, kCtasPerSm<NT>)
   bool ok = true;
   Share w = share_at(f0);
   load_q(w, 0);
+  {
+    int h;
+    const int32_t *e0 = entry_of(lane, h), *e1 = entry_of(32 + lane, head_next);
+    const int block = *e0;
+    block_next = *e1;
+    win = slab_of(block, h);
+  }
+  while (issued < kRing && issued < mine) issue();
   cp_async_wait();
   __syncthreads();
+  // the segment that the range begins inside: ends in it (1) or not (0)
+  const int first_ends = f0 == w.seg0 ? -1 : w.seg1 <= f1;
+  int recs = 0;
   for (int fc = f0;; buf ^= 1, ++shares) {
     // ------------------------------------------------ one segment's share
     const int fe = w.end, cols = w.s.n * rep;
@@ -587,19 +648,24 @@ __global__ void __launch_bounds__(kWarpsOf<NT> * 32, kCtasPerSm<NT>)
     if (SCORES && d.one) {  // this CTA's scores, all of the segment's columns
       __syncthreads();
       for (int t = tid; t < w.s.len; t += kWarps * 32)
-        add_weight(d, w.s, w.h, t, d.scores + (score0 + static_cast<size_t>(w.seg0) * kPageTokens + t) * d.score_ld,
+        add_weight(d, w.s.sid, w.h, t, d.scores + (score0 + static_cast<size_t>(w.seg0) * kPageTokens + t) * d.score_ld,
                    sm.fin, cols);
       break;
     }
     if (d.one) break;
-    if (fe == f1) {
-      // the only segment of the range that can start in it and go on
-      if (tid == 0 && blockIdx.y == 0)
-        d.desc[b] = fc == w.seg0 && fe < w.seg1
-                        ? make_int4(w.seg, range_of(total, w.seg1 - 1, ctas) - b + 1, w.s.row0, cols)
-                        : make_int4(-1, 0, 0, 0);
-      break;
+    if (tid == 0 && blockIdx.y == 0) {
+      if (SCORES && recs < d.rec_ld)
+        d.rec[static_cast<size_t>(b) * d.rec_ld + recs] =
+            Rec{w.seg, w.seg0, fc - w.seg0, fe - w.seg0, w.s.sid, w.h, w.s.len, cols};
+      if (SCORES && recs >= d.rec_ld) set_status(a.c.status, kStatusBadArgs);
+      if (fe == f1) {
+        // the only segment of the range that can start in it and go on
+        d.desc[b] = make_int4(fc == w.seg0 && fe < w.seg1 ? w.seg : -1, w.s.row0, cols, first_ends);
+        if (SCORES) d.rec_n[b] = min(recs + 1, d.rec_ld);
+      }
     }
+    ++recs;
+    if (fe == f1) break;
     fc = fe;
     w = next;
   }
@@ -624,6 +690,25 @@ __device__ __forceinline__ float2 join_ml(const float2* ml, size_t stride, int p
   return make_float2(M, warp_sum(L));
 }
 
+// Ranges after b that go on with the segment that starts in b and does not end there.
+__device__ __forceinline__ int parts_after(const DecodeArgs& d, int b) {
+  const int lane = threadIdx.x & 31;
+  for (int n = 0;; n += 32) {
+    const int at = b + 1 + n + lane;
+    const unsigned ends = __ballot_sync(0xffffffffu, at >= d.ctas || d.desc[at].w != 0);
+    if (ends) return n + __ffs(ends);
+  }
+}
+// The range before b in which segment `seg` starts.
+__device__ __forceinline__ int owner_before(const DecodeArgs& d, int b, int seg) {
+  const int lane = threadIdx.x & 31;
+  for (int n = b - 1;; n -= 32) {
+    const int at = n - lane;
+    const unsigned hit = __ballot_sync(0xffffffffu, at < 0 || d.desc[at].x == seg);
+    if (hit) return max(n - (__ffs(hit) - 1), 0);
+  }
+}
+
 // blockIdx.y < d.join_y: joins the parts of the segment that starts in range
 // blockIdx.x and goes on in others, a column a CTA, parts over the warps.
 // blockIdx.y >= d.join_y (with weights): adds the probabilities of the slots of
@@ -637,9 +722,10 @@ __global__ void __launch_bounds__(kJoinThreads) kv4_join_kernel(const DecodeArgs
   if (blockIdx.y < d.join_y) {
     __shared__ float4 red[kJoinWarps][kHeadDim / 4];
     pdl_wait();
-    const int4 ds = d.desc[b];  // segment, its parts, first row, columns
+    const int4 ds = d.desc[b];
     if (ds.x < 0) return;
-    for (int col = blockIdx.y; col < ds.w; col += d.join_y) {
+    const int parts = 1 + parts_after(d, b);
+    for (int col = blockIdx.y; col < ds.z; col += d.join_y) {
       const size_t first = static_cast<size_t>(b + ds.x) * stride + col;
       const float4* po = reinterpret_cast<const float4*>(d.part_o) + first * (kHeadDim / 4) + lane;
       const float2* ml = reinterpret_cast<const float2*>(d.part_ml) + first;
@@ -649,10 +735,10 @@ __global__ void __launch_bounds__(kJoinThreads) kv4_join_kernel(const DecodeArgs
 #pragma unroll
       for (int e = 0; e < PRE; ++e) {
         const int p = warp + kJoinWarps * e;
-        pre[e] = p < ds.y ? po[p * stride * (kHeadDim / 4)] : make_float4(0.f, 0.f, 0.f, 0.f);
-        pm[e] = p < ds.y ? ml[p * stride].x : -INFINITY;
+        pre[e] = p < parts ? po[p * stride * (kHeadDim / 4)] : make_float4(0.f, 0.f, 0.f, 0.f);
+        pm[e] = p < parts ? ml[p * stride].x : -INFINITY;
       }
-      const float2 all = join_ml(ml, stride, ds.y);
+      const float2 all = join_ml(ml, stride, parts);
       float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
       auto add = [&](const float4& v, float mp) {
         const float f = mp == -INFINITY ? 0.f : ex2(mp - all.x);
@@ -664,7 +750,7 @@ __global__ void __launch_bounds__(kJoinThreads) kv4_join_kernel(const DecodeArgs
 #pragma unroll
       for (int e = 0; e < PRE; ++e) add(pre[e], pm[e]);
 #pragma unroll 4
-      for (int p = warp + kJoinWarps * PRE; p < ds.y; p += kJoinWarps)
+      for (int p = warp + kJoinWarps * PRE; p < parts; p += kJoinWarps)
         add(po[p * stride * (kHeadDim / 4)], ml[p * stride].x);
       red[warp][lane] = O;
       __syncthreads();
@@ -672,7 +758,7 @@ __global__ void __launch_bounds__(kJoinThreads) kv4_join_kernel(const DecodeArgs
         float v = 0.f;
 #pragma unroll
         for (int w = 0; w < kJoinWarps; ++w) v += reinterpret_cast<const float*>(red[w])[tid];
-        static_cast<Act*>(a.out)[(ds.z + col / rep) * a.out_ld + ((ds.x % H) * rep + col % rep) * kHeadDim +
+        static_cast<Act*>(a.out)[(ds.y + col / rep) * a.out_ld + ((ds.x % H) * rep + col % rep) * kHeadDim +
                                  place_dim(tid)] =
             ActTraits<Act>::from_f(all.y != 0.f ? v / all.y * a.c.v_scale : 0.f);
       }
@@ -680,38 +766,28 @@ __global__ void __launch_bounds__(kJoinThreads) kv4_join_kernel(const DecodeArgs
     }
     return;
   }
-  __shared__ int cum[kSeqChunk + 1];
-  __shared__ int sums[kJoinWarps];
   __shared__ float2 ml[kKv4DecodeCols];  // (m, 1 / l) of the segment's columns
-  page_prefix<kJoinThreads>(a, 0, a.seqs, cum, sums);
   pdl_wait();
-  const int total = cum[a.seqs] * H;
-  const int ctas = ranges_of(total, d.ctas, kWarpsOf<NT>);
-  if (b >= ctas) return;
-  const int f0 = range_start(total, b, ctas), f1 = range_start(total, b + 1, ctas);
-  const int y = blockIdx.y - d.join_y, ys = gridDim.y - d.join_y;
-  for (int fc = f0; fc < f1;) {
-    const int si = seq_at(cum, a.seqs, fc / H);
-    const int np = cum[si + 1] - cum[si], base = cum[si] * H;
-    const int h = (fc - base) / np, seg0 = base + h * np, seg1 = seg0 + np;
-    const int fe = min(f1, seg1), seg = si * H + h;
-    Kv4Seq s;
-    kv4_seq(a, si, s);
-    const int cols = s.n * rep;
-    const int b0 = range_of(total, seg0, ctas), b1 = range_of(total, seg1 - 1, ctas);
-    for (int col = warp; col < cols; col += kJoinWarps) {
+  const int y = blockIdx.y - d.join_y, ys = gridDim.y - d.join_y, n = d.rec_n[b];
+  for (int k = 0; k < n; ++k) {
+    const Rec r = d.rec[static_cast<size_t>(b) * d.rec_ld + k];
+    // ranges that hold parts of the segment: from the one it starts in
+    const int b0 = r.page0 == 0 ? b : owner_before(d, b, r.seg);
+    const bool ends = k + 1 < n || d.desc[b].x != r.seg;  // in this range, if it starts here
+    const int parts = r.page0 == 0 && ends ? 1 : 1 + parts_after(d, b0);
+    for (int col = warp; col < r.cols; col += kJoinWarps) {
       const float2 v = join_ml(reinterpret_cast<const float2*>(d.part_ml) +
-                                   static_cast<size_t>(b0 + seg) * stride + col,
-                               stride, b1 - b0 + 1);
+                                   static_cast<size_t>(b0 + r.seg) * stride + col,
+                               stride, parts);
       if (lane == 0) ml[col] = make_float2(v.x == -INFINITY ? 0.f : v.x, v.y > 0.f ? 1.f / v.y : 0.f);
     }
     __syncthreads();
-    const int upto = min((fe - seg0) * kPageTokens, s.len);
-    for (int t = (fc - seg0) * kPageTokens + y * kJoinThreads + tid; t < upto; t += ys * kJoinThreads) {
-      add_weight(d, s, h, t, d.scores + (static_cast<size_t>(seg0) * kPageTokens + t) * d.score_ld, ml, cols);
-    }
+    const int upto = min(r.page1 * kPageTokens, r.len);
+#pragma unroll 2
+    for (int t = r.page0 * kPageTokens + y * kJoinThreads + tid; t < upto; t += ys * kJoinThreads)
+      add_weight(d, r.sid, r.h, t, d.scores + (static_cast<size_t>(r.seg0) * kPageTokens + t) * d.score_ld, ml,
+                 r.cols);
     __syncthreads();
-    fc = fe;
   }
 }
 
@@ -731,7 +807,8 @@ struct Plan {
   int nt, groups, ctas, cols, score_ld, pages_max;
   bool one;
   long long pages;  // pages of all segments at most
-  size_t desc, part_o, part_ml, scores;
+  int rec_ld;
+  size_t desc, rec, part_o, part_ml, scores;
 };
 
 Plan plan_of(int q_heads, int kv_heads, long long seqs, long long max_q, long long max_len,
@@ -761,6 +838,13 @@ Plan plan_of(int q_heads, int kv_heads, long long seqs, long long max_q, long lo
   p.desc = p.one ? 0 : up(static_cast<size_t>(p.ctas) * sizeof(int4));
   p.part_o = up(rows * kHeadDim * 4);
   p.part_ml = up(rows * 8);
+  // a share costs kSegPad pages at least, and a segment has one in a range; with
+  // k < ctas ranges (few pages: 8 k at most) a range has 8 k shares at most
+  const long long segs = seqs * kv_heads;
+  long long shares = (p.pages + kSegPad * segs) / (static_cast<long long>(p.ctas) * kSegPad) + 8;
+  shares += static_cast<long long>(sqrt(8. * static_cast<double>(segs))) + 1;
+  p.rec_ld = static_cast<int>(shares < segs ? shares : segs);
+  p.rec = weights && !p.one ? up(static_cast<size_t>(p.ctas) * (4 + static_cast<size_t>(p.rec_ld) * sizeof(Rec)) + 128) : 0;
   p.scores = weights ? up(static_cast<size_t>(p.pages) * kPageTokens * p.score_ld * 4) : 0;
   return p;
 }
@@ -768,8 +852,8 @@ Plan plan_of(int q_heads, int kv_heads, long long seqs, long long max_q, long lo
 // Sequences a launch takes: the prefix in shared memory holds kSeqChunk, and
 // page numbers are 32-bit.
 long long chunk_of(int kv_heads, long long seqs, long long max_len) {
-  const long long per = (max_len + kPageTokens - 1) / kPageTokens * kv_heads;
-  long long n = per > 0 ? INT32_MAX / per : kSeqChunk;
+  const long long per = ((max_len + kPageTokens - 1) / kPageTokens + kSegPad) * kv_heads;
+  long long n = INT32_MAX / per;
   n = n < kSeqChunk ? n : kSeqChunk;
   return n < seqs ? n : seqs;
 }
@@ -788,7 +872,7 @@ cudaError_t launch_nt(const DecodeArgs& d, cudaStream_t s) {
       e = kv4_start(kv4_decode_kernel<Act, NT, false>, dim3(d.ctas, d.groups), kWarpsOf<NT> * 32, smem, s, d);
   }
   if (e != cudaSuccess || d.one) return e;
-  return kv4_start(kv4_join_kernel<Act, NT>, dim3(d.ctas, d.join_y + (d.scores ? 2 : 0)), kJoinThreads, 0, s, d);
+  return kv4_start(kv4_join_kernel<Act, NT>, dim3(d.ctas, d.join_y + (d.scores ? 4 : 0)), kJoinThreads, 0, s, d);
 }
 
 }  // namespace
@@ -798,7 +882,7 @@ size_t kv4_decode_scratch(int q_heads, int kv_heads, long long seqs, long long m
   const long long n = chunk_of(kv_heads, seqs, max_len);
   if (n < 1) return 0;
   const Plan p = plan_of(q_heads, kv_heads, n, max_q, max_len, weights, 148);
-  return p.desc + p.part_o + p.part_ml + p.scores;
+  return p.desc + p.rec + p.part_o + p.part_ml + p.scores;
 }
 
 cudaError_t kv4_decode_launch(const Kv4AttnArgs& a, int act, cudaStream_t s) {
@@ -826,9 +910,14 @@ cudaError_t kv4_decode_launch(const Kv4AttnArgs& a, int act, cudaStream_t s) {
     d.score_ld = p.score_ld;
     uint8_t* w = static_cast<uint8_t*>(a.scratch);
     d.desc = reinterpret_cast<int4*>(w);
-    d.part_o = reinterpret_cast<float*>(w + p.desc);
-    d.part_ml = reinterpret_cast<float*>(w + p.desc + p.part_o);
-    d.scores = a.c.weights ? reinterpret_cast<float*>(w + p.desc + p.part_o + p.part_ml) : nullptr;
+    w += p.desc;
+    d.rec_ld = p.rec_ld;
+    d.rec = reinterpret_cast<Rec*>(w);
+    d.rec_n = reinterpret_cast<int*>(w + static_cast<size_t>(p.ctas) * p.rec_ld * sizeof(Rec));
+    w += p.rec;
+    d.part_o = reinterpret_cast<float*>(w);
+    d.part_ml = reinterpret_cast<float*>(w + p.part_o);
+    d.scores = a.c.weights ? reinterpret_cast<float*>(w + p.part_o + p.part_ml) : nullptr;
     d.join_y = p.cols < 16 ? p.cols : 16;
     const bool bf = act == DIAL_ACT_BF16;
     const cudaError_t e = p.nt == 1 ? (bf ? launch_nt<__nv_bfloat16, 1>(d, s) : launch_nt<__half, 1>(d, s))

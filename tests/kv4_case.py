@@ -116,10 +116,9 @@ class Cache:
 
     def values(self, sid, n):
         """k and v [n, kv_heads, 128] of the session's slots."""
-        b, o = self.at(sid, n)
-        k, ks, v, vs = unpack(self.pages)
-        return (decode(k[b, :, o], ks[b, :, o], self.k_scale),
-                decode(v[b, :, o], vs[b, :, o], self.v_scale))
+        k, ks, v, vs = unpack(self.pages[self.table[sid, :-(-n // PAGE)]])  # [pages, heads, 16, .]
+        flat = lambda x: x.transpose(0, 2, 1, 3).reshape(-1, self.H, x.shape[-1])[:n]  # noqa: E731
+        return (decode(flat(k), flat(ks), self.k_scale), decode(flat(v), flat(vs), self.v_scale))
 
     def put(self, sid, slot, k, v, pos):
         """One token's k and v [kv_heads, 128] into its slot."""

@@ -192,6 +192,17 @@ def test_attention_prompts(cuda, queries, lens, heads):
                     spare_rows=1, stride=64)
 
 
+@pytest.mark.parametrize("weights", [False, True])
+def test_attention_of_many_ragged_sequences(cuda, weights):
+    """More sequences than one launch takes, most of them short or empty, a few
+    long: ranges with many segments, and segments over many ranges."""
+    c = Cache(19, 300, 900, 4, 2)
+    lens = [int(n) for n in c.rng.integers(0, 40, 300)]
+    for i, n in ((7, 900), (150, 777), (151, 0), (299, 899)):
+        lens[i] = n
+    check_attention(c, cuda, [(s, n, 1) for s, n in enumerate(lens)], weights=weights)
+
+
 def test_attention_long_split(cuda):
     """One session long enough for every split, at an odd length; the largest
     score in the first and in the last slot."""
@@ -361,3 +372,242 @@ def test_a_run_of_steps_with_eviction(cuda):
             same_slabs(host(cache.pages), c.pages)
             np.testing.assert_array_equal(host(cache.weights), c.weights)
             np.testing.assert_array_equal(host(cache.positions), c.positions)
+
+
+# ------------------------------------------- streams, graphs, devices, refusals
+STATUS_BAD_ARGS = 0x104  # kStatusBadArgs (csrc/common.cuh)
+
+
+def test_a_captured_step_replays_on_new_inputs(cuda):
+    """append -> attention with weights -> eviction captured once and replayed with
+    other rows, lengths and pages: as the same calls made eagerly."""
+    from dial_b200 import kv4
+
+    c = Cache(41, 3, 1024, 8, 2)
+    base, table = c.device(cuda)
+    runs = []
+    for graph in (False, True):
+        cache = kv4.Kv4Cache(base.pages.clone(), base.weights.clone(), base.positions.clone())
+        x = torch.zeros(3, 12 * DIM, dtype=BF16, device=cuda)
+        sids, slots, lens = i32(cuda, 0, 1, 2), i32(cuda, 0, 0, 0), i32(cuda, 0, 0, 0)
+        pos = i32(cuda, 0, 0, 0)
+        new = torch.zeros_like(lens)
+        q = torch.zeros(3, 8 * DIM, dtype=BF16, device=cuda)
+        out = torch.zeros_like(q)
+        s1 = torch.empty(kv4.attention_scratch_bytes(c.sh, 3, 3, 1, 1024, True) + 16, dtype=torch.uint8,
+                         device=cuda)
+        s2 = torch.empty(kv4.evict_scratch_bytes(c.sh, 3, 1024, 700), dtype=torch.uint8, device=cuda)
+
+        def step():
+            kv4.kv4_append(c.sh, cache, x, table, sids, slots, pos, q_out=q)
+            kv4.kv4_attention(c.sh, cache, q, table, sids, lens, 1024, accumulate=True, out=out,
+                              scratch=s1)
+            kv4.kv4_evict(c.sh, cache, table, sids, lens, 1024, 700, 100, lens_out=new, scratch=s2)
+
+        if graph:
+            side = torch.cuda.Stream(cuda)
+            side.wait_stream(torch.cuda.current_stream(cuda))
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.stream(side), torch.cuda.graph(g, stream=side):
+                step()
+            torch.cuda.synchronize()
+        got = []
+        gen = torch.Generator(device=cuda)
+        gen.manual_seed(1)
+        for n in ([900, 1, 33], [701, 700, 2], [17, 1000, 699]):
+            x.copy_(torch.randn(x.shape, generator=gen, device=cuda))
+            lens.copy_(i32(cuda, *n))
+            slots.copy_(lens - 1)
+            pos.copy_(lens + 3)
+            g.replay() if graph else step()
+            got.append([t.clone() for t in (out, new, cache.pages, cache.weights, cache.positions)])
+        torch.cuda.synchronize()
+        runs.append(got)
+    for eager, replayed in zip(*runs):
+        for a, b in zip(eager, replayed):
+            assert torch.equal(a, b)
+
+
+def test_two_streams_with_scratch_of_their_own(cuda):
+    """Calls that overlap in time, each with its own scratch, on streams other than
+    their tensors', as the same calls alone."""
+    from dial_b200 import kv4
+
+    c = Cache(42, 2, 3000, 8, 2)
+    cache, table = c.device(cuda)
+    q = (torch.randn(2, 8 * DIM, device=cuda) * 2).to(BF16)
+    qs = (torch.randn(300, 8 * DIM, device=cuda) * 2).to(BF16)
+
+    def call(kind):
+        if kind == 0:
+            return kv4.kv4_attention(c.sh, cache, q, table, i32(cuda, 0, 1), i32(cuda, 3000, 2999), 3000)
+        return kv4.kv4_attention(c.sh, cache, qs, table, i32(cuda, 1), i32(cuda, 2500), 3000,
+                                 q_starts=i32(cuda, 0, 300), max_q=300)
+
+    want = [call(0), call(1)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(cuda) for _ in range(2)]
+    for _ in range(10):
+        got = [None, None]
+        for k, s in enumerate(streams):
+            s.wait_stream(torch.cuda.current_stream(cuda))
+            with torch.cuda.stream(s):
+                got[k] = call(k)
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
+
+
+def test_repeated_calls_give_the_same_bits(cuda):
+    c = Cache(43, 4, 5000, 32, 8)
+    cache, table = c.device(cuda)
+    q = (torch.randn(4, 32 * DIM, device=cuda) * 2).to(BF16)
+    lens = i32(cuda, 5000, 17, 4001, 900)
+    from dial_b200 import kv4
+
+    outs, weights = [], []
+    for _ in range(6):
+        w = kv4.Kv4Cache(cache.pages, cache.weights.clone(), cache.positions)
+        outs.append(kv4.kv4_attention(c.sh, w, q, table, i32(cuda, 0, 1, 2, 3), lens, 5000, accumulate=True))
+        weights.append(w.weights)
+    assert all(torch.equal(o, outs[0]) for o in outs) and all(torch.equal(w, weights[0]) for w in weights)
+
+
+def test_pages_past_four_gigabytes(cuda):
+    """Pages whose byte offset passes 32 bits, at the end of a pool of 5 GB."""
+    from dial_b200 import kv4
+
+    c = Cache(44, 1, 200, 8, 4)
+    blocks = (5 << 30) // (4 * 2304)
+    small, _ = c.device(cuda)
+    big = kv4.Kv4Cache(torch.empty(blocks, 4, 2304, dtype=torch.uint8, device=cuda),
+                       torch.zeros(blocks, 4, PAGE, device=cuda),
+                       torch.zeros(blocks, 4, PAGE, dtype=torch.int32, device=cuda))
+    shift = blocks - c.pages.shape[0]
+    big.pages[shift:] = small.pages
+    big.weights[shift:] = small.weights
+    c.table = c.table + shift
+    c.sh.num_blocks = blocks
+    table = torch.from_numpy(c.table).to(cuda)
+    q = (torch.randn(1, 8 * DIM, device=cuda) * 2).to(BF16)
+    out = kv4.kv4_attention(c.sh, big, q, table, i32(cuda, 0), i32(cuda, 200), 200, accumulate=True)
+    new = kv4.kv4_evict(c.sh, big, table, i32(cuda, 0), i32(cuda, 200), 200, 90)
+    k, v = kv4.kv4_read(c.sh, big, table, i32(cuda, 0), new, 90)
+    c.table = c.table - shift
+    o, b, s, _ = c.attend(host(q), 0, 200)
+    assert (np.abs(host(out) - o) <= b).all()
+    # the same on the small pool, bit for bit
+    ref, table = c.device(cuda)
+    c.sh.num_blocks = c.pages.shape[0]
+    out2 = kv4.kv4_attention(c.sh, ref, q, table, i32(cuda, 0), i32(cuda, 200), 200, accumulate=True)
+    kv4.kv4_evict(c.sh, ref, table, i32(cuda, 0), i32(cuda, 200), 200, 90)
+    k2, v2 = kv4.kv4_read(c.sh, ref, table, i32(cuda, 0), new, 90)
+    assert int(new[0]) == 90 and torch.equal(out, out2) and torch.equal(k, k2) and torch.equal(v, v2)
+    assert torch.equal(big.weights[shift:], ref.weights) and torch.equal(big.pages[shift:], ref.pages)
+    del big
+    torch.cuda.empty_cache()
+
+
+def test_bad_rows_are_left_out_and_reported(cuda):
+    """Sessions, slots, positions, lengths and block ids out of range: the status is
+    set, the good rows are as without the bad ones, memory outside is untouched."""
+    import dial_b200
+    from dial_b200 import kv4
+
+    c = Cache(45, 4, 160, 8, 2, max_pos=200)
+    good, table = c.device(cuda)
+    x = torch.randn(6, 12 * DIM, device=cuda).to(BF16)
+    ang = torch.zeros(200, 64, dtype=BF16, device=cuda)
+    # rows 1-4 are bad: session 4, slot past the table, position past the tables, negative session
+    cache = kv4.Kv4Cache(good.pages.clone(), good.weights.clone(), good.positions.clone())
+    q = kv4.kv4_append(c.sh, cache, x, table, i32(cuda, 0, 4, 1, 1, -1, 2), i32(cuda, 5, 1, 160, 7, 3, 9),
+                       i32(cuda, 1, 1, 1, 200, 1, 1), cos=ang + 1, sin=ang,
+                       q_out=torch.full((6, 8 * DIM), 3.0, dtype=BF16, device=cuda))
+    assert dial_b200.device_status(clear=True) == STATUS_BAD_ARGS
+    assert (q[1:5] == 3.0).all() and (q[0] != 3.0).any() and (q[5] != 3.0).any()
+    want = kv4.Kv4Cache(good.pages.clone(), good.weights.clone(), good.positions.clone())
+    kv4.kv4_append(c.sh, want, x[[0, 5]].contiguous(), table, i32(cuda, 0, 2), i32(cuda, 5, 9), i32(cuda, 1, 1),
+                   cos=ang + 1, sin=ang)
+    for a, b in ((cache.pages, want.pages), (cache.weights, want.weights), (cache.positions, want.positions)):
+        assert torch.equal(a, b)
+    assert dial_b200.device_status() == 0
+    # attention: a bad session, a length past max_len, a negative one, rows out of order
+    for queries in (1, 40):
+        starts = i32(cuda, *[i * queries for i in range(5)])
+        qq = (torch.randn(4 * queries, 8 * DIM, device=cuda)).to(BF16)
+        for bad_sids, bad_lens in (((0, 9, 2, 3), (150, 9, 80, 0)), ((0, 1, 2, 3), (150, 161, 80, -1))):
+            w = good.weights.clone()
+            cc = kv4.Kv4Cache(good.pages, w, good.positions)
+            out = torch.full_like(qq, 5.0)
+            kv4.kv4_attention(c.sh, cc, qq, table, i32(cuda, *bad_sids), i32(cuda, *bad_lens), 160,
+                              q_starts=starts, max_q=queries, accumulate=True, out=out)
+            assert dial_b200.device_status(clear=True) == STATUS_BAD_ARGS
+            for i in (0, 2):
+                o, b, _, _ = c.attend(host(qq[i * queries:(i + 1) * queries]), i, (150, 0, 80)[i])
+                d = np.abs(host(out[i * queries:(i + 1) * queries]) - o)
+                assert (d <= b).all()
+            assert (out[queries:2 * queries] == 5.0).all()
+            w_sum = host(w - good.weights)
+            blk, _ = c.at(1, 160)
+            assert (w_sum[blk] == 0).all()
+    # block ids outside the pool: page 0 is read, nothing is written outside
+    bad = table.clone()
+    bad[0, 2] = c.sh.num_blocks
+    bad[1, 0] = -7
+    out = kv4.kv4_attention(c.sh, good, x[:2, :8 * DIM], bad, i32(cuda, 0, 1), i32(cuda, 100, 30), 160)
+    assert dial_b200.device_status(clear=True) == STATUS_BAD_ARGS
+    c2 = Cache(45, 4, 160, 8, 2, max_pos=200)
+    c2.pages, c2.table = c.pages, c.table.copy()
+    c2.table[0, 2] = c2.table[1, 0] = 0
+    for i, n in ((0, 100), (1, 30)):
+        o, b, _, _ = c2.attend(host(x[i:i + 1, :8 * DIM]), i, n)
+        assert (np.abs(host(out[i:i + 1]) - o) <= b).all()
+    before = good.pages.clone()
+    kv4.kv4_append(c.sh, good, x[:1], bad, i32(cuda, 1), i32(cuda, 3), i32(cuda, 0))
+    assert torch.equal(good.pages, before)
+    assert dial_b200.device_status(clear=True) == STATUS_BAD_ARGS
+    # eviction of a bad sequence: its length stays, the good one's is cut
+    lens = i32(cuda, 150, 170, 80)
+    kv4.kv4_evict(c.sh, good, table, i32(cuda, 0, 1, 2), lens, 160, 50, 10, lens_out=lens)
+    assert lens.tolist() == [50, 170, 50]
+    assert dial_b200.device_status(clear=True) == STATUS_BAD_ARGS
+
+
+def test_append_and_read_of_strided_rows(cuda):
+    """qkv, q_out, q and out as columns of wider tensors; the columns beside stay."""
+    from dial_b200 import kv4
+
+    c = Cache(46, 1, 64, 4, 2)
+    cache, table = c.device(cuda)
+    wide = torch.randn(5, 8 * DIM + 64, device=cuda).to(BF16)
+    qw = torch.full((5, 4 * DIM + 128), 9.0, dtype=BF16, device=cuda)
+    kv4.kv4_append(c.sh, cache, wide[:, 64:], table, i32(cuda, 0, 0, 0, 0, 0), i32(cuda, 0, 1, 2, 3, 4),
+                   i32(cuda, 0, 1, 2, 3, 4), q_out=qw[:, 128:])
+    assert (qw[:, :128] == 9.0).all() and torch.equal(qw[:, 128:], wide[:, 64:64 + 4 * DIM])
+    ref, _ = c.device(cuda)
+    kv4.kv4_append(c.sh, ref, wide[:, 64:].contiguous(), table, i32(cuda, 0, 0, 0, 0, 0),
+                   i32(cuda, 0, 1, 2, 3, 4), i32(cuda, 0, 1, 2, 3, 4))
+    assert torch.equal(cache.pages, ref.pages)
+
+
+def test_empty_calls(cuda):
+    from dial_b200 import kv4
+
+    c = Cache(47, 1, 64, 4, 2)
+    cache, table = c.device(cuda)
+    none = torch.zeros(0, dtype=torch.int32, device=cuda)
+    q = torch.zeros(0, 4 * DIM, dtype=BF16, device=cuda)
+    assert kv4.kv4_attention(c.sh, cache, q, table, none, none, 64).shape == (0, 4 * DIM)
+    k, _ = kv4.kv4_read(c.sh, cache, table, none, none, 3)
+    assert k.shape == (0, 3, 2, DIM)
+    assert kv4.kv4_append(c.sh, cache, torch.zeros(0, 8 * DIM, dtype=BF16, device=cuda), table, none, none,
+                          none).shape == (0, 4 * DIM)
+    assert kv4.kv4_evict(c.sh, cache, table, none, none, 64, 8).shape == (0,)
+    # max_len 0: every query sees nothing
+    out = kv4.kv4_attention(c.sh, cache, torch.ones(2, 4 * DIM, dtype=BF16, device=cuda), table,
+                            i32(cuda, 0, 0), i32(cuda, 0, 0), 0)
+    assert (out == 0).all()
+    out = kv4.kv4_attention(c.sh, cache, torch.ones(90, 4 * DIM, dtype=BF16, device=cuda), table, i32(cuda, 0),
+                            i32(cuda, 0), 0, q_starts=i32(cuda, 0, 90), max_q=90, accumulate=True)
+    assert (out == 0).all()
+    torch.cuda.synchronize()
