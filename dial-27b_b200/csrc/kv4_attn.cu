@@ -57,7 +57,7 @@ extern "C" int dial_b200_kv4_attention(const dial_b200_kv4_shape* sh, const void
   Kv4AttnArgs a{};
   int rc = kv4_cache_of(sh, pages, weights, nullptr, block_table, sessions, &a.c, err, n);
   if (rc != DIAL_OK) return rc;
-  if (!q || !sids || !lens || !out)
+  if (seqs != 0 && rows != 0 && (!q || !sids || !lens || !out))
     return kv4_fail(err, n, DIAL_ERR_INVALID, "null pointer argument");
   if (seqs < 0 || seqs > 65535)
     return kv4_fail(err, n, DIAL_ERR_INVALID, "seqs %lld outside [0, 65535]", (long long)seqs);

@@ -408,11 +408,11 @@ extern "C" int dial_b200_kv4_append(const dial_b200_kv4_shape* sh, const void* q
   AppendArgs a{};
   int rc = kv4_cache_of(sh, pages, weights, positions_pool, block_table, sessions, &a.c, err, n);
   if (rc != DIAL_OK) return rc;
-  if (!qkv || !sids || !slots)
+  if (rows != 0 && (!qkv || !sids || !slots))
     return kv4_fail(err, n, DIAL_ERR_INVALID, "null pointer argument");
   if (!q_norm_w != !k_norm_w || !cos != !sin)
     return kv4_fail(err, n, DIAL_ERR_INVALID, "q_norm_w and k_norm_w, cos and sin go in pairs");
-  if ((cos || positions_pool) && !positions)
+  if ((cos || positions_pool) && !positions && rows != 0)
     return kv4_fail(err, n, DIAL_ERR_INVALID, "RoPE and a positions pool need positions");
   if (cos && sh->max_pos < 1)
     return kv4_fail(err, n, DIAL_ERR_INVALID, "max_pos %d must be positive with RoPE", sh->max_pos);
@@ -469,7 +469,7 @@ extern "C" int dial_b200_kv4_read(const dial_b200_kv4_shape* sh, const void* pag
   ReadArgs a{};
   int rc = kv4_cache_of(sh, pages, nullptr, nullptr, block_table, sessions, &a.c, err, n);
   if (rc != DIAL_OK) return rc;
-  if (!sids || !lens || !k_out || !v_out)
+  if (seqs != 0 && count != 0 && (!sids || !lens || !k_out || !v_out))
     return kv4_fail(err, n, DIAL_ERR_INVALID, "null pointer argument");
   if (!aligned(k_out, 16) || !aligned(v_out, 16))
     return kv4_fail(err, n, DIAL_ERR_INVALID, "k_out and v_out must be 16-byte aligned");

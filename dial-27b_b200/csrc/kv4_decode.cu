@@ -307,9 +307,9 @@ __global__ void __launch_bounds__(kWarpsOf<NT> * 32, kCtasPerSm<NT>)
   // number of one page of a window of 32 and copies that page itself; the next
   // window's table loads go out a window ahead
   const int mine = f1 - f0 > warp ? (f1 - f0 - warp + kWarps - 1) / kWarps : 0;
-  // table entry of the warp's page i, and its kv head
+  // table entry of the warp's page i (past its last: of a page of the range), and its kv head
   auto entry_of = [&](int i, int& h) -> const int32_t* {
-    const int f = f0 + warp + kWarps * min(i, max(mine - 1, 0));
+    const int f = min(f0 + warp + kWarps * min(i, max(mine - 1, 0)), f1 - 1);
     const int s = seq_at(sm.cum, seqs, f / H);
     const int np = sm.cum[s + 1] - sm.cum[s], r = f - sm.cum[s] * H;
     Kv4Seq q;
@@ -879,7 +879,8 @@ cudaError_t launch_nt(const DecodeArgs& d, cudaStream_t s) {
 
 size_t kv4_decode_scratch(int q_heads, int kv_heads, long long seqs, long long max_q,
                           long long max_len, bool weights) {
-  const long long n = chunk_of(kv_heads, seqs, max_len);
+  // no fewer sequences than a launch with a shorter max_len takes
+  const long long n = seqs < kSeqChunk ? seqs : kSeqChunk;
   if (n < 1) return 0;
   const Plan p = plan_of(q_heads, kv_heads, n, max_q, max_len, weights, 148);
   return p.desc + p.rec + p.part_o + p.part_ml + p.scores;

@@ -306,7 +306,7 @@ extern "C" int dial_b200_kv4_evict(const dial_b200_kv4_shape* sh, void* pages, f
   EvictArgs a{};
   int rc = kv4_cache_of(sh, pages, weights, positions, block_table, sessions, &a.c, err, n);
   if (rc != DIAL_OK) return rc;
-  if (!weights || !sids || !lens || !lens_out)
+  if (!weights || (seqs != 0 && (!sids || !lens || !lens_out)))
     return kv4_fail(err, n, DIAL_ERR_INVALID, "null pointer argument");
   if (seqs < 0 || seqs > 65535)
     return kv4_fail(err, n, DIAL_ERR_INVALID, "seqs %lld outside [0, 65535]", (long long)seqs);

@@ -201,7 +201,11 @@ int dial_b200_attention_decode_noalloc(const dial_b200_attn_shape* sh, const voi
  * table, a position outside the tables or a length outside [0, max_len]
  * records the bad-argument device status, and that row or sequence is left
  * out, its outputs as they were; a block id outside [0, num_blocks) records it
- * too, and reads use page 0, writes are dropped. */
+ * too, and reads use page 0, writes are dropped.
+ * Rows of activations (qkv, q, q_out, out, k_out, v_out), norm weights, cos / sin,
+ * pages and scratch start on 16-byte boundaries, strides are multiples of 8; other
+ * arrays need their type's alignment.  A call without rows or sequences does
+ * nothing; its per-row pointers may be NULL. */
 #define DIAL_B200_KV4_SLAB_BYTES 2304
 
 typedef struct {
@@ -260,7 +264,8 @@ int64_t dial_b200_kv4_attention_scratch_bytes(const dial_b200_kv4_shape* sh, int
  *   out [rows, out_ld] = softmax(softmax_scale * q . k) . v, f32 inside;
  *   weights (if not NULL): weights[slot] += the slot's probabilities summed
  *   over the sequence's queries and the query heads of the kv head.  Sequences
- *   must then name distinct sessions.
+ *   must then name distinct sessions that share no page (a sum is one load and
+ *   one store).
  * max_q and max_len bound n and lens[i] (host); rows no sequence names are left as
  * they were.  `scratch` needs no preparation; two calls that may run at the
  * same time need two. */

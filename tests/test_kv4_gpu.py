@@ -203,6 +203,15 @@ def test_attention_of_many_ragged_sequences(cuda, weights):
     check_attention(c, cuda, [(s, n, 1) for s, n in enumerate(lens)], weights=weights)
 
 
+def test_many_sequences_of_many_queries(cuda):
+    """More sequences than one launch takes, each with rows for several tiles,
+    one of one query, one of none."""
+    c = Cache(20, 530, 70, 4, 2)
+    seqs = [(s, int(n), 33) for s, n in enumerate(c.rng.integers(0, 70, 530))]
+    seqs[5], seqs[511], seqs[513] = (5, 70, 1), (511, 66, 70), (513, 12, 0)
+    check_attention(c, cuda, seqs, spare_rows=2)
+
+
 def test_attention_long_split(cuda):
     """One session long enough for every split, at an odd length; the largest
     score in the first and in the last slot."""
