@@ -208,26 +208,53 @@ struct DecodeSmem {
   int sums[kWarps];
 };
 
-// The probabilities of slot t (scores x, the columns' (m, 1 / l) in ml) into its
-// running weight.
-__device__ __forceinline__ void add_weight(const DecodeArgs& d, int sid, int h, int t, const float* x,
-                                           const float2* ml, int cols) {
+// The probabilities of slots t, t + step .. below `upto` of segment (sid, h) into
+// their running weights: scores x [slot][score_ld], the columns' (m, 1 / l) in ml.
+// B slots at once, whose loads all precede the stores.
+template <int B>
+__device__ __forceinline__ void add_weights(const DecodeArgs& d, int sid, int h, int t, int step, int upto,
+                                            const float* x, const float2* ml, int cols) {
   const Kv4AttnArgs& a = d.a;
-  const int block = kv4_block(a.c, a.c.block_table, sid, t / kPageTokens);
-  float* to = a.c.weights + kv4_slab_index(a.c, max(block, 0), h) * kPageTokens + t % kPageTokens;
-  const float old = *to;
-  float sum = 0.f;
-  int col = 0;
-  if ((d.score_ld & 3) == 0)
-    for (; col + 4 <= cols; col += 4) {
-      const float4 v = *reinterpret_cast<const float4*>(x + col);
-      sum = fmaf(ex2(v.x - ml[col].x), ml[col].y, sum);
-      sum = fmaf(ex2(v.y - ml[col + 1].x), ml[col + 1].y, sum);
-      sum = fmaf(ex2(v.z - ml[col + 2].x), ml[col + 2].y, sum);
-      sum = fmaf(ex2(v.w - ml[col + 3].x), ml[col + 3].y, sum);
+  for (; t < upto; t += B * step) {
+    int block[B];
+    float* to[B];
+    float old[B], sum[B];
+#pragma unroll
+    for (int e = 0; e < B; ++e) {
+      const int at = t + e * step;
+      block[e] = at < upto ? kv4_block(a.c, a.c.block_table, sid, at / kPageTokens) : -1;
     }
-  for (; col < cols; ++col) sum = fmaf(ex2(x[col] - ml[col].x), ml[col].y, sum);
-  if (block >= 0) *to = old + sum;
+#pragma unroll
+    for (int e = 0; e < B; ++e) {
+      const int at = t + e * step;
+      to[e] = a.c.weights + kv4_slab_index(a.c, max(block[e], 0), h) * kPageTokens + at % kPageTokens;
+      old[e] = block[e] >= 0 ? *to[e] : 0.f;
+      sum[e] = 0.f;
+    }
+    int col = 0;
+    if ((d.score_ld & 3) == 0)
+      for (; col + 4 <= cols; col += 4) {
+        float4 v[B];
+#pragma unroll
+        for (int e = 0; e < B; ++e)
+          v[e] = *reinterpret_cast<const float4*>(x + static_cast<size_t>(min(t + e * step, upto - 1)) * d.score_ld + col);
+#pragma unroll
+        for (int e = 0; e < B; ++e) {
+          sum[e] = fmaf(ex2(v[e].x - ml[col].x), ml[col].y, sum[e]);
+          sum[e] = fmaf(ex2(v[e].y - ml[col + 1].x), ml[col + 1].y, sum[e]);
+          sum[e] = fmaf(ex2(v[e].z - ml[col + 2].x), ml[col + 2].y, sum[e]);
+          sum[e] = fmaf(ex2(v[e].w - ml[col + 3].x), ml[col + 3].y, sum[e]);
+        }
+      }
+    for (; col < cols; ++col)
+#pragma unroll
+      for (int e = 0; e < B; ++e)
+        sum[e] = fmaf(ex2(x[static_cast<size_t>(min(t + e * step, upto - 1)) * d.score_ld + col] - ml[col].x),
+                      ml[col].y, sum[e]);
+#pragma unroll
+    for (int e = 0; e < B; ++e)
+      if (block[e] >= 0) *to[e] = old[e] + sum[e];
+  }
 }
 
 // One segment's share of a range.
@@ -647,9 +674,8 @@ __global__ void __launch_bounds__(kWarpsOf<NT> * 32, kCtasPerSm<NT>)
     }
     if (SCORES && d.one) {  // this CTA's scores, all of the segment's columns
       __syncthreads();
-      for (int t = tid; t < w.s.len; t += kWarps * 32)
-        add_weight(d, w.s.sid, w.h, t, d.scores + (score0 + static_cast<size_t>(w.seg0) * kPageTokens + t) * d.score_ld,
-                   sm.fin, cols);
+      add_weights<2>(d, w.s.sid, w.h, tid, kWarps * 32, w.s.len,
+                     d.scores + (score0 + static_cast<size_t>(w.seg0) * kPageTokens) * d.score_ld, sm.fin, cols);
       break;
     }
     if (d.one) break;
@@ -676,56 +702,84 @@ __global__ void __launch_bounds__(kWarpsOf<NT> * 32, kCtasPerSm<NT>)
 }
 
 constexpr int kJoinThreads = 256, kJoinWarps = kJoinThreads / 32;
+constexpr int kWeightCtas = 4;  // of a range
+constexpr int kFewParts = 16;   // of a segment, up to which a warp joins a column
 
-// max over a segment's parts of column `col`, and the sum l under it; one warp.
+// max over a segment's parts of a column, and the sum l under it; G lanes share them.
+template <int G>
 __device__ __forceinline__ float2 join_ml(const float2* ml, size_t stride, int parts) {
-  const int lane = threadIdx.x & 31;
-  float M = -INFINITY, L = 0.f;
-  for (int p = lane; p < parts; p += 32) M = fmaxf(M, ml[p * stride].x);
-  M = warp_max(M);
-  for (int p = lane; p < parts; p += 32) {
+  const int lane = threadIdx.x % G;
+  float2 own = lane < parts ? ml[lane * stride] : make_float2(-INFINITY, 0.f);
+  float M = own.x;
+  for (int p = lane + G; p < parts; p += G) M = fmaxf(M, ml[p * stride].x);
+#pragma unroll
+  for (int o = G / 2; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+  float L = own.x == -INFINITY ? 0.f : ex2(own.x - M) * own.y;
+  for (int p = lane + G; p < parts; p += G) {
     const float2 v = ml[p * stride];
     if (v.x != -INFINITY) L = fmaf(ex2(v.x - M), v.y, L);
   }
-  return make_float2(M, warp_sum(L));
+#pragma unroll
+  for (int o = G / 2; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+  return make_float2(M, L);
 }
 
-// Ranges after b that go on with the segment that starts in b and does not end there.
-__device__ __forceinline__ int parts_after(const DecodeArgs& d, int b) {
-  const int lane = threadIdx.x & 31;
-  for (int n = 0;; n += 32) {
-    const int at = b + 1 + n + lane;
-    const unsigned ends = __ballot_sync(0xffffffffu, at >= d.ctas || d.desc[at].w != 0);
-    if (ends) return n + __ffs(ends);
+// (m, 1 / l) of a segment's columns, G lanes a column.
+template <int G>
+__device__ __forceinline__ void column_ml(const float2* first, size_t stride, int parts, int cols, float2* ml) {
+  for (int c0 = threadIdx.x / 32 * (32 / G); c0 < cols; c0 += kJoinThreads / G) {  // warp-uniform
+    const int col = c0 + threadIdx.x % 32 / G;
+    const float2 v = join_ml<G>(first + min(col, cols - 1), stride, parts);
+    if (threadIdx.x % G == 0 && col < cols)
+      ml[col] = make_float2(v.x == -INFINITY ? 0.f : v.x, v.y > 0.f ? 1.f / v.y : 0.f);
   }
 }
-// The range before b in which segment `seg` starts.
-__device__ __forceinline__ int owner_before(const DecodeArgs& d, int b, int seg) {
+
+// Ranges after b that go on with the segment that b begins or continues and does not
+// end; `ends`: whether it ends in range b + 1 + lane.
+__device__ __forceinline__ int parts_after(const DecodeArgs& d, int b, bool ends) {
+  const int lane = threadIdx.x & 31;
+  for (int n = 0;; n += 32) {
+    if (n > 0) ends = b + 1 + n + lane >= d.ctas || d.desc[b + 1 + n + lane].w != 0;
+    const unsigned any = __ballot_sync(0xffffffffu, ends);
+    if (any) return n + __ffs(any);
+  }
+}
+// The range before b in which segment `seg` starts; `starts`: the segment that starts
+// in range b - 1 - lane and goes on.
+__device__ __forceinline__ int owner_before(const DecodeArgs& d, int b, int seg, int starts) {
   const int lane = threadIdx.x & 31;
   for (int n = b - 1;; n -= 32) {
     const int at = n - lane;
-    const unsigned hit = __ballot_sync(0xffffffffu, at < 0 || d.desc[at].x == seg);
+    if (n < b - 1) starts = at < 0 ? seg : d.desc[at].x;
+    const unsigned hit = __ballot_sync(0xffffffffu, starts == seg || at < 0);
     if (hit) return max(n - (__ffs(hit) - 1), 0);
   }
 }
 
-// blockIdx.y < d.join_y: joins the parts of the segment that starts in range
-// blockIdx.x and goes on in others, a column a CTA, parts over the warps.
-// blockIdx.y >= d.join_y (with weights): adds the probabilities of the slots of
-// range blockIdx.x to the running weights.
+// With weights, blockIdx.y < kWeightCtas: adds the probabilities of the slots of
+// range blockIdx.x to the running weights.  The other blockIdx.y: joins the parts
+// of the segment that starts in the range and goes on in others, a column a CTA,
+// parts over the warps.
 template <typename Act, int NT>
-__global__ void __launch_bounds__(kJoinThreads) kv4_join_kernel(const DecodeArgs d) {
+__global__ void __launch_bounds__(kJoinThreads, 4) kv4_join_kernel(const DecodeArgs d) {
   const Kv4AttnArgs& a = d.a;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, b = blockIdx.x;
   const int H = a.c.kv_heads, rep = a.c.q_heads / H;
   const size_t stride = static_cast<size_t>(d.groups) * NT * 8;  // columns of a part
-  if (blockIdx.y < d.join_y) {
+  pdl_wait();
+  // what range b and its neighbours hold, loaded at once
+  const int4 ds = d.desc[b];
+  const bool ends = b + 1 + lane >= d.ctas || d.desc[b + 1 + lane].w != 0;
+  const int ys = d.scores ? kWeightCtas : 0;
+  if (blockIdx.y >= ys) {
     __shared__ float4 red[kJoinWarps][kHeadDim / 4];
-    pdl_wait();
-    const int4 ds = d.desc[b];
     if (ds.x < 0) return;
-    const int parts = 1 + parts_after(d, b);
-    for (int col = blockIdx.y; col < ds.z; col += d.join_y) {
+    const int parts = 1 + parts_after(d, b, ends);
+    // few parts: a column a warp; else a column a CTA, its parts over the warps
+    const bool few = parts <= kFewParts;
+    const int y = blockIdx.y - ys, gy = gridDim.y - ys, W = few ? 1 : kJoinWarps, part0 = few ? 0 : warp;
+    for (int col = few ? y * kJoinWarps + warp : y; col < ds.z; col += few ? gy * kJoinWarps : gy) {
       const size_t first = static_cast<size_t>(b + ds.x) * stride + col;
       const float4* po = reinterpret_cast<const float4*>(d.part_o) + first * (kHeadDim / 4) + lane;
       const float2* ml = reinterpret_cast<const float2*>(d.part_ml) + first;
@@ -734,11 +788,11 @@ __global__ void __launch_bounds__(kJoinThreads) kv4_join_kernel(const DecodeArgs
       float pm[PRE];
 #pragma unroll
       for (int e = 0; e < PRE; ++e) {
-        const int p = warp + kJoinWarps * e;
+        const int p = part0 + W * e;
         pre[e] = p < parts ? po[p * stride * (kHeadDim / 4)] : make_float4(0.f, 0.f, 0.f, 0.f);
         pm[e] = p < parts ? ml[p * stride].x : -INFINITY;
       }
-      const float2 all = join_ml(ml, stride, parts);
+      const float2 all = join_ml<32>(ml, stride, parts);
       float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
       auto add = [&](const float4& v, float mp) {
         const float f = mp == -INFINITY ? 0.f : ex2(mp - all.x);
@@ -750,43 +804,46 @@ __global__ void __launch_bounds__(kJoinThreads) kv4_join_kernel(const DecodeArgs
 #pragma unroll
       for (int e = 0; e < PRE; ++e) add(pre[e], pm[e]);
 #pragma unroll 4
-      for (int p = warp + kJoinWarps * PRE; p < parts; p += kJoinWarps)
+      for (int p = part0 + W * PRE; p < parts; p += W)
         add(po[p * stride * (kHeadDim / 4)], ml[p * stride].x);
+      Act* out = static_cast<Act*>(a.out) + (ds.y + col / rep) * a.out_ld + ((ds.x % H) * rep + col % rep) * kHeadDim;
+      const float scale = all.y != 0.f ? a.c.v_scale / all.y : 0.f;
+      if (few) {
+        const float v[4] = {O.x, O.y, O.z, O.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) out[place_dim(lane * 4 + e)] = ActTraits<Act>::from_f(v[e] * scale);
+        continue;
+      }
       red[warp][lane] = O;
       __syncthreads();
       if (tid < kHeadDim) {
         float v = 0.f;
 #pragma unroll
         for (int w = 0; w < kJoinWarps; ++w) v += reinterpret_cast<const float*>(red[w])[tid];
-        static_cast<Act*>(a.out)[(ds.y + col / rep) * a.out_ld + ((ds.x % H) * rep + col % rep) * kHeadDim +
-                                 place_dim(tid)] =
-            ActTraits<Act>::from_f(all.y != 0.f ? v / all.y * a.c.v_scale : 0.f);
+        out[place_dim(tid)] = ActTraits<Act>::from_f(v * scale);
       }
       __syncthreads();
     }
     return;
   }
   __shared__ float2 ml[kKv4DecodeCols];  // (m, 1 / l) of the segment's columns
-  pdl_wait();
-  const int y = blockIdx.y - d.join_y, ys = gridDim.y - d.join_y, n = d.rec_n[b];
+  const Rec* recs = d.rec + static_cast<size_t>(b) * d.rec_ld;
+  const int n = d.rec_n[b];
+  const int starts = b - 1 - lane >= 0 ? d.desc[b - 1 - lane].x : -1;
+  Rec r = recs[0];
   for (int k = 0; k < n; ++k) {
-    const Rec r = d.rec[static_cast<size_t>(b) * d.rec_ld + k];
-    // ranges that hold parts of the segment: from the one it starts in
-    const int b0 = r.page0 == 0 ? b : owner_before(d, b, r.seg);
-    const bool ends = k + 1 < n || d.desc[b].x != r.seg;  // in this range, if it starts here
-    const int parts = r.page0 == 0 && ends ? 1 : 1 + parts_after(d, b0);
-    for (int col = warp; col < r.cols; col += kJoinWarps) {
-      const float2 v = join_ml(reinterpret_cast<const float2*>(d.part_ml) +
-                                   static_cast<size_t>(b0 + r.seg) * stride + col,
-                               stride, parts);
-      if (lane == 0) ml[col] = make_float2(v.x == -INFINITY ? 0.f : v.x, v.y > 0.f ? 1.f / v.y : 0.f);
-    }
+    // ranges that hold parts of the segment: from the one it starts in, b0, on
+    const int b0 = r.page0 == 0 ? b : owner_before(d, b, r.seg, starts);
+    const bool here = k + 1 < n || (r.page0 == 0 ? ds.x != r.seg : ds.w != 0);  // it ends in this range
+    const int parts = b - b0 + 1 + (here ? 0 : parts_after(d, b, ends));
+    const float2* first = reinterpret_cast<const float2*>(d.part_ml) + static_cast<size_t>(b0 + r.seg) * stride;
+    if (parts <= kFewParts) column_ml<8>(first, stride, parts, r.cols, ml);
+    else column_ml<32>(first, stride, parts, r.cols, ml);
     __syncthreads();
-    const int upto = min(r.page1 * kPageTokens, r.len);
-#pragma unroll 2
-    for (int t = r.page0 * kPageTokens + y * kJoinThreads + tid; t < upto; t += ys * kJoinThreads)
-      add_weight(d, r.sid, r.h, t, d.scores + (static_cast<size_t>(r.seg0) * kPageTokens + t) * d.score_ld, ml,
-                 r.cols);
+    add_weights<4>(d, r.sid, r.h, r.page0 * kPageTokens + blockIdx.y * kJoinThreads + tid, kWeightCtas * kJoinThreads,
+                   min(r.page1 * kPageTokens, r.len),
+                   d.scores + static_cast<size_t>(r.seg0) * kPageTokens * d.score_ld, ml, r.cols);
+    if (k + 1 < n) r = recs[k + 1];
     __syncthreads();
   }
 }
@@ -872,7 +929,7 @@ cudaError_t launch_nt(const DecodeArgs& d, cudaStream_t s) {
       e = kv4_start(kv4_decode_kernel<Act, NT, false>, dim3(d.ctas, d.groups), kWarpsOf<NT> * 32, smem, s, d);
   }
   if (e != cudaSuccess || d.one) return e;
-  return kv4_start(kv4_join_kernel<Act, NT>, dim3(d.ctas, d.join_y + (d.scores ? 4 : 0)), kJoinThreads, 0, s, d);
+  return kv4_start(kv4_join_kernel<Act, NT>, dim3(d.ctas, d.join_y + (d.scores ? kWeightCtas : 0)), kJoinThreads, 0, s, d);
 }
 
 }  // namespace
@@ -919,7 +976,7 @@ cudaError_t kv4_decode_launch(const Kv4AttnArgs& a, int act, cudaStream_t s) {
     d.part_o = reinterpret_cast<float*>(w);
     d.part_ml = reinterpret_cast<float*>(w + p.part_o);
     d.scores = a.c.weights ? reinterpret_cast<float*>(w + p.part_o + p.part_ml) : nullptr;
-    d.join_y = p.cols < 16 ? p.cols : 16;
+    d.join_y = p.cols < 8 ? p.cols : 8;
     const bool bf = act == DIAL_ACT_BF16;
     const cudaError_t e = p.nt == 1 ? (bf ? launch_nt<__nv_bfloat16, 1>(d, s) : launch_nt<__half, 1>(d, s))
                                     : (bf ? launch_nt<__nv_bfloat16, 2>(d, s) : launch_nt<__half, 2>(d, s));
