@@ -24,7 +24,7 @@
 namespace dialb200 {
 namespace {
 
-constexpr int kThreads = 14 * 32;
+constexpr int kThreads = 22 * 32;
 constexpr int kSeqChunk = 512;  // sequences a launch
 constexpr int kKeys = 256;      // of an item
 constexpr int kChunk = 32;      // query tiles of an item at most
@@ -48,7 +48,7 @@ constexpr int kSmemBytes = kOffMisc + sizeof(Misc) + 1024;
 struct ColsumArgs {
   Kv4AttnArgs a;
   Kv4Rows r;
-  float* part;  // [seqs][kv_heads][kb_max][chunks][256]
+  float* part;  // [seqs][kv_heads][kb_max][chunks][2][256]
   int kb_max, chunks;
 };
 
@@ -78,7 +78,7 @@ __device__ __forceinline__ void tiles_seeing(const Kv4Seq& s, int rep, int kb, i
 }
 
 __device__ __forceinline__ size_t part_at(const ColsumArgs& d, int i, int h, int kb, int c) {
-  return (((static_cast<size_t>(i) * d.a.c.kv_heads + h) * d.kb_max + kb) * d.chunks + c) * kKeys;
+  return (((static_cast<size_t>(i) * d.a.c.kv_heads + h) * d.kb_max + kb) * d.chunks + c) * 2 * kKeys;
 }
 
 // Item f of all (cum: items of a kv head of the sequences before).
@@ -133,17 +133,17 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_colsum_kernel(const __grid_co
     }
     for (int i = 0; i < kSBufs; ++i) {
       mbar_init(&sm.sfull[i], 1);
-      mbar_init(&sm.sfree[i], 4);
+      mbar_init(&sm.sfree[i], 8);
     }
     for (int i = 0; i < kCBufs; ++i) {
       mbar_init(&sm.cfull[i], 1);
-      mbar_init(&sm.cfree[i], 8);
+      mbar_init(&sm.cfree[i], 16);
     }
     mbar_init(&sm.fin, 1);
     sm.failed = 0;
     fence_mbar_init();
   }
-  if (warp == 13) {
+  if (warp == 21) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&sm.tmem)));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
@@ -181,9 +181,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_colsum_kernel(const __grid_co
     return __all_sync(0xffffffffu, ok) != 0;
   };
 
-  if (warp < 8) {
-    // ------------------------------------------------ sums, one key a thread
-    const int grp = warp >> 2, quarter = warp & 3, r = quarter * 32 + lane;
+  if (warp < 16) {
+    // --------------------------- sums, one key and half of a tile's rows a thread
+    const int half = warp >> 3, grp = warp >> 2 & 1, quarter = warp & 3, r = quarter * 32 + lane;
     const uint32_t lane_off = static_cast<uint32_t>(32 * quarter) << 16;
     uint32_t n = 0;  // tiles so far
     for (long long f = blockIdx.x; f < total; f += gridDim.x) {
@@ -196,8 +196,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_colsum_kernel(const __grid_co
         ok = ok && wait(&sm.cfull[cb], n / kCBufs & 1u) && wait(&sm.sfull[sb], n / 2 & 1u);
         if (!ok) continue;
         fence_after();
-        const uint32_t tS = sm.tmem + sb * 128 + lane_off;
-        const float *fc = sm.fac[cb], *of = sm.off[cb];
+        const uint32_t tS = sm.tmem + sb * 128 + half * 64 + lane_off;
+        const float *fc = sm.fac[cb] + half * 64, *of = sm.off[cb] + half * 64;
+        const int* seen = sm.seen[cb] + half * 64;
         // every row of the tile is there and sees the whole block
         if ((T + 1) * 128 <= w.s.n * rep && w.s.len - w.s.n + 1 + T * 128 / rep >= key0 + 128) {
           uint32_t x[32], y[32];
@@ -217,16 +218,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_colsum_kernel(const __grid_co
           ld32(tS + 32, y);
           add(x, 0);
           ld_wait(y);
-          ld32(tS + 64, x);
           add(y, 32);
-          ld_wait(x);
-          ld32(tS + 96, y);
-          add(x, 64);
-          ld_wait(y);
-          add(y, 96);
         } else {
 #pragma unroll 1
-          for (int c = 0; c < 128; c += 16) {
+          for (int c = 0; c < 64; c += 16) {
             uint32_t x[16];
             ld16(tS + c, x);
             ld_wait16(x);
@@ -234,7 +229,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_colsum_kernel(const __grid_co
             for (int e = 0; e < 16; e += 2) {
               const float z0 = fmaf(__uint_as_float(x[e]), fc[c + e], of[c + e]);
               const float z1 = fmaf(__uint_as_float(x[e + 1]), fc[c + e + 1], of[c + e + 1]);
-              s0 = add2(s0, pair(key < sm.seen[cb][c + e] ? ex2(z0) : 0.f, key < sm.seen[cb][c + e + 1] ? ex2(z1) : 0.f));
+              s0 = add2(s0, pair(key < seen[c + e] ? ex2(z0) : 0.f, key < seen[c + e + 1] ? ex2(z1) : 0.f));
             }
             __syncwarp();
           }
@@ -247,11 +242,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_colsum_kernel(const __grid_co
         }
       }
       const uint64_t s = add2(s0, s1);
-      if (w.t1 > w.t0) d.part[w.part + grp * 128 + r] = lo_of(s) + hi_of(s);
+      if (w.t1 > w.t0) d.part[w.part + half * kKeys + grp * 128 + r] = lo_of(s) + hi_of(s);
     }
-  } else if (warp < 12) {
+  } else if (warp < 20) {
     // ------------------------------------------------------- K codes, once an item
-    const int dw = warp - 8, q = lane & 3, tok = lane >> 2;
+    const int dw = warp - 16, q = lane & 3, tok = lane >> 2;
     uint4 kc[2][4];
     uint32_t ks[2][4], items = 0;
     auto fetch = [&](const Item& w) {
@@ -278,7 +273,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_colsum_kernel(const __grid_co
       f = next_with_tiles(d, sm.cum, f + gridDim.x, total);
       if (f < total) fetch(item_at(d, sm.cum, f));
     }
-  } else if (warp == 12) {
+  } else if (warp == 20) {
     // ------------------------------------- query tiles (TMA) and their constants
     uint32_t n = 0, issued = 0;
     bool ok = true;
@@ -369,7 +364,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_colsum_kernel(const __grid_co
   fence_before();
   __syncthreads();
   fence_after();
-  if (warp == 13)
+  if (warp == 21)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(sm.tmem));
 }
 
@@ -386,7 +381,8 @@ __global__ void __launch_bounds__(kKeys) kv4_colsum_add_kernel(const ColsumArgs 
     int t0, t1;
     tiles_seeing(s, rep, kb, c, t0, t1);
     if (t1 <= t0) break;
-    sum += d.part[part_at(d, i, h, kb, c) + threadIdx.x];
+    const float* part = d.part + part_at(d, i, h, kb, c) + threadIdx.x;
+    sum += part[0] + part[kKeys];
   }
   const int block = kv4_block(a.c, a.c.block_table, s.sid, key / kPageTokens);
   if (block >= 0) a.c.weights[kv4_slab_index(a.c, block, h) * kPageTokens + key % kPageTokens] += sum;
@@ -432,7 +428,7 @@ size_t kv4_colsum_scratch(int q_heads, int kv_heads, long long seqs, long long m
                           long long max_len) {
   const long long n = seqs < kSeqChunk ? seqs : kSeqChunk;
   return static_cast<size_t>(n) * kv_heads * ((max_len + kKeys - 1) / kKeys) * chunks_max(q_heads / kv_heads, max_q) *
-         kKeys * sizeof(float);
+         2 * kKeys * sizeof(float);
 }
 
 cudaError_t kv4_colsum_launch(const Kv4AttnArgs& a, const Kv4Rows& rows, void* scratch,
