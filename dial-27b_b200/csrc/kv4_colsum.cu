@@ -199,12 +199,17 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_colsum_kernel(const __grid_co
         const uint32_t tS = sm.tmem + sb * 128 + half * 64 + lane_off;
         const float *fc = sm.fac[cb] + half * 64, *of = sm.off[cb] + half * 64;
         const int* seen = sm.seen[cb] + half * 64;
+        auto free_scores = [&]() {
+          fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sm.sfree[sb]);
+        };
         // every row of the tile is there and sees the whole block
         if ((T + 1) * 128 <= w.s.n * rep && w.s.len - w.s.n + 1 + T * 128 / rep >= key0 + 128) {
-          uint32_t x[32], y[32];
+          uint32_t x[16], y[16];
           auto add = [&](const uint32_t* v, int c0) {
 #pragma unroll
-            for (int e = 0; e < 32; e += 4) {
+            for (int e = 0; e < 16; e += 4) {
               const ulonglong2 f2 = *reinterpret_cast<const ulonglong2*>(fc + c0 + e);
               const ulonglong2 o2 = *reinterpret_cast<const ulonglong2*>(of + c0 + e);
               const uint64_t z0 = fma2(pair(__uint_as_float(v[e]), __uint_as_float(v[e + 1])), f2.x, o2.x);
@@ -213,12 +218,19 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_colsum_kernel(const __grid_co
               s1 = add2(s1, pair(ex2(lo_of(z1)), ex2(hi_of(z1))));
             }
           };
-          ld32(tS, x);
-          ld_wait(x);
-          ld32(tS + 32, y);
+          ld16(tS, x);
+          ld_wait16(x);
+          ld16(tS + 16, y);
           add(x, 0);
-          ld_wait(y);
-          add(y, 32);
+          ld_wait16(y);
+          ld16(tS + 32, x);
+          add(y, 16);
+          ld_wait16(x);
+          ld16(tS + 48, y);
+          add(x, 32);
+          ld_wait16(y);
+          free_scores();
+          add(y, 48);
         } else {
 #pragma unroll 1
           for (int c = 0; c < 64; c += 16) {
@@ -233,13 +245,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_colsum_kernel(const __grid_co
             }
             __syncwarp();
           }
+          free_scores();
         }
-        fence_before();
         __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(&sm.sfree[sb]);
-          mbar_arrive(&sm.cfree[cb]);
-        }
+        if (lane == 0) mbar_arrive(&sm.cfree[cb]);
       }
       const uint64_t s = add2(s0, s1);
       if (w.t1 > w.t0) d.part[w.part + half * kKeys + grp * 128 + r] = lo_of(s) + hi_of(s);
