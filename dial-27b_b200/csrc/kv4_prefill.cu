@@ -383,72 +383,94 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const PrefillA
           }
           st_wait();
         }
-        // the probabilities under the reference so far, 16 scores at a time, the
-        // load of one chunk beside the work on the other; where one would exceed
-        // 2^kRaise the reference moves to the row's maximum and all is done again
-        uint32_t p[64];
-        uint64_t sum0, sum1;
-        float top;
-        auto probs = [&]() {
-          const uint64_t off2 = pair(-ref, -ref);
-          uint32_t x[16], y[16];
-          float t0 = -INFINITY, t1 = -INFINITY;
-          sum0 = sum1 = 0;
-          auto chunk = [&](const uint32_t* v, uint32_t* to) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const uint64_t z = fma2(pair(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])), fac2, off2);
-              if (e & 1) t1 = max3(t1, lo_of(z), hi_of(z));
-              else t0 = max3(t0, lo_of(z), hi_of(z));
-              const float p0 = ex2(lo_of(z)), p1 = ex2(hi_of(z));
-              if (e & 1) sum1 = add2(sum1, pair(p0, p1));
-              else sum0 = add2(sum0, pair(p0, p1));
-              to[e] = pack_f16(p0, p1);
-            }
-          };
-          ld16(tS, x);
-#pragma unroll
-          for (int c = 0; c < 8; c += 2) {
-            ld_wait16(x);
-            ld16(tS + 16 * c + 16, y);
-            chunk(x, p + 8 * c);
-            ld_wait16(y);
-            if (c < 6) ld16(tS + 16 * c + 32, x);
-            chunk(y, p + 8 * c + 8);
-          }
-          top = fmaxf(t0, t1);
-        };
-        probs();
-        if (__any_sync(0xffffffffu, top > kRaise || (m == -INFINITY && top > -INFINITY))) {
-          const float mn = fmaxf(m, top + ref);
-          const float al = m == -INFINITY ? 0.f : ex2(m - mn);
-          m = mn;
-          ref = mn == -INFINITY ? 0.f : mn;
-          l2 = pair(lo_of(l2) * al, hi_of(l2) * al);
-          if (kb > begin) {  // S of this block was issued after P V of the one before
+        // a half of the block after the other: the probabilities under the reference
+        // so far, 16 scores at a time, the load of one chunk beside the work on the
+        // other; where one would exceed 2^kRaise the reference moves to the row's
+        // maximum and the half is done again.  References are whole numbers, so that
+        // what is rescaled (sums, O, the P of the half before) stays exact.
 #pragma unroll 1
-            for (int cb = 0; cb < 8; ++cb) {
-              uint32_t o[16];
-              ld16(tO + cb * 16, o);
-              ld_wait16(o);
+        for (int hf = 0; hf < 2; ++hf) {
+          uint32_t p[32];
+          uint64_t sum0, sum1;
+          float top;
+          const uint32_t tH = tS + 64 * hf;
+          auto probs = [&]() {
+            const uint64_t off2 = pair(-ref, -ref);
+            uint32_t x[16], y[16];
+            float t0 = -INFINITY, t1 = -INFINITY;
+            sum0 = sum1 = 0;
+            auto chunk = [&](const uint32_t* v, uint32_t* to) {
 #pragma unroll
-              for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * al);
-              __syncwarp();
-              st16(tO + cb * 16, o);
-            }
-          }
+              for (int e = 0; e < 8; ++e) {
+                const uint64_t z = fma2(pair(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])), fac2, off2);
+                if (e & 1) t1 = max3(t1, lo_of(z), hi_of(z));
+                else t0 = max3(t0, lo_of(z), hi_of(z));
+                const float p0 = ex2(lo_of(z)), p1 = ex2(hi_of(z));
+                if (e & 1) sum1 = add2(sum1, pair(p0, p1));
+                else sum0 = add2(sum0, pair(p0, p1));
+                to[e] = pack_f16(p0, p1);
+              }
+            };
+            ld16(tH, x);
+            ld_wait16(x);
+            ld16(tH + 16, y);
+            chunk(x, p);
+            ld_wait16(y);
+            ld16(tH + 32, x);
+            chunk(y, p + 8);
+            ld_wait16(x);
+            ld16(tH + 48, y);
+            chunk(x, p + 16);
+            ld_wait16(y);
+            chunk(y, p + 24);
+            top = fmaxf(t0, t1);
+          };
           probs();
+          if (__any_sync(0xffffffffu, top > kRaise || (m == -INFINITY && top > -INFINITY))) {
+            const float mn = fmaxf(m, ceilf(top + ref));
+            const float al = m == -INFINITY ? 0.f : ex2(m - mn);
+            m = mn;
+            ref = mn == -INFINITY ? 0.f : mn;
+            l2 = pair(lo_of(l2) * al, hi_of(l2) * al);
+            if (kb > begin) {  // S of this block was issued after P V of the one before
+#pragma unroll 1
+              for (int cb = 0; cb < 8; ++cb) {
+                uint32_t o[16];
+                ld16(tO + cb * 16, o);
+                ld_wait16(o);
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * al);
+                __syncwarp();
+                st16(tO + cb * 16, o);
+              }
+            }
+            if (hf == 1) {
+              const uint32_t al2 = pack_f16(al, al);
+              st_wait();
+#pragma unroll 1
+              for (int cb = 0; cb < 2; ++cb) {
+                uint32_t o[16];
+                ld16(tS + cb * 16, o);
+                ld_wait16(o);
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[e] = hmul2(o[e], al2);
+                __syncwarp();
+                st16(tS + cb * 16, o);
+              }
+            }
+            probs();
+          }
+          l2 = add2(l2, add2(sum0, sum1));
+          __syncwarp();
+          st16(tS + 32 * hf, p);
+          st16(tS + 32 * hf + 16, p + 16);
         }
-        l2 = add2(l2, add2(sum0, sum1));
         if (kb + 1 == last && f < f1) {
           // the tile's queries are read: the next item's may take their place
           find_next(f);
           fetched = next->j0 < min(next->j1, next->blocks[t]);
           if (fetched) fetch_q(*next);
         }
-        __syncwarp();
-#pragma unroll
-        for (int c = 0; c < 4; ++c) st16(tS + 16 * c, p + 16 * c);
         st_wait();
         fence_before();
         __syncwarp();
