@@ -307,7 +307,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const PrefillA
       const int j = mine ? R / rep : 0;
       long long at = (x.s.row0 + j) * a.q_ld + (x.h * rep + (mine ? R - j * rep : 0)) * kHeadDim;
       if (!mine) at = -1;
-#pragma unroll
+#pragma unroll 4
       for (int e = 0; e < 16; ++e) {
         const int row = 2 * e + (lane >> 4), c = lane & 15;
         const long long from = __shfl_sync(0xffffffffu, at, row);
@@ -332,7 +332,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const PrefillA
         // f16 after 2^-e of the row's largest exponent: exact for values down to
         // 2^-14 of it, and off by at most 2^-25 of it below
         float top = 0.f;
-#pragma unroll
+#pragma unroll 2
         for (int e = 0; e < 16; ++e) {
           const uint4 raw = *reinterpret_cast<const uint4*>(q_row + (e >> 3) * kHalf + (((e & 7) ^ (r & 7)) << 4));
           const Act* v = reinterpret_cast<const Act*>(&raw);
@@ -343,7 +343,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const PrefillA
         const float down = exp2i(-ex);
         fac = exp2i(ex) * a.scale * a.c.k_scale * 1.4426950408889634f;
         const bool keep_q = d.off && live && begin == 0;
-#pragma unroll
+#pragma unroll 2
         for (int e = 0; e < 16; ++e) {
           uint4* at = reinterpret_cast<uint4*>(q_row + (e >> 3) * kHalf + (((e & 7) ^ (r & 7)) << 4));
           const uint4 raw = *at;
@@ -465,16 +465,16 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const PrefillA
           st16(tS + 32 * hf, p);
           st16(tS + 32 * hf + 16, p + 16);
         }
+        st_wait();
+        fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.pready[t]);
         if (kb + 1 == last && f < f1) {
           // the tile's queries are read: the next item's may take their place
           find_next(f);
           fetched = next->j0 < min(next->j1, next->blocks[t]);
           if (fetched) fetch_q(*next);
         }
-        st_wait();
-        fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sm.pready[t]);
       }
       // ------------------------------------------------------------ output
       const bool whole = w.j0 == 0 && w.j1 == w.nb;
@@ -488,27 +488,25 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const PrefillA
           const float inv = l != 0.f ? a.c.v_scale / l : 0.f;
           Act* dst = static_cast<Act*>(a.out) + (w.s.row0 + j) * a.out_ld + head * kHeadDim;
           float* part = d.part_o + (static_cast<size_t>(slot) * 2 * kRows + t * kRows + r) * kHeadDim;
-#pragma unroll
-          for (int cb = 0; cb < 2; ++cb) {
-            uint32_t o[64];
-            ld32(tO + cb * 64, o);
-            ld32(tO + cb * 64 + 32, o + 32);
+#pragma unroll 1
+          for (int cb = 0; cb < 4; ++cb) {
+            uint32_t o[32];
+            ld32(tO + cb * 32, o);
             ld_wait(o);
-            ld_wait(o + 32);
             if (live && whole) {
 #pragma unroll
-              for (int e = 0; e < 8; ++e) {
+              for (int e = 0; e < 4; ++e) {
                 uint4 out;
                 Act* h = reinterpret_cast<Act*>(&out);
 #pragma unroll
                 for (int u = 0; u < 8; ++u)
                   h[u] = ActTraits<Act>::from_f(l != 0.f ? __uint_as_float(o[8 * e + u]) * inv : 0.f);
-                reinterpret_cast<uint4*>(dst)[cb * 8 + e] = out;
+                reinterpret_cast<uint4*>(dst)[cb * 4 + e] = out;
               }
             } else if (live) {
 #pragma unroll
-              for (int e = 0; e < 16; ++e)
-                reinterpret_cast<uint4*>(part)[cb * 16 + e] =
+              for (int e = 0; e < 8; ++e)
+                reinterpret_cast<uint4*>(part)[cb * 8 + e] =
                     make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
             }
             __syncwarp();
