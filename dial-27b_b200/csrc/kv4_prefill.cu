@@ -33,7 +33,7 @@ namespace {
 constexpr int kRows = 128;                  // rows of a tile
 constexpr int kKeys = 128;                  // keys of a block
 constexpr int kThreads = 13 * 32;
-constexpr int kPad = 2;                     // an item's own cost, in blocks
+constexpr int kPad = 4;                     // an item's own cost, in blocks
 constexpr int kSeqChunk = 512;              // sequences a launch
 constexpr int kOffQ = 0;                    // [2]
 constexpr int kOffK = 2 * kTile;            // [2]
@@ -201,6 +201,13 @@ __device__ void work_prefix(const Kv4AttnArgs& a, long long* cum) {
   __syncthreads();
 }
 
+// 32 bytes, on a 32-byte boundary: a row's stores are whole sectors.
+__device__ __forceinline__ void st_global8(void* to, const uint32_t* v) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(v[0]), "r"(v[1]),
+               "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
+
 template <typename Act>
 __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const PrefillArgs d) {
   extern __shared__ uint8_t smem_raw[];
@@ -298,6 +305,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const PrefillA
       __syncwarp();
     };
     bool ok = true, fetched = false;
+    const bool wide = (reinterpret_cast<uintptr_t>(a.out) & 31) == 0 && a.out_ld % 16 == 0;
     // whether the item the range begins inside ends in it (1) or not (0)
     const int first = cur->j0 == 0 ? -1 : cur->j1 == cur->nb;
     // the warp's 32 rows of the tile's queries, raw, where their f16 form will be
@@ -362,6 +370,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const PrefillA
         if (lane == 0) mbar_arrive(&sm.qfull[t]);
       }
       fetched = false;
+      if (f < f1) find_next(f);  // beside the first S
       const uint64_t fac2 = pair(fac, fac);
       for (int kb = begin; kb < last; ++kb) {
         ok = __all_sync(0xffffffffu, ok && wait(&sm.sfull[t], sphase & 1u));
@@ -471,7 +480,6 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const PrefillA
         if (lane == 0) mbar_arrive(&sm.pready[t]);
         if (kb + 1 == last && f < f1) {
           // the tile's queries are read: the next item's may take their place
-          find_next(f);
           fetched = next->j0 < min(next->j1, next->blocks[t]);
           if (fetched) fetch_q(*next);
         }
@@ -495,19 +503,23 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const PrefillA
             ld_wait(o);
             if (live && whole) {
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                uint4 out;
-                Act* h = reinterpret_cast<Act*>(&out);
+              for (int e = 0; e < 2; ++e) {
+                uint32_t v[8];
+                Act* h = reinterpret_cast<Act*>(v);
 #pragma unroll
-                for (int u = 0; u < 8; ++u)
-                  h[u] = ActTraits<Act>::from_f(l != 0.f ? __uint_as_float(o[8 * e + u]) * inv : 0.f);
-                reinterpret_cast<uint4*>(dst)[cb * 4 + e] = out;
+                for (int u = 0; u < 16; ++u)
+                  h[u] = ActTraits<Act>::from_f(l != 0.f ? __uint_as_float(o[16 * e + u]) * inv : 0.f);
+                Act* to = dst + cb * 32 + e * 16;
+                if (wide) {
+                  st_global8(to, v);
+                } else {
+                  reinterpret_cast<uint4*>(to)[0] = make_uint4(v[0], v[1], v[2], v[3]);
+                  reinterpret_cast<uint4*>(to)[1] = make_uint4(v[4], v[5], v[6], v[7]);
+                }
               }
             } else if (live) {
 #pragma unroll
-              for (int e = 0; e < 8; ++e)
-                reinterpret_cast<uint4*>(part)[cb * 8 + e] =
-                    make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+              for (int e = 0; e < 4; ++e) st_global8(part + cb * 32 + e * 8, o + 8 * e);
             }
             __syncwarp();
           }
@@ -526,9 +538,6 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const PrefillA
         if (tid == 0)
           d.desc[b] = w.j0 == 0 && w.j1 < w.nb ? make_int4(w.i, w.h, w.tp, first) : make_int4(-1, 0, 0, first);
         break;
-      }
-      if (w.j0 >= last) {  // nothing of this item for the tile: the next is not known yet
-        find_next(f);
       }
       Share* was = cur;
       cur = next;
