@@ -10,7 +10,13 @@
 namespace dialb200 {
 namespace {
 
-constexpr int kFewCols = 64;
+// (query, head of the group) columns of a sequence up to which the decode kernel
+// takes a call: its MMAs are 8 columns wide and a page costs it about the same
+// instructions for each 16, while the tcgen05 kernels have 128 rows a tile whatever
+// a sequence brings.  Measured, decode / tcgen05, 32 heads of 8, 8 sessions of 4096
+// slots: 32 columns 38 / 52 us, 64 61 / 53, 96 85 / 54; one of 65536: 61 / 84, 100 / 85,
+// 144 / 86; with weights, 8 of 4096: 61 / 99, 113 / 101, 193 / 102.
+constexpr int kFewCols = 48;
 
 // Scratch of the attention of many queries; that of their weights follows.
 size_t rows_part(int q_heads, long long rows) {

@@ -156,8 +156,8 @@ __device__ __forceinline__ void encode8(const float (&x)[8], float mult, uint32_
 // A CTA for a row and a share (blockIdx.y) of its head units, a half warp a unit: unit
 // u < kv_heads is a kv head (k and v), the others query heads.  A warp's norm weights,
 // cos and sin serve all its units, U of which are loaded at once.
-// Bound by instructions for long prompts (about half of them the quantisation), by
-// latency for a token.
+// Bound by instructions for long prompts (14.6 M for 2048 rows, about half of them the
+// quantisation; 2.46 a clock, DRAM at 12 %), by latency for a token (7 us cold).
 template <typename Act, int U>
 __global__ void __launch_bounds__(256) kv4_append_kernel(const AppendArgs a) {
   const int lane = threadIdx.x & 31, l = lane & 15, m = blockIdx.x;
@@ -301,7 +301,10 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const ReadArgs a) {
 template <typename Act>
 cudaError_t launch_read(const ReadArgs& a, cudaStream_t s) {
   const long long units = static_cast<long long>(a.rows) * a.c.kv_heads;
-  if (a.rows <= 148 * 64)  // few: every (slot, kv head) a warp of its own
+  // Few: every (slot, kv head) a warp of its own, for latency; many: a warp two rows.
+  // 8 kv heads, own / shared: 256 rows 2.7 / 6.5 us, 2048 5.2 / 6.9, 4096 9.1 / 7.7,
+  // 9472 17.1 / 9.3, 65536 115 / 67 (302 MB: 4.5 TB/s, bound by the loads' latency).
+  if (a.rows <= 148 * 20)
     return kv4_start(kv4_read_kernel<Act, false>, dim3(static_cast<unsigned>((units + 7) / 8)), 256, 0, s, a);
   return kv4_start(kv4_read_kernel<Act, true>, dim3((a.rows + 15) / 16), 256, 0, s, a);
 }
@@ -447,11 +450,15 @@ extern "C" int dial_b200_kv4_append(const dial_b200_kv4_shape* sh, const void* q
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   cudaError_t e;
   const int most = (a.units + 15) / 16;
-  if (rows * most <= 1184) {  // a unit a half warp while the GPU's 148 SMs have room for more CTAs
+  // A unit a half warp while 148 SMs have room for the CTAs (8 of 256 threads each);
+  // else a row a CTA, three of a half warp's units in flight.  32 heads of 8 (3 CTAs a
+  // row), unit / row: 16 rows 3.0 / 4.0 us, 256 4.9 / 4.8, 394 6.0 / 6.4, 1024 13.3 / 10.3,
+  // 2048 24.7 / 18.5.
+  if (rows * most <= 1184) {
     const dim3 grid(static_cast<unsigned>(rows), most);
     e = sh->act == DIAL_ACT_BF16 ? kv4_start(kv4_append_kernel<__nv_bfloat16, 1>, grid, 256, 0, s, a)
                                  : kv4_start(kv4_append_kernel<__half, 1>, grid, 256, 0, s, a);
-  } else {  // a row a CTA, three of a half warp's units in flight
+  } else {
     const dim3 grid(static_cast<unsigned>(rows), 1);
     e = sh->act == DIAL_ACT_BF16 ? kv4_start(kv4_append_kernel<__nv_bfloat16, 3>, grid, 256, 0, s, a)
                                  : kv4_start(kv4_append_kernel<__half, 3>, grid, 256, 0, s, a);

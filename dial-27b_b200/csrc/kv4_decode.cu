@@ -20,13 +20,19 @@
 // one vote a page instead of a shuffle tree.
 //
 // Work split: the pages of all (sequence, kv head) segments laid end to end and
-// cut into equal ranges, one a CTA, so ragged lengths balance; the pages of a
-// range go round its 4 warps, each with its own ring of bulk copies that runs on
+// cut into ranges of equal cost, one a CTA, so ragged lengths balance; the pages of a
+// range go round its warps, each with its own ring of bulk copies that runs on
 // across segment borders.  A segment inside one range is finished there; the
 // others leave (m, l, O) parts that kv4_join_kernel adds in order.  With running
-// weights the scores are kept in scratch (16 columns' f32 are a ninth of the
-// page's bytes at 4 heads a group) and the join turns them into probabilities
-// once m and l are known, one thread a slot, no atomics.
+// weights the scores are kept in scratch (16 bytes a slot at 4 heads a group, a ninth
+// of the page's) and the join turns them into probabilities once m and l are known, a
+// slot a thread, no atomics.
+//
+// Measured, kernel and join by themselves with cold caches: 32 sessions of 128 to 8192 slots (180 MB) 49 + 6 us, one of
+// 131071 (151 MB) 39 + 8, 9 of 900 to 30001 with weights 48 + 17, five queries of 8
+// sessions of 700 to 4099 with weights 36 + 15, 201 slots 10.  Bound by
+// instructions: 320 a page, warp and column tile (dequantisation 130, MMA 72,
+// softmax 60), 2.45 a clock; DRAM at 46 %, the tensor pipe at 21 %.
 #include <cmath>
 #include <type_traits>
 
@@ -47,9 +53,12 @@ template <int NT>
 constexpr int kCtasPerSm = NT == 1 ? 2 : 3;
 constexpr int kRing = 4;           // pages in flight a warp
 constexpr int kSeqChunk = 256;     // sequences a launch
-constexpr int kSegPad = 20;        // a segment's own cost (its start, and the merge of its parts), in pages
+// A segment's own cost (its start, and the merge of its parts), in pages.  32 ragged
+// sessions of 128 to 8192 slots: 55.7 us at 1, 53.3 at 10, 51.0 at 20, 50.8 at 30; five
+// queries of 8 sessions with weights 55.0 at 1, 50.2 at 20.
+constexpr int kSegPad = 20;
 constexpr int kInfo = 6;           // sequences of a range kept in shared memory
-constexpr int kOneLen = 512;       // slots up to which a CTA takes a whole segment
+constexpr int kOneLen = 1024;      // slots up to which a CTA takes a whole segment
 constexpr float kRaise = 8.f;      // log2 headroom of a probability above 1
 constexpr int kColStride = kHeadDim + 8;
 
@@ -702,8 +711,10 @@ __global__ void __launch_bounds__(kWarpsOf<NT> * 32, kCtasPerSm<NT>)
 }
 
 constexpr int kJoinThreads = 256, kJoinWarps = kJoinThreads / 32;
-constexpr int kWeightCtas = 4;  // of a range
-constexpr int kFewParts = 16;   // of a segment, up to which a warp joins a column
+constexpr int kWeightCtas = 4;  // of a range, scheduled first: 17 us against 20 when last
+// Parts of a segment up to which a warp joins a column by itself (more: a CTA).  Five
+// queries of 8 sessions, 4 parts a segment: the join takes 14 us against 21.
+constexpr int kFewParts = 16;
 
 // max over a segment's parts of a column, and the sum l under it; G lanes share them.
 template <int G>
@@ -879,9 +890,11 @@ Plan plan_of(int q_heads, int kv_heads, long long seqs, long long max_q, long lo
   p.pages = seqs * per * kv_heads;
   // a page a warp at least, as many CTAs as are resident at once at most
   p.pages_max = static_cast<int>(per);
-  // Short sequences: a CTA for each segment, which nothing has to join.  A
-  // segment of kOneLen slots takes one CTA about as long as the join of ranges
-  // (3 us) and its launch; the weights of several column groups need the join.
+  // Short sequences: a CTA for each segment, which nothing has to join; without the
+  // second launch, the prefix and the parts.  A CTA a segment / ranges, 32 heads of 8:
+  // one session of 256 slots 5.4 / 7.5 us, of 1024 9.1 / 9.3; 32 sessions of 256 7.7 /
+  // 15.1, of 1024 13.6 / 20.7; 128 of 1024 44.7 / 52.3.  The weights of several column
+  // groups need the join.
   p.one = max_len <= kOneLen && !(weights && p.groups > 1);
   const int warps = p.nt == 1 ? kWarpsOf<1> : kWarpsOf<2>;
   const long long want = (p.pages + warps - 1) / warps;

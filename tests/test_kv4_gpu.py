@@ -203,6 +203,23 @@ def test_attention_of_many_ragged_sequences(cuda, weights):
     check_attention(c, cuda, [(s, n, 1) for s, n in enumerate(lens)], weights=weights)
 
 
+@pytest.mark.parametrize("weights", [False, True])
+def test_ranges_of_many_ragged_sequences(cuda, weights):
+    """The same with one sequence too long for a CTA a segment, in a call of more
+    sequences than one launch takes."""
+    c = Cache(21, 270, 1100, 3, 1)
+    lens = [int(n) for n in c.rng.integers(0, 30, 270)]
+    lens[130], lens[131], lens[264], lens[269] = 1100, 1025, 1090, 0
+    check_attention(c, cuda, [(s, n, 1) for s, n in enumerate(lens)], weights=weights)
+
+
+@pytest.mark.parametrize("queries", [8, 9, 12, 13])
+def test_attention_around_the_few_queries_rule(cuda, queries):
+    c = Cache(22, 2, 1500, 8, 2)
+    check_attention(c, cuda, [(0, 1500, queries), (1, 1023, queries)])
+    check_attention(c, cuda, [(0, 1024, queries), (1, 1000, 3)], weights=False)
+
+
 def test_many_sequences_of_many_queries(cuda):
     """More sequences than one launch takes, each with rows for several tiles,
     one of one query, one of none."""
