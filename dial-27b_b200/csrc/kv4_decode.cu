@@ -31,8 +31,9 @@
 // Measured, kernel and join by themselves with cold caches: 32 sessions of 128 to 8192 slots (180 MB) 49 + 6 us, one of
 // 131071 (151 MB) 39 + 8, 9 of 900 to 30001 with weights 48 + 17, five queries of 8
 // sessions of 700 to 4099 with weights 36 + 15, 201 slots 10.  Bound by
-// instructions: 320 a page, warp and column tile (dequantisation 130, MMA 72,
-// softmax 60), 2.45 a clock; DRAM at 46 %, the tensor pipe at 21 %.
+// instructions: 320 a page and column tile (16 MMAs, 64 conversions and 64 packed
+// products of the codes with what arranges them, the softmax of 128 scores), 2.45 a
+// clock; DRAM at 46 %, the tensor pipe at 21 %.
 #include <cmath>
 #include <type_traits>
 

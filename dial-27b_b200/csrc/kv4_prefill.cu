@@ -21,7 +21,7 @@
 // (290 against 332).
 //
 // Measured: a 2048-token prompt, 32 heads of 8 (34 GFLOP) 72 us with the join of 15; 512
-// tokens each on 9500 and 16897 slots, 40 heads of 8 (137 GFLOP) 290-330 by the
+// tokens each on 9500 and 16897 slots, 40 heads of 8 (271 GFLOP) 290-317 by the
 // clock.  Two tiles' 128-key block takes 2.4 us against 1.1 for its MMAs and 1.1 for
 // its exponentials: bound by the chain S, softmax, P V of each tile, of which two
 // are all that TMEM's 512 columns hold.  Sixteen softmax warps, two a row, took 420

@@ -267,7 +267,7 @@ int64_t dial_b200_kv4_attention_scratch_bytes(const dial_b200_kv4_shape* sh, int
  *   must then name distinct sessions that share no page (a sum is one load and
  *   one store).
  * max_q and max_len bound n and lens[i] (host); rows no sequence names are left as
- * they were.  `scratch` needs no preparation; two calls that may run at the
+ * they were; out must not overlap q.  `scratch` needs no preparation; two calls that may run at the
  * same time need two. */
 int dial_b200_kv4_attention(const dial_b200_kv4_shape* sh, const void* q, int64_t q_ld,
                             const void* pages, float* weights, const int32_t* block_table,
