@@ -616,6 +616,48 @@ def test_append_and_read_of_strided_rows(cuda):
     assert torch.equal(cache.pages, ref.pages)
 
 
+@pytest.mark.parametrize("dt", [BF16, F16])
+def test_prompt_rows_on_sixteen_byte_boundaries(cuda, dt):
+    """q and out that start on 16-byte but not on 32-byte boundaries, whole items and
+    items cut over the GPU: the bits of an aligned call, the columns beside untouched."""
+    from dial_b200 import kv4
+
+    c = Cache(48, 2, 2600, 8, 2, dt=dt)
+    cache, table = c.device(cuda)
+    width, rows = 8 * DIM, 230
+    wide = (torch.randn(rows, width + 24, device=cuda) * 2).to(dt)
+    out = torch.full((rows, width + 24), 3.0, dtype=dt, device=cuda)
+    args = (table, i32(cuda, 1, 0), i32(cuda, 2600, 70), 2600, i32(cuda, 0, 200, 230), 200)
+    kv4.kv4_attention(c.sh, cache, wide[:, 8:8 + width], *args, out=out[:, 8:8 + width])
+    want = kv4.kv4_attention(c.sh, cache, wide[:, 8:8 + width].contiguous(), *args)
+    assert torch.equal(out[:, 8:8 + width], want)
+    assert (out[:, :8] == 3.0).all() and (out[:, 8 + width:] == 3.0).all()
+    o, b, _, _ = c.attend(host(wide[:200, 8:8 + width]), 1, 2600)
+    assert (np.abs(host(want[:200]) - o) <= b).all()
+
+
+def test_evict_twice_and_the_same_bits(cuda):
+    """An eviction repeated on what it left changes nothing; two runs give the same
+    bits; sessions evicted beside each other as one by one."""
+    from dial_b200 import kv4
+
+    c = Cache(49, 3, 900, 4, 2)
+    runs = []
+    for one_by_one in (False, True, False):
+        cache, table = c.device(cuda)
+        if one_by_one:
+            new = torch.cat([kv4.kv4_evict(c.sh, cache, table, i32(cuda, s), i32(cuda, n), 900, 300, 40)
+                             for s, n in ((0, 900), (1, 299), (2, 640))])
+        else:
+            new = kv4.kv4_evict(c.sh, cache, table, i32(cuda, 0, 1, 2), i32(cuda, 900, 299, 640), 900, 300, 40)
+        runs.append((new, cache.pages.clone(), cache.weights.clone(), cache.positions.clone()))
+        again = kv4.kv4_evict(c.sh, cache, table, i32(cuda, 0, 1, 2), new, 900, 300, 40)
+        assert again.tolist() == [300, 299, 300]
+        assert torch.equal(cache.pages, runs[-1][1]) and torch.equal(cache.weights, runs[-1][2])
+    for r in runs[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(r, runs[0]))
+
+
 def test_empty_calls(cuda):
     from dial_b200 import kv4
 
