@@ -258,43 +258,60 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const ReadArgs a) {
   const int codes_at = (part ? kKv4VCodes : 0) + l * 4;
   const int scales_at = (part ? kKv4VScales : kKv4KScales) + (l >> 1);
   const unsigned unit = blockIdx.x * 8 + (threadIdx.x >> 5);
+  constexpr unsigned R = HEADS ? 2 : 1, B = HEADS ? 4 : 1;  // rows, and heads at once
+  const unsigned h0 = HEADS ? 0 : unit % H, h1 = HEADS ? H : h0 + 1;
+  // the rows' look-ups beside each other, then the loads of B heads of them
+  bool write[R], there[R];
+  const uint8_t* slab[R];
+  int t[R];
 #pragma unroll
-  for (unsigned e = 0; e < (HEADS ? 2u : 1u); ++e) {
-    const unsigned row = HEADS ? unit * 2 + e : unit / H;
-    if (row >= a.rows) return;
-    const unsigned h0 = HEADS ? 0 : unit - row * H, h1 = HEADS ? H : h0 + 1;
-    const unsigned i = row / static_cast<unsigned>(a.count);
+  for (unsigned e = 0; e < R; ++e) {
+    const unsigned row = HEADS ? unit * R + e : unit / H;
+    write[e] = row < a.rows;
+    const unsigned i = write[e] ? row / static_cast<unsigned>(a.count) : 0;
     const int sid = a.sids[i];
     const long long slot = (a.first ? a.first[i] : 0) + static_cast<long long>(row - i * a.count);
-    const bool there = slot >= 0 && slot < a.lens[i];
-    if (there && (static_cast<unsigned>(sid) >= static_cast<unsigned>(a.c.sessions) ||
-                  slot >= static_cast<long long>(a.c.max_blocks) * kPageTokens)) {
+    there[e] = write[e] && slot >= 0 && slot < a.lens[i];
+    if (there[e] && (static_cast<unsigned>(sid) >= static_cast<unsigned>(a.c.sessions) ||
+                     slot >= static_cast<long long>(a.c.max_blocks) * kPageTokens)) {
       if (lane == 0) set_status(a.c.status, kStatusBadArgs);
-      continue;
+      write[e] = there[e] = false;
     }
-    const int t = there ? static_cast<int>(slot % kPageTokens) : 0;
-    const int block = there ? max(0, kv4_block(a.c, a.c.block_table, sid, static_cast<int>(slot / kPageTokens))) : 0;
-    const uint8_t* slab = a.c.pages + kv4_slab_index(a.c, block, 0) * kKv4Slab;
-    Act* out = static_cast<Act*>(part ? a.v_out : a.k_out) + static_cast<size_t>(row) * H * kHeadDim + l * 8;
-#pragma unroll 4
-    for (unsigned h = h0; h < h1; ++h) {
-      uint32_t w = 0, sc = 0;
-      if (there) {
-        w = *reinterpret_cast<const uint32_t*>(slab + h * kKv4Slab + codes_at + t * 64);
-        sc = slab[h * kKv4Slab + scales_at + t * 8];
-      }
-      const float f = e4m3_value(sc) * mult;
-      uint32_t o[4];
-      e2m1x8_to_f16x2x4(w, o);
-      uint4 r;
-      typename Pair<Act>::T* p = reinterpret_cast<typename Pair<Act>::T*>(&r);
+    t[e] = there[e] ? static_cast<int>(slot % kPageTokens) : 0;
+    const int block = there[e] ? max(0, kv4_block(a.c, a.c.block_table, sid, static_cast<int>(slot / kPageTokens))) : 0;
+    slab[e] = a.c.pages + kv4_slab_index(a.c, block, 0) * kKv4Slab;
+  }
+  for (unsigned h = h0; h < h1; h += B) {
+    uint32_t w[R][B], sc[R][B];
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&o[q]));
-        p[q] = Pair<Act>::of(v.x * f, v.y * f);
+    for (unsigned e = 0; e < R; ++e)
+#pragma unroll
+      for (unsigned u = 0; u < B; ++u) {
+        w[e][u] = sc[e][u] = 0;
+        if (there[e] && h + u < h1) {
+          const uint8_t* from = slab[e] + (h + u) * kKv4Slab;
+          w[e][u] = *reinterpret_cast<const uint32_t*>(from + codes_at + t[e] * 64);
+          sc[e][u] = from[scales_at + t[e] * 8];
+        }
       }
-      *reinterpret_cast<uint4*>(out + static_cast<size_t>(h) * kHeadDim) = r;
-    }
+#pragma unroll
+    for (unsigned e = 0; e < R; ++e)
+#pragma unroll
+      for (unsigned u = 0; u < B; ++u) {
+        if (!write[e] || h + u >= h1) continue;
+        const float f = e4m3_value(sc[e][u]) * mult;
+        uint32_t o[4];
+        e2m1x8_to_f16x2x4(w[e][u], o);
+        uint4 r;
+        typename Pair<Act>::T* p = reinterpret_cast<typename Pair<Act>::T*>(&r);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&o[q]));
+          p[q] = Pair<Act>::of(v.x * f, v.y * f);
+        }
+        const size_t row = HEADS ? unit * R + e : unit / H;
+        *reinterpret_cast<uint4*>(static_cast<Act*>(part ? a.v_out : a.k_out) + (row * H + h + u) * kHeadDim + l * 8) = r;
+      }
   }
 }
 
@@ -302,9 +319,10 @@ template <typename Act>
 cudaError_t launch_read(const ReadArgs& a, cudaStream_t s) {
   const long long units = static_cast<long long>(a.rows) * a.c.kv_heads;
   // Few: every (slot, kv head) a warp of its own, for latency; many: a warp two rows.
-  // 8 kv heads, own / shared: 256 rows 2.7 / 6.5 us, 2048 5.2 / 6.9, 4096 9.1 / 7.7,
-  // 9472 17.1 / 9.3, 65536 115 / 67 (302 MB: 4.5 TB/s, bound by the loads' latency).
-  if (a.rows <= 148 * 20)
+  // 8 kv heads, own / shared: 256 rows 2.5 / 4.1 us, 2048 5.3 / 4.3, 4096 9.1 / 5.6, 65536
+  // 115 / 59 (302 MB: 5.1 TB/s).  Four heads of two rows are loaded before the first is
+  // stored (stores hold back the loads behind them): 59 against 67; eight 60.
+  if (a.rows <= 148 * 8)
     return kv4_start(kv4_read_kernel<Act, false>, dim3(static_cast<unsigned>((units + 7) / 8)), 256, 0, s, a);
   return kv4_start(kv4_read_kernel<Act, true>, dim3((a.rows + 15) / 16), 256, 0, s, a);
 }
