@@ -39,9 +39,11 @@ using namespace dialb200;
 extern "C" int64_t dial_b200_kv4_attention_scratch_bytes(const dial_b200_kv4_shape* sh,
                                                          int64_t seqs, int64_t rows, int64_t max_q,
                                                          int64_t max_len, int32_t with_weights) {
-  if (!sh || sh->q_heads < 1 || sh->kv_heads < 1 || sh->q_heads % sh->kv_heads != 0 || seqs < 0 || rows < 0 || max_q < 0 ||
-      max_len < 0)
+  if (!sh || sh->q_heads < 1 || sh->kv_heads < 1 || sh->kv_heads > 1024 || sh->q_heads % sh->kv_heads != 0 ||
+      sh->q_heads / sh->kv_heads > 16 || seqs < 0 || seqs > 65535 || rows < 0 || rows > (1 << 26) || max_q < 0 ||
+      max_q > (1 << 24) || max_len < 0 || max_len > 16LL << 26)
     return -1;
+  if (seqs == 0 || rows == 0 || max_q == 0) return 0;  // the call does nothing
   // enough for every call within the sizes, whichever kernels it takes
   const int rep = sh->q_heads / sh->kv_heads;
   const int64_t few = max_q < kFewCols / rep ? max_q : kFewCols / rep;

@@ -96,6 +96,11 @@ def _rows(name: str, t, dtype, rows, width: int, idx: int):
          f"got {t.dtype} {tuple(t.shape)} strides {t.stride()} on {t.device}")
 
 
+def _max_len(sh: Kv4Shape, max_len: int):
+    if not 0 <= max_len <= PAGE_TOKENS * sh.max_blocks:
+        _bad(f"max_len {max_len} exceeds the block table's {PAGE_TOKENS * sh.max_blocks} slots")
+
+
 def _launch(name: str, idx: int, *args):
     """The call on the current stream of device `idx`, which is made current."""
     if idx < 0:
@@ -119,7 +124,7 @@ def _current_device() -> int:
 def _scratch(given, nbytes: int, like):
     """Address of the scratch, and what keeps it alive during the call."""
     if given is None:
-        if not nbytes:
+        if nbytes <= 0:  # none is needed, or the call refuses its sizes
             return 0, None
         given = torch.empty(nbytes, dtype=torch.uint8, device=like.device)
     elif (given.get_device() != like.get_device() or not given.is_contiguous()
@@ -211,6 +216,7 @@ def kv4_attention(sh: Kv4Shape, cache: Kv4Cache, q, block_table, sids, lens, max
         if not p_w:
             _bad("accumulate needs a cache with weights")
     p_bt, sessions = _table("block_table", block_table, sh.max_blocks, idx)
+    _max_len(sh, max_len)
     p_s, keep = _scratch(scratch, attention_scratch_bytes(sh, n, rows, max_q, max_len, accumulate), q)
     _launch("dial_b200_kv4_attention", idx, C.byref(sh), p_q, ld,
             _need("pages", cache.pages, torch.uint8, slabs * SLAB_BYTES, idx), p_w, p_bt,
@@ -236,8 +242,9 @@ def kv4_evict(sh: Kv4Shape, cache: Kv4Cache, block_table, sids, lens, max_len: i
     or into the pages of dst_table.  Returns the new lengths [seqs]."""
     idx, i32, H, nb = sids.get_device(), torch.int32, sh.kv_heads, sh.num_blocks
     n, slots = sids.numel(), nb * H * PAGE_TOKENS
-    if keep < 0 or max_len < 0:
-        _bad(f"keep {keep} / max_len {max_len} is negative")
+    if keep < 0:
+        _bad(f"keep {keep} is negative")
+    _max_len(sh, max_len)
     if lens_out is None:
         lens_out = torch.empty(n, dtype=i32, device=sids.device)
     p_bt, sessions = _table("block_table", block_table, sh.max_blocks, idx)

@@ -92,6 +92,46 @@ def test_null_shape_and_sizes():
     assert _abi.lib.dial_b200_kv4_attention_scratch_bytes(C.byref(sh), -1, 1, 1, 1, 0) == -1
 
 
+@pytest.mark.parametrize("q_heads,kv_heads", [(1, 1), (16, 1), (40, 8), (1024, 1024)])
+def test_scratch_of_every_size(q_heads, kv_heads):
+    """Sizes at the ends of their ranges: never an arithmetic fault, none for a call
+    that does nothing, and no less for a larger call than for a smaller one."""
+    sh = kv4.make_shape(q_heads, kv_heads, 64, 640)
+    size = kv4.attention_scratch_bytes
+    for weights in (False, True):
+        for seqs, rows, max_q, max_len in ((0, 5, 5, 99), (3, 0, 5, 99), (3, 5, 0, 99)):
+            assert size(sh, seqs, rows, max_q, max_len, weights) == 0
+        for seqs, rows, max_q in ((1, 1, 1), (7, 60, 9), (300, 300, 1), (300, 9000, 48), (65535, 65535, 1)):
+            last = 0
+            for max_len in (0, 1, 511, 1024, 1025, 4096, 70000, 1 << 20):
+                got = size(sh, seqs, rows, max_q, max_len, weights)
+                assert got >= last, (seqs, rows, max_q, max_len)
+                last = got
+        for max_len in (700, 1500, 40000):
+            last = 0
+            for q in (1, 2, 3, 4, 9, 10, 12, 13, 48, 49, 100, 1000):
+                got = size(sh, 8, 8 * q, q, max_len, weights)
+                assert got >= last, (q, max_len)
+                last = got
+            last = 0
+            for seqs in (1, 2, 9, 100, 255, 256, 257, 600, 5000):
+                got = size(sh, seqs, seqs, 1, max_len, weights)
+                assert got >= last, (seqs, max_len)
+                last = got
+
+
+def test_scratch_of_refused_sizes():
+    raw, ev = _abi.lib.dial_b200_kv4_attention_scratch_bytes, _abi.lib.dial_b200_kv4_evict_scratch_bytes
+    for heads in ((17, 1), (64, 1), (30, 4), (0, 1), (4096, 2048)):
+        assert raw(C.byref(kv4.make_shape(*heads, 64, 64)), 1, 1, 1, 64, 1) == -1
+    sh = kv4.make_shape(32, 8, 64, 64)
+    for sizes in ((65536, 1, 1, 64), (1, 1 << 27, 1, 64), (1, 1, 1 << 25, 64), (1, 1, 1, 1 << 31), (1, 1, 1, -1)):
+        assert raw(C.byref(sh), *sizes, 0) == -1
+    assert ev(C.byref(sh), 65536, 64, 8) == -1 and ev(C.byref(sh), 1, 64, -1) == -1
+    with pytest.raises(dial_b200.DialError, match="exceeds the block table"):
+        kv4._max_len(sh, 64 * 16 + 1)
+
+
 def test_python_checks_name_the_tensor():
     c = Cache(1, 2, 64, 4, 2)
     cache, table = c.device("cpu")

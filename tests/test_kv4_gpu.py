@@ -658,6 +658,13 @@ def test_evict_twice_and_the_same_bits(cuda):
         assert all(torch.equal(a, b) for a, b in zip(r, runs[0]))
 
 
+def test_sequences_without_queries(cuda):
+    """max_q 0, and sequences whose rows are all spare."""
+    c = Cache(50, 2, 60, 8, 2)
+    check_attention(c, cuda, [(0, 40, 0), (1, 0, 0)], spare_rows=3)
+    check_attention(c, cuda, [(0, 40, 0), (1, 33, 0)], spare_rows=3, max_q=5, weights=False)
+
+
 def test_empty_calls(cuda):
     from dial_b200 import kv4
 
