@@ -23,6 +23,10 @@ size_t rows_part(int q_heads, long long rows) {
   return (kv4_prefill_scratch(q_heads, rows, true) + 127) & ~static_cast<size_t>(127);
 }
 
+// The caller's scratch starts on a 16-byte boundary, what is laid out in it on this
+// one: the tensor-core kernel stores its parts 32 bytes at a time.
+constexpr size_t kScratchAlign = 128;
+
 cudaError_t launch(const Kv4AttnArgs& a, int act, cudaStream_t s) {
   if (a.max_q * (a.c.q_heads / a.c.kv_heads) <= kFewCols) return kv4_decode_launch(a, act, s);
   const cudaError_t e = kv4_prefill_launch(a, act, s);
@@ -47,12 +51,14 @@ extern "C" int64_t dial_b200_kv4_attention_scratch_bytes(const dial_b200_kv4_sha
   // enough for every call within the sizes, whichever kernels it takes
   const int rep = sh->q_heads / sh->kv_heads;
   const int64_t few = max_q < kFewCols / rep ? max_q : kFewCols / rep;
-  const size_t a = kv4_decode_scratch(sh->q_heads, sh->kv_heads, seqs, few, max_len, with_weights != 0);
-  if (max_q * rep <= kFewCols) return static_cast<int64_t>(a);
-  const size_t b = with_weights ? rows_part(sh->q_heads, rows) +
-                                      kv4_colsum_scratch(sh->q_heads, sh->kv_heads, seqs, max_q, max_len)
-                                : kv4_prefill_scratch(sh->q_heads, rows, false);
-  return static_cast<int64_t>(a > b ? a : b);
+  size_t bytes = kv4_decode_scratch(sh->q_heads, sh->kv_heads, seqs, few, max_len, with_weights != 0);
+  if (max_q * rep > kFewCols) {
+    const size_t many = with_weights ? rows_part(sh->q_heads, rows) +
+                                           kv4_colsum_scratch(sh->q_heads, sh->kv_heads, seqs, max_q, max_len)
+                                     : kv4_prefill_scratch(sh->q_heads, rows, false);
+    bytes = bytes > many ? bytes : many;
+  }
+  return static_cast<int64_t>(bytes > 0 ? bytes + kScratchAlign - 16 : 0);
 }
 
 extern "C" int dial_b200_kv4_attention(const dial_b200_kv4_shape* sh, const void* q, int64_t q_ld,
@@ -96,7 +102,8 @@ extern "C" int dial_b200_kv4_attention(const dial_b200_kv4_shape* sh, const void
   a.lens = lens;
   a.q_starts = q_starts;
   a.out = out;
-  a.scratch = scratch;
+  a.scratch = reinterpret_cast<void*>((reinterpret_cast<uintptr_t>(scratch) + kScratchAlign - 1) &
+                                      ~static_cast<uintptr_t>(kScratchAlign - 1));
   a.q_ld = q_ld;
   a.out_ld = out_ld;
   a.seqs = static_cast<int>(seqs);
