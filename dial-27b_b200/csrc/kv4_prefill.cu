@@ -737,8 +737,9 @@ __global__ void __launch_bounds__(256) kv4_prefill_join_kernel(const PrefillArgs
   for (int p = 0; p < parts; ++p) M = fmaxf(M, d.part_ml[slot(p)].x);
   for (int p = 0; p < parts; ++p) {
     const float2 ml = d.part_ml[slot(p)];
-    if (ml.x == -INFINITY) continue;
-    const float f = ex2(ml.x - M);
+    if (ml.x == -INFINITY && ml.y == 0.f) continue;  // the row sees nothing there
+    // scores that are all NaN leave no maximum, but a sum
+    const float f = ml.x == -INFINITY ? 1.f : ex2(ml.x - M);
     const float4 v = reinterpret_cast<const float4*>(d.part_o)[slot(p) * (kHeadDim / 4) + lane];
     L = fmaf(f, ml.y, L);
     O.x = fmaf(f, v.x, O.x);

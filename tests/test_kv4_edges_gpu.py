@@ -53,3 +53,47 @@ def test_scratch_on_every_sixteen_byte_boundary(cuda, queries, weights):
         got = call(buf[start:start + n])
         assert all(torch.equal(x, y) for x, y in zip(got, want)), start
         assert (buf[:start] == 0xA5).all() and (buf[start + n:] == 0xA5).all(), start
+
+
+# ------------------------------------------------- queries that are not finite
+@pytest.mark.parametrize("lens,queries", [((40, 33), (5, 2)), ((2600, 90), (200, 90)), ((2600, 1500), (1, 5)),
+                                          ((300, 20), (60, 17)), ((1100, 1024), (12, 1))])
+@pytest.mark.parametrize("dt", [BF16, F16])
+def test_queries_of_nan_and_infinity(cuda, lens, queries, dt):
+    """A query head with a NaN gives NaN wherever it sees a slot, whole or cut over
+    the GPU, in out and in the weights of the slots it sees; one with an infinity
+    NaN in out; neither reaches another query, head, or a slot it does not see."""
+    from dial_b200 import kv4
+
+    c = Cache(62, 2, max(lens), 8, 2, dt=dt)
+    cache, table = c.device(cuda)
+    q = torch.randn(sum(queries), 8 * DIM, device=cuda).to(dt)
+    clean = host(q)
+    bad = [(0, 1, float("nan")), (queries[0] - 1, 6, float("nan")), (sum(queries) - 1, 3, float("inf")),
+           (sum(queries) - 1, 4, float("-inf"))]
+    want = np.zeros((sum(queries), 8), bool)
+    for row, head, value in bad:
+        q[row, head * DIM + 5] = value
+        want[row, head] = True
+    before = host(cache.weights)
+    out = kv4.kv4_attention(c.sh, cache, q, table, i32(cuda, 0, 1), i32(cuda, *lens), max(lens),
+                            q_starts=i32(cuda, 0, queries[0], sum(queries)), max_q=max(queries),
+                            accumulate=True)
+    out, w = host(out).reshape(-1, 8, DIM), host(cache.weights)
+    np.testing.assert_array_equal(np.isnan(out), np.broadcast_to(want[..., None], out.shape))
+    at = 0
+    for s, (n, m) in enumerate(zip(lens, queries)):
+        o, b, sums, sb = c.attend(clean[at:at + m], s, n)
+        fine = ~want[at:at + m]
+        d = np.abs(out[at:at + m] - o.reshape(m, 8, DIM))[fine]
+        assert (d <= b.reshape(m, 8, DIM)[fine]).all()
+        if s == 0:
+            nan = np.zeros((n, 2), bool)
+            for row, head, value in bad[:2]:
+                nan[:max(0, n - m + 1 + row), head // 4] = True
+            blk, off = c.at(0, n)
+            got, old = w[blk, :, off], before[blk, :, off]
+            np.testing.assert_array_equal(np.isnan(got), nan)
+            d, lim = np.abs(got - old - sums), sb + 2.0 ** -23 * (2 * np.abs(old) + sums)
+            assert (d <= lim)[~nan].all()
+        at += m
