@@ -443,9 +443,7 @@ __global__ void __launch_bounds__(kWarpsOf<NT> * 32, kCtasPerSm<NT>)
       for (int e = 0; e < 32; ++e) top = fmaxf(top, fabsf(qv[e]));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      // 2^-e of the row's largest exponent: the f16 copy is exact for values down
-      // to 2^-14 of it, and off by at most 2^-25 of it below
-      const int ex = min(max(static_cast<int>(__float_as_uint(top) >> 23) - 127, -100), 100);
+      const int ex = query_exp(top);
       const float down = exp2i(-ex);
 #pragma unroll
       for (int e = 0; e < 16; ++e) qf[nt][e] = pack_f16(qv[2 * e] * down, qv[2 * e + 1] * down);

@@ -55,6 +55,13 @@ __device__ __forceinline__ float quotient(float x, float s, float y) {
   return fabsf(q) < 1e30f ? fmaf(fmaf(-q, s, x), y, q) : __fdiv_rn(x, s);
 }
 
+// Queries enter the MMAs as f16 after 2^-e, e the exponent of the row's largest value
+// `top` (within f32's normal powers): exact for values down to 2^-14 of it, and off by
+// at most 2^-25 of it below.
+__device__ __forceinline__ int query_exp(float top) {
+  return min(max(static_cast<int>(__float_as_uint(top) >> 23) - 127, -126), 126);
+}
+
 // A sequence of an attention call: its session, slots, first row and rows.
 struct Kv4Seq {
   int sid, len, row0, n;

@@ -349,8 +349,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const PrefillA
         if (!fetched) fetch_q(w);
         cp_async_wait();
         __syncwarp();
-        // f16 after 2^-e of the row's largest exponent: exact for values down to
-        // 2^-14 of it, and off by at most 2^-25 of it below
+        // to f16 (query_exp)
         float top = 0.f;
 #pragma unroll 2
         for (int e = 0; e < 16; ++e) {
@@ -359,7 +358,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const PrefillA
 #pragma unroll
           for (int u = 0; u < 8; ++u) top = fmaxf(top, fabsf(ActTraits<Act>::to_f(v[u])));
         }
-        const int ex = min(max(static_cast<int>(__float_as_uint(top) >> 23) - 127, -100), 100);
+        const int ex = query_exp(top);
         const float down = exp2i(-ex);
         fac = exp2i(ex) * a.scale * a.c.k_scale * 1.4426950408889634f;
         const bool keep_q = d.off && live && begin == 0;

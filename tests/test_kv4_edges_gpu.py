@@ -97,3 +97,27 @@ def test_queries_of_nan_and_infinity(cuda, lens, queries, dt):
             d, lim = np.abs(got - old - sums), sb + 2.0 ** -23 * (2 * np.abs(old) + sums)
             assert (d <= lim)[~nan].all()
         at += m
+
+
+# ---------------------------------------------------------- ends of the range
+@pytest.mark.parametrize("power", [100, 116, 125, -110])
+@pytest.mark.parametrize("queries,n", [(1, 900), (5, 1300), (70, 700)])
+def test_queries_near_the_ends_of_bf16(cuda, power, queries, n):
+    """Finite queries up to 2^127 and down to 2^-112, with a softmax scale that brings
+    their scores back: as for ordinary ones."""
+    from dial_b200 import kv4
+
+    c = Cache(63, 1, n, 8, 2)
+    scale = float(np.float32(2.0 ** (-power if power > 0 else 99) * DIM ** -0.5))
+    sh = kv4.make_shape(8, 2, c.max_blocks, c.pages.shape[0], k_scale=c.k_scale, v_scale=c.v_scale,
+                        softmax_scale=scale)
+    cache, table = c.device(cuda)
+    q = (torch.randn(queries, 8 * DIM, device=cuda).clamp(-3.9, 3.9).double() * 2.0 ** power).to(BF16)
+    before = host(cache.weights)
+    out = kv4.kv4_attention(sh, cache, q, table, i32(cuda, 0), i32(cuda, n), n, q_starts=i32(cuda, 0, queries),
+                            max_q=queries, accumulate=True)
+    o, b, s, sb = c.attend(host(q), 0, n, scale)
+    assert np.isfinite(b).all() and (np.abs(host(out) - o) <= b).all()
+    blk, off = c.at(0, n)
+    d = np.abs(host(cache.weights)[blk, :, off] - before[blk, :, off] - s)
+    assert (d <= sb + 2.0 ** -23 * (2 * before[blk, :, off] + s)).all()
