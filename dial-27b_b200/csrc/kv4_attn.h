@@ -15,7 +15,10 @@ struct Kv4AttnArgs {
   void* scratch;
   long long q_ld, out_ld;
   int seqs, rows, max_q, max_len;
-  float scale;
+  // unit 2^unit_exp = softmax_scale k_scale log2(e), unit in [1/2, 1]: from q . k of the
+  // codes and e4m3 scales to base-2 scores
+  float unit;
+  int unit_exp;
 };
 
 // Few queries a sequence: mma.sync, the cache streamed once for up to 16

@@ -447,7 +447,7 @@ __global__ void __launch_bounds__(kWarpsOf<NT> * 32, kCtasPerSm<NT>)
       const float down = exp2i(-ex);
 #pragma unroll
       for (int e = 0; e < 16; ++e) qf[nt][e] = pack_f16(qv[2 * e] * down, qv[2 * e + 1] * down);
-      const float mine_f = exp2i(ex) * a.scale * a.c.k_scale * 1.4426950408889634f;
+      const float mine_f = score_scale(a, ex);
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         fac[nt][e] = __shfl_sync(0xffffffffu, mine_f, (2 * c + e) * 4);

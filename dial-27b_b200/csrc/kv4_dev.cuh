@@ -61,6 +61,11 @@ __device__ __forceinline__ float quotient(float x, float s, float y) {
 __device__ __forceinline__ int query_exp(float top) {
   return min(max(static_cast<int>(__float_as_uint(top) >> 23) - 127, -126), 126);
 }
+// What such a row's sums are multiplied by to become base-2 scores.  Kept within f32's
+// normal numbers, so that a masked score, -inf, stays -inf under any scale.
+__device__ __forceinline__ float score_scale(const Kv4AttnArgs& a, int e) {
+  return a.unit * exp2i(min(max(e + a.unit_exp, -125), 127));
+}
 
 // A sequence of an attention call: its session, slots, first row and rows.
 struct Kv4Seq {

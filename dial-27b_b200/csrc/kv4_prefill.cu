@@ -360,7 +360,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const PrefillA
         }
         const int ex = query_exp(top);
         const float down = exp2i(-ex);
-        fac = exp2i(ex) * a.scale * a.c.k_scale * 1.4426950408889634f;
+        fac = score_scale(a, ex);
         const bool keep_q = d.off && live && begin == 0;
 #pragma unroll 2
         for (int e = 0; e < 16; ++e) {

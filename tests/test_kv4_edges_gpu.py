@@ -121,3 +121,25 @@ def test_queries_near_the_ends_of_bf16(cuda, power, queries, n):
     blk, off = c.at(0, n)
     d = np.abs(host(cache.weights)[blk, :, off] - before[blk, :, off] - s)
     assert (d <= sb + 2.0 ** -23 * (2 * before[blk, :, off] + s)).all()
+
+
+@pytest.mark.parametrize("queries", [3, 60])
+def test_scales_that_leave_nothing_of_a_score(cuda, queries):
+    """Zero queries and ordinary ones under a scale of 1e-30: every slot that a query
+    sees has the same weight, the others none."""
+    from dial_b200 import kv4
+
+    c = Cache(64, 1, 200, 8, 2)
+    sh = kv4.make_shape(8, 2, c.max_blocks, c.pages.shape[0], k_scale=c.k_scale, v_scale=c.v_scale,
+                        softmax_scale=1e-30)
+    cache, table = c.device(cuda)
+    q = torch.randn(queries, 8 * DIM, device=cuda).to(BF16)
+    q[1] = 0
+    before = host(cache.weights)
+    out = kv4.kv4_attention(sh, cache, q, table, i32(cuda, 0), i32(cuda, 200), 200,
+                            q_starts=i32(cuda, 0, queries), max_q=queries, accumulate=True)
+    o, b, s, sb = c.attend(host(q), 0, 200, float(np.float32(1e-30)))
+    assert (np.abs(host(out) - o) <= b).all()
+    blk, off = c.at(0, 200)
+    d = np.abs(host(cache.weights)[blk, :, off] - before[blk, :, off] - s)
+    assert (d <= sb + 2.0 ** -23 * (2 * before[blk, :, off] + s)).all()
