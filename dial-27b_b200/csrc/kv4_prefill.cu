@@ -550,6 +550,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const PrefillA
           d.desc[b] = w.j0 == 0 && w.j1 < w.nb ? make_int4(w.i, w.h, w.tp, first) : make_int4(-1, 0, 0, first);
         break;
       }
+      __syncwarp();  // every lane has read *cur, which takes the item after the next one
       Share* was = cur;
       cur = next;
       next = was;

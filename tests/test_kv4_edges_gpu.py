@@ -143,3 +143,28 @@ def test_scales_that_leave_nothing_of_a_score(cuda, queries):
     blk, off = c.at(0, 200)
     d = np.abs(host(cache.weights)[blk, :, off] - before[blk, :, off] - s)
     assert (d <= sb + 2.0 ** -23 * (2 * before[blk, :, off] + s)).all()
+
+
+# ------------------------------------------------------- items of one tile
+def test_items_without_blocks_in_a_tile(cuda):
+    """Sequences of one tile of rows, of two, and of two of which the first sees no
+    slot, in turn and several to a CTA: each item's results go to its own rows."""
+    from dial_b200 import kv4
+
+    c = Cache(66, 40, 502, 32, 8)
+    seqs = [((330, 33), (270, 14), (20, 60), (499, 17))[i % 4] for i in range(40)]
+    seqs = [(n + i % 4, m) for i, (n, m) in enumerate(seqs)]
+    cache, table = c.device(cuda)
+    starts = np.cumsum([0] + [m for _, m in seqs])
+    q = torch.randn(int(starts[-1]), 32 * DIM, device=cuda).to(BF16)
+    before = host(cache.weights)
+    out = host(kv4.kv4_attention(c.sh, cache, q, table, torch.arange(40, dtype=torch.int32, device=cuda),
+                                 i32(cuda, *[n for n, _ in seqs]), 502, q_starts=i32(cuda, *starts.tolist()),
+                                 max_q=60, accumulate=True))
+    w = host(cache.weights)
+    for i, (n, m) in enumerate(seqs):
+        o, b, s, sb = c.attend(host(q[starts[i]:starts[i + 1]]), i, n)
+        assert (np.abs(out[starts[i]:starts[i + 1]] - o) <= b).all(), i
+        blk, off = c.at(i, n)
+        d = np.abs(w[blk, :, off] - before[blk, :, off] - s)
+        assert (d <= sb + 2.0 ** -23 * (2 * before[blk, :, off] + s)).all(), i
