@@ -13,11 +13,12 @@
 //                conversion, which then gives the operand's token pairs.
 // e2m1 times e4m3 is exact in f16 (6 significant bits, 2^-10 .. 2688), so K and V
 // enter the MMA as the values the cache stands for; queries enter as f16 after
-// an exact power-of-two scale, P as f16 (2^-11 relative), and scores, sums and
+// an exact power-of-two scale, P as f16 (2^-11 relative, for the rate of its MMA, and
+// lifted by 2^7 so that a long tail of small ones counts), and scores, sums and
 // accumulators are f32.  Columns are (query, head of the group) pairs, so the
 // 8 columns of an MMA cost the same for 1 and for 8.
-// The softmax reference m moves only when a score exceeds it by 2^8, found by
-// one vote a page instead of a shuffle tree.
+// The softmax reference m moves only when a score exceeds the one it was set by by more
+// than 8 (base 2), found by one vote a page instead of a shuffle tree.
 //
 // Work split: the pages of all (sequence, kv head) segments laid end to end and
 // cut into ranges of equal cost, one a CTA, so ragged lengths balance; the pages of a
@@ -60,7 +61,10 @@ constexpr int kSeqChunk = 256;     // sequences a launch
 constexpr int kSegPad = 20;
 constexpr int kInfo = 6;           // sequences of a range kept in shared memory
 constexpr int kOneLen = 1024;      // slots up to which a CTA takes a whole segment
-constexpr float kRaise = 8.f;      // log2 headroom of a probability above 1
+// Probabilities are taken against a reference kLift below the largest score, base 2:
+// f16 keeps them to 2^-32 of the largest, and the f32 sums lose more over as many slots.
+// The reference moves when one would exceed 2^kTop.
+constexpr float kLift = 7.f, kTop = 15.f;
 constexpr int kColStride = kHeadDim + 8;
 
 // A range's share of a segment, for its weights.
@@ -540,7 +544,7 @@ __global__ void __launch_bounds__(kWarpsOf<NT> * 32, kCtasPerSm<NT>)
             }
         }
       }
-      // `high` is (m + kRaise) / fac: the vote needs no scaled scores
+      // m is the reference, `high` (m + kTop) / fac: the vote needs no scaled scores
       float top[NT][2];
       bool raise = false;
 #pragma unroll
@@ -560,11 +564,11 @@ __global__ void __launch_bounds__(kWarpsOf<NT> * 32, kCtasPerSm<NT>)
             float t = top[nt][e];
 #pragma unroll
             for (int i = 4; i < 32; i <<= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, i));
-            const float mn = fmaxf(m[nt][e], t * fac[nt][e]);
+            const float mn = fmaxf(m[nt][e], t * fac[nt][e] - kLift);
             const float al = m[nt][e] == -INFINITY ? 0.f : ex2(m[nt][e] - mn);
             m[nt][e] = mn;
             ref[nt][e] = mn == -INFINITY ? 0.f : mn;
-            high[nt][e] = __fdiv_rn(mn + kRaise, fac[nt][e]);
+            high[nt][e] = __fdiv_rn(mn + kTop, fac[nt][e]);
             l[nt][e] *= al;
 #pragma unroll
             for (int mt = 0; mt < 8; ++mt) {

@@ -13,8 +13,10 @@
 // P (f16) takes the first 64 of its own S's 128 columns, 32 for each half of the
 // keys, once the scores there are read.  S_t of block j + 1 is issued right after P V
 // of block j, so one tile's softmax runs beside the other's MMAs.
-// The exponent's reference moves only when a score exceeds it by 2^8: a block is
-// taken in one pass, without its maximum first, and O in TMEM is rarely rescaled.
+// The exponent's reference moves only when a score exceeds the one it was set by by more
+// than 8 (base 2): a block is taken in one pass, without its maximum first, and O in
+// TMEM is rarely rescaled.  P is f16 (2^-11 relative), which its MMA's rate asks for; scores,
+// sums and O are f32.
 // A block goes in halves of 64 keys, so that the first half's P is stored beside the
 // second's work (332 us against 363 for the 512-token chunk); code that runs once
 // an item is kept in rolled loops, since its instructions are fetched anew each time
@@ -51,7 +53,10 @@ constexpr int kOffQ = 0;                    // [2]
 constexpr int kOffK = 2 * kTile;            // [2]
 constexpr int kOffV = 4 * kTile;            // [2]
 constexpr int kOffMisc = 6 * kTile;
-constexpr float kRaise = 8.f;               // log2 headroom of a probability above 1
+// Probabilities are taken against a reference kLift below a row's largest score, base 2:
+// f16 keeps them to 2^-32 of the largest, and the f32 sums lose more over as many slots.
+// The reference moves when one would exceed 2^kTop.
+constexpr float kLift = 7.f, kTop = 15.f;
 constexpr int kStatusKv4Prefill = 0x601;
 
 struct Misc {
@@ -405,8 +410,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const PrefillA
         }
         // a half of the block after the other: the probabilities under the reference
         // so far, 16 scores at a time, the load of one chunk beside the work on the
-        // other; where one would exceed 2^kRaise the reference moves to the row's
-        // maximum and the half is done again.  References are whole numbers, so that
+        // other; where one would exceed 2^kTop the reference moves to kLift below the
+        // row's maximum and the half is done again.  References are whole numbers, so that
         // what is rescaled (sums, O, the P of the half before) stays exact.
 #pragma unroll 1
         for (int hf = 0; hf < 2; ++hf) {
@@ -446,8 +451,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const PrefillA
             top = fmaxf(t0, t1);
           };
           probs();
-          if (__any_sync(0xffffffffu, top > kRaise || (m == -INFINITY && top > -INFINITY))) {
-            const float mn = fmaxf(m, ceilf(top + ref));
+          if (__any_sync(0xffffffffu, top > kTop || (m == -INFINITY && top > -INFINITY))) {
+            const float mn = fmaxf(m, ceilf(top + ref) - kLift);
             const float al = m == -INFINITY ? 0.f : ex2(m - mn);
             m = mn;
             ref = mn == -INFINITY ? 0.f : mn;

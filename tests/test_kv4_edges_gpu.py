@@ -168,3 +168,48 @@ def test_items_without_blocks_in_a_tile(cuda):
         blk, off = c.at(i, n)
         d = np.abs(w[blk, :, off] - before[blk, :, off] - s)
         assert (d <= sb + 2.0 ** -23 * (2 * before[blk, :, off] + s)).all(), i
+
+
+# ------------------------------------------------------------ long flat tails
+@pytest.mark.parametrize("sessions,n,heads,queries,tops", [(37, 1 << 20, (8, 8), 1, 8),
+                                                           (1, 1 << 17, (64, 8), 608, 1)])
+def test_a_long_tail_far_below_the_largest(cuda, sessions, n, heads, queries, tops):
+    """`tops` slots share the largest score (one for each warp that takes a share of a
+    sequence) and all others lie 2^-25.1 of it below: their sum counts, 0.4 % here,
+    whatever the length.  Values are -a for the first and a for the others, so that
+    out = a (T - 1) / (T + 1) with T the tail's sum.  Bound, on a (T + 1) / (T + 1) = a: f16
+    probabilities 2^-11; f32 sums: a warp or row takes 2^17 slots, 16 a step of the
+    product, each of the 2^13 partial sums off by 2^-23 at most (truncated), 2^-10, and l by
+    2^13 additions rounded to 2^-24, 2^-11; half a step of f16, 2^-11.  All sessions
+    read the same three pages."""
+    from dial_b200 import kv4
+    from kv4_case import PAGE, pack
+
+    q_heads, H = heads
+    blocks = n // PAGE
+    sh = kv4.make_shape(q_heads, H, blocks, 4, k_scale=0.5, v_scale=0.0625, softmax_scale=1.0, dtype=F16)
+    one = np.full((3, H, PAGE, 8), 0x38, np.uint8)  # scale 1
+    k = np.zeros((3, H, PAGE, DIM), np.uint8)
+    v = np.full((3, H, PAGE, DIM), 7, np.uint8)     # +6
+    k[1, :, 5, 0] = 7
+    v[1, :, 5] = 15                                 # -6
+    pages = np.zeros((4, H, 2304), np.uint8)
+    pages[:3] = pack(k, one, v, one)
+    table = torch.zeros(sessions, blocks, dtype=torch.int32, device=cuda)
+    table[:, :tops] = 1
+    cache = kv4.Kv4Cache(torch.from_numpy(pages).to(cuda))
+    t = np.float64(np.float16(25.1 * np.log(2) / 3))
+    q = torch.zeros(sessions * queries, q_heads, DIM, dtype=F16, device=cuda)
+    q[..., 0] = float(t)
+    out = kv4.kv4_attention(sh, cache, q.reshape(-1, q_heads * DIM), table,
+                            torch.arange(sessions, dtype=torch.int32, device=cuda),
+                            torch.full((sessions,), n, dtype=torch.int32, device=cuda), n,
+                            q_starts=i32(cuda, *range(0, sessions * queries + 1, queries)), max_q=queries)
+    seen = np.tile(n - queries + 1 + np.arange(queries), sessions)
+    tail = (seen - tops) * np.exp(-3 * t) / tops
+    a = 6 * 0.0625
+    want = (a * (tail - 1) / (tail + 1))[:, None]
+    assert tail.min() > 0.0035
+    d = np.abs(host(out) - want)
+    bound = a * (2.0 ** -11 + 2.0 ** -10 + 2.0 ** -11 + 2.0 ** -11)
+    assert (d <= bound).all(), (d.max(), bound)
