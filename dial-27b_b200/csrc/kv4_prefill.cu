@@ -412,7 +412,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const PrefillA
         // so far, 16 scores at a time, the load of one chunk beside the work on the
         // other; where one would exceed 2^kTop the reference moves to kLift below the
         // row's maximum and the half is done again.  References are whole numbers, so that
-        // what is rescaled (sums, O, the P of the half before) stays exact.
+        // sums and O are rescaled exactly, and the P of the half before to f16's smallest step.
 #pragma unroll 1
         for (int hf = 0; hf < 2; ++hf) {
           uint32_t p[32];
@@ -470,7 +470,6 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const PrefillA
               }
             }
             if (hf == 1) {
-              const uint32_t al2 = pack_f16(al, al);
               st_wait();
 #pragma unroll 1
               for (int cb = 0; cb < 2; ++cb) {
@@ -478,7 +477,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const PrefillA
                 ld16(tS + cb * 16, o);
                 ld_wait16(o);
 #pragma unroll
-                for (int e = 0; e < 16; ++e) o[e] = hmul2(o[e], al2);
+                for (int e = 0; e < 16; ++e) {
+                  const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&o[e]));
+                  o[e] = pack_f16(x.x * al, x.y * al);
+                }
                 __syncwarp();
                 st16(tS + cb * 16, o);
               }

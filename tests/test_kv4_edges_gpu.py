@@ -213,3 +213,38 @@ def test_a_long_tail_far_below_the_largest(cuda, sessions, n, heads, queries, to
     d = np.abs(host(out) - want)
     bound = a * (2.0 ** -11 + 2.0 ** -10 + 2.0 ** -11 + 2.0 ** -11)
     assert (d <= bound).all(), (d.max(), bound)
+
+
+def test_a_large_score_in_the_second_half_of_a_block(cuda):
+    """A block of 128 keys whose first 64 score 7.5 above the keys before (base 2) and
+    whose second half holds one of 27: the 64 add 2^-13.5 to its weight, twelve
+    times that to the values here.  Bound: half a step of f16, and 2^-16 of the largest value
+    for the rest: scores of 27 off by 2^-18.6 (the f32 scale and the exponential), sums
+    of 300 terms; probabilities in f16 are off by 2^-11 of that 2^-13.5.  Sessions
+    enough, all on the same pages, that CTAs take whole items."""
+    from dial_b200 import kv4
+
+    n, queries, sessions = 316, 60, 40
+    c = Cache(67, 1, n, 8, 8, dt=F16)
+    score = np.zeros(n)
+    score[128:192], score[192:256], score[222], score[256:] = 7.5, -39.0, 27.0, -39.0
+    for slot in range(n):
+        k, v = np.zeros((8, DIM)), np.full((8, DIM), 2.0 ** -5)
+        k[:, 0] = score[slot]
+        if 128 <= slot < 192:
+            v[:] = 0.375
+        c.put(0, slot, k, v, 0)
+    assert np.array_equal(c.values(0, n)[0][:, 7, 0], score)
+    sh = kv4.make_shape(8, 8, c.max_blocks, c.pages.shape[0], k_scale=c.k_scale, v_scale=c.v_scale,
+                        softmax_scale=float(np.float32(np.log(2))), dtype=F16)
+    cache, table = c.device(cuda)
+    q = torch.zeros(sessions * queries, 8 * DIM, dtype=F16, device=cuda)
+    q[:, ::DIM] = 1
+    out = host(kv4.kv4_attention(sh, cache, q, table.expand(sessions, -1).contiguous(),
+                                 torch.arange(sessions, dtype=torch.int32, device=cuda),
+                                 i32(cuda, *[n] * sessions), n,
+                                 q_starts=i32(cuda, *range(0, sessions * queries + 1, queries)),
+                                 max_q=queries)).reshape(sessions, queries, -1)
+    want = c.attend(host(q[:queries]), 0, n, float(np.float32(np.log(2))))[0]
+    d = np.abs(out - want)
+    assert (d <= 2.0 ** -11 * np.abs(want) + 2.0 ** -16 * 0.375).all(), d.max()
