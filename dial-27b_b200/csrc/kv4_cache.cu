@@ -272,8 +272,8 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const ReadArgs a) {
     const int sid = a.sids[i];
     const long long slot = (a.first ? a.first[i] : 0) + static_cast<long long>(row - i * a.count);
     there[e] = write[e] && slot >= 0 && slot < a.lens[i];
-    if (there[e] && (static_cast<unsigned>(sid) >= static_cast<unsigned>(a.c.sessions) ||
-                     slot >= static_cast<long long>(a.c.max_blocks) * kPageTokens)) {
+    if (write[e] && (static_cast<unsigned>(sid) >= static_cast<unsigned>(a.c.sessions) ||
+                     (there[e] && slot >= static_cast<long long>(a.c.max_blocks) * kPageTokens))) {
       if (lane == 0) set_status(a.c.status, kStatusBadArgs);
       write[e] = there[e] = false;
     }

@@ -248,3 +248,31 @@ def test_a_large_score_in_the_second_half_of_a_block(cuda):
     want = c.attend(host(q[:queries]), 0, n, float(np.float32(np.log(2))))[0]
     d = np.abs(out - want)
     assert (d <= 2.0 ** -11 * np.abs(want) + 2.0 ** -16 * 0.375).all(), d.max()
+
+
+# -------------------------------------------------------------- bad sequences
+def test_read_leaves_bad_sessions_out(cuda):
+    """Sequences of no session: reported, and their rows stay as they were, those past
+    their length among them."""
+    import ctypes as C
+
+    import dial_b200
+    from dial_b200 import _abi
+
+    c = Cache(65, 2, 64, 4, 2)
+    cache, table = c.device(cuda)
+    k = torch.full((4, 5, 2, DIM), 3.0, dtype=BF16, device=cuda)
+    v = torch.full_like(k, 4.0)
+    sids, lens = i32(cuda, 1, 2, -1, 0), i32(cuda, 3, 2, 0, 64)
+    _abi.call("dial_b200_kv4_read", C.byref(c.sh), cache.pages.data_ptr(), table.data_ptr(), 2, sids.data_ptr(),
+              None, lens.data_ptr(), 4, 5, k.data_ptr(), v.data_ptr(),
+              torch.cuda.current_stream(cuda).cuda_stream)
+    torch.cuda.synchronize()
+    assert dial_b200.device_status(clear=True) == 0x104
+    assert (k[1:3] == 3.0).all() and (v[1:3] == 4.0).all()
+    assert (k[0, 3:] == 0).all() and (v[0, 3:] == 0).all()
+    for i, (sid, n) in ((0, (1, 3)), (3, (0, 5))):
+        kk, vv = c.values(sid, n)
+        want = torch.from_numpy(kk.astype(np.float32)).to(BF16)
+        assert torch.equal(k[i, :n].cpu(), want)
+        assert torch.equal(v[i, :n].cpu(), torch.from_numpy(vv.astype(np.float32)).to(BF16))
