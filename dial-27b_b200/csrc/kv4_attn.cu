@@ -93,6 +93,7 @@ extern "C" int dial_b200_kv4_attention(const dial_b200_kv4_shape* sh, const void
       (reinterpret_cast<uintptr_t>(q) & 15) != 0 || (reinterpret_cast<uintptr_t>(out) & 15) != 0)
     return kv4_fail(err, n, DIAL_ERR_INVALID,
                     "q and out rows must hold q_heads heads and start on 16-byte boundaries");
+  if (!q_starts) max_q = 1;  // row i is sequence i's
   if (seqs == 0 || rows == 0 || max_q == 0) return DIAL_OK;
   if (dial_b200_kv4_attention_scratch_bytes(sh, seqs, rows, max_q, max_len, weights != nullptr) > 0 &&
       (!scratch || (reinterpret_cast<uintptr_t>(scratch) & 15) != 0))
@@ -108,7 +109,7 @@ extern "C" int dial_b200_kv4_attention(const dial_b200_kv4_shape* sh, const void
   a.out_ld = out_ld;
   a.seqs = static_cast<int>(seqs);
   a.rows = static_cast<int>(rows);
-  a.max_q = static_cast<int>(q_starts ? max_q : 1);
+  a.max_q = static_cast<int>(max_q);
   a.max_len = static_cast<int>(max_len);
   const float scale = sh->softmax_scale > 0.f ? sh->softmax_scale : 1.f / sqrtf(static_cast<float>(kHeadDim));
   a.unit = static_cast<float>(frexp(1.4426950408889634 * scale * sh->k_scale, &a.unit_exp));

@@ -198,8 +198,8 @@ def kv4_attention(sh: Kv4Shape, cache: Kv4Cache, q, block_table, sids, lens, max
     """Attention of q [rows, q_heads * 128] over the cached slots, causal at the
     end of each sequence: sequence i's queries are rows q_starts[i] ..
     q_starts[i + 1] - 1 (default: row i), the last of them sees slots 0 ..
-    lens[i] - 1 of session sids[i].  max_q and max_len bound the queries and
-    slots of a sequence.  accumulate adds each slot's probabilities to
+    lens[i] - 1 of session sids[i].  max_q (with q_starts) and max_len bound the
+    queries and slots of a sequence.  accumulate adds each slot's probabilities to
     cache.weights.  Returns out [rows, q_heads * 128]."""
     idx, dt, i32 = q.get_device(), _DTYPE[sh.act], torch.int32
     H, rows, n, width = sh.kv_heads, q.size(0), sids.numel(), sh.q_heads * HEAD_DIM
@@ -217,6 +217,8 @@ def kv4_attention(sh: Kv4Shape, cache: Kv4Cache, q, block_table, sids, lens, max
             _bad("accumulate needs a cache with weights")
     p_bt, sessions = _table("block_table", block_table, sh.max_blocks, idx)
     _max_len(sh, max_len)
+    if q_starts is None:
+        max_q = 1
     p_s, keep = _scratch(scratch, attention_scratch_bytes(sh, n, rows, max_q, max_len, accumulate), q)
     _launch("dial_b200_kv4_attention", idx, C.byref(sh), p_q, ld,
             _need("pages", cache.pages, torch.uint8, slabs * SLAB_BYTES, idx), p_w, p_bt,

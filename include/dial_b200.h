@@ -267,9 +267,9 @@ int64_t dial_b200_kv4_attention_scratch_bytes(const dial_b200_kv4_shape* sh, int
  *   over the sequence's queries and the query heads of the kv head.  Sequences
  *   must then name distinct sessions that share no page (a sum is one load and
  *   one store).
- * max_q and max_len bound n and lens[i] (host); rows no sequence names are left as
- * they were; out must not overlap q.  `scratch` needs no preparation; two calls that may run at the
- * same time need two. */
+ * max_q and max_len bound n and lens[i] (host; max_q counts with q_starts only, n is 1
+ * without); rows no sequence names are left as they were; out must not overlap q.
+ * `scratch` needs no preparation; two calls that may run at the same time need two. */
 int dial_b200_kv4_attention(const dial_b200_kv4_shape* sh, const void* q, int64_t q_ld,
                             const void* pages, float* weights, const int32_t* block_table,
                             int64_t sessions, const int32_t* sids, const int32_t* lens,

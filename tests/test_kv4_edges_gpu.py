@@ -276,3 +276,18 @@ def test_read_leaves_bad_sessions_out(cuda):
         want = torch.from_numpy(kk.astype(np.float32)).to(BF16)
         assert torch.equal(k[i, :n].cpu(), want)
         assert torch.equal(v[i, :n].cpu(), torch.from_numpy(vv.astype(np.float32)).to(BF16))
+
+
+# -------------------------------------------------------------- arguments
+def test_single_queries_take_no_max_q(cuda):
+    """Without q_starts, max_q is not looked at."""
+    from dial_b200 import kv4
+
+    c = Cache(68, 2, 1200, 8, 2)
+    cache, table = c.device(cuda)
+    q = torch.randn(2, 8 * DIM, device=cuda).to(BF16)
+    args = (c.sh, cache, q, table, i32(cuda, 0, 1), i32(cuda, 1200, 37), 1200)
+    want = kv4.kv4_attention(*args)
+    for max_q in (0, 9, 100):
+        out = torch.full_like(q, 5.0)
+        assert torch.equal(kv4.kv4_attention(*args, max_q=max_q, out=out), want)
