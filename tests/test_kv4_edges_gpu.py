@@ -8,6 +8,7 @@ import pytest
 import torch
 
 from kv4_case import DIM, Cache, i32
+from test_kv4_gpu import check_attention
 
 pytestmark = pytest.mark.gpu
 BF16, F16 = torch.bfloat16, torch.float16
@@ -291,3 +292,43 @@ def test_single_queries_take_no_max_q(cuda):
     for max_q in (0, 9, 100):
         out = torch.full_like(q, 5.0)
         assert torch.equal(kv4.kv4_attention(*args, max_q=max_q, out=out), want)
+
+
+# ------------------------------------------------------------ the rarer paths
+@pytest.mark.parametrize("n,queries,heads,dt", [
+    (1200, 1100, (8, 1), BF16),   # 69 tiles of rows: items of three chunks, 35 pairs of tiles
+    (3000, 700, (16, 2), F16),    # 44 tiles over twelve key blocks, as few see the last
+    (700, 40, (16, 1), F16), (300, 300, (16, 1), BF16),  # 16 heads a group
+    (900, 130, (8, 2), F16)])
+def test_prompts_with_weights(cuda, n, queries, heads, dt):
+    c = Cache(69, 3, n, *heads, dt=dt)
+    check_attention(c, cuda, [(2, n, queries), (0, min(n, 77), 5), (1, 33, 20)], spare_rows=1)
+
+
+@pytest.mark.parametrize("out_of_place", [False, True])
+def test_evict_of_a_session_past_shared_memory(cuda, out_of_place):
+    """More slots than a CTA keeps the keys of (24576), weights with many ties."""
+    from dial_b200 import kv4
+
+    n, keep, recent = 25003, 9001, 500
+    c = Cache(70, 1, n, 2, 2)
+    b, o = c.at(0, n)
+    for h in range(2):
+        c.positions[b, h, o] = np.cumsum(c.rng.integers(1, 3, n))
+    c.weights = np.round(c.weights * 8).astype(np.float32)
+    dst = c.table.copy()
+    if out_of_place:
+        kb, first = -(-keep // 16), c.sh.num_blocks
+        for x in ("pages", "weights", "positions"):
+            a = getattr(c, x)
+            setattr(c, x, np.concatenate([a, a[:1].repeat(kb, 0)]))
+        c.sh.num_blocks = first + kb
+        dst[:] = -1
+        dst[0, :kb] = np.arange(first, first + kb)
+    cache, table = c.device(cuda)
+    new = kv4.kv4_evict(c.sh, cache, table, i32(cuda, 0), i32(cuda, n), n, keep, recent,
+                        dst_table=torch.from_numpy(dst).to(cuda) if out_of_place else None)
+    assert host(new).tolist() == [c.evict(0, n, keep, recent, dst)]
+    np.testing.assert_array_equal(host(cache.pages), c.pages)
+    np.testing.assert_array_equal(host(cache.weights), c.weights)
+    np.testing.assert_array_equal(host(cache.positions), c.positions)
