@@ -45,7 +45,7 @@ extern "C" int64_t dial_b200_kv4_attention_scratch_bytes(const dial_b200_kv4_sha
                                                          int64_t max_len, int32_t with_weights) {
   if (!sh || sh->q_heads < 1 || sh->kv_heads < 1 || sh->kv_heads > 1024 || sh->q_heads % sh->kv_heads != 0 ||
       sh->q_heads / sh->kv_heads > 16 || seqs < 0 || seqs > 65535 || rows < 0 || rows > (1 << 26) || max_q < 0 ||
-      max_q > (1 << 24) || max_len < 0 || max_len > 16LL << 26)
+      max_q > (1 << 24) || max_len < 0 || max_len > 16LL << 26 || rows * sh->q_heads > INT32_MAX)
     return -1;
   if (seqs == 0 || rows == 0 || max_q == 0) return 0;  // the call does nothing
   // enough for every call within the sizes, whichever kernels it takes

@@ -298,7 +298,7 @@ using namespace dialb200;
 extern "C" int64_t dial_b200_kv4_evict_scratch_bytes(const dial_b200_kv4_shape* sh, int64_t seqs,
                                                      int64_t max_len, int64_t keep) {
   if (!sh || sh->kv_heads < 1 || sh->kv_heads > 1024 || seqs < 0 || seqs > 65535 || max_len < 0 ||
-      max_len > 16LL << 26 || keep < 0)
+      max_len > 16LL << 26 || keep < 0 || keep > INT32_MAX)
     return -1;
   const int64_t most = keep < max_len ? keep : max_len;
   return seqs * sh->kv_heads * (2 + 2 * most) * 4 + 16;

@@ -253,7 +253,7 @@ int dial_b200_kv4_read(const dial_b200_kv4_shape* sh, const void* pages,
                        void* k_out, void* v_out, void* stream, char* err, size_t err_size);
 
 /* Scratch of dial_b200_kv4_attention for calls of at most these sizes; -1 for sizes
- * that it refuses. */
+ * that it refuses whatever the block table. */
 int64_t dial_b200_kv4_attention_scratch_bytes(const dial_b200_kv4_shape* sh, int64_t seqs,
                                               int64_t rows, int64_t max_q, int64_t max_len,
                                               int32_t with_weights);
@@ -278,7 +278,7 @@ int dial_b200_kv4_attention(const dial_b200_kv4_shape* sh, const void* q, int64_
                             void* stream, char* err, size_t err_size);
 
 /* Scratch of dial_b200_kv4_evict for calls of at most these sizes; -1 for sizes that
- * it refuses. */
+ * it refuses whatever the block table. */
 int64_t dial_b200_kv4_evict_scratch_bytes(const dial_b200_kv4_shape* sh, int64_t seqs,
                                           int64_t max_len, int64_t keep);
 
