@@ -91,7 +91,7 @@ def _rows(name: str, t, dtype, rows, width: int, idx: int):
     if (t.dtype is dtype and t.dim() == 2 and t.size(1) == width
             and (rows is None or t.size(0) == rows) and t.stride(1) == 1
             and t.get_device() == idx):
-        return t.data_ptr(), t.stride(0) if t.size(0) > 1 else max(t.stride(0), width)
+        return t.data_ptr(), t.stride(0) if t.size(0) > 1 else width
     _bad(f"{name}: expected {dtype} rows [{'rows' if rows is None else rows}, {width}] on device {idx}, "
          f"got {t.dtype} {tuple(t.shape)} strides {t.stride()} on {t.device}")
 

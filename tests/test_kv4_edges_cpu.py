@@ -2,6 +2,8 @@
 
 import ctypes as C
 
+import torch
+
 from dial_b200 import _abi, kv4
 from test_kv4_cpu import ATTN, EVICT, refused, shape
 
@@ -28,3 +30,12 @@ def test_scratch_sizes_of_calls_that_are_refused():
     rc, _ = refused("dial_b200_kv4_evict", *{**EVICT, "sh": shape(), "keep": 2 ** 31}.values())
     assert rc == _abi.DIAL_ERR_INVALID
     assert size(C.byref(sh), 2, 64, 2 ** 31) == -1 and size(C.byref(sh), 2, 64, 2 ** 31 - 1) > 0
+
+
+def test_one_row_of_any_stride():
+    """A single row has no stride to be refused for."""
+    x = torch.zeros(3, 515, dtype=torch.bfloat16)
+    for row in (x[:1, :512], x[:0, :512], x.t()[:512].t()[:1], torch.zeros(512, 1, dtype=torch.bfloat16).t()):
+        assert row.shape[1] == 512
+        assert kv4._rows("q", row, torch.bfloat16, None, 512, -1) == (row.data_ptr(), 512)
+    assert kv4._rows("q", x[:2, :512], torch.bfloat16, 2, 512, -1) == (x.data_ptr(), 515)
