@@ -10,14 +10,6 @@
 namespace dialb200 {
 namespace {
 
-// (query, head of the group) columns of a sequence up to which the decode kernel
-// takes a call: its MMAs are 8 columns wide and a page costs it about the same
-// instructions for each 16, while the tcgen05 kernels have 128 rows a tile whatever
-// a sequence brings.  Measured, decode / tcgen05, 32 heads of 8, 8 sessions of 4096
-// slots: 32 columns 38 / 52 us, 64 61 / 53, 96 85 / 54; one of 65536: 61 / 84, 100 / 85,
-// 144 / 86; with weights, 8 of 4096: 61 / 99, 113 / 101, 193 / 102.
-constexpr int kFewCols = 48;
-
 // Scratch of the attention of many queries; that of their weights follows.
 size_t rows_part(int q_heads, long long rows) {
   return (kv4_prefill_scratch(q_heads, rows, true) + 127) & ~static_cast<size_t>(127);
@@ -28,7 +20,7 @@ size_t rows_part(int q_heads, long long rows) {
 constexpr size_t kScratchAlign = 128;
 
 cudaError_t launch(const Kv4AttnArgs& a, int act, cudaStream_t s) {
-  if (a.max_q * (a.c.q_heads / a.c.kv_heads) <= kFewCols) return kv4_decode_launch(a, act, s);
+  if (a.max_q * (a.c.q_heads / a.c.kv_heads) <= kKv4FewCols) return kv4_decode_launch(a, act, s);
   const cudaError_t e = kv4_prefill_launch(a, act, s);
   if (e != cudaSuccess || !a.c.weights) return e;
   return kv4_colsum_launch(a, kv4_prefill_rows(a),
@@ -50,9 +42,9 @@ extern "C" int64_t dial_b200_kv4_attention_scratch_bytes(const dial_b200_kv4_sha
   if (seqs == 0 || rows == 0 || max_q == 0) return 0;  // the call does nothing
   // enough for every call within the sizes, whichever kernels it takes
   const int rep = sh->q_heads / sh->kv_heads;
-  const int64_t few = max_q < kFewCols / rep ? max_q : kFewCols / rep;
+  const int64_t few = max_q < kKv4FewCols / rep ? max_q : kKv4FewCols / rep;
   size_t bytes = kv4_decode_scratch(sh->q_heads, sh->kv_heads, seqs, few, max_len, with_weights != 0);
-  if (max_q * rep > kFewCols) {
+  if (max_q * rep > kKv4FewCols) {
     const size_t many = with_weights ? rows_part(sh->q_heads, rows) +
                                            kv4_colsum_scratch(sh->q_heads, sh->kv_heads, seqs, max_q, max_len)
                                      : kv4_prefill_scratch(sh->q_heads, rows, false);

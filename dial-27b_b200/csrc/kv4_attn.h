@@ -23,7 +23,14 @@ struct Kv4AttnArgs {
 
 // Few queries a sequence: mma.sync, the cache streamed once for up to 16
 // (query, head) columns (kv4_decode.cu).
-constexpr int kKv4DecodeCols = 512;  // (query, head) columns of a kv head at most
+//
+// (query, head of the group) columns of a sequence up to which it takes a call: its
+// MMAs are 8 columns wide and a page costs it about the same instructions for each 16,
+// while the tcgen05 kernels have 128 rows a tile whatever a sequence brings.
+// Measured, decode / tcgen05, 32 heads of 8, 8 sessions of 4096 slots: 32 columns 38 / 52
+// us, 64 61 / 53, 96 85 / 54; one of 65536: 61 / 84, 100 / 85, 144 / 86; with weights, 8
+// of 4096: 61 / 99, 113 / 101, 193 / 102.
+constexpr int kKv4FewCols = 48;
 size_t kv4_decode_scratch(int q_heads, int kv_heads, long long seqs, long long max_q,
                           long long max_len, bool weights);
 cudaError_t kv4_decode_launch(const Kv4AttnArgs& a, int act, cudaStream_t s);

@@ -840,7 +840,7 @@ __global__ void __launch_bounds__(kJoinThreads, 4) kv4_join_kernel(const DecodeA
     }
     return;
   }
-  __shared__ float2 ml[kKv4DecodeCols];  // (m, 1 / l) of the segment's columns
+  __shared__ float2 ml[kKv4FewCols];  // (m, 1 / l) of the segment's columns
   const Rec* recs = d.rec + static_cast<size_t>(b) * d.rec_ld;
   const int n = d.rec_n[b];
   const int starts = b - 1 - lane >= 0 ? d.desc[b - 1 - lane].x : -1;
@@ -901,8 +901,7 @@ Plan plan_of(int q_heads, int kv_heads, long long seqs, long long max_q, long lo
   p.one = max_len <= kOneLen && !(weights && p.groups > 1);
   const int warps = p.nt == 1 ? kWarpsOf<1> : kWarpsOf<2>;
   const long long want = (p.pages + warps - 1) / warps;
-  long long most = static_cast<long long>(sms) * (p.nt == 1 ? kCtasPerSm<1> : kCtasPerSm<2>) / p.groups;
-  if (most < sms / 4) most = sms / 4;
+  const long long most = static_cast<long long>(sms) * (p.nt == 1 ? kCtasPerSm<1> : kCtasPerSm<2>) / p.groups;
   p.ctas = static_cast<int>(want < 1 ? 1 : want < most ? want : most);
   if (p.one) p.ctas = static_cast<int>(seqs * kv_heads);
   p.score_ld = (p.cols + 1) & ~1;
