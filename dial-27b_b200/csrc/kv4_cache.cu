@@ -156,8 +156,8 @@ __device__ __forceinline__ void encode8(const float (&x)[8], float mult, uint32_
 // A CTA for a row and a share (blockIdx.y) of its head units, a half warp a unit: unit
 // u < kv_heads is a kv head (k and v), the others query heads.  A warp's norm weights,
 // cos and sin serve all its units, U of which are loaded at once.
-// Bound by instructions for long prompts (14.6 M for 2048 rows, about half of them the
-// quantisation; 2.46 a clock, DRAM at 12 %), by latency for a token (7 us cold).
+// 2048 rows: 14.6 M instructions, about half of them the quantisation, at 2.45 of 4 a
+// clock: a row's loads are waited for (DRAM 12 %, ALU 42 %).  A token: latency (7 us cold).
 template <typename Act, int U>
 __global__ void __launch_bounds__(256) kv4_append_kernel(const AppendArgs a) {
   const int lane = threadIdx.x & 31, l = lane & 15, m = blockIdx.x;
@@ -468,11 +468,11 @@ extern "C" int dial_b200_kv4_append(const dial_b200_kv4_shape* sh, const void* q
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   cudaError_t e;
   const int most = (a.units + 15) / 16;
-  // A unit a half warp while 148 SMs have room for the CTAs (8 of 256 threads each);
-  // else a row a CTA, three of a half warp's units in flight.  32 heads of 8 (3 CTAs a
-  // row), unit / row: 16 rows 3.0 / 4.0 us, 256 4.9 / 4.8, 394 6.0 / 6.4, 1024 13.3 / 10.3,
-  // 2048 24.7 / 18.5.
-  if (rows * most <= 1184) {
+  // A unit a half warp up to two rounds of the 592 CTAs that are resident (four an SM, at
+  // 64 registers a thread); from there on a row a CTA, three of a half warp's units in
+  // flight.  32 heads of 8 (3 CTAs a row), unit / row: 16 rows 3.0 / 4.0 us, 256 4.9 / 4.8,
+  // 394 (1182 CTAs) 6.0 / 6.4, 1024 13.3 / 10.3, 2048 24.7 / 18.5.
+  if (rows * most <= 2 * 592) {
     const dim3 grid(static_cast<unsigned>(rows), most);
     e = sh->act == DIAL_ACT_BF16 ? kv4_start(kv4_append_kernel<__nv_bfloat16, 1>, grid, 256, 0, s, a)
                                  : kv4_start(kv4_append_kernel<__half, 1>, grid, 256, 0, s, a);

@@ -7,7 +7,7 @@
 // (kv4_prefill.cu).  Half that attention's MMAs and all of its exponentials; bound
 // by the exponentials (16 a clock and SM).  S^T = K Q^T has a key in every TMEM
 // lane, so a thread adds up its own key's row and nothing is exchanged.
-// Measured: 512 tokens each on 9500 and 16897 slots, 40 heads of 8, 244-263 us by
+// Measured: 512 tokens each on 9500 and 16897 slots, 40 heads of 8, 244-265 us by
 // the clock, the exponentials' unit 70 % busy, tensor pipe 33 %.  With one warp a key and
 // tile (8, not 16) 325; with scores in runs of 32, not 16, 280.
 //

@@ -29,12 +29,13 @@
 // of the page's) and the join turns them into probabilities once m and l are known, a
 // slot a thread, no atomics.
 //
-// Measured, kernel and join by themselves with cold caches: 32 sessions of 128 to 8192 slots (180 MB) 49 + 6 us, one of
-// 131071 (151 MB) 39 + 8, 9 of 900 to 30001 with weights 48 + 17, five queries of 8
-// sessions of 700 to 4099 with weights 36 + 15, 201 slots 10.  Bound by
-// instructions: 320 a page and column tile (16 MMAs, 64 conversions and 64 packed
-// products of the codes with what arranges them, the softmax of 128 scores), 2.45 a
-// clock; DRAM at 46 %, the tensor pipe at 21 %.
+// Measured, kernel and join by themselves with cold caches: 32 sessions of 128 to 8192
+// slots (180 MB) 48 + 4 us, one of 131071 (151 MB) 38 + 6, 9 of 900 to 30001 with weights
+// 47 + 16, five queries of 8 sessions of 700 to 4099 with weights 34 + 14, 201 slots 8.
+// No unit is full: a page and column tile takes 320 instructions (16 MMAs, 64
+// conversions and 64 packed products of the codes with what arranges them, the softmax
+// of 128 scores), each waiting for one before it, and the 16 warps an SM that registers
+// leave issue 2.45 of 4 a clock (ALU 52 %, DRAM 46 %, tensor pipe 21 %).
 #include <cmath>
 #include <type_traits>
 
@@ -55,9 +56,11 @@ template <int NT>
 constexpr int kCtasPerSm = NT == 1 ? 2 : 3;
 constexpr int kRing = 4;           // pages in flight a warp
 constexpr int kSeqChunk = 256;     // sequences a launch
-// A segment's own cost (its start, and the merge of its parts), in pages.  32 ragged
-// sessions of 128 to 8192 slots: 55.7 us at 1, 53.3 at 10, 51.0 at 20, 50.8 at 30; five
-// queries of 8 sessions with weights 55.0 at 1, 50.2 at 20.
+// A segment's own cost (its start, and the merge of its parts), in pages.  At 10 / 20 / 30
+// / 45: 32 sessions of 128 to 8192 slots 50.1 / 48.1 / 47.9 / 49.3 us; 100 of 1200 to 2500
+// 63.1 / 61.7 / 61.4 / 61.4, with weights 90.3 / 87.7 / 86.9 / 87.0; five queries of 8
+// sessions with weights 44.8 / 42.7 / 43.0 / 45.1; four of 20 sessions of 1000 to 9000
+// slots 56.0 / 54.7 / 55.3 / 56.5.
 constexpr int kSegPad = 20;
 constexpr int kInfo = 6;           // sequences of a range kept in shared memory
 constexpr int kOneLen = 1024;      // slots up to which a CTA takes a whole segment

@@ -13,9 +13,9 @@
 //     ballots.
 //  2. kv4_move_kernel: eight lanes an entry, four entries a warp and step.
 //
-// Measured: 16 sessions of 3500 to 8192 slots, 8 kv heads, halved: select 32 us (128 CTAs,
-// one wave; bound by the passes' latency), move 38 (bound by the latency of 64-byte
-// pieces; DRAM at 48 %).  Keys in shared memory / read anew each pass, both kernels:
+// Measured: 16 sessions of 3500 to 8192 slots, 8 kv heads, halved: select 30 us (128 CTAs,
+// one wave: the passes take about 330 instructions for 32 slots, 1.96 of 4 a clock), move
+// 37 (waits for its loads of 64-byte pieces; DRAM at 48 %).  Keys in shared memory / read anew each pass, both kernels:
 // one session of 4096 19 / 27 us, 16 of 8192 40 / 57, 4 of 24576 63 / 127.
 #include "kv4_dev.cuh"
 #include "kv4_launch.h"

@@ -22,7 +22,7 @@
 // an item is kept in rolled loops, since its instructions are fetched anew each time
 // (290 against 332).
 //
-// Measured: a 2048-token prompt, 32 heads of 8 (34 GFLOP) 72 us with the join of 15; 512
+// Measured: a 2048-token prompt, 32 heads of 8 (34 GFLOP) 73 us with the join of 14; 512
 // tokens each on 9500 and 16897 slots, 40 heads of 8 (271 GFLOP) 290-317 by the
 // clock.  Two tiles' 128-key block takes 2.4 us against 1.1 for its MMAs and 1.1 for
 // its exponentials: bound by the chain S, softmax, P V of each tile, of which two
@@ -45,8 +45,10 @@ namespace {
 constexpr int kRows = 128;                  // rows of a tile
 constexpr int kKeys = 128;                  // keys of a block
 constexpr int kThreads = 13 * 32;
-// An item's own cost (its start and output), in blocks: a 2048-token prompt takes 80.8
-// us at 2, 72.4 at 4, 75.5 at 6.
+// An item's own cost (its start and output), in blocks.  At 2 / 4 / 6: a prompt of 1024
+// tokens 41.1 / 39.3 / 36.5 us, of 2048 81.1 / 72.9 / 75.8, of 4096 195 / 181 / 186; 300
+// queries each of 4 sessions of 2000 to 6000 slots 137 / 140 / 142; 512 each on 9500
+// and 16897 the same within 0.4 %.
 constexpr int kPad = 4;
 constexpr int kSeqChunk = 512;              // sequences a launch
 constexpr int kOffQ = 0;                    // [2]

@@ -262,7 +262,11 @@ int64_t dial_b200_kv4_attention_scratch_bytes(const dial_b200_kv4_shape* sh, int
  * queries of sequence i are rows q_starts[i] .. q_starts[i + 1] - 1 of q [rows,
  * q_ld] (q_starts NULL: row i), n of them, and query j sees slots 0 ..
  * lens[i] - n + j of session sids[i]; a query that sees none gives zeros.
- *   out [rows, out_ld] = softmax(softmax_scale * q . k) . v, f32 inside;
+ *   out [rows, out_ld] = softmax(softmax_scale * q . k) . v.  Scores, sums and
+ *   accumulators are f32; queries enter their product as f16 after an exact power of
+ *   two (off by 2^-25 of the row's largest value at most), probabilities theirs as f16
+ *   (off by 2^-11 of themselves, or 2^-32 of the row's largest).  A query head with a NaN
+ *   gives NaN, and adds NaN to the weights of the slots that it sees;
  *   weights (if not NULL): weights[slot] += the slot's probabilities summed
  *   over the sequence's queries and the query heads of the kv head.  Sequences
  *   must then name distinct sessions that share no page (a sum is one load and
