@@ -468,8 +468,8 @@ extern "C" int dial_b200_kv4_append(const dial_b200_kv4_shape* sh, const void* q
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   cudaError_t e;
   const int most = (a.units + 15) / 16;
-  // A unit a half warp up to two rounds of the 592 CTAs that are resident (four an SM, at
-  // 64 registers a thread); from there on a row a CTA, three of a half warp's units in
+  // A unit a half warp up to twice the 592 CTAs that are resident (four an SM, at 64
+  // registers a thread); from there on a row a CTA, three of a half warp's units in
   // flight.  32 heads of 8 (3 CTAs a row), unit / row: 16 rows 3.0 / 4.0 us, 256 4.9 / 4.8,
   // 394 (1182 CTAs) 6.0 / 6.4, 1024 13.3 / 10.3, 2048 24.7 / 18.5.
   if (rows * most <= 2 * 592) {
