@@ -104,6 +104,7 @@ extern "C" int dial_b200_kv4_attention(const dial_b200_kv4_shape* sh, const void
   a.max_q = static_cast<int>(max_q);
   a.max_len = static_cast<int>(max_len);
   const float scale = sh->softmax_scale > 0.f ? sh->softmax_scale : 1.f / sqrtf(static_cast<float>(kHeadDim));
+  a.zeros = 0;
   a.unit = static_cast<float>(frexp(1.4426950408889634 * scale * sh->k_scale, &a.unit_exp));
   if ((rc = kv4_ready(&a.c, err, n)) != DIAL_OK) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);

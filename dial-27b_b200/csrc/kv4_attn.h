@@ -19,6 +19,7 @@ struct Kv4AttnArgs {
   // codes and e4m3 scales to base-2 scores
   float unit;
   int unit_exp;
+  uint64_t zeros;  // two f32 zeros, not known when the kernels are compiled (score2)
 };
 
 // Few queries a sequence: mma.sync, the cache streamed once for up to 16

@@ -36,6 +36,7 @@ constexpr int kOffK = 0;                     // [2], the item's two key blocks
 constexpr int kOffQ = 2 * kTile;             // [kQBufs]
 constexpr int kOffMisc = (2 + kQBufs) * kTile;
 constexpr int kStatusKv4Colsum = 0x602;
+constexpr float kLarge = 4096.f;
 
 struct Misc {
   uint64_t kfull, kfree, qfull[kQBufs], qfree[kQBufs], sfull[kSBufs], sfree[kSBufs], cfull[kCBufs], cfree[kCBufs], fin;
@@ -44,6 +45,10 @@ struct Misc {
   alignas(16) float fac[kCBufs][128];
   alignas(16) float off[kCBufs][128];
   alignas(16) int seen[kCBufs][128];    // slots the row sees
+  // slots that all of a tile's 128 rows see; 0 for fewer rows, and for a log-sum-exp above
+  // kLarge, of whose rounding an fma would keep too much in the exponent (2^-13 at kLarge;
+  // rounding every score first, in the path of whole tiles too, takes 290 us for 266)
+  int all_see[kCBufs];
   long long cum[kSeqChunk + 1];         // items of one kv head of the sequences before
 };
 constexpr int kSmemBytes = kOffMisc + sizeof(Misc) + 1024;
@@ -207,8 +212,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_colsum_kernel(const __grid_co
           __syncwarp();
           if (lane == 0) mbar_arrive(&sm.sfree[sb]);
         };
-        // every row of the tile is there and sees the whole block
-        if ((T + 1) * 128 <= w.s.n * rep && w.s.len - w.s.n + 1 + T * 128 / rep >= key0 + 128) {
+        if (sm.all_see[cb] >= key0 + 128) {
           uint32_t x[16], y[16];
           auto add = [&](const uint32_t* v, int c0) {
 #pragma unroll
@@ -242,8 +246,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_colsum_kernel(const __grid_co
             ld_wait16(x);
 #pragma unroll
             for (int e = 0; e < 16; e += 2) {
-              const float z0 = fmaf(__uint_as_float(x[e]), fc[c + e], of[c + e]);
-              const float z1 = fmaf(__uint_as_float(x[e + 1]), fc[c + e + 1], of[c + e + 1]);
+              // scores rounded as the log-sum-exps have them
+              const float z0 = __fmul_rn(__uint_as_float(x[e]), fc[c + e]) + of[c + e];
+              const float z1 = __fmul_rn(__uint_as_float(x[e + 1]), fc[c + e + 1]) + of[c + e + 1];
               s0 = add2(s0, pair(key < seen[c + e] ? ex2(z0) : 0.f, key < seen[c + e + 1] ? ex2(z1) : 0.f));
             }
             __syncwarp();
@@ -314,12 +319,17 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_colsum_kernel(const __grid_co
         ++issued;
         ok = wait(&sm.cfree[cb], (n / kCBufs & 1u) ^ 1u);
         if (!ok) break;
+        bool large = false;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
+          large |= fabsf(ov[e]) > kLarge && ov[e] != -INFINITY;
           sm.fac[cb][e * 32 + lane] = fv[e];
           sm.off[cb][e * 32 + lane] = ov[e];
           sm.seen[cb][e * 32 + lane] = sv[e];
         }
+        large = __any_sync(0xffffffffu, large);
+        if (lane == 0)
+          sm.all_see[cb] = large || (T + 1) * 128 > w.s.n * rep ? 0 : w.s.len - w.s.n + 1 + T * 128 / rep;
         __syncwarp();
         if (lane == 0) mbar_arrive(&sm.cfull[cb]);
       }

@@ -509,6 +509,15 @@ __global__ void __launch_bounds__(kWarpsOf<NT> * 32, kCtasPerSm<NT>)
           }
         }
       }
+      // scores, rounded: the same in the reference and here, so that the largest one's
+      // difference is right however large they are (an fma would keep the rounding of the
+      // reference, 2^-24 of it, in the exponent)
+#pragma unroll
+      for (int u = 0; u < N; ++u)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[u][nt][e] = __fmul_rn(x[u][nt][e], fac[nt][e & 1]);
       uint32_t there[N][2];  // V scales to keep: slots past the end may hold anything
 #pragma unroll
       for (int u = 0; u < N; ++u) there[u][0] = there[u][1] = 0xFFFFFFFFu;
@@ -541,13 +550,12 @@ __global__ void __launch_bounds__(kWarpsOf<NT> * 32, kCtasPerSm<NT>)
 #pragma unroll
             for (int u = 0; u < N; ++u) {
               float* to = d.scores + (score0 + static_cast<size_t>(w.seg0 + page0 + kWarps * u) * kPageTokens + t0) * d.score_ld + cc;
-              *reinterpret_cast<float2*>(to) = make_float2(x[u][nt][0] * fac[nt][0], x[u][nt][1] * fac[nt][1]);
-              *reinterpret_cast<float2*>(to + 8 * d.score_ld) =
-                  make_float2(x[u][nt][2] * fac[nt][0], x[u][nt][3] * fac[nt][1]);
+              *reinterpret_cast<float2*>(to) = make_float2(x[u][nt][0], x[u][nt][1]);
+              *reinterpret_cast<float2*>(to + 8 * d.score_ld) = make_float2(x[u][nt][2], x[u][nt][3]);
             }
         }
       }
-      // m is the reference, `high` (m + kTop) / fac: the vote needs no scaled scores
+      // m is the reference, `high` m + kTop
       float top[NT][2];
       bool raise = false;
 #pragma unroll
@@ -567,11 +575,11 @@ __global__ void __launch_bounds__(kWarpsOf<NT> * 32, kCtasPerSm<NT>)
             float t = top[nt][e];
 #pragma unroll
             for (int i = 4; i < 32; i <<= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, i));
-            const float mn = fmaxf(m[nt][e], t * fac[nt][e] - kLift);
+            const float mn = fmaxf(m[nt][e], t - kLift);
             const float al = m[nt][e] == -INFINITY ? 0.f : ex2(m[nt][e] - mn);
             m[nt][e] = mn;
             ref[nt][e] = mn == -INFINITY ? 0.f : mn;
-            high[nt][e] = __fdiv_rn(mn + kTop, fac[nt][e]);
+            high[nt][e] = __fadd_rd(mn, kTop);
             l[nt][e] *= al;
 #pragma unroll
             for (int mt = 0; mt < 8; ++mt) {
@@ -585,10 +593,10 @@ __global__ void __launch_bounds__(kWarpsOf<NT> * 32, kCtasPerSm<NT>)
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int u = 0; u < N; ++u) {
-          const float p0 = ex2(fmaf(x[u][nt][0], fac[nt][0], -ref[nt][0]));
-          const float p1 = ex2(fmaf(x[u][nt][1], fac[nt][1], -ref[nt][1]));
-          const float p2 = ex2(fmaf(x[u][nt][2], fac[nt][0], -ref[nt][0]));
-          const float p3 = ex2(fmaf(x[u][nt][3], fac[nt][1], -ref[nt][1]));
+          const float p0 = ex2(x[u][nt][0] - ref[nt][0]);
+          const float p1 = ex2(x[u][nt][1] - ref[nt][1]);
+          const float p2 = ex2(x[u][nt][2] - ref[nt][0]);
+          const float p3 = ex2(x[u][nt][3] - ref[nt][1]);
           l[nt][0] += p0 + p2;
           l[nt][1] += p1 + p3;
           pf[u][nt][0] = transpose8(pack_f16(p0, p1));

@@ -56,12 +56,10 @@ __device__ __forceinline__ float quotient(float x, float s, float y) {
 }
 
 // Queries enter the MMAs as f16 after 2^-e, e the exponent of the row's largest value
-// `top`: exact for values down to 2^-14 of it, and off by at most 2^-25 of it below.  No
-// less than -100, where values of 2^-125 still count: rows of zeros, the columns of an
-// MMA past the last query, keep a scale by which the decode kernel divides without the
-// slow path of the smallest numbers (32 ragged sessions 48.2 us, at -126 49.5).
+// `top` (within f32's normal powers): exact for values down to 2^-14 of it, and off by
+// at most 2^-25 of it below.
 __device__ __forceinline__ int query_exp(float top) {
-  return min(max(static_cast<int>(__float_as_uint(top) >> 23) - 127, -100), 126);
+  return min(max(static_cast<int>(__float_as_uint(top) >> 23) - 127, -126), 126);
 }
 // What such a row's sums are multiplied by to become base-2 scores.  Kept within f32's
 // normal numbers, so that a masked score, -inf, stays -inf under any scale.

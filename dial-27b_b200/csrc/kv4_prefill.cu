@@ -429,9 +429,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const PrefillA
             auto chunk = [&](const uint32_t* v, uint32_t* to) {
 #pragma unroll
               for (int e = 0; e < 8; ++e) {
-                const uint64_t z = fma2(pair(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])), fac2, off2);
-                if (e & 1) t1 = max3(t1, lo_of(z), hi_of(z));
-                else t0 = max3(t0, lo_of(z), hi_of(z));
+                const uint64_t s = score2(a, pair(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])), fac2);
+                if (e & 1) t1 = max3(t1, lo_of(s), hi_of(s));
+                else t0 = max3(t0, lo_of(s), hi_of(s));
+                const uint64_t z = add2(s, off2);
                 const float p0 = ex2(lo_of(z)), p1 = ex2(hi_of(z));
                 if (e & 1) sum1 = add2(sum1, pair(p0, p1));
                 else sum0 = add2(sum0, pair(p0, p1));
@@ -453,8 +454,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const PrefillA
             top = fmaxf(t0, t1);
           };
           probs();
-          if (__any_sync(0xffffffffu, top > kTop || (m == -INFINITY && top > -INFINITY))) {
-            const float mn = fmaxf(m, ceilf(top + ref) - kLift);
+          if (__any_sync(0xffffffffu, top > __fadd_rd(m, kTop))) {
+            const float mn = fmaxf(m, ceilf(top) - kLift);
             const float al = m == -INFINITY ? 0.f : ex2(m - mn);
             m = mn;
             ref = mn == -INFINITY ? 0.f : mn;

@@ -143,6 +143,14 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
   return d;
 }
+// x f, rounded, two at a time: scores as their references and log-sum-exps have them,
+// so that what is subtracted from the largest one leaves the right exponent however
+// large they are (an fma would keep a reference's rounding, 2^-24 of it, in the
+// exponent).  Written with a zero that the compiler does not know: a product and the
+// sum after it are made into one fma, in this form too.
+__device__ __forceinline__ uint64_t score2(const Kv4AttnArgs& a, uint64_t x, uint64_t f) {
+  return fma2(x, f, a.zeros);
+}
 __device__ __forceinline__ float lo_of(uint64_t v) { return __uint_as_float(static_cast<uint32_t>(v)); }
 __device__ __forceinline__ float hi_of(uint64_t v) { return __uint_as_float(static_cast<uint32_t>(v >> 32)); }
 

@@ -124,6 +124,53 @@ def test_queries_near_the_ends_of_bf16(cuda, power, queries, n):
     assert (d <= sb + 2.0 ** -23 * (2 * before[blk, :, off] + s)).all()
 
 
+@pytest.mark.parametrize("power", [14, 19, 22, 24, 25, 26, 27, 28, 30, 40, 80, 120])
+@pytest.mark.parametrize("queries,n", [(1, 900), (1, 3000), (5, 1300), (70, 700)])
+def test_scores_far_beyond_f32s_whole_numbers(cuda, power, queries, n):
+    """Queries of 2^power under the ordinary scale: a head takes its best slot's values
+    and adds 1 to its weight wherever the runner-up is further off than the roundings of
+    32-bit scores (2^-18 of sum |q k|, twice attend's bound) and than 40; where it is
+    not, the result lies between the values.  f16 probabilities cost 2^-11, the output
+    half a step; the weight of a lone slot is 1 but for 2^-20 (exponentials and 1 / l)."""
+    from dial_b200 import kv4
+
+    c = Cache(71, 2, n, 8, 2)
+    cache, table = c.device(cuda)
+    q = (torch.randn(queries + 1, 8 * DIM, device=cuda).clamp(-3.9, 3.9).double() * 2.0 ** power).to(BF16)
+    before = host(cache.weights)
+    out = host(kv4.kv4_attention(c.sh, cache, q, table, i32(cuda, 1, 0), i32(cuda, n, 77), n,
+                                 q_starts=i32(cuda, 0, queries, queries + 1), max_q=queries,
+                                 accumulate=True)).reshape(queries + 1, 8, DIM)
+    assert np.isfinite(out).all()
+    added, decided = host(cache.weights) - before, 0
+    for sid, rows, length in ((1, range(queries), n), (0, [queries], 77)):
+        K, V = c.values(sid, length)
+        Q = host(q).reshape(-1, 8, DIM)
+        want, open_ = np.zeros((length, 2)), np.zeros(2)
+        for j in rows:
+            seen = length - len(rows) + 1 + j - rows[0]
+            for h in range(8):
+                k, v = K[:seen, h // 4], V[:seen, h // 4]
+                s = (k @ Q[j, h]) * DIM ** -0.5
+                best = int(s.argmax())
+                gap = s[best] - np.delete(s, best).max()
+                noise = 2.0 ** -18 * (np.abs(k) @ np.abs(Q[j, h])).max() * DIM ** -0.5
+                if gap > max(noise, 40.0):
+                    decided += 1
+                    want[best, h // 4] += 1
+                    d = np.abs(out[j, h] - v[best])
+                    assert (d <= (2.0 ** -11 + 2.0 ** -8) * np.abs(v[best]) + 2.0 ** -30).all()
+                else:
+                    open_[h // 4] += 1
+                    eps = 2.0 ** -7 * np.abs(v).max()
+                    assert (out[j, h] >= v.min(0) - eps).all() and (out[j, h] <= v.max(0) + eps).all()
+        blk, off = c.at(sid, length)
+        d = added[blk, :, off] - want
+        lim = 2.0 ** -20 * want + 2.0 ** -22 * (before[blk, :, off] + want)
+        assert (d >= -lim).all() and (d <= lim + open_ * (1 + 2.0 ** -10)).all()
+    assert decided > 0.8 * 8 * (queries + 1) or power < 19
+
+
 @pytest.mark.parametrize("queries", [3, 60])
 def test_scales_that_leave_nothing_of_a_score(cuda, queries):
     """Zero queries and ordinary ones under a scale of 1e-30: every slot that a query
