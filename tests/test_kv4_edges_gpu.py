@@ -7,7 +7,7 @@ import numpy as np
 import pytest
 import torch
 
-from kv4_case import DIM, Cache, i32
+from kv4_case import DIM, Cache, act_round, i32, norm_rope, same_slabs
 from test_kv4_gpu import check_attention
 
 pytestmark = pytest.mark.gpu
@@ -379,3 +379,37 @@ def test_evict_of_a_session_past_shared_memory(cuda, out_of_place):
     np.testing.assert_array_equal(host(cache.pages), c.pages)
     np.testing.assert_array_equal(host(cache.weights), c.weights)
     np.testing.assert_array_equal(host(cache.positions), c.positions)
+
+
+@pytest.mark.parametrize("dt", [BF16, F16])
+def test_append_of_rows_at_the_ends_of_the_type(cuda, dt):
+    """Heads of values near the type's largest and smallest, of one value beside zeros, and
+    of zeros alone, with norm and RoPE: q and the slabs equal the reference."""
+    from dial_b200 import kv4
+
+    c = Cache(72, 1, 64, 6, 2, dt=dt, fill=False, max_pos=300)
+    cache, table = c.device(cuda)
+    rows = 40
+    lo, hi = (-14, 14) if dt == F16 else (-126, 125)
+    x = c.rng.standard_normal((rows, 10, DIM)).clip(-3.5, 3.5)
+    x *= 2.0 ** c.rng.integers(lo, hi + 1, (rows, 10, 1))
+    x[0] = 0
+    x[1, :, 1:] = 0
+    x[2, :, ::2] *= 2.0 ** -9
+    x = act_round(x.reshape(rows, -1), dt)
+    slots = np.arange(rows, dtype=np.int32)
+    pos = (slots * 7).astype(np.int32)
+    tab = np.arange(300)[:, None] * 1e6 ** (-np.arange(64) / 64)
+    cos, sin = (act_round(f(tab), dt) for f in (np.cos, np.sin))
+    w = act_round(1 + 0.2 * c.rng.standard_normal(DIM), dt)
+    t = lambda a: torch.from_numpy(np.ascontiguousarray(a)).to(cuda).to(dt)  # noqa: E731
+    q = kv4.kv4_append(c.sh, cache, t(x), table, i32(cuda, *[0] * rows), i32(cuda, *slots.tolist()),
+                       i32(cuda, *pos.tolist()), t(w), t(w), t(cos), t(sin))
+    hd = x.reshape(rows, -1, DIM)
+    eps = float(np.float32(1e-6))
+    qr = norm_rope(hd[:, :6], w, cos[pos], sin[pos], eps, dt)
+    kr = norm_rope(hd[:, 6:8], w, cos[pos], sin[pos], eps, dt)
+    np.testing.assert_array_equal(host(q), qr.reshape(rows, -1))
+    for m in range(rows):
+        c.put(0, m, kr[m], hd[m, 8:], pos[m])
+    same_slabs(host(cache.pages), c.pages)
