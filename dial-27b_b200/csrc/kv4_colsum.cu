@@ -7,8 +7,8 @@
 // (kv4_prefill.cu).  Half that attention's MMAs and all of its exponentials; bound
 // by the exponentials (16 a clock and SM).  S^T = K Q^T has a key in every TMEM
 // lane, so a thread adds up its own key's row and nothing is exchanged.
-// Measured: 512 tokens each on 9500 and 16897 slots, 40 heads of 8, 244-265 us by
-// the clock, the exponentials' unit 70 % busy, tensor pipe 33 %.  With one warp a key and
+// Measured: 512 tokens each on 9500 and 16897 slots, 40 heads of 8, 258 us cold,
+// the exponentials' unit 69 % busy, tensor pipe 34 %.  With one warp a key and
 // tile (8, not 16) 325; with scores in runs of 32, not 16, 280.
 //
 // Items: two 128-key blocks of a (sequence, kv head), so that a query tile fetched
@@ -47,7 +47,7 @@ struct Misc {
   alignas(16) int seen[kCBufs][128];    // slots the row sees
   // slots that all of a tile's 128 rows see; 0 for fewer rows, and for a log-sum-exp above
   // kLarge, of whose rounding an fma would keep too much in the exponent (2^-13 at kLarge;
-  // rounding every score first, in the path of whole tiles too, takes 290 us for 266)
+  // rounding every score first, in the path of whole tiles too, takes 290 us)
   int all_see[kCBufs];
   long long cum[kSeqChunk + 1];         // items of one kv head of the sequences before
 };

@@ -31,7 +31,7 @@
 //
 // Measured, kernel and join by themselves with cold caches: 32 sessions of 128 to 8192
 // slots (180 MB) 48 + 4 us, one of 131071 (151 MB) 38 + 6, 9 of 900 to 30001 with weights
-// 47 + 16, five queries of 8 sessions of 700 to 4099 with weights 34 + 14, 201 slots 8.
+// 46 + 16, five queries of 8 sessions of 700 to 4099 with weights 34 + 14, 201 slots 7.
 // No unit is full: a page and column tile takes 320 instructions (16 MMAs, 64
 // conversions and 64 packed products of the codes with what arranges them, the softmax
 // of 128 scores), each waiting for one before it, and the 16 warps an SM that registers
